@@ -248,6 +248,47 @@ LB_API int lb_encode_encrypt(lb_context *ctx, const uint64_t *pk, const void *va
 LB_API int lb_decode(lb_context *ctx, int size_l, const uint64_t *pt, double scale, int sparse_slots, double *out_complex, void *stream);
 /* pt[batch][size_l][N] -> out_complex[batch][sparse_slots] (re, im) pairs */
 LB_API int lb_decode_batch(lb_context *ctx, int size_l, int batch, const uint64_t *pt, double scale, int sparse_slots, double *out_complex, void *stream);
+/* ---- 8-bit updates (no counterpart in the reference) ------------------------------------------
+ * Clients' updates held, compared and multiplied as 8-bit integers with scales.  The cache is `n_slots` slots of `page`
+ * codes (slot s at codes + s * code_stride) and one scale per group of `group` columns (at scales + s * scale_stride); group is a
+ * power of two from 32 on, or 0 for one group in a page.  page and code_stride are multiples of 16, codes starts on a 16-byte
+ * boundary.  A row of n_cols values covers ceil(n_cols / page) pages; slots (DEVICE, may be NULL: in order) names the
+ * slot of page p of row i at [i * pages + p].  A page whose slot lies outside [0, n_slots) is not in the cache: it is
+ * not written, and reads as zeros.  The slots that one call writes must be distinct.
+ * dtype: 1 = float, 3 = bfloat16, 4 = IEEE half (lb_encode's numbers, continued).  Strides are in elements and count between
+ * rows, which must not overlap.  workspace: DEVICE memory on a 16-byte boundary that belongs to the call until it has run, at
+ * least as much as the call's _workspace_bytes says (NULL where that is 0); these calls leave the context's own scratch alone. */
+
+/* t = values + residual (residual NULL: 0) in 32 bits, 0 from lengths[i] columns of row i on (lengths DEVICE; NULL: n_cols; clamped to
+ * [0, n_cols]).  Per group: m = max|t|, scale = m / 127 rounded to 32 bits, code = the integer nearest to t / scale, ties to
+ * even.  A group of zeros has scale 0; one that holds an infinity or NaN has scale NaN and codes 0, so that it reads as NaN.
+ * residual_out (NULL, residual itself, or memory apart from it) gets t - code * scale, exactly, for the columns below the row's
+ * length (0 in a group whose scale is NaN); the columns from there on are left as they are.  A page is always written whole, with
+ * zeros behind the row's end. */
+LB_API size_t lb_quantize_rows_workspace_bytes(int64_t n_rows, int64_t n_cols, int64_t page, int64_t group);
+LB_API int lb_quantize_rows(lb_context *ctx, const void *values, int dtype, int64_t n_rows, int64_t n_cols, int64_t value_stride,
+                     const int32_t *lengths, const float *residual, float *residual_out, int64_t residual_stride, const int32_t *slots,
+                     int64_t n_slots, int64_t page, int64_t group, int8_t *codes, int64_t code_stride, float *scales, int64_t scale_stride,
+                     void *workspace, size_t workspace_bytes, void *stream);
+/* out[i][c] = code * scale (32 bits, then rounded to dtype) of column c % page of the slot of page c / page of row i */
+LB_API int lb_dequantize_rows(lb_context *ctx, const int8_t *codes, int64_t code_stride, const float *scales, int64_t scale_stride,
+                       int64_t n_slots, int64_t page, int64_t group, const int32_t *slots, int64_t n_rows, int64_t n_cols, void *out,
+                       int dtype, int64_t out_stride, void *stream);
+/* out[i][j] = (sum over k of a[i][k] b[j][k]) * a_scale[i] * b_scale[j]: an exact integer sum (k <= 131071), scaled in 32 bits, rounded to
+ * dtype.  a [m][k], b [n][k], any alignment of their rows (rows off a 16-byte boundary are copied into the workspace first).
+ * a_scale [m], b_scale [n]; out must not overlap an operand. */
+LB_API size_t lb_int8_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t a_stride, const int8_t *b, int64_t b_stride);
+LB_API int lb_int8_matmul(lb_context *ctx, int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t a_stride, const float *a_scale,
+                   const int8_t *b, int64_t b_stride, const float *b_scale, void *out, int dtype, int64_t out_stride, void *workspace,
+                   size_t workspace_bytes, void *stream);
+/* The selection rule's pair distances in the clear (lancelot-main-GPU/utils/byzantine_fl.py:162-171,527-536) over cached updates:
+ * out[i][j] (DEVICE, n x n doubles) = the squared distance of rows i and j of the cache, 0 for i == j.  slots [n][n_pages]; the
+ * pages of a row count whole (what lb_quantize_rows wrote behind a row's end are zeros).  n <= 4096. */
+LB_API size_t lb_int8_distances_workspace_bytes(const lb_context *ctx, int64_t n, int64_t n_pages, int64_t page);
+LB_API int lb_int8_distances(lb_context *ctx, const int8_t *codes, int64_t code_stride, const float *scales, int64_t scale_stride,
+                      int64_t n_slots, int64_t page, int64_t group, const int32_t *slots, int64_t n, int64_t n_pages, double *out,
+                      void *workspace, size_t workspace_bytes, void *stream);
+
 /* Synchronises the stream and reports (then clears) conditions kernels could only flag. */
 LB_API int lb_check_status(lb_context *ctx, void *stream);
 

@@ -725,6 +725,145 @@ int lb_decode_batch(lb_context *h, int size_l, int batch, const uint64_t *pt, do
     return decode(C(h), size_l, batch, pt, scale, sparse_slots, out_complex, S(stream));
 }
 
+// ---- 8-bit updates ---------------------------------------------------------------------------
+
+static int cache_ok(const int8_t *codes, int64_t code_stride, const float *scales, int64_t scale_stride, int64_t n_slots, int64_t page,
+                    int64_t group)
+{
+    REQUIRE(page >= 16 && page % 16 == 0 && page <= (1 << 30), "a page holds a multiple of 16 codes, at most 2^30");
+    REQUIRE(group == 0 || (group >= 32 && group <= (1 << 30) && (group & (group - 1)) == 0), "group is 0 or a power of two from 32 on");
+    REQUIRE(n_slots >= 0 && n_slots <= (int64_t)1 << 40, "n_slots is out of range");
+    REQUIRE(n_slots == 0 || (codes && scales), "operand is null");
+    REQUIRE((uintptr_t)codes % 16 == 0 && code_stride % 16 == 0 && code_stride >= page, "the slots of a cache start on 16-byte boundaries and do not overlap");
+    const int64_t groups = group && group < page ? (page + group - 1) / group : 1;
+    REQUIRE((uintptr_t)scales % 4 == 0 && scale_stride >= groups, "the scales of two slots overlap");
+    return LB_OK;
+}
+
+static int value_size(int dtype) { return dtype == 1 ? 4 : dtype == 3 || dtype == 4 ? 2 : 0; }
+
+// rows x cols of elements of `size` bytes at p, `stride` elements apart
+static int rows_ok(const void *p, int64_t rows, int64_t cols, int64_t stride, int size)
+{
+    REQUIRE(p, "operand is null");
+    REQUIRE((uintptr_t)p % size == 0, "an operand is not aligned to its type");
+    REQUIRE(rows <= 1 || (stride >= cols && stride <= (int64_t)1 << 40), "the rows of an operand overlap");
+    return LB_OK;
+}
+
+// warps that a call over `pages` pages launches at most: their number has to fit the grid's arithmetic
+static int pages_ok(int64_t n_rows, int64_t n_cols, int64_t page)
+{
+    REQUIRE(n_rows >= 0 && n_cols >= 0 && n_rows <= ((int64_t)1 << 31) - 1 && n_cols <= (int64_t)1 << 40, "n_rows or n_cols is out of range");
+    const int64_t pages = (n_cols + page - 1) / page, per_page = (page + 31) / 32;
+    REQUIRE(pages == 0 || n_rows <= (((int64_t)1 << 31) - 1) / pages / per_page, "too many rows for one call");
+    return LB_OK;
+}
+
+static int workspace_ok(const void *workspace, size_t have, size_t need)
+{
+    REQUIRE(have >= need && (need == 0 || workspace), "the workspace is too small");
+    REQUIRE(need == 0 || (uintptr_t)workspace % 16 == 0, "the workspace is not on a 16-byte boundary");
+    return LB_OK;
+}
+
+size_t lb_quantize_rows_workspace_bytes(int64_t n_rows, int64_t n_cols, int64_t page, int64_t group)
+{
+    if (page < 16 || page > (1 << 30) || n_rows < 1 || n_cols < 1 || group < 0) return 0;
+    return quantize_workspace_bytes(n_rows, n_cols, (int)page, (int)(group > page ? page : group));
+}
+
+int lb_quantize_rows(lb_context *h, const void *values, int dtype, int64_t n_rows, int64_t n_cols, int64_t value_stride, const int32_t *lengths,
+                     const float *residual, float *residual_out, int64_t residual_stride, const int32_t *slots, int64_t n_slots, int64_t page,
+                     int64_t group, int8_t *codes, int64_t code_stride, float *scales, int64_t scale_stride, void *workspace,
+                     size_t workspace_bytes, void *stream)
+{
+    int rc = bind(h);
+    if (rc) return rc;
+    REQUIRE(value_size(dtype), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+    if ((rc = cache_ok(codes, code_stride, scales, scale_stride, n_slots, page, group))) return rc;
+    if ((rc = pages_ok(n_rows, n_cols, page))) return rc;
+    if (n_rows == 0 || n_cols == 0) return LB_OK;
+    if ((rc = rows_ok(values, n_rows, n_cols, value_stride, value_size(dtype)))) return rc;
+    if (residual && (rc = rows_ok(residual, n_rows, n_cols, residual_stride, 4))) return rc;
+    if (residual_out && (rc = rows_ok(residual_out, n_rows, n_cols, residual_stride, 4))) return rc;
+    const int64_t span = (n_rows - 1) * residual_stride + n_cols;
+    REQUIRE(!residual || !residual_out || residual == residual_out || residual + span <= residual_out || residual_out + span <= residual,
+            "residual_out is residual itself or apart from it");
+    REQUIRE((uintptr_t)lengths % 4 == 0 && (uintptr_t)slots % 4 == 0, "an operand is not aligned to its type");
+    REQUIRE(slots || n_rows * ((n_cols + page - 1) / page) <= n_slots, "the cache has too few slots");
+    if ((rc = workspace_ok(workspace, workspace_bytes, lb_quantize_rows_workspace_bytes(n_rows, n_cols, page, group)))) return rc;
+    return quantize_rows(values, dtype, n_rows, n_cols, value_stride, lengths, residual, residual_out, residual_stride, slots, n_slots, (int)page,
+                         (int)(group > page ? page : group), reinterpret_cast<signed char *>(codes), code_stride, scales, scale_stride, workspace,
+                         S(stream));
+}
+
+int lb_dequantize_rows(lb_context *h, const int8_t *codes, int64_t code_stride, const float *scales, int64_t scale_stride, int64_t n_slots,
+                       int64_t page, int64_t group, const int32_t *slots, int64_t n_rows, int64_t n_cols, void *out, int dtype,
+                       int64_t out_stride, void *stream)
+{
+    int rc = bind(h);
+    if (rc) return rc;
+    REQUIRE(value_size(dtype), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+    if ((rc = cache_ok(codes, code_stride, scales, scale_stride, n_slots, page, group))) return rc;
+    if ((rc = pages_ok(n_rows, n_cols, page))) return rc;
+    if (n_rows == 0 || n_cols == 0) return LB_OK;
+    if ((rc = rows_ok(out, n_rows, n_cols, out_stride, value_size(dtype)))) return rc;
+    REQUIRE((uintptr_t)slots % 4 == 0, "an operand is not aligned to its type");
+    REQUIRE(slots || n_rows * ((n_cols + page - 1) / page) <= n_slots, "the cache has too few slots");
+    return dequantize_rows(reinterpret_cast<const signed char *>(codes), code_stride, scales, scale_stride, n_slots, (int)page,
+                           (int)(group > page ? 0 : group), slots, n_rows, n_cols, out, dtype, out_stride, S(stream));
+}
+
+size_t lb_int8_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t a_stride, const int8_t *b, int64_t b_stride)
+{
+    if (m < 1 || n < 1 || k < 0 || m > (1 << 30) || n > (1 << 30) || k > 131071) return 0;
+    return int8_matmul_workspace_bytes((int)m, (int)n, (int)k, a, a_stride, b, b_stride);
+}
+
+int lb_int8_matmul(lb_context *h, int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b,
+                   int64_t b_stride, const float *b_scale, void *out, int dtype, int64_t out_stride, void *workspace, size_t workspace_bytes,
+                   void *stream)
+{
+    int rc = bind(h);
+    if (rc) return rc;
+    REQUIRE(value_size(dtype), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+    REQUIRE(m >= 0 && n >= 0 && k >= 0 && m <= (1 << 30) && n <= (1 << 30), "m, n or k is out of range");
+    REQUIRE(k <= 131071, "a sum of more than 131071 products of 8-bit integers may pass 32 bits");
+    if (m == 0 || n == 0) return LB_OK;
+    if ((rc = rows_ok(out, m, n, out_stride, value_size(dtype)))) return rc;
+    if (k > 0 && ((rc = rows_ok(a, m, k, a_stride, 1)) || (rc = rows_ok(b, n, k, b_stride, 1)))) return rc;
+    REQUIRE(a_scale && b_scale, "operand is null");
+    REQUIRE((uintptr_t)a_scale % 4 == 0 && (uintptr_t)b_scale % 4 == 0, "an operand is not aligned to its type");
+    if ((rc = workspace_ok(workspace, workspace_bytes, lb_int8_matmul_workspace_bytes(m, n, k, a, a_stride, b, b_stride)))) return rc;
+    return int8_matmul(C(h), (int)m, (int)n, (int)k, reinterpret_cast<const signed char *>(a), a_stride, a_scale,
+                       reinterpret_cast<const signed char *>(b), b_stride, b_scale, out, dtype, out_stride, workspace, S(stream));
+}
+
+size_t lb_int8_distances_workspace_bytes(const lb_context *h, int64_t n, int64_t n_pages, int64_t page)
+{
+    if (!h || !h->c || n < 1 || n > 4096 || n_pages < 0 || page < 16 || page > (1 << 30)) return 0;
+    return int8_distances_workspace_bytes(h->c, (int)n, n_pages, (int)page);
+}
+
+int lb_int8_distances(lb_context *h, const int8_t *codes, int64_t code_stride, const float *scales, int64_t scale_stride, int64_t n_slots,
+                      int64_t page, int64_t group, const int32_t *slots, int64_t n, int64_t n_pages, double *out, void *workspace,
+                      size_t workspace_bytes, void *stream)
+{
+    int rc = bind(h);
+    if (rc) return rc;
+    if ((rc = cache_ok(codes, code_stride, scales, scale_stride, n_slots, page, group))) return rc;
+    REQUIRE(n >= 0 && n <= 4096, "n is at most 4096");
+    REQUIRE(n_pages >= 0 && n_pages <= (((int64_t)1 << 31) - 1) / ((page + 127) / 128), "too many pages for one call");
+    if (n == 0) return LB_OK;
+    REQUIRE(out, "operand is null");
+    REQUIRE((uintptr_t)out % 8 == 0 && (uintptr_t)slots % 4 == 0, "an operand is not aligned to its type");
+    REQUIRE(slots || n * n_pages <= n_slots, "the cache has too few slots");
+    if ((rc = workspace_ok(workspace, workspace_bytes, lb_int8_distances_workspace_bytes(h, n, n_pages, page)))) return rc;
+    return int8_distances(C(h), reinterpret_cast<const signed char *>(codes), code_stride, scales, scale_stride, n_slots, (int)page,
+                          (int)(group > page ? 0 : group), slots, (int)n, (int)n_pages, out, workspace, S(stream));
+}
+
 int lb_check_status(lb_context *h, void *stream)
 {
     int rc = bind(h);
@@ -737,6 +876,10 @@ int lb_check_status(lb_context *h, void *stream)
         if (flags & 1) {
             set_error("encoded values are too large");
             return LB_ERR_INVALID_ARG;
+        }
+        if (flags & 2) {
+            set_error("a wait inside a kernel ran out: the results of the calls before this one are not complete");
+            return LB_ERR_LOGIC;
         }
         set_error("device-side status flag raised");
         return LB_ERR_LOGIC;

@@ -194,4 +194,20 @@ int decode(Context *ctx, int size_l, int batch, const u64 *pt, double scale, int
 int encrypt_asymmetric(Context *ctx, const u64 *pk, const u64 *pt, int pt_is_coeff, const uint8_t *host_seeds, int batch, u64 *ct,
                        cudaStream_t stream);
 
+
+// 8-bit updates: cache rows (quantize.cu), products (int8_product.cu), pair distances (int8_distances.cu).  Value types are
+// numbered like the encoder's: 1 = float, 3 = bfloat16, 4 = half; group 0 = one group in a page
+size_t quantize_workspace_bytes(long n_rows, long n_cols, int page, int group);
+int quantize_rows(const void *values, int dtype, long n_rows, long n_cols, long value_stride, const int *lengths, const float *residual,
+                  float *residual_out, long residual_stride, const int *slots, long n_slots, int page, int group, signed char *codes,
+                  long code_stride, float *scales, long scale_stride, void *workspace, cudaStream_t stream);
+int dequantize_rows(const signed char *codes, long code_stride, const float *scales, long scale_stride, long n_slots, int page, int group,
+                    const int *slots, long n_rows, long n_cols, void *out, int dtype, long out_stride, cudaStream_t stream);
+size_t int8_matmul_workspace_bytes(int m, int n, int k, const void *a, long a_stride, const void *b, long b_stride);
+int int8_matmul(Context *ctx, int m, int n, int k, const signed char *a, long a_stride, const float *a_scale, const signed char *b, long b_stride,
+                const float *b_scale, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream);
+size_t int8_distances_workspace_bytes(const Context *ctx, int n, long pages, int page);
+int int8_distances(Context *ctx, const signed char *codes, long code_stride, const float *scales, long scale_stride, long n_slots, int page,
+                   int group, const int *slots, int n, int pages, double *out, void *workspace, cudaStream_t stream);
+
 } // namespace lb

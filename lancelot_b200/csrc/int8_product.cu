@@ -1,0 +1,564 @@
+// Matrix product of 8-bit integers with a scale per row of either operand:
+//   out[m][n] = (sum over k of a[m][k] b[n][k]) * a_scale[m] * b_scale[n]
+// Sums are exact 32-bit integers; the two scales are applied in 32-bit floats and the result is rounded once to its type.
+// The reference has no integer matrix product; updates of low rank are formed with it from their two factors before they are
+// encrypted (the mean of products is not the product of means, so the factors themselves cannot be averaged).
+//
+// Two kernels.  With few rows on one side the other side is read once and that bounds the call: rows go from memory straight into
+// the registers of the warp's matrix instruction.  Otherwise the tiles run on the tensor cores' own memory: operands by TMA
+// into 128-byte swizzled shared memory, tcgen05.mma into TMEM, results out of TMEM while the next tile is being multiplied.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "context.h"
+
+namespace lb {
+
+namespace {
+
+// ---- results ------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void put(float *p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
+
+__device__ __forceinline__ float scaled(int sum, float sa, float sb) { return __int2float_rn(sum) * sa * sb; }
+
+// ---- rows copied to a 16-byte pitch --------------------------------------------------------------------------------------
+// Operands whose rows start off a 16-byte boundary are copied once, zeros up to the pitch: a TMA row and a 16-byte load have to
+// start on such a boundary.
+__global__ void __launch_bounds__(256) pack_kernel(const signed char *__restrict__ src, const long stride, const long rows, const int cols,
+                                                   signed char *__restrict__ dst, const int pitch)
+{
+    const long per_row = pitch / 4, total = rows * per_row;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long r = i / per_row;
+        const int c = (int)(i - r * per_row) * 4;
+        const signed char *p = src + r * stride + c;
+        unsigned v = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < cols) v |= (unsigned)(unsigned char)p[e] << (8 * e);
+        *reinterpret_cast<unsigned *>(dst + r * pitch + c) = v;
+    }
+}
+
+// ---- few rows on one side -------------------------------------------------------------------------------------------------
+// A block forms 16 rows of the long side (the rows of A of m16n8k32) against up to 32 rows of the short side; its eight warps
+// split k and add up through shared memory.  As in the pair distances, the order of k inside a product is free, so lane (g, t) loads
+// 16 consecutive bytes of a row and uses them as four k-slots on either side.
+constexpr int kSkinnyWarps = 8;
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct SkinnyArgs {
+    const signed char *w, *x; // long side [rows][k], short side [cols][k]
+    long w_stride, x_stride;
+    const float *w_scale, *x_scale;
+    int rows, cols, k; // k a multiple of 16
+    void *out;
+    long row_step, col_step; // of the result
+};
+
+template <typename T, int NB> __global__ void __launch_bounds__(kSkinnyWarps * 32) skinny_kernel(const SkinnyArgs a)
+{
+    __shared__ int part[kSkinnyWarps][16][NB * 8 + 1];
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
+    const long r0 = (long)blockIdx.x * 16;
+    const bool in0 = r0 + g < a.rows, in1 = r0 + g + 8 < a.rows;
+    const signed char *w0 = a.w + (r0 + g) * a.w_stride, *w1 = w0 + 8 * a.w_stride;
+    int acc[NB][4];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = 0;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int k = warp * 64 + t * 16; k < a.k + t * 16; k += kSkinnyWarps * 64) { // the warp stays together: mma.sync wants all lanes
+        const bool in = k < a.k;
+        const uint4 u = in && in0 ? __ldcs(reinterpret_cast<const uint4 *>(w0 + k)) : zero;
+        const uint4 v = in && in1 ? __ldcs(reinterpret_cast<const uint4 *>(w1 + k)) : zero;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const uint4 x = in && j * 8 + g < a.cols ? __ldg(reinterpret_cast<const uint4 *>(a.x + (j * 8 + g) * a.x_stride + k)) : zero;
+            mma_s8(acc[j], u.x, v.x, u.y, v.y, x.x, x.y);
+            mma_s8(acc[j], u.z, v.z, u.w, v.w, x.z, x.w);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[warp][g + (e >> 1) * 8][j * 8 + t * 2 + (e & 1)] = acc[j][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * NB * 8; i += kSkinnyWarps * 32) {
+        const int r = i & 15, c = i >> 4;
+        if (r0 + r >= a.rows || c >= a.cols) continue;
+        int sum = 0;
+#pragma unroll
+        for (int s = 0; s < kSkinnyWarps; ++s) sum += part[s][r][c];
+        put(reinterpret_cast<T *>(a.out) + (r0 + r) * a.row_step + c * a.col_step, scaled(sum, a.w_scale[r0 + r], a.x_scale[c]));
+    }
+}
+
+template <typename T> int launch_skinny(const SkinnyArgs &a, cudaStream_t stream)
+{
+    const unsigned grid = (unsigned)((a.rows + 15) / 16);
+    if (a.cols <= 8) skinny_kernel<T, 1><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
+    else if (a.cols <= 16) skinny_kernel<T, 2><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
+    else skinny_kernel<T, 4><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
+    LB_CUDA(cudaGetLastError());
+    return LB_OK;
+}
+
+// ---- tiles on tcgen05 -------------------------------------------------------------------------------------------------------
+// One CTA per SM walks over tiles of 128 x BN.  Warp 0 brings 128-byte wide blocks of k by TMA into a ring of stages, warp 1
+// issues the products (four of k = 32 a stage), warps 2 to 5 take a finished tile out of TMEM.  TMEM holds two tiles, so
+// a tile leaves while the next one is being formed.
+constexpr int kTileM = 128, kTileK = 128, kTileThreads = 192;
+constexpr int kWaitNs = 2000000000; // a wait gives up after two seconds
+
+__device__ __forceinline__ unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(unsigned bar, unsigned count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(unsigned bar, unsigned bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity)
+{
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return done;
+}
+__device__ __forceinline__ unsigned long long now_ns()
+{
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// false: the wait ran out, here or in another warp of the block
+__device__ __noinline__ bool mbar_wait_slow(unsigned bar, unsigned parity, volatile int *failed)
+{
+    const unsigned long long began = now_ns();
+    while (!*failed) {
+        for (int i = 0; i < 64; ++i)
+            if (mbar_try(bar, parity)) return true;
+        if (now_ns() - began > kWaitNs) {
+            *failed = 1;
+            break;
+        }
+    }
+    return false;
+}
+__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int *failed)
+{
+    for (int i = 0; i < 16; ++i)
+        if (mbar_try(bar, parity)) return true;
+    return mbar_wait_slow(bar, parity, failed);
+}
+__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, int x, int y, unsigned bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+// rows of 128 bytes, 128-byte swizzle: groups of eight rows 1024 bytes apart
+__device__ __forceinline__ unsigned long long operand_desc(unsigned addr)
+{
+    return (unsigned long long)((addr & 0x3ffff) >> 4) | 1ull << 16 | (unsigned long long)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+__device__ __forceinline__ void mma_i8(unsigned d, unsigned long long a, unsigned long long b, unsigned desc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+                 "r"(desc), "r"((unsigned)add)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_commit(unsigned bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_load32(unsigned addr, int (&v)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+                   "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+                   "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+template <int BN> struct Tile {
+    static constexpr int kStageBytes = (kTileM + BN) * kTileK;
+    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int kSmem = kStages * kStageBytes + 1024 + 4 * 256 * 4 + 256;
+    // D 32-bit signed, A and B 8-bit signed, both k-major
+    static constexpr unsigned kDesc = 2u << 4 | 1u << 7 | 1u << 10 | (unsigned)(BN >> 3) << 17 | (unsigned)(kTileM >> 4) << 24;
+};
+
+struct ProductArgs {
+    int m, n, k_blocks;
+    int tiles_m, tiles_n, band; // tiles are walked in bands of `band` rows of tiles, so that a wave reads few distinct rows of a and b
+    const float *a_scale, *b_scale;
+    void *out;
+    long out_stride;
+    int align; // 32, 16: the result's rows start on such a boundary; 0: on none
+    int *status;
+};
+
+__device__ __forceinline__ void tile_at(const ProductArgs &a, int t, int &tm, int &tn)
+{
+    const int per_band = a.band * a.tiles_n, b = t / per_band, in = t - b * per_band;
+    const int rows = min(a.band, a.tiles_m - b * a.band);
+    tn = in / rows;
+    tm = b * a.band + (in - tn * rows);
+}
+
+// 32 results of a row, column n0 on
+__device__ __forceinline__ void put32(float *p, const float (&v)[32], int valid, int align)
+{
+    if (valid >= 32 && align == 32) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p + e), "r"(__float_as_uint(v[e])), "r"(__float_as_uint(v[e + 1])),
+                         "r"(__float_as_uint(v[e + 2])), "r"(__float_as_uint(v[e + 3])), "r"(__float_as_uint(v[e + 4])),
+                         "r"(__float_as_uint(v[e + 5])), "r"(__float_as_uint(v[e + 6])), "r"(__float_as_uint(v[e + 7]))
+                         : "memory");
+    } else if (valid >= 32 && align >= 16) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (e < valid) p[e] = v[e];
+    }
+}
+__device__ __forceinline__ unsigned pack2(const __nv_bfloat16 *, float a, float b)
+{
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<unsigned *>(&v);
+}
+__device__ __forceinline__ unsigned pack2(const __half *, float a, float b)
+{
+    __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<unsigned *>(&v);
+}
+template <typename T> __device__ __forceinline__ void put32(T *p, const float (&v)[32], int valid, int align)
+{
+    if (valid >= 32 && align >= 16) {
+        unsigned w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack2(p, v[2 * e], v[2 * e + 1]);
+        if (align == 32) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p + 2 * e), "r"(w[e]), "r"(w[e + 1]), "r"(w[e + 2]),
+                             "r"(w[e + 3]), "r"(w[e + 4]), "r"(w[e + 5]), "r"(w[e + 6]), "r"(w[e + 7])
+                             : "memory");
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4 *>(p + 2 * e) = make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (e < valid) put(p + e, v[e]);
+    }
+}
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(kTileThreads, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                  const ProductArgs a)
+{
+    using C = Tile<BN>;
+    extern __shared__ unsigned char raw[];
+    unsigned char *stages = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    float *scales = reinterpret_cast<float *>(stages + C::kStages * C::kStageBytes); // [4][256], one set per warp that takes results out
+    unsigned char *tail = reinterpret_cast<unsigned char *>(scales + 1024);
+    unsigned long long *bars = reinterpret_cast<unsigned long long *>(tail); // full[stages], empty[stages], done[2], freed[2], drained
+    unsigned *tmem_at = reinterpret_cast<unsigned *>(bars + 2 * C::kStages + 5);
+    volatile int *failed = reinterpret_cast<volatile int *>(tmem_at + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned full = smem_u32(bars), empty = full + 8 * C::kStages, done = empty + 8 * C::kStages, freed = done + 16, drained = freed + 16;
+    const unsigned stage0 = smem_u32(stages);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(done + 8 * i, 1);
+            mbar_init(freed + 8 * i, 128);
+        }
+        mbar_init(drained, 1);
+        *failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_at)), "n"(2 * BN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tmem = *tmem_at;
+    const int tiles = a.tiles_m * a.tiles_n;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+                int tm, tn;
+                tile_at(a, t, tm, tn);
+                for (int k = 0; k < a.k_blocks && ok; ++k, ++it) {
+                    const int s = it % C::kStages;
+                    if (it >= C::kStages) ok = mbar_wait(empty + 8 * s, (it / C::kStages - 1) & 1, failed);
+                    if (!ok) break;
+                    mbar_expect(full + 8 * s, C::kStageBytes);
+                    tma_load(stage0 + s * C::kStageBytes, &map_a, k * kTileK, tm * kTileM, full + 8 * s);
+                    tma_load(stage0 + s * C::kStageBytes + kTileM * kTileK, &map_b, k * kTileK, tn * BN, full + 8 * s);
+                }
+            }
+            // nothing may be in flight into shared memory when the block ends; after a success the products have waited for it
+            if (!ok) {
+                for (int i = it > C::kStages ? it - C::kStages : 0; i < it; ++i)
+                    for (int n = 0; n < 1 << 20; ++n)
+                        if (mbar_try(full + 8 * (i % C::kStages), (i / C::kStages) & 1)) break;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int it = 0, done_tiles = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++done_tiles) {
+                const int buf = done_tiles & 1;
+                if (done_tiles >= 2) ok = mbar_wait(freed + 8 * buf, (done_tiles / 2 - 1) & 1, failed);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int k = 0; k < a.k_blocks; ++k, ++it) {
+                    const int s = it % C::kStages;
+                    ok = mbar_wait(full + 8 * s, (it / C::kStages) & 1, failed);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned at = stage0 + s * C::kStageBytes;
+                    const unsigned long long da = operand_desc(at), db = operand_desc(at + kTileM * kTileK);
+#pragma unroll
+                    for (int e = 0; e < kTileK / 32; ++e) mma_i8(tmem + buf * BN, da + 2 * e, db + 2 * e, C::kDesc, k > 0 || e > 0);
+                    mma_commit(empty + 8 * s);
+                }
+                if (ok) mma_commit(done + 8 * buf);
+            }
+            if (!ok) { // products that are still under way end before their memory is given back
+                mma_commit(drained);
+                for (int n = 0; n < 1 << 20; ++n)
+                    if (mbar_try(drained, 0)) break;
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3;
+        float *sb = scales + quarter * 256;
+        int done_tiles = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++done_tiles) {
+            const int buf = done_tiles & 1;
+            int tm, tn;
+            tile_at(a, t, tm, tn);
+            __syncwarp();
+            for (int c = lane; c < BN; c += 32) sb[c] = tn * BN + c < a.n ? a.b_scale[tn * BN + c] : 0.f;
+            __syncwarp();
+            const int row = tm * kTileM + quarter * 32 + lane;
+            const float sa = row < a.m ? a.a_scale[row] : 0.f;
+            ok = mbar_wait(done + 8 * buf, (done_tiles / 2) & 1, failed);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride + tn * BN;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 32) {
+                if (tn * BN + c >= a.n) break;
+                int v[32];
+                tmem_load32(tmem + buf * BN + c + ((unsigned)quarter << 21), v);
+                float f[32];
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 s4 = *reinterpret_cast<const float4 *>(sb + c + e);
+                    f[e] = scaled(v[e], sa, s4.x);
+                    f[e + 1] = scaled(v[e + 1], sa, s4.y);
+                    f[e + 2] = scaled(v[e + 2], sa, s4.z);
+                    f[e + 3] = scaled(v[e + 3], sa, s4.w);
+                }
+                if (row < a.m) put32(out + c, f, a.n - tn * BN - c, a.align);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            mbar_arrive(freed + 8 * buf);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (threadIdx.x == 0 && *failed) atomicOr(a.status, 2);
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * BN) : "memory");
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int encode_map(CUtensorMap *map, const void *base, long rows, int cols, long stride, int box_rows)
+{
+    static EncodeTiled encode = nullptr;
+    if (!encode) {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        LB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found));
+        if (found != cudaDriverEntryPointSuccess || !f) {
+            set_error("the driver has no cuTensorMapEncodeTiled");
+            return LB_ERR_CUDA;
+        }
+        encode = reinterpret_cast<EncodeTiled>(f);
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows}, steps[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+        return LB_ERR_CUDA;
+    }
+    return LB_OK;
+}
+
+template <typename T, int BN> int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const ProductArgs &a, cudaStream_t stream)
+{
+    using C = Tile<BN>;
+    static bool set[64] = {};
+    if (ctx->device < 64 && !set[ctx->device]) {
+        LB_CUDA(cudaFuncSetAttribute(product_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        set[ctx->device] = true;
+    }
+    const int tiles = a.tiles_m * a.tiles_n;
+    product_kernel<T, BN><<<tiles < ctx->sm_count ? tiles : ctx->sm_count, kTileThreads, C::kSmem, stream>>>(ma, mb, a);
+    LB_CUDA(cudaGetLastError());
+    return LB_OK;
+}
+
+constexpr int kSkinny = 32; // rows on the short side up to which the long side is streamed
+
+struct ProductPlan {
+    bool pack_a, pack_b;
+    int pitch;      // of packed rows
+    size_t a_bytes; // of packed a
+    size_t bytes;
+};
+ProductPlan product_plan(int m, int n, int k, const void *a, long a_stride, const void *b, long b_stride)
+{
+    ProductPlan p;
+    auto off = [&](const void *x, long stride, int rows) { return (uintptr_t)x % 16 != 0 || (rows > 1 && stride % 16 != 0) || k % 16 != 0 || k == 0; };
+    p.pack_a = off(a, a_stride, m);
+    p.pack_b = off(b, b_stride, n);
+    p.pitch = k ? (k + 15) / 16 * 16 : 16;
+    p.a_bytes = p.pack_a ? ((size_t)m * p.pitch + 255) / 256 * 256 : 0;
+    p.bytes = p.a_bytes + (p.pack_b ? (size_t)n * p.pitch : 0);
+    return p;
+}
+
+template <typename T>
+int product_typed(Context *ctx, int m, int n, int k, const signed char *a, long a_stride, const float *a_scale, const signed char *b, long b_stride,
+                  const float *b_scale, void *out, long out_stride, cudaStream_t stream)
+{
+    const double bytes = (double)m * k + (double)n * k + (double)m * n * sizeof(T);
+    if (m <= kSkinny || n <= kSkinny) {
+        SkinnyArgs s;
+        const bool turned = m > n; // the long side is the rows of a
+        s.w = turned ? a : b;
+        s.x = turned ? b : a;
+        s.w_stride = turned ? a_stride : b_stride;
+        s.x_stride = turned ? b_stride : a_stride;
+        s.w_scale = turned ? a_scale : b_scale;
+        s.x_scale = turned ? b_scale : a_scale;
+        s.rows = turned ? m : n;
+        s.cols = turned ? n : m;
+        s.k = k;
+        s.out = out;
+        s.row_step = turned ? out_stride : 1;
+        s.col_step = turned ? 1 : out_stride;
+        count_launch("int8_skinny", stream, bytes);
+        return launch_skinny<T>(s, stream);
+    }
+    ProductArgs p;
+    p.m = m;
+    p.n = n;
+    p.k_blocks = (k + kTileK - 1) / kTileK;
+    p.tiles_m = (m + kTileM - 1) / kTileM;
+    p.a_scale = a_scale;
+    p.b_scale = b_scale;
+    p.out = out;
+    p.out_stride = out_stride;
+    const uintptr_t at = (uintptr_t)out | (uintptr_t)(out_stride * (long)sizeof(T));
+    p.align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
+    p.status = ctx->d_status;
+    p.band = 8;
+    // the widest tile that still gives every SM one
+    const int bn = (long)p.tiles_m * ((n + 255) / 256) >= ctx->sm_count ? 256 : (long)p.tiles_m * ((n + 127) / 128) >= ctx->sm_count ? 128 : 64;
+    p.tiles_n = (n + bn - 1) / bn;
+    CUtensorMap ma, mb;
+    int rc = encode_map(&ma, a, m, k, a_stride, kTileM);
+    if (rc) return rc;
+    if ((rc = encode_map(&mb, b, n, k, b_stride, bn))) return rc;
+    count_launch("int8_tiles", stream, bytes);
+    if (bn == 256) return launch_tiles<T, 256>(ctx, ma, mb, p, stream);
+    if (bn == 128) return launch_tiles<T, 128>(ctx, ma, mb, p, stream);
+    return launch_tiles<T, 64>(ctx, ma, mb, p, stream);
+}
+
+} // namespace
+
+size_t int8_matmul_workspace_bytes(int m, int n, int k, const void *a, long a_stride, const void *b, long b_stride)
+{
+    return product_plan(m, n, k, a, a_stride, b, b_stride).bytes;
+}
+
+int int8_matmul(Context *ctx, int m, int n, int k, const signed char *a, long a_stride, const float *a_scale, const signed char *b, long b_stride,
+                const float *b_scale, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream)
+{
+    const ProductPlan p = product_plan(m, n, k, a, a_stride, b, b_stride);
+    auto pack = [&](const signed char *&x, long &stride, long rows, signed char *to) -> int {
+        const long total = rows * (p.pitch / 4), blocks = (total + 255) / 256, most = (long)ctx->sm_count * 16;
+        count_launch("int8_pack", stream, 2.0 * rows * k);
+        pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(x, stride, rows, k, to, p.pitch);
+        LB_CUDA(cudaGetLastError());
+        x = to;
+        stride = p.pitch;
+        return LB_OK;
+    };
+    signed char *ws = reinterpret_cast<signed char *>(workspace);
+    int rc;
+    if (p.pack_a && (rc = pack(a, a_stride, m, ws))) return rc;
+    if (p.pack_b && (rc = pack(b, b_stride, n, ws + p.a_bytes))) return rc;
+    k = p.pitch; // k itself where a side is not packed: a ragged k packs both
+    switch (dtype) {
+    case 1: return product_typed<float>(ctx, m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
+    case 3: return product_typed<__nv_bfloat16>(ctx, m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
+    default: return product_typed<__half>(ctx, m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
+    }
+}
+
+} // namespace lb

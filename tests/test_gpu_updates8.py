@@ -1,0 +1,398 @@
+"""8-bit updates on the GPU against plain 64-bit formulas: cache rows written and read back, the 8-bit matrix product, pair distances.
+
+Codes, scales and residuals are compared for equality (the definition leaves no choice); a product may be off by the roundings it
+makes: the integer sum to 32 bits, two products by a scale, the result's type.  Distances are sums of 64-bit floats."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+F32, F64 = 2.0 ** -24, 2.0 ** -53  # half a step, relative
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    from lancelot_b200 import cabi
+
+    return cabi.Context(12, cabi.coeff_modulus_create(1 << 12, [40, 40]), 1)
+
+
+def gen(seed):
+    import torch
+
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def quantized(t, page, group):
+    """t [rows][cols] float32 -> codes [rows * pages][page], scales, lost [rows][cols], from the definition with 64-bit quotients"""
+    import torch
+
+    rows, cols = t.shape
+    pages = -(-cols // page)
+    size = group if 0 < group < page else page
+    groups = -(-page // size)
+    x = torch.zeros(rows, pages * page, device=t.device)
+    x[:, :cols] = t
+    x = x.view(rows * pages, page)
+    x = torch.nn.functional.pad(x, (0, groups * size - page)).view(rows * pages, groups, size)
+    most = x.abs().amax(2)
+    scale = torch.where(most.isfinite(), most / torch.full_like(most, 127), torch.full_like(most, math.nan))
+    s = scale.double()[:, :, None]
+    code = (x.double() / s).round().clamp(-127, 127)
+    code = torch.where(s > 0, code, torch.zeros_like(code))
+    lost = torch.where(s.isnan(), torch.zeros_like(s), x.double() - code * s.nan_to_num())
+    assert torch.equal(lost, lost.float().double())  # what is lost fits 32 bits
+    codes = code.view(rows * pages, -1)[:, :page].to(torch.int8)
+    lost = lost.float().view(rows * pages, -1)[:, :page].reshape(rows, -1)[:, :cols]
+    return codes, scale, lost
+
+
+def same(x, y):
+    import torch
+
+    return torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(), y.nan_to_num()) if x.is_floating_point() else torch.equal(x, y)
+
+
+def expanded(codes, scales, group):
+    page = codes.shape[1]
+    return codes.float() * scales.repeat_interleave(group if 0 < group < page else page, 1)[:, :page]
+
+
+GROUPS = [0, 32, 64, 128, 256, 512, 1024, 4096, 65536]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("rows,cols,page", [(1, 1, 16), (3, 33, 48), (5, 1000, 1008), (2, 5000, 2048), (1, 70001, 32768), (2, 100000, 98304)])
+def test_rows_written_and_read_back(ctx, dtype, rows, cols, page):
+    import torch
+
+    dt = getattr(torch, dtype)
+    for group in GROUPS:
+        g = gen(rows * cols + group)
+        v = (torch.randn(rows, cols, generator=g, device="cuda") * torch.rand(rows, 1, generator=g, device="cuda")).to(dt)
+        v[:, ::7] = 0
+        pages, groups = -(-cols // page), -(-page // group) if 0 < group < page else 1
+        codes = torch.full((rows * pages, page), 99, dtype=torch.int8, device="cuda")
+        scales = torch.full((rows * pages, groups), 99.0, device="cuda")
+        lost = torch.empty(rows, cols, device="cuda")
+        ctx.quantize_rows(v, codes, scales, group=group, residual_out=lost)
+        want_codes, want_scales, want_lost = quantized(v.float(), page, group)
+        assert torch.equal(codes, want_codes) and torch.equal(scales, want_scales) and torch.equal(lost, want_lost), group
+        back = ctx.dequantize_rows(codes, scales, cols, group=group, dtype=dt)
+        want = expanded(codes, scales, group).view(rows, pages * page)[:, :cols].to(dt)
+        assert torch.equal(back, want), group
+
+
+def test_borders_between_codes_are_decided_exactly(ctx):
+    """values on and next to the half steps of the scale, where a 32-bit quotient rounds to the wrong side"""
+    import torch
+
+    g = gen(5)
+    rows, cols = 64, 4096
+    most = torch.rand(rows, 1, generator=g, device="cuda") * 10 + 0.1
+    s = most / torch.full_like(most, 127)
+    half = (torch.randint(-126, 126, (rows, cols), generator=g, device="cuda") + 0.5).double() * s.double()
+    v = half.float()
+    step = torch.randint(-1, 2, (rows, cols), generator=g, device="cuda", dtype=torch.int32)
+    v = (v.view(torch.int32) + step).view(torch.float32)
+    v[:, :1] = most
+    codes = torch.empty(rows, cols, dtype=torch.int8, device="cuda")
+    scales = torch.empty(rows, 1, device="cuda")
+    lost = torch.empty(rows, cols, device="cuda")
+    ctx.quantize_rows(v, codes, scales, residual_out=lost)
+    want = quantized(v, cols, 0)
+    assert torch.equal(codes, want[0]) and torch.equal(scales, want[1]) and torch.equal(lost, want[2])
+    # exact ties go to the even code: a scale of 2^-5 and odd multiples of 2^-6
+    v = (torch.arange(-253, 254, device="cuda") / 64.0).view(1, -1)
+    v[0, 0] = 127 / 32
+    codes, scales = torch.empty(1, 512, dtype=torch.int8, device="cuda"), torch.empty(1, 1, device="cuda")
+    ctx.quantize_rows(v, codes, scales)
+    assert float(scales) == 1 / 32 and torch.equal(codes[0, 1:507].float(), (v[0, 1:] * 32).round())
+
+
+@pytest.mark.parametrize("group", [0, 64, 1024])
+def test_infinities_nan_and_tiny_values(ctx, group):
+    import torch
+
+    v = torch.randn(9, 4096, generator=gen(1), device="cuda")
+    v[0, 5] = math.inf
+    v[1, 4095] = -math.inf
+    v[2, 1024] = math.nan
+    v[3] *= 2.0 ** -130  # the scales of these rows are below the normal range
+    v[4] *= 2.0 ** -148
+    v[5] = 0
+    v[6] = -0.0
+    v[7] *= 1e38
+    v[8] = torch.finfo(torch.float32).max
+    n = 4096 // group if group else 1
+    codes, scales, lost = torch.empty(9, 4096, dtype=torch.int8, device="cuda"), torch.empty(9, n, device="cuda"), torch.empty(9, 4096, device="cuda")
+    v.clamp_(-torch.finfo(torch.float32).max, torch.finfo(torch.float32).max)[0, 5] = math.inf
+    v[1, 4095] = -math.inf
+    ctx.quantize_rows(v, codes, scales, group=group, residual_out=lost)
+    want = quantized(v, 4096, group)
+    assert torch.equal(codes, want[0]) and same(scales, want[1]) and torch.equal(lost, want[2])
+    back = ctx.dequantize_rows(codes, scales, 4096, group=group)
+    assert same(back, expanded(codes, scales, group))
+    assert back[0].isnan().any() and back[2].isnan().any() and not back[3:].isnan().any()
+
+
+@pytest.mark.parametrize("group", [0, 128])
+def test_lengths_slots_residual_and_strides(ctx, group):
+    """ragged rows (empty ones among them), slots in any order with some outside the cache, strided rows off their alignment, the residual in
+    place; what a call does not own stays as it was"""
+    import torch
+
+    g = gen(3)
+    rows, cols, page = 7, 1003, 512
+    pages, groups = 2, page // group if group else 1
+    wide = torch.randn(rows, 1100, generator=g, device="cuda")
+    v = wide[:, 13:13 + cols]
+    res_wide = torch.randn(rows, 1050, generator=g, device="cuda") * 0.01
+    res = res_wide[:, 5:5 + cols]
+    lengths = torch.tensor([0, 1, 512, 513, 1003, 5000, -4], dtype=torch.int32, device="cuda")
+    slots = torch.randperm(20, generator=g, device="cuda")[: rows * pages].to(torch.int32).view(rows, pages)
+    slots[2, 1], slots[4, 0] = -1, 20
+    codes = torch.full((20, page + 16), 77, dtype=torch.int8, device="cuda")[:, :page]
+    scales = torch.full((20, groups), 77.0, device="cuda")
+    before, res_before = res_wide.clone(), res.clone()
+    ctx.quantize_rows(v, codes, scales, group=group, slots=slots, lengths=lengths, residual=res, residual_out=res)
+    inside = torch.arange(cols, device="cuda") < lengths[:, None]
+    t = torch.where(inside, v + res_before, torch.zeros(()).cuda())
+    want_codes, want_scales, want_lost = quantized(t, page, group)
+    written = torch.zeros(20, dtype=torch.bool, device="cuda")
+    for i in range(rows):
+        for p in range(pages):
+            s, lo, hi = int(slots[i, p]), p * page, min((p + 1) * page, cols)
+            if 0 <= s < 20:
+                written[s] = True
+                assert torch.equal(codes[s], want_codes[i * pages + p]) and torch.equal(scales[s], want_scales[i * pages + p])
+                want = torch.where(inside[i, lo:hi], want_lost[i, lo:hi], res_before[i, lo:hi])
+                assert torch.equal(res[i, lo:hi], want)
+            else:
+                assert torch.equal(res[i, lo:hi], res_before[i, lo:hi])
+    assert bool((codes[~written] == 77).all()) and bool((scales[~written] == 77).all())
+    res_wide[:, 5:5 + cols] = 0
+    before[:, 5:5 + cols] = 0
+    assert torch.equal(res_wide, before)
+    out = torch.full((rows, 1111), 5.0, device="cuda")
+    back = ctx.dequantize_rows(codes, scales, cols, group=group, slots=slots, out=out[:, 3:3 + cols])
+    full = torch.zeros(rows, pages, page, device="cuda")
+    for i in range(rows):
+        for p in range(pages):
+            s = int(slots[i, p])
+            if 0 <= s < 20:
+                full[i, p] = expanded(codes[s:s + 1], scales[s:s + 1], group)[0]
+    assert torch.equal(back, full.view(rows, -1)[:, :cols])
+    assert bool((out[:, :3] == 5).all()) and bool((out[:, 3 + cols:] == 5).all())
+
+
+def test_error_feedback_over_rounds_loses_nothing(ctx):
+    """sum of what was sent plus the residual left = sum of the updates (to the roundings of the 32-bit sums t)"""
+    import torch
+
+    g = gen(8)
+    res = torch.zeros(2, 3000, device="cuda")
+    sent, total, slack = torch.zeros(2, 3000, dtype=torch.float64, device="cuda"), torch.zeros(2, 3000, dtype=torch.float64, device="cuda"), 0.0
+    codes, scales = torch.empty(2, 3008, dtype=torch.int8, device="cuda"), torch.empty(2, 47, device="cuda")
+    for _ in range(5):
+        v = torch.randn(2, 3000, generator=g, device="cuda")
+        slack += F32 * float((v + res).abs().max())
+        ctx.quantize_rows(v, codes, scales, group=64, residual=res, residual_out=res)
+        sent += (codes.double() * scales.double().repeat_interleave(64, 1))[:, :3000]
+        total += v.double()
+    assert float((sent + res.double() - total).abs().max()) <= slack
+
+
+PRODUCTS = [(1, 1, 1), (1, 4096, 4096), (8, 64, 16), (9, 100, 33), (17, 130, 64), (32, 77, 1000), (300, 5, 260), (33, 33, 128), (128, 256, 128),
+            (129, 257, 129), (64, 1000, 16), (200, 300, 8), (333, 1111, 2047), (1024, 2048, 512), (2500, 2600, 384), (256, 512, 4160), (40, 48, 131071),
+            (5, 48, 131071), (50, 60, 0), (3, 4, 0)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_product(ctx, m, n, k, dtype):
+    import torch
+
+    dt = getattr(torch, dtype)
+    g = gen(m * n + k)
+    a = torch.randint(-128, 128, (m, k), generator=g, device="cuda", dtype=torch.int8)
+    b = torch.randint(-128, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    sa = torch.rand(m, generator=g, device="cuda") * 1e-2 / math.sqrt(k + 1)
+    sb = torch.rand(n, generator=g, device="cuda") * 1e-2
+    got = ctx.int8_matmul(a, b, sa, sb, dtype=dt)
+    ctx.check_status()
+    check_product(got, a, b, sa, sb)
+
+
+def check_product(got, a, b, sa, sb):
+    import torch
+
+    want = (a.double() @ b.double().T) * sa.double()[:, None] * sb.double()
+    # sum, two products, and the type; numbers below the type's normal range are off by half of its smallest step
+    rel = 3 * F32 + (0 if got.dtype == torch.float32 else torch.finfo(got.dtype).eps / 2)
+    tiny = torch.finfo(got.dtype).tiny * torch.finfo(got.dtype).eps / 2
+    assert bool(((got.double() - want).abs() <= want.abs() * rel * (1 + 1e-6) + tiny).all())
+
+
+def test_product_of_the_largest_sums(ctx):
+    """all codes at the ends of their range: the sums need all 32 bits"""
+    import torch
+
+    for m, n in [(3, 40), (64, 70)]:
+        for x, y in [(-128, -128), (127, -128), (127, 127)]:
+            a = torch.full((m, 131071), x, dtype=torch.int8, device="cuda")
+            b = torch.full((n, 131071), y, dtype=torch.int8, device="cuda")
+            one = torch.ones(max(m, n), device="cuda")
+            got = ctx.int8_matmul(a, b, one[:m].contiguous(), one[:n].contiguous(), dtype=torch.float32)
+            assert bool((got == float(torch.tensor(x * y * 131071).float())).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 256), (20, 40, 96), (150, 500, 256), (300, 300, 100)])
+def test_product_of_strided_rows(ctx, m, n, k):
+    """operands and results that are columns of wider matrices, at every alignment; what lies beside them stays as it was"""
+    import torch
+
+    g = gen(k)
+    for off, pad in [(0, 16), (16, 0), (1, 15), (4, 3), (7, 0)]:
+        a = torch.randint(-127, 128, (m, off + k + pad), generator=g, device="cuda", dtype=torch.int8)[:, off:off + k]
+        b = torch.randint(-127, 128, (n, off + k + 2 * pad), generator=g, device="cuda", dtype=torch.int8)[:, off:off + k]
+        sa, sb = torch.rand(m + 1, generator=g, device="cuda")[1:], torch.rand(n + 3, generator=g, device="cuda")[3:]
+        for dt in (torch.float32, torch.bfloat16):
+            wide = torch.full((m, off + n + pad), 7.0, dtype=dt, device="cuda")
+            got = ctx.int8_matmul(a, b, sa, sb, out=wide[:, off:off + n])
+            check_product(got, a, b, sa, sb)
+            assert bool((wide[:, :off] == 7).all()) and bool((wide[:, off + n:] == 7).all())
+
+
+def distances(codes, scales, slots, group):
+    """from differences, in 64 bits, and how far sums of 64-bit floats may be off"""
+    import torch
+
+    n, pages = slots.shape
+    page = codes.shape[1]
+    x = torch.zeros(n, pages, page, dtype=torch.float64, device="cuda")
+    wide = codes.double() * scales.double().repeat_interleave(group if 0 < group < page else page, 1)[:, :page]
+    there = (slots >= 0) & (slots < codes.shape[0])
+    x[there] = wide[slots[there].long()]
+    x = x.view(n, -1)
+    want = torch.stack([(x - x[i]).square().sum(1) for i in range(n)])
+    norm = x.square().sum(1)
+    return want, (norm[:, None] + norm) * F64 * (x.shape[1] + 8)
+
+
+@pytest.mark.parametrize("n,pages,page", [(1, 1, 16), (2, 1, 32), (4, 7, 8192), (9, 3, 1008), (17, 2, 2048), (20, 5, 4096), (32, 1, 48), (33, 2, 512),
+                                          (70, 3, 1040), (100, 2, 4096)])
+@pytest.mark.parametrize("group", [0, 32, 64, 128, 1024])
+def test_pair_distances(ctx, n, pages, page, group):
+    import torch
+
+    g = gen(n * page + group)
+    groups = -(-page // group) if 0 < group < page else 1
+    codes = torch.randint(-127, 128, (n * pages + 2, page), generator=g, device="cuda", dtype=torch.int8)
+    scales = torch.rand(n * pages + 2, groups, generator=g, device="cuda")
+    slots = torch.randperm(n * pages + 2, generator=g, device="cuda")[: n * pages].to(torch.int32).view(n, pages)
+    if n > 2:
+        slots[1] = slots[2]  # two rows that are the same
+        slots[0, 0] = -1     # a page that is not there
+    got = ctx.int8_distances(codes, scales, slots, group=group)
+    want, slack = distances(codes, scales, slots, group)
+    assert bool(((got - want).abs() <= slack).all())
+    assert torch.equal(got, got.T) and bool((got.diagonal() == 0).all())
+    if n > 2:
+        assert float(got[1, 2]) == 0.0 and torch.equal(got[1], got[2])
+
+
+def test_distances_of_a_row_that_is_not_a_number(ctx):
+    import torch
+
+    codes = torch.randint(-127, 128, (5, 256), generator=gen(2), device="cuda", dtype=torch.int8)
+    scales = torch.rand(5, 2, generator=gen(3), device="cuda")
+    scales[3, 1] = math.nan
+    d = ctx.int8_distances(codes, scales, torch.arange(5, dtype=torch.int32, device="cuda").view(5, 1), group=128)
+    others = [i for i in range(5) if i != 3]
+    assert bool(d[3, others].isnan().all()) and bool(d[others, 3].isnan().all()) and not d[others][:, others].isnan().any()
+    assert float(d[3, 3]) == 0.0
+
+
+def test_a_chain_is_captured_and_replayed(ctx):
+    """write, read back, distances and a product of the written codes in one CUDA graph, on values that change between replays"""
+    import torch
+
+    n, cols, page = 6, 2000, 1024
+    v = torch.zeros(n, cols, device="cuda")
+    codes, scales = torch.zeros(2 * n, page, dtype=torch.int8, device="cuda"), torch.zeros(2 * n, 8, device="cuda")
+    slots = torch.arange(2 * n, dtype=torch.int32, device="cuda").view(n, 2)
+    whole, whole_scale = torch.zeros(n, 2000, dtype=torch.int8, device="cuda"), torch.zeros(n, 1, device="cuda")
+    weight = torch.randint(-127, 128, (200, 2000), generator=gen(1), device="cuda", dtype=torch.int8)
+    weight_scale = torch.rand(200, generator=gen(2), device="cuda")
+
+    def work():
+        ctx.quantize_rows(v, codes, scales, group=128, slots=slots)
+        ctx.quantize_rows(v, whole, whole_scale)
+        return (ctx.dequantize_rows(codes, scales, cols, group=128, slots=slots), ctx.int8_distances(codes, scales, slots, group=128),
+                ctx.int8_matmul(whole, weight, whole_scale.view(-1), weight_scale, dtype=torch.float32))
+
+    work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for seed in range(3):
+        v.copy_(torch.randn(n, cols, generator=gen(seed), device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in got]
+        for x, y in zip(replayed, work()):
+            assert torch.equal(x, y)
+
+
+def test_calls_on_another_stream(ctx):
+    import torch
+
+    v = torch.randn(3, 40000, generator=gen(4), device="cuda")
+    side = torch.cuda.Stream()
+    codes, scales = torch.zeros(3, 40000, dtype=torch.int8, device="cuda"), torch.zeros(3, 1, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        ctx.quantize_rows(v, codes, scales)
+        back = ctx.dequantize_rows(codes, scales, 40000)
+    side.synchronize()
+    want = quantized(v, 40000, 0)
+    assert torch.equal(codes, want[0]) and torch.equal(back, expanded(codes, scales, 0))
+
+
+def test_refusals(ctx):
+    import torch
+
+    from lancelot_b200._lib import InvalidArgument
+
+    v = torch.zeros(2, 64, device="cuda")
+    codes, scales = torch.zeros(2, 64, dtype=torch.int8, device="cuda"), torch.zeros(2, 1, device="cuda")
+    bad = [lambda: ctx.quantize_rows(v.double(), codes, scales), lambda: ctx.quantize_rows(v.cpu(), codes, scales),
+           lambda: ctx.quantize_rows(v, codes, scales, group=48), lambda: ctx.quantize_rows(v, codes, scales, group=16),
+           lambda: ctx.quantize_rows(v, codes, scales, group=-32), lambda: ctx.quantize_rows(v, codes, scales, group=32),  # two scales a slot
+           lambda: ctx.quantize_rows(v, codes[:, :60], scales), lambda: ctx.quantize_rows(v, codes[:1], scales),
+           lambda: ctx.quantize_rows(v, codes, scales[:1]), lambda: ctx.quantize_rows(v, codes, scales, lengths=torch.zeros(3, dtype=torch.int32, device="cuda")),
+           lambda: ctx.quantize_rows(v, codes, scales, slots=torch.zeros(3, dtype=torch.int32, device="cuda")),
+           lambda: ctx.quantize_rows(v, codes, scales, slots=torch.zeros(2, dtype=torch.int64, device="cuda")),
+           lambda: ctx.quantize_rows(v, codes, scales, residual=torch.zeros(2, 63, device="cuda")),
+           lambda: ctx.quantize_rows(v.t()[:2], codes, scales), lambda: ctx.quantize_rows(v[:1].expand(2, 64), codes, scales),
+           lambda: ctx.dequantize_rows(codes, scales, 64, dtype=torch.float64), lambda: ctx.dequantize_rows(codes, scales, 64, n_rows=3),
+           lambda: ctx.dequantize_rows(codes, scales, 64, out=torch.zeros(2, 65, device="cuda")),
+           lambda: ctx.int8_matmul(codes, codes[:, :32], v[0, :2], v[0, :2]), lambda: ctx.int8_matmul(codes, codes, v[0, :3], v[0, :2]),
+           lambda: ctx.int8_matmul(codes, codes, v[0, :2], v[0, :2], dtype=torch.int32), lambda: ctx.int8_matmul(codes.to(torch.uint8), codes, v[0, :2], v[0, :2]),
+           lambda: ctx.int8_matmul(*[torch.zeros(1, 131072, dtype=torch.int8, device="cuda")] * 2, v[0, :1], v[0, :1]),
+           lambda: ctx.int8_distances(codes, scales, torch.zeros(2, dtype=torch.int32, device="cuda")),
+           lambda: ctx.int8_distances(codes, scales, torch.zeros(5000, 1, dtype=torch.int32, device="cuda"))]
+    for i, call in enumerate(bad):
+        with pytest.raises(InvalidArgument):
+            call()
+            pytest.fail("call %d was not refused" % i)
+    assert not codes.any() and not scales.any()
+    # rows of no columns and no rows at all are served
+    ctx.quantize_rows(v[:0], codes, scales)
+    ctx.quantize_rows(v[:, :0], codes, scales)
+    assert ctx.dequantize_rows(codes, scales, 0, n_rows=2).shape == (2, 0)
+    assert ctx.int8_matmul(codes[:0], codes, v[0, :0], v[0, :2]).shape == (0, 2)
+    assert ctx.int8_distances(codes, scales, torch.zeros(0, 1, dtype=torch.int32, device="cuda")).shape == (0, 0)
