@@ -732,7 +732,7 @@ static int cache_ok(const int8_t *codes, int64_t code_stride, const float *scale
 {
     REQUIRE(page >= 16 && page % 16 == 0 && page <= (1 << 30), "a page holds a multiple of 16 codes, at most 2^30");
     REQUIRE(group == 0 || (group >= 32 && group <= (1 << 30) && (group & (group - 1)) == 0), "group is 0 or a power of two from 32 on");
-    REQUIRE(n_slots >= 0 && n_slots <= (int64_t)1 << 40, "n_slots is out of range");
+    REQUIRE(n_slots >= 0 && n_slots < (int64_t)1 << 31, "n_slots is out of range");
     REQUIRE(n_slots == 0 || (codes && scales), "operand is null");
     REQUIRE((uintptr_t)codes % 16 == 0 && code_stride % 16 == 0 && code_stride >= page, "the slots of a cache start on 16-byte boundaries and do not overlap");
     const int64_t groups = group && group < page ? (page + group - 1) / group : 1;
@@ -856,6 +856,7 @@ int lb_int8_distances(lb_context *h, const int8_t *codes, int64_t code_stride, c
     REQUIRE(n >= 0 && n <= 4096, "n is at most 4096");
     REQUIRE(n_pages >= 0 && n_pages <= (((int64_t)1 << 31) - 1) / ((page + 127) / 128), "too many pages for one call");
     if (n == 0) return LB_OK;
+    REQUIRE(n * n_pages < (int64_t)1 << 31 && code_stride < (int64_t)1 << 31 && scale_stride < (int64_t)1 << 31, "the cache is too large for one call");
     REQUIRE(out, "operand is null");
     REQUIRE((uintptr_t)out % 8 == 0 && (uintptr_t)slots % 4 == 0, "an operand is not aligned to its type");
     REQUIRE(slots || n * n_pages <= n_slots, "the cache has too few slots");

@@ -11,20 +11,15 @@
 // instruction: a row of A and a column of B are both "a client's codes along k", and the order of k inside the product does not
 // matter as long as both sides agree, so lane (g, t) loads 16 consecutive bytes of client g and uses them as four k-slots of A and
 // of B at once.  No shared memory, no transposition, one load per code.
-#include "context.h"
+#include <type_traits>
+
+#include "tcgen05.cuh"
 
 namespace lb {
 
 namespace {
 
 constexpr int kWarps = 8;
-
-__device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
-{
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 struct DistanceArgs {
     const signed char *codes;
@@ -34,7 +29,7 @@ struct DistanceArgs {
     long n_slots;
     const int *slots; // [n][pages]; nullptr: in order
     int n, pages, page;
-    int group;          // columns of a group; page for one group in a page
+    int group;          // columns of a group; 2^30 for one group in a page
     int unit;           // columns a warp takes at a time, within a page
     unsigned units_per_page, units;
     int blocks; // blocks per tile
@@ -188,15 +183,535 @@ __device__ void gram_tile(const DistanceArgs &a, const int row_a, const int row_
     }
 }
 
-template <int RB, bool DIAG_ONLY, int BYTES>
-__global__ void __launch_bounds__(kWarps * 32) gram_kernel(const DistanceArgs a, const int n_blocks)
+template <int BYTES> __global__ void __launch_bounds__(kWarps * 32) gram_kernel(const DistanceArgs a, const int n_blocks)
 {
     __shared__ double sum[32 * 32];
-    int i = 0, j = 0;
-    if (!DIAG_ONLY) tile_of(blockIdx.x, n_blocks, i, j);
+    int i, j;
+    tile_of(blockIdx.x, n_blocks, i, j);
     double *out = a.partial + ((size_t)blockIdx.x * a.blocks + blockIdx.y) * 1024;
-    if (DIAG_ONLY || i == j) gram_tile<RB, true, BYTES>(a, i * 32, j * 32, sum, out);
-    else gram_tile<RB, false, BYTES>(a, i * 32, j * 32, sum, out);
+    if (i == j) gram_tile<4, true, BYTES>(a, i * 32, j * 32, sum, out);
+    else gram_tile<4, false, BYTES>(a, i * 32, j * 32, sum, out);
+}
+
+// ---- pieces of the kernels for up to 128 clients ----------------------------------------------------------------------------------
+constexpr int kRingBytes = 216 * 1024;
+constexpr int kMaxScales = 4; // copies of scales that a thread makes for one stage
+
+// An integer sum as a 64-bit float, without the conversion unit (which takes 8 cycles for what the FP64 pipe does in 2): sums start
+// from -2^31 instead of 0, and 2^52 + 2^31 + x has just those bits below an exponent of 52.  Where there is time, every
+// fourth sum goes through the conversion unit all the same, beside the others.
+constexpr int kBias = (int)0x80000000;
+__device__ __forceinline__ double unbiased(int x) { return __hiloint2double(0x43300000, x) - 4503601774854144.0; }
+
+struct Ring {
+    int rows;        // of clients, rounded up to eight: what a stage has room for
+    int groups;      // scales of a row in a stage
+    int stage_bytes; // codes [rows][pitch], then scales [rows][groups] in 32 bits
+    int stages;
+    int spare;       // bytes behind the ring that a read of rows beyond `rows` may reach
+};
+
+// Eight rows of codes at columns `at` of a stage, as four (two) k-slots of the matrix instruction
+template <int BYTES> __device__ __forceinline__ void load_rows(unsigned (&w)[BYTES / 4], const unsigned char *at)
+{
+    if constexpr (BYTES == 16) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(at);
+        w[0] = x.x;
+        w[1] = x.y;
+        w[2] = x.z;
+        w[3] = x.w;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(at);
+        w[0] = x.x;
+        w[1] = x.y;
+    }
+}
+
+__device__ __forceinline__ void apply_scales(double (&total)[4], const int (&acc)[4], double lo, double hi, double2 col)
+{
+    total[0] += (lo * col.x) * unbiased(acc[0]);
+    total[1] += (lo * col.y) * unbiased(acc[1]);
+    total[2] += (hi * col.x) * unbiased(acc[2]);
+    total[3] += (hi * col.y) * unbiased(acc[3]);
+}
+
+// All pairs of up to 32 clients.  The 8 x 8 blocks of pairs that are wanted come in twos: the instruction forms 16 rows against 8
+// columns, and block (i, j) serves as (j, i).  Three blocks of clients take three instructions this way instead of four for the
+// upper triangle as it stands.
+template <int TILES, unsigned LO, unsigned HI, unsigned COL> struct Tiles { // one hexadecimal digit per instruction, the first one last
+    static constexpr int kTiles = TILES;
+    static constexpr __host__ __device__ int lo(int v) { return LO >> 4 * v & 15; }                                     // block of rows 0 to 7
+    static constexpr __host__ __device__ int hi(int v) { return (HI >> 4 * v & 15) == 15 ? -1 : (int)(HI >> 4 * v & 15); } // of rows 8 to 15; f: none
+    static constexpr __host__ __device__ int col(int v) { return COL >> 4 * v & 15; }                                   // of the columns
+};
+template <int NB> struct Cover;
+template <> struct Cover<1> : Tiles<1, 0x0, 0xf, 0x0> {};
+template <> struct Cover<2> : Tiles<2, 0x00, 0xf1, 0x01> {};
+template <> struct Cover<3> : Tiles<3, 0x100, 0x212, 0x210> {};
+template <> struct Cover<4> : Tiles<6, 0x103210, 0xff0321, 0x320321> {};
+
+// all pairs of 32 clients, columns [begin, end) of the rows from `codes` on, one scale each from `scales` on
+template <int BYTES>
+__device__ __forceinline__ void triangle(double (&total)[8][4], const unsigned char *codes, const double *scales, int pitch, int begin, int end)
+{
+    using V = Cover<4>;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const unsigned char *at = codes + g * pitch + t * BYTES;
+    int acc[V::kTiles][4];
+    auto step = [&](int c, auto first) {
+        unsigned w[5][BYTES / 4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) load_rows<BYTES>(w[r], at + r * 8 * pitch + c);
+#pragma unroll
+        for (int k = 0; k < BYTES / 4; ++k) w[4][k] = 0;
+#pragma unroll
+        for (int k = 0; k < BYTES / 4; k += 2)
+#pragma unroll
+            for (int v = 0; v < V::kTiles; ++v) {
+                const int lo = V::lo(v), hi = V::hi(v) >= 0 ? V::hi(v) : 4, col = V::col(v);
+                if (decltype(first)::value && k == 0) mma_s8_from(acc[v], kBias, w[lo][k], w[hi][k], w[lo][k + 1], w[hi][k + 1], w[col][k], w[col][k + 1]);
+                else mma_s8(acc[v], w[lo][k], w[hi][k], w[lo][k + 1], w[hi][k + 1], w[col][k], w[col][k + 1]);
+            }
+    };
+    step(begin, std::true_type());
+    for (int c = begin + 4 * BYTES; c < end; c += 4 * BYTES) step(c, std::false_type());
+    double row[4];
+    double2 col[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        row[r] = scales[r * 8 + g];
+        col[r] = *reinterpret_cast<const double2 *>(scales + r * 8 + t * 2);
+    }
+#pragma unroll
+    for (int v = 0; v < V::kTiles; ++v) apply_scales(total[v], acc[v], row[V::lo(v)], V::hi(v) >= 0 ? row[V::hi(v) >= 0 ? V::hi(v) : 0] : 0.0, col[V::col(v)]);
+}
+
+// 32 clients with the first `blocks` x 8 of 32 others, `apart` rows further down
+template <int BYTES>
+__device__ __forceinline__ void square(double (&total)[8][4], const unsigned char *codes, const double *scales, int apart, int blocks, int pitch, int begin, int end)
+{
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const unsigned char *at = codes + g * pitch + t * BYTES, *other = at + apart * pitch;
+    int acc[8][4];
+    auto step = [&](int c, auto first) {
+        unsigned a[4][BYTES / 4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) load_rows<BYTES>(a[r], at + r * 8 * pitch + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j >= blocks) break;
+            unsigned b[BYTES / 4];
+            load_rows<BYTES>(b, other + j * 8 * pitch + c);
+#pragma unroll
+            for (int k = 0; k < BYTES / 4; k += 2) {
+                if (decltype(first)::value && k == 0) {
+                    mma_s8_from(acc[2 * j], kBias, a[0][k], a[1][k], a[0][k + 1], a[1][k + 1], b[k], b[k + 1]);
+                    mma_s8_from(acc[2 * j + 1], kBias, a[2][k], a[3][k], a[2][k + 1], a[3][k + 1], b[k], b[k + 1]);
+                } else {
+                    mma_s8(acc[2 * j], a[0][k], a[1][k], a[0][k + 1], a[1][k + 1], b[k], b[k + 1]);
+                    mma_s8(acc[2 * j + 1], a[2][k], a[3][k], a[2][k + 1], a[3][k + 1], b[k], b[k + 1]);
+                }
+            }
+        }
+    };
+    step(begin, std::true_type());
+    for (int c = begin + 4 * BYTES; c < end; c += 4 * BYTES) step(c, std::false_type());
+    double row[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) row[r] = scales[r * 8 + g];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j >= blocks) break;
+        const double2 col = *reinterpret_cast<const double2 *>(scales + apart + j * 8 + t * 2);
+        apply_scales(total[2 * j], acc[2 * j], row[0], row[1], col);
+        apply_scales(total[2 * j + 1], acc[2 * j + 1], row[2], row[3], col);
+    }
+}
+
+// ---- up to 32 clients: no shared memory ----------------------------------------------------------------------------------------
+// A warp takes a unit of a page's columns, kChunk columns at a time, the next ones on their way in registers while these are multiplied.
+// 16 warps an SM, none of which waits for another.  A client that is not there (or a page of one) is read as the cache's first
+// slot with scales of 0, so that no load needs a condition.
+template <int NB, int BYTES, int CHUNK, int GROUPS> // GROUPS: scales of a chunk
+__global__ void __launch_bounds__(kWarps * 32, NB == 4 ? 1 : 2) gram_direct_kernel(const DistanceArgs a)
+{
+    using V = Cover<NB>;
+    constexpr int STEP = BYTES * 4, STEPS = CHUNK / STEP, W = BYTES / 4;
+    __shared__ double sum[NB * 8][NB * 8];
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
+    const int log_group = 31 - __clz(a.group), code_stride = (int)a.code_stride, scale_stride = (int)a.scale_stride;
+    double total[V::kTiles][4];
+#pragma unroll
+    for (int v = 0; v < V::kTiles; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[v][e] = 0.0;
+
+    // where the next chunk lies
+    const unsigned stride = a.blocks * kWarps;
+    unsigned u = blockIdx.x * kWarps + warp;
+    int at = 0, end = 0; // columns of the page
+    int entry[NB], slot[NB];
+    const signed char *src[NB];
+    const float *scl[NB];
+    unsigned there = 0;
+#pragma unroll
+    for (int r = 0; r < NB; ++r) entry[r] = min(r * 8 + g, a.n - 1) * a.pages;
+    auto look_up = [&](unsigned unit) {
+        const int page = (int)(min(unit, a.units - 1) / a.units_per_page);
+        if (a.slots) { // (not a choice for each slot: that would wait for it)
+#pragma unroll
+            for (int r = 0; r < NB; ++r) slot[r] = __ldg(a.slots + entry[r] + page);
+        } else {
+#pragma unroll
+            for (int r = 0; r < NB; ++r) slot[r] = entry[r] + page;
+        }
+    };
+    auto enter = [&]() {
+        there = 0;
+        at = (int)(u % a.units_per_page) * a.unit;
+        end = min(at + a.unit, a.page);
+#pragma unroll
+        for (int r = 0; r < NB; ++r) {
+            const bool is = r * 8 + g < a.n && (unsigned)slot[r] < (unsigned)a.n_slots;
+            there |= (unsigned)is << r;
+            const int s = is ? slot[r] : 0;
+            src[r] = a.codes + (long)s * code_stride + t * BYTES;
+            scl[r] = a.scales + (long)s * scale_stride;
+        }
+        look_up(u + stride); // on their way while this unit is multiplied
+    };
+    struct Chunk {
+        unsigned w[NB][STEPS][W];
+        float s[NB][GROUPS];
+    };
+    auto load = [&](Chunk &k) {
+        const bool whole = at + CHUNK <= end;
+#pragma unroll
+        for (int r = 0; r < NB; ++r) {
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i) {
+                const bool inside = whole || at + i * STEP + t * BYTES < end;
+                if constexpr (BYTES == 16) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (inside) x = __ldg(reinterpret_cast<const uint4 *>(src[r] + at + i * STEP));
+                    k.w[r][i][0] = x.x;
+                    k.w[r][i][1] = x.y;
+                    k.w[r][i][2] = x.z;
+                    k.w[r][i][3] = x.w;
+                } else {
+                    uint2 x = make_uint2(0, 0);
+                    if (inside) x = __ldg(reinterpret_cast<const uint2 *>(src[r] + at + i * STEP));
+                    k.w[r][i][0] = x.x;
+                    k.w[r][i][1] = x.y;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < GROUPS; ++q) {
+                k.s[r][q] = 0.f;
+                if ((there >> r & 1) && (q == 0 || at + q * (CHUNK / GROUPS) < end)) k.s[r][q] = __ldg(scl[r] + (at >> log_group) + q);
+            }
+        }
+        at += CHUNK;
+        if (at >= end) {
+            u += stride;
+            if (u < a.units) enter();
+        }
+    };
+    auto multiply = [&](const Chunk &k) {
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) {
+            int acc[V::kTiles][4];
+#pragma unroll
+            for (int i = q * STEPS / GROUPS; i < (q + 1) * STEPS / GROUPS; ++i)
+#pragma unroll
+                for (int j = 0; j < W; j += 2)
+#pragma unroll
+                    for (int v = 0; v < V::kTiles; ++v) {
+                        const int lo = V::lo(v), hi = V::hi(v) >= 0 ? V::hi(v) : 0, col = V::col(v);
+                        const unsigned h0 = V::hi(v) >= 0 ? k.w[hi][i][j] : 0, h1 = V::hi(v) >= 0 ? k.w[hi][i][j + 1] : 0;
+                        if (i == q * STEPS / GROUPS && j == 0) mma_s8_from(acc[v], kBias, k.w[lo][i][j], h0, k.w[lo][i][j + 1], h1, k.w[col][i][j], k.w[col][i][j + 1]);
+                        else mma_s8(acc[v], k.w[lo][i][j], h0, k.w[lo][i][j + 1], h1, k.w[col][i][j], k.w[col][i][j + 1]);
+                    }
+            // accumulator e of a lane: row g (+ 8 for e >= 2) of A, column 2 t + (e & 1) of B
+            double row[NB];
+            double2 col[NB];
+#pragma unroll
+            for (int r = 0; r < NB; ++r) {
+                row[r] = k.s[r][q];
+                col[r].x = __shfl_sync(0xffffffffu, k.s[r][q], t * 8);
+                col[r].y = __shfl_sync(0xffffffffu, k.s[r][q], t * 8 + 4);
+            }
+#pragma unroll
+            for (int v = 0; v < V::kTiles; ++v) apply_scales(total[v], acc[v], row[V::lo(v)], V::hi(v) >= 0 ? row[V::hi(v) >= 0 ? V::hi(v) : 0] : 0.0, col[V::col(v)]);
+        }
+    };
+
+    look_up(u);
+    if (u < a.units) {
+        enter();
+        Chunk one, two;
+        load(one);
+        while (true) {
+            const bool more = u < a.units;
+            if (more) load(two);
+            multiply(one);
+            if (!more) break;
+            const bool again = u < a.units;
+            if (again) load(one);
+            multiply(two);
+            if (!again) break;
+        }
+    }
+    // the block's warps one after the other: the order of the additions is fixed
+    for (int k = 0; k < kWarps; ++k) {
+        if (warp == k) {
+#pragma unroll
+            for (int v = 0; v < V::kTiles; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int block = e < 2 ? V::lo(v) : V::hi(v);
+                    if (block < 0) continue;
+                    const int x = block * 8 + g, y = V::col(v) * 8 + t * 2 + (e & 1);
+                    if (block == V::col(v) && x > y) continue;
+                    double *to = &sum[min(x, y)][max(x, y)];
+                    *to = k ? *to + total[v][e] : total[v][e];
+                }
+        }
+        __syncthreads();
+    }
+    constexpr int kRows = NB * 8;
+    double *out = a.partial + (size_t)blockIdx.x * (kRows * kRows + kRows);
+    for (int i = threadIdx.x; i < kRows * kRows; i += kWarps * 32) {
+        const int x = i / kRows, y = i % kRows;
+        if (x <= y) {
+            out[i] = sum[x][y];
+            if (x == y) out[kRows * kRows + x] = sum[x][x];
+        }
+    }
+}
+
+// ---- up to 128 clients: a ring of shared memory --------------------------------------------------------------------------------
+// One CTA per SM.  All its warps together copy the codes and scales of some hundred columns of all clients into the ring, several stages
+// ahead (cp.async; one barrier a stage), and each warp multiplies two groups of 32 clients, or one with itself.  Rows lie 64 bytes off
+// a multiple of 128 apart, so that the 16-byte loads of eight rows fall on different banks.
+//
+// NB: blocks of eight clients: 8, 12 or 16.  SETS warps split the columns of a stage, 2^LOG_UNIT, for the same pairs.  (Sizes are constants because instructions are what this kernel runs short of: with
+// divisions by a unit of run-time size it took 870 a warp and stage, four times what follows.)
+template <int NB, int LOG_UNIT, int BYTES, int WARPS, int SETS>
+__global__ void __launch_bounds__(WARPS * 32, 1) gram_ring_kernel(const DistanceArgs a, const Ring r)
+{
+    constexpr int kThreads = WARPS * 32;
+    constexpr int kUnit = 1 << LOG_UNIT, kPitch = kUnit + 64, kWide = NB * 8;
+    constexpr int kLanes = kUnit < 512 ? kUnit / 16 : 32;                         // that copy one row together
+    constexpr int kRowsACopy = 32 / kLanes, kCopiesARow = kUnit / (kLanes * 16); // of a warp
+    constexpr int kFill = (kWide / kRowsACopy * kCopiesARow + WARPS - 1) / WARPS; // copies that a warp makes for one stage, at most
+    extern __shared__ __align__(128) unsigned char ring[];
+    double *wide_scales = reinterpret_cast<double *>(ring + r.stages * r.stage_bytes + r.spare); // [2][groups][kWide]: of this stage and the next
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int code_bytes = r.rows * kPitch;
+    const int log_group = 31 - __clz(a.group), log_groups = 31 - __clz(r.groups), scales_a_stage = a.n << log_groups;
+
+    // where a unit lies; units are taken in turn by the CTAs
+    const int page_step = (int)(gridDim.x / a.units_per_page), part_step = (int)(gridDim.x % a.units_per_page);
+    struct Place {
+        int page, begin;
+    };
+    auto advance = [&](Place &p) {
+        p.page += page_step;
+        p.begin += part_step << LOG_UNIT;
+        if (p.begin >= a.page) {
+            ++p.page;
+            p.begin -= (int)a.units_per_page << LOG_UNIT;
+        }
+    };
+    Place now = {(int)(blockIdx.x / a.units_per_page), (int)(blockIdx.x % a.units_per_page) << LOG_UNIT};
+    Place ahead = now; // the next unit to be copied
+
+    // What this thread copies of every stage: 16 bytes of the same columns of every kRowsApart-th row, and some scales.  The slots are
+    // looked up a stage ahead; none of these loads is behind a branch, and nothing looks at the slots before fill does
+    static_assert(WARPS % kCopiesARow == 0, "a warp's copies are of the same columns");
+    constexpr int kRowsApart = WARPS / kCopiesARow * kRowsACopy;
+    const int first_row = warp / kCopiesARow * kRowsACopy + lane / kLanes, column = warp % kCopiesARow * 512 + lane % kLanes * 16;
+    const unsigned first_to = smem_u32(ring) + first_row * kPitch + column;
+    const int n_slots = (int)a.n_slots, code_stride = (int)a.code_stride, scale_stride = (int)a.scale_stride;
+    int code_entry[kFill], scale_entry[kMaxScales], code_slot[kFill], scale_slot[kMaxScales];
+#pragma unroll
+    for (int k = 0; k < kFill; ++k) code_entry[k] = min(first_row + k * kRowsApart, a.n - 1) * a.pages;
+#pragma unroll
+    for (int k = 0; k < kMaxScales; ++k) scale_entry[k] = min((int)(threadIdx.x + k * kThreads) >> log_groups, a.n - 1) * a.pages;
+    auto look_up = [&](int page) {
+        const int at = min(page, a.pages - 1);
+        if (a.slots) { // (not a choice for each slot: that would wait for it)
+#pragma unroll
+            for (int k = 0; k < kFill; ++k) code_slot[k] = __ldg(a.slots + code_entry[k] + at);
+#pragma unroll
+            for (int k = 0; k < kMaxScales; ++k)
+                if (k * kThreads < scales_a_stage) scale_slot[k] = __ldg(a.slots + scale_entry[k] + at);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kFill; ++k) code_slot[k] = code_entry[k] + at;
+#pragma unroll
+            for (int k = 0; k < kMaxScales; ++k) scale_slot[k] = scale_entry[k] + at;
+        }
+    };
+    auto fill = [&](const Place &p, int stage) { // a page that is not there leaves old codes, and scales of 0
+        if (p.page < a.pages) {
+            const unsigned to = first_to + stage * r.stage_bytes;
+            const signed char *from = a.codes + p.begin + column;
+            const bool inside = p.begin + column < a.page;
+#pragma unroll
+            for (int k = 0; k < kFill; ++k)
+                if (first_row + k * kRowsApart < a.n && (unsigned)code_slot[k] < (unsigned)n_slots) // zeros behind the page's end
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * kRowsApart * kPitch), "l"(inside ? from + (long)code_slot[k] * code_stride : a.codes),
+                                 "r"(inside ? 16 : 0));
+            const unsigned scales_to = smem_u32(ring) + stage * r.stage_bytes + code_bytes;
+#pragma unroll
+            for (int k = 0; k < kMaxScales; ++k) {
+                const int i = threadIdx.x + k * kThreads;
+                if (i < scales_a_stage) {
+                    const int q = (p.begin >> log_group) + (i & (r.groups - 1));
+                    const bool there = (unsigned)scale_slot[k] < (unsigned)n_slots && (long)q << log_group < a.page;
+                    const float *src = there ? a.scales + (long)scale_slot[k] * scale_stride + q : a.scales;
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scales_to + i * 4), "l"(src), "r"(there ? 4 : 0));
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto widen = [&](int stage, int parity) { // a stage's scales as 64-bit floats, [group][client]
+        const float *from = reinterpret_cast<const float *>(ring + (size_t)stage * r.stage_bytes + code_bytes);
+        double *to = wide_scales + parity * r.groups * kWide;
+        for (int i = threadIdx.x; i < scales_a_stage; i += kThreads) to[(i & (r.groups - 1)) * kWide + (i >> log_groups)] = from[i];
+    };
+
+    // the pairs of this warp: rows from row0 on with rows from col0 on
+    const int set = warp % SETS;
+    int row0 = 0, col0 = warp / SETS;
+    constexpr int kGroups = NB / 4;
+    while (col0 >= kGroups - row0) col0 -= kGroups - row0++;
+    col0 = (row0 + col0) * 32;
+    row0 *= 32;
+    const int col_blocks = min(4, (a.n - col0 + 7) / 8);
+    constexpr int kPer = kUnit / SETS; // columns of a warp
+    const int step = min(a.group, kPer);
+    double total[8][4];
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[v][e] = 0.0;
+
+    look_up(ahead.page);
+    for (int s = 0; s < r.stages - 1; ++s) {
+        fill(ahead, s);
+        advance(ahead);
+        look_up(ahead.page);
+    }
+    // a stage and the next one have come in when all but the last stages - 3 copies have
+    auto wait = [&]() {
+        switch (r.stages) {
+        case 3: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+        case 4: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+        case 5: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+        case 6: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        case 7: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+        default: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+        }
+    };
+    wait();
+    __syncthreads();
+    widen(0, 0);
+    int s = 0, parity = 0;
+    for (; now.page < a.pages; advance(now)) {
+        wait();
+        __syncthreads(); // this stage and the next have come in, the last one has been read
+        const int next = s + 1 == r.stages ? 0 : s + 1;
+        fill(ahead, s ? s - 1 : r.stages - 1);
+        advance(ahead);
+        look_up(ahead.page);
+        widen(next, parity ^ 1); // (behind the last unit: old scales, and nobody reads them)
+        const int columns = min(kUnit, a.page - now.begin);
+        const unsigned char *codes = ring + (size_t)s * r.stage_bytes;
+        const int to = min((set + 1) * kPer, columns);
+        const double *scales = wide_scales + parity * r.groups * kWide;
+        for (int c = set * kPer; c < to; c += step) {
+            const double *sc = scales + (c >> log_group) * kWide; // a stage begins where a group does, or has only one
+            if (row0 == col0) triangle<BYTES>(total, codes + row0 * kPitch, sc + row0, kPitch, c, c + step);
+            else square<BYTES>(total, codes + row0 * kPitch, sc + row0, col0 - row0, col_blocks, kPitch, c, c + step);
+        }
+        s = next;
+        parity ^= 1;
+    }
+    // the ring's memory takes the sums now; the order in which the warps of a set add them up is fixed
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    double *sums = reinterpret_cast<double *>(ring);
+    const int g = lane >> 2, t = lane & 3;
+    for (int k = 0; k < SETS; ++k) {
+        __syncthreads();
+        if (set != k) continue;
+        auto put = [&](int x, int y, double v) {
+            double *at = sums + min(x, y) * kWide + max(x, y);
+            *at = k ? *at + v : v;
+        };
+        if (row0 == col0) {
+            using V = Cover<4>;
+#pragma unroll
+            for (int v = 0; v < V::kTiles; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int block = e < 2 ? V::lo(v) : V::hi(v);
+                    if (block < 0) continue;
+                    const int x = block * 8 + g, y = V::col(v) * 8 + t * 2 + (e & 1);
+                    if (block != V::col(v) || x <= y) put(row0 + x, row0 + y, total[v][e]);
+                }
+        } else {
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) put(row0 + (v & 1) * 16 + (e >> 1) * 8 + g, col0 + (v >> 1) * 8 + t * 2 + (e & 1), total[v][e]);
+        }
+    }
+    __syncthreads();
+    double *out = a.partial + (size_t)blockIdx.x * (kWide * kWide + kWide);
+    for (int i = threadIdx.x; i < kWide * kWide; i += kThreads) {
+        const int x = i / kWide, y = i - x * kWide;
+        if (x <= y && y < a.n) {
+            out[i] = sums[i];
+            if (x == y) out[kWide * kWide + x] = sums[i];
+        }
+    }
+}
+
+// A block per row i: the sums of all blocks, then the distances of row i.  LANES clients side by side, and as many slices of the blocks
+// as the 1024 threads give, the same ones for every sum
+template <int LANES>
+__global__ void __launch_bounds__(1024) distance_rows_kernel(const double *__restrict__ partial, const int n, const int rows, const int blocks, double *__restrict__ out)
+{
+    constexpr int kSlices = 1024 / LANES;
+    __shared__ double dots[kSlices][LANES], norms[kSlices][LANES];
+    const int i = blockIdx.x, j = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+    const long pitch = (long)rows * rows + rows;
+    double dot = 0.0, norm = 0.0;
+    if (j < n) {
+        const double *p = partial + (long)min(i, j) * rows + max(i, j), *q = partial + (long)rows * rows + j;
+#pragma unroll 8
+        for (int b = slice; b < blocks; b += kSlices) {
+            dot += p[b * pitch];
+            norm += q[b * pitch];
+        }
+    }
+    dots[slice][j] = dot;
+    norms[slice][j] = norm;
+    __syncthreads();
+    for (int half = kSlices / 2; half; half /= 2) {
+        if (slice < half) {
+            dots[slice][j] += dots[slice + half][j];
+            norms[slice][j] += norms[slice + half][j];
+        }
+        __syncthreads();
+    }
+    if (slice || j >= n) return;
+    const double x = norms[0][i], y = norms[0][j], z = dots[0][j], d = (x - z) + (y - z);
+    out[(long)i * n + j] = i == j ? 0.0 : d < 0.0 ? 0.0 : d; // below 0: rounding of nearly equal updates; NaN stays
 }
 
 // a warp per pair i <= j: the partial sums of the blocks, then the distance
@@ -229,8 +744,11 @@ __global__ void __launch_bounds__(256) distance_finish_kernel(const double *__re
 }
 
 struct DistancePlan {
-    int n_blocks, tiles, blocks, unit;
+    int n_blocks, tiles, blocks; // gram_kernel: blocks of 32 clients, pairs of them, blocks per pair
+    int unit, least_unit;        // columns taken at a time
+    int rows;                          // gram_ring_kernel: its rows; 0: gram_kernel
     long units;
+    size_t bytes;
 };
 
 DistancePlan distance_plan(int sm_count, int n, long pages, int page)
@@ -238,37 +756,94 @@ DistancePlan distance_plan(int sm_count, int n, long pages, int page)
     DistancePlan p;
     p.n_blocks = (n + 31) / 32;
     p.tiles = p.n_blocks * (p.n_blocks + 1) / 2;
-    // a warp takes 1024 columns of a page at a time; fewer where that would leave warps without work
-    p.unit = 1024;
-    while (p.unit > 128 && pages * ((page + p.unit - 1) / p.unit) * p.tiles < (long)sm_count * 2 * kWarps) p.unit >>= 1;
+    p.rows = n <= 32 ? (n + 7) / 8 * 8 : n <= 128 ? (n + 31) / 32 * 32 : 0;
+    // what a warp (gram_ring_kernel: a CTA) takes at a time: as much as leaves all of them work
+    const bool ring = n > 32 && n <= 128;
+    const int warp_blocks = p.rows ? (p.rows == 32 ? 1 : 2) * sm_count : (2 * sm_count + p.tiles - 1) / p.tiles;
+    const long takers = ring ? sm_count : (long)warp_blocks * kWarps;
+    p.unit = !ring ? 1024 : p.rows > 64 ? 256 : 512;
+    p.least_unit = !ring ? 128 : 256;
+    while (p.unit > p.least_unit && pages * ((page + p.unit - 1) / p.unit) < takers) p.unit >>= 1;
     p.units = pages * ((page + p.unit - 1) / p.unit);
-    const long want = (p.units + kWarps - 1) / kWarps, most = (sm_count * 2 + p.tiles - 1) / p.tiles;
-    p.blocks = (int)(want < most ? want : most);
-    if (p.blocks < 1) p.blocks = 1;
+    if (p.rows) {
+        const long want = ring ? p.units : (p.units + kWarps - 1) / kWarps, most = ring ? sm_count : warp_blocks;
+        p.blocks = (int)(want < most ? want : most);
+        if (p.blocks < 1) p.blocks = 1;
+        p.bytes = (size_t)p.blocks * (p.rows * p.rows + p.rows) * sizeof(double);
+    } else {
+        const long want = (p.units + kWarps - 1) / kWarps, most = (sm_count * 2 + p.tiles - 1) / p.tiles;
+        p.blocks = (int)(want < most ? want : most);
+        if (p.blocks < 1) p.blocks = 1;
+        p.bytes = (size_t)p.tiles * p.blocks * 1024 * sizeof(double);
+    }
     return p;
 }
 
-template <int BYTES> void launch_gram(const DistanceArgs &a, const DistancePlan &p, cudaStream_t stream)
+template <int NB, int LOG_UNIT, int BYTES, int WARPS, int SETS> int launch_ring(Context *ctx, const DistanceArgs &a, const DistancePlan &p, cudaStream_t stream)
 {
-    const dim3 grid((unsigned)p.tiles, (unsigned)p.blocks);
-    if (p.n_blocks > 1) gram_kernel<4, false, BYTES><<<grid, kWarps * 32, 0, stream>>>(a, p.n_blocks);
-    else if (a.n > 24) gram_kernel<4, true, BYTES><<<grid, kWarps * 32, 0, stream>>>(a, 1);
-    else if (a.n > 16) gram_kernel<3, true, BYTES><<<grid, kWarps * 32, 0, stream>>>(a, 1);
-    else if (a.n > 8) gram_kernel<2, true, BYTES><<<grid, kWarps * 32, 0, stream>>>(a, 1);
-    else gram_kernel<1, true, BYTES><<<grid, kWarps * 32, 0, stream>>>(a, 1);
+    constexpr int kUnit = 1 << LOG_UNIT, kPitch = kUnit + 64;
+    Ring r;
+    r.rows = (a.n + 7) / 8 * 8;
+    r.groups = a.group < kUnit ? kUnit / a.group : 1;
+    r.stage_bytes = (r.rows * kPitch + r.rows * r.groups * 4 + 127) / 128 * 128;
+    r.spare = (NB * 8 - r.rows) * kPitch;
+    const int wide = 2 * r.groups * NB * 8 * 8;
+    r.stages = (kRingBytes - r.spare - wide) / r.stage_bytes;
+    if (r.stages > 8) r.stages = 8;
+    static bool set[64] = {};
+    if (ctx->device >= 64 || !set[ctx->device]) {
+        LB_CUDA(cudaFuncSetAttribute(gram_ring_kernel<NB, LOG_UNIT, BYTES, WARPS, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
+        if (ctx->device < 64) set[ctx->device] = true;
+    }
+    gram_ring_kernel<NB, LOG_UNIT, BYTES, WARPS, SETS><<<p.blocks, WARPS * 32, r.stages * r.stage_bytes + r.spare + wide, stream>>>(a, r);
+    return LB_OK;
+}
+
+template <int NB, int BYTES, int CHUNK> int launch_direct(const DistanceArgs &a, const DistancePlan &p, cudaStream_t stream)
+{
+    if constexpr (BYTES == 8) {
+        gram_direct_kernel<NB, 8, CHUNK, CHUNK / 32><<<p.blocks, kWarps * 32, 0, stream>>>(a);
+    } else if constexpr (CHUNK == 256) {
+        if (a.group < 128) gram_direct_kernel<NB, 16, CHUNK, 4><<<p.blocks, kWarps * 32, 0, stream>>>(a);
+        else if (a.group < CHUNK) gram_direct_kernel<NB, 16, CHUNK, 2><<<p.blocks, kWarps * 32, 0, stream>>>(a);
+        else gram_direct_kernel<NB, 16, CHUNK, 1><<<p.blocks, kWarps * 32, 0, stream>>>(a);
+    } else if constexpr (CHUNK == 128) {
+        if (a.group < CHUNK) gram_direct_kernel<NB, 16, CHUNK, 2><<<p.blocks, kWarps * 32, 0, stream>>>(a);
+        else gram_direct_kernel<NB, 16, CHUNK, 1><<<p.blocks, kWarps * 32, 0, stream>>>(a);
+    } else {
+        gram_direct_kernel<NB, 16, CHUNK, 1><<<p.blocks, kWarps * 32, 0, stream>>>(a);
+    }
+    return LB_OK;
+}
+
+template <int BYTES> int launch_gram(Context *ctx, const DistanceArgs &a, const DistancePlan &p, cudaStream_t stream)
+{
+    const bool small = p.unit == p.least_unit;
+    switch (p.rows / 8) {
+    case 1: return launch_direct<1, BYTES, 256>(a, p, stream);
+    case 2: return launch_direct<2, BYTES, BYTES == 8 ? 128 : 256>(a, p, stream);
+    case 3: return launch_direct<3, BYTES, 128>(a, p, stream);
+    case 4: return launch_direct<4, BYTES, 64>(a, p, stream);
+    case 8: return small ? launch_ring<8, 8, BYTES, 12, 4>(ctx, a, p, stream) : launch_ring<8, 9, BYTES, 12, 4>(ctx, a, p, stream); // three pairs of groups of 32
+    case 12: return launch_ring<12, 8, BYTES, 12, 2>(ctx, a, p, stream); // six
+    case 16: return launch_ring<16, 8, BYTES, 10, 1>(ctx, a, p, stream); // ten
+    }
+    gram_kernel<BYTES><<<dim3((unsigned)p.tiles, (unsigned)p.blocks), kWarps * 32, 0, stream>>>(a, p.n_blocks);
+    return LB_OK;
 }
 
 } // namespace
 
-size_t int8_distances_workspace_bytes(const Context *ctx, int n, long pages, int page)
-{
-    const DistancePlan p = distance_plan(ctx->sm_count, n, pages, page);
-    return (size_t)p.tiles * p.blocks * 1024 * sizeof(double);
-}
+size_t int8_distances_workspace_bytes(const Context *ctx, int n, long pages, int page) { return distance_plan(ctx->sm_count, n, pages, page).bytes; }
 
 int int8_distances(Context *ctx, const signed char *codes, long code_stride, const float *scales, long scale_stride, long n_slots, int page,
                    int group, const int *slots, int n, int pages, double *out, void *workspace, cudaStream_t stream)
 {
+    if (n_slots == 0) pages = 0; // no page is there: all distances are 0
+    if (n == 1 || pages == 0) {
+        LB_CUDA(cudaMemsetAsync(out, 0, (size_t)n * n * sizeof(double), stream));
+        return LB_OK;
+    }
     const DistancePlan p = distance_plan(ctx->sm_count, n, pages, page);
     DistanceArgs a;
     a.codes = codes;
@@ -280,18 +855,21 @@ int int8_distances(Context *ctx, const signed char *codes, long code_stride, con
     a.n = n;
     a.pages = pages;
     a.page = page;
-    a.group = group == 0 || group > page ? page : group;
+    a.group = group == 0 || group >= page ? 1 << 30 : group;
     a.unit = p.unit;
     a.units_per_page = (unsigned)((page + p.unit - 1) / p.unit);
     a.units = (unsigned)p.units;
     a.blocks = p.blocks;
     a.partial = reinterpret_cast<double *>(workspace);
     count_launch("int8_gram", stream, (double)n * pages * page);
-    if (a.group % 64 == 0 || a.group == a.page) launch_gram<16>(a, p, stream);
-    else launch_gram<8>(a, p, stream);
+    // 16 bytes a lane cover 64 columns, which have to share their scale; 8 bytes cover 32
+    int rc = a.group % 64 == 0 ? launch_gram<16>(ctx, a, p, stream) : launch_gram<8>(ctx, a, p, stream);
+    if (rc) return rc;
     LB_CUDA(cudaGetLastError());
     count_launch("int8_distances", stream, 8.0 * n * n);
-    distance_finish_kernel<<<(unsigned)(((long)n * n + 7) / 8), 256, 0, stream>>>(a.partial, n, p.n_blocks, p.blocks, out);
+    if (p.rows && n <= 32) distance_rows_kernel<32><<<n, 1024, 0, stream>>>(a.partial, n, p.rows, p.blocks, out);
+    else if (p.rows) distance_rows_kernel<128><<<n, 1024, 0, stream>>>(a.partial, n, p.rows, p.blocks, out);
+    else distance_finish_kernel<<<(unsigned)(((long)n * n + 7) / 8), 256, 0, stream>>>(a.partial, n, p.n_blocks, p.blocks, out);
     LB_CUDA(cudaGetLastError());
     return LB_OK;
 }

@@ -7,11 +7,10 @@
 // Two kernels.  With few rows on one side the other side is read once and that bounds the call: rows go from memory straight into
 // the registers of the warp's matrix instruction.  Otherwise the tiles run on the tensor cores' own memory: operands by TMA
 // into 128-byte swizzled shared memory, tcgen05.mma into TMEM, results out of TMEM while the next tile is being multiplied.
-#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "context.h"
+#include "tcgen05.cuh"
 
 namespace lb {
 
@@ -48,13 +47,6 @@ __global__ void __launch_bounds__(256) pack_kernel(const signed char *__restrict
 // split k and add up through shared memory.  As in the pair distances, the order of k inside a product is free, so lane (g, t) loads
 // 16 consecutive bytes of a row and uses them as four k-slots on either side.
 constexpr int kSkinnyWarps = 8;
-
-__device__ __forceinline__ void mma_s8(int (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
-{
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 struct SkinnyArgs {
     const signed char *w, *x; // long side [rows][k], short side [cols][k]
@@ -120,90 +112,6 @@ template <typename T> int launch_skinny(const SkinnyArgs &a, cudaStream_t stream
 // issues the products (four of k = 32 a stage), warps 2 to 5 take a finished tile out of TMEM.  TMEM holds two tiles, so
 // a tile leaves while the next one is being formed.
 constexpr int kTileM = 128, kTileK = 128, kTileThreads = 192;
-constexpr int kWaitNs = 2000000000; // a wait gives up after two seconds
-
-__device__ __forceinline__ unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(unsigned bar, unsigned count)
-{
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect(unsigned bar, unsigned bytes)
-{
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(unsigned bar)
-{
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity)
-{
-    unsigned done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done)
-                 : "r"(bar), "r"(parity)
-                 : "memory");
-    return done;
-}
-__device__ __forceinline__ unsigned long long now_ns()
-{
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-// false: the wait ran out, here or in another warp of the block
-__device__ __noinline__ bool mbar_wait_slow(unsigned bar, unsigned parity, volatile int *failed)
-{
-    const unsigned long long began = now_ns();
-    while (!*failed) {
-        for (int i = 0; i < 64; ++i)
-            if (mbar_try(bar, parity)) return true;
-        if (now_ns() - began > kWaitNs) {
-            *failed = 1;
-            break;
-        }
-    }
-    return false;
-}
-__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int *failed)
-{
-    for (int i = 0; i < 16; ++i)
-        if (mbar_try(bar, parity)) return true;
-    return mbar_wait_slow(bar, parity, failed);
-}
-__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, int x, int y, unsigned bar)
-{
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
-                 "r"(x), "r"(y), "r"(bar)
-                 : "memory");
-}
-// rows of 128 bytes, 128-byte swizzle: groups of eight rows 1024 bytes apart
-__device__ __forceinline__ unsigned long long operand_desc(unsigned addr)
-{
-    return (unsigned long long)((addr & 0x3ffff) >> 4) | 1ull << 16 | (unsigned long long)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
-__device__ __forceinline__ void mma_i8(unsigned d, unsigned long long a, unsigned long long b, unsigned desc, bool add)
-{
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-                 "r"(desc), "r"((unsigned)add)
-                 : "memory");
-}
-__device__ __forceinline__ void mma_commit(unsigned bar)
-{
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tmem_load32(unsigned addr, int (&v)[32])
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
-                   "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
-                   "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-                 : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
 template <int BN> struct Tile {
     static constexpr int kStageBytes = (kTileM + BN) * kTileK;
     static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
@@ -346,34 +254,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) product_kernel(const __grid_c
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            int it = 0, done_tiles = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++done_tiles) {
-                const int buf = done_tiles & 1;
-                if (done_tiles >= 2) ok = mbar_wait(freed + 8 * buf, (done_tiles / 2 - 1) & 1, failed);
+        const unsigned elected = elect_one();
+        int it = 0, done_tiles = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++done_tiles) {
+            const int buf = done_tiles & 1;
+            if (done_tiles >= 2) ok = mbar_wait_warp(freed + 8 * buf, (done_tiles / 2 - 1) & 1, failed);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int k = 0; k < a.k_blocks; ++k, ++it) {
+                const int s = it % C::kStages;
+                ok = mbar_wait_warp(full + 8 * s, (it / C::kStages) & 1, failed);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int k = 0; k < a.k_blocks; ++k, ++it) {
-                    const int s = it % C::kStages;
-                    ok = mbar_wait(full + 8 * s, (it / C::kStages) & 1, failed);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned at = stage0 + s * C::kStageBytes;
-                    const unsigned long long da = operand_desc(at), db = operand_desc(at + kTileM * kTileK);
+                const unsigned at = stage0 + s * C::kStageBytes;
+                const unsigned long long da = operand_desc(at), db = operand_desc(at + kTileM * kTileK);
 #pragma unroll
-                    for (int e = 0; e < kTileK / 32; ++e) mma_i8(tmem + buf * BN, da + 2 * e, db + 2 * e, C::kDesc, k > 0 || e > 0);
-                    mma_commit(empty + 8 * s);
-                }
-                if (ok) mma_commit(done + 8 * buf);
+                for (int e = 0; e < kTileK / 32; ++e) mma_i8(elected, tmem + buf * BN, da + 2 * e, db + 2 * e, C::kDesc, k > 0 || e > 0);
+                mma_commit(elected, empty + 8 * s);
             }
-            if (!ok) { // products that are still under way end before their memory is given back
-                mma_commit(drained);
-                for (int n = 0; n < 1 << 20; ++n)
-                    if (mbar_try(drained, 0)) break;
-            }
+            if (ok) mma_commit(elected, done + 8 * buf);
         }
-        __syncwarp();
+        if (!ok) { // products that are still under way end before their memory is given back
+            mma_commit(elected, drained);
+            for (int n = 0; n < 1 << 20; ++n)
+                if (mbar_try(drained, 0)) break;
+        }
     } else {
         const int quarter = warp & 3;
         float *sb = scales + quarter * 256;
@@ -417,33 +323,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) product_kernel(const __grid_c
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (threadIdx.x == 0 && *failed) atomicOr(a.status, 2);
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * BN) : "memory");
-}
-
-typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-int encode_map(CUtensorMap *map, const void *base, long rows, int cols, long stride, int box_rows)
-{
-    static EncodeTiled encode = nullptr;
-    if (!encode) {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        LB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found));
-        if (found != cudaDriverEntryPointSuccess || !f) {
-            set_error("the driver has no cuTensorMapEncodeTiled");
-            return LB_ERR_CUDA;
-        }
-        encode = reinterpret_cast<EncodeTiled>(f);
-    }
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
-    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows}, steps[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        set_error("cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
-        return LB_ERR_CUDA;
-    }
-    return LB_OK;
 }
 
 template <typename T, int BN> int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const ProductArgs &a, cudaStream_t stream)
@@ -520,9 +399,9 @@ int product_typed(Context *ctx, int m, int n, int k, const signed char *a, long 
     const int bn = (long)p.tiles_m * ((n + 255) / 256) >= ctx->sm_count ? 256 : (long)p.tiles_m * ((n + 127) / 128) >= ctx->sm_count ? 128 : 64;
     p.tiles_n = (n + bn - 1) / bn;
     CUtensorMap ma, mb;
-    int rc = encode_map(&ma, a, m, k, a_stride, kTileM);
+    int rc = encode_map(&ma, a, m, k, a_stride, kTileK, kTileM);
     if (rc) return rc;
-    if ((rc = encode_map(&mb, b, n, k, b_stride, bn))) return rc;
+    if ((rc = encode_map(&mb, b, n, k, b_stride, kTileK, bn))) return rc;
     count_launch("int8_tiles", stream, bytes);
     if (bn == 256) return launch_tiles<T, 256>(ctx, ma, mb, p, stream);
     if (bn == 128) return launch_tiles<T, 128>(ctx, ma, mb, p, stream);

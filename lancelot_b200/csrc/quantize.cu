@@ -102,6 +102,52 @@ template <bool VEC> __device__ __forceinline__ void store4(__half *p, float4 v, 
     if (valid > 3) p[3] = __float2half_rn(v.w);
 }
 
+// Rows that start off a 16-byte boundary (an odd number of values a row is the rule for updates).  The warp's run of columns
+// is still contiguous, so it moves in aligned pieces and the lanes hand the values on to where they belong: `off` values of a piece
+// belong to the lane before.  All 32 lanes take part; lane l stands for columns col .. col + 3, col = (lane 0's) + 4 l.  Only values with
+// 0 <= column < limit are touched.
+template <typename T> __device__ __forceinline__ float4 load_piece(const T *row, long at, long limit)
+{
+    if (at >= 0 && at + 4 <= limit) return load4<true>(row + at, 4);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at >= 0 && at < limit) v.x = (float)row[at];
+    if (at + 1 >= 0 && at + 1 < limit) v.y = (float)row[at + 1];
+    if (at + 2 >= 0 && at + 2 < limit) v.z = (float)row[at + 2];
+    if (at + 3 >= 0 && at + 3 < limit) v.w = (float)row[at + 3];
+    return v;
+}
+template <typename T> __device__ __forceinline__ float4 load_shifted(const T *row, long col, long limit)
+{
+    const int off = (int)((uintptr_t)(row + col) / sizeof(T)) & 3;
+    const float4 a = load_piece(row, col - off, limit);
+    if (off == 0) return a;
+    float4 next = make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool last = (threadIdx.x & 31) == 31;
+    if (last) next = load_piece(row, col - off + 4, limit);
+    const float x = __shfl_down_sync(0xffffffffu, a.x, 1), y = __shfl_down_sync(0xffffffffu, a.y, 1), z = __shfl_down_sync(0xffffffffu, a.z, 1);
+    if (!last) next = make_float4(x, y, z, 0.f);
+    if (off == 1) return make_float4(a.y, a.z, a.w, next.x);
+    if (off == 2) return make_float4(a.z, a.w, next.x, next.y);
+    return make_float4(a.w, next.x, next.y, next.z);
+}
+template <typename T> __device__ __forceinline__ void store_shifted(T *row, long col, float4 v, long limit)
+{
+    const int off = (int)((uintptr_t)(row + col) / sizeof(T)) & 3;
+    if (off == 0) {
+        store4<true>(row + col, v, limit - col);
+        return;
+    }
+    const float y = __shfl_up_sync(0xffffffffu, v.y, 1), z = __shfl_up_sync(0xffffffffu, v.z, 1), w = __shfl_up_sync(0xffffffffu, v.w, 1);
+    const int lane = threadIdx.x & 31;
+    const float4 piece = off == 1 ? make_float4(w, v.x, v.y, v.z) : off == 2 ? make_float4(z, w, v.x, v.y) : make_float4(y, z, w, v.x);
+    if (lane == 0) store4<false>(row + col, v, min(limit - col, 4L - off)); // the rest of the piece is not this warp's
+    else store4<true>(row + col - off, piece, limit - col + off);
+    if (lane == 31) {
+        const float4 rest = off == 1 ? make_float4(v.w, 0.f, 0.f, 0.f) : off == 2 ? make_float4(v.z, v.w, 0.f, 0.f) : make_float4(v.y, v.z, v.w, 0.f);
+        store4<false>(row + col + 4 - off, rest, min(limit - col - 4 + off, (long)off));
+    }
+}
+
 // The scale of a group from the bits of its largest magnitude.  The bit patterns of magnitudes are ordered like the magnitudes
 // with infinities and NaN above all numbers, so an integer maximum carries them along: such a group gets NaN
 __device__ __forceinline__ float scale_of(unsigned most)
@@ -187,18 +233,27 @@ __device__ __forceinline__ long row_limit(const QuantizeArgs &a, long row)
     return a.lengths ? min((long)max(a.lengths[row], 0), a.n_cols) : a.n_cols;
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ float4 load_sum(const QuantizeArgs &a, long row, long col, long valid)
+// t for columns col .. col + 3 of a row, 0 from column `limit` on.  VEC: all rows start on the boundary of a vector
+template <typename T, bool VEC> __device__ __forceinline__ float4 load_sum(const QuantizeArgs &a, long row, long col, long limit)
 {
-    float4 v = load4<VEC>(reinterpret_cast<const T *>(a.values) + row * a.value_stride + col, valid);
+    const T *values = reinterpret_cast<const T *>(a.values) + row * a.value_stride;
+    float4 v = VEC ? load4<true>(values + col, limit - col) : load_shifted(values, col, limit);
     if (a.residual) {
-        const float4 r = load4<VEC>(a.residual + row * a.residual_stride + col, valid);
+        const float *res = a.residual + row * a.residual_stride;
+        const float4 r = VEC ? load4<true>(res + col, limit - col) : load_shifted(res, col, limit);
         v.x += r.x;
         v.y += r.y;
         v.z += r.z;
         v.w += r.w;
     }
     return v;
+}
+template <bool VEC> __device__ __forceinline__ void store_lost(const QuantizeArgs &a, long row, long col, const float4 &v, long limit)
+{
+    if (!a.residual_out) return;
+    float *out = a.residual_out + row * a.residual_stride;
+    if (VEC) store4<true>(out + col, v, limit - col);
+    else store_shifted(out, col, v, limit);
 }
 
 // ---- groups of 32 to 512 columns: a warp takes 512 columns, four of each lane's values side by side -------------------
@@ -214,13 +269,13 @@ __global__ void __launch_bounds__(256) quantize_warp_kernel(const QuantizeArgs a
     const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
     long slot;
     if (!page_slot(a, page_index, slot)) return;
-    const long limit = row_limit(a, row);
+    const long limit = min(row_limit(a, row), (long)(page + 1) * a.page);
     const int in_page = tile * 512 + lane * 4;
     const long col = (long)page * a.page + in_page;
     float4 v[4];
     unsigned m[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = load_sum<T, VEC>(a, row, col + j * 128, in_page + j * 128 < a.page ? limit - col - j * 128 : 0);
+    for (int j = 0; j < 4; ++j) v[j] = load_sum<T, VEC>(a, row, col + j * 128, limit);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         m[j] = most4(v[j]);
@@ -241,12 +296,13 @@ __global__ void __launch_bounds__(256) quantize_warp_kernel(const QuantizeArgs a
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int c = in_page + j * 128;
-        if (c >= a.page) break;
         const float s = scale_of(m[j]);
-        if ((c & ((1 << LOG_G) - 1)) == 0) a.scales[slot * a.scale_stride + (c >> LOG_G)] = s;
         const unsigned q = codes4(v[j], s);
-        *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
-        if (a.residual_out) store4<VEC>(a.residual_out + row * a.residual_stride + col + j * 128, v[j], limit - col - j * 128);
+        if (c < a.page) {
+            if ((c & ((1 << LOG_G) - 1)) == 0) a.scales[slot * a.scale_stride + (c >> LOG_G)] = s;
+            *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
+        }
+        store_lost<VEC>(a, row, col + j * 128, v[j], limit);
     }
 }
 
@@ -259,15 +315,14 @@ __global__ void __launch_bounds__(THREADS) quantize_block_kernel(const QuantizeA
     const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
     long slot;
     if (!page_slot(a, page_index, slot)) return;
-    const long limit = row_limit(a, row);
     const int first = g * a.group, end = min(a.page, first + a.group); // columns of the group inside the page
+    const long limit = min(row_limit(a, row), (long)page * a.page + end);
     const int in_page = first + threadIdx.x * 4;
     const long col = (long)page * a.page + in_page;
     float4 v[V];
     unsigned m = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-        v[j] = load_sum<T, VEC>(a, row, col + j * THREADS * 4, in_page + j * THREADS * 4 < end ? limit - col - j * THREADS * 4 : 0);
+    for (int j = 0; j < V; ++j) v[j] = load_sum<T, VEC>(a, row, col + j * THREADS * 4, limit);
 #pragma unroll
     for (int j = 0; j < V; ++j) m = max(m, most4(v[j]));
     m = __reduce_max_sync(0xffffffffu, m);
@@ -280,10 +335,9 @@ __global__ void __launch_bounds__(THREADS) quantize_block_kernel(const QuantizeA
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int c = in_page + j * THREADS * 4;
-        if (c >= end) break;
         const unsigned q = codes4(v[j], s);
-        *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
-        if (a.residual_out) store4<VEC>(a.residual_out + row * a.residual_stride + col + j * THREADS * 4, v[j], limit - col - j * THREADS * 4);
+        if (c < end) *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
+        store_lost<VEC>(a, row, col + j * THREADS * 4, v[j], limit);
     }
 }
 
@@ -299,9 +353,9 @@ __global__ void __launch_bounds__(1024) quantize_part_kernel(const QuantizeArgs 
     const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
     long slot;
     if (!page_slot(a, page_index, slot)) return;
-    const long limit = row_limit(a, row);
     const long first = (long)g * a.group;
     const long end = min((long)a.page, first + a.group);
+    const long limit = min(row_limit(a, row), (long)page * a.page + end);
     const long in_page = first + (long)part * kPart + threadIdx.x * 4;
     const long col = (long)page * a.page + in_page;
     unsigned m = 0;
@@ -314,12 +368,11 @@ __global__ void __launch_bounds__(1024) quantize_part_kernel(const QuantizeArgs 
 #pragma unroll 4
     for (int j = 0; j < kPart / 4096; ++j) {
         const long c = in_page + j * 4096;
-        if (c >= end) break;
-        float4 v = load_sum<T, VEC>(a, row, col + j * 4096, limit - col - j * 4096);
+        float4 v = load_sum<T, VEC>(a, row, col + j * 4096, limit);
         if (WRITE) {
             const unsigned q = codes4(v, s);
-            *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
-            if (a.residual_out) store4<VEC>(a.residual_out + row * a.residual_stride + col + j * 4096, v, limit - col - j * 4096);
+            if (c < end) *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
+            store_lost<VEC>(a, row, col + j * 4096, v, limit);
         } else {
             m = max(m, most4(v));
         }
@@ -404,14 +457,14 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a,
             s[j] = __ldg(a.scales + slot * a.scale_stride + (c >> a.log_group));
         }
     }
-    T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride + col;
+    T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride;
+    const long limit = min(a.n_cols, (long)(page + 1) * a.page);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int c = in_page + j * 128;
-        if (c >= a.page) break;
         const float4 v = make_float4(s[j] * (float)(signed char)(q[j] & 255), s[j] * (float)(signed char)(q[j] >> 8 & 255),
                                      s[j] * (float)(signed char)(q[j] >> 16 & 255), s[j] * (float)(signed char)(q[j] >> 24));
-        store4<VEC>(out + j * 128, v, a.n_cols - col - j * 128);
+        if (VEC) store4<true>(out + col + j * 128, v, limit - col - j * 128);
+        else store_shifted(out, col + j * 128, v, limit);
     }
 }
 

@@ -282,7 +282,8 @@ def distances(codes, scales, slots, group):
 
 
 @pytest.mark.parametrize("n,pages,page", [(1, 1, 16), (2, 1, 32), (4, 7, 8192), (9, 3, 1008), (17, 2, 2048), (20, 5, 4096), (32, 1, 48), (33, 2, 512),
-                                          (70, 3, 1040), (100, 2, 4096)])
+                                          (70, 3, 1040), (100, 2, 4096), (5, 40, 8192), (64, 4, 2048), (97, 1, 1200), (100, 30, 8192), (70, 33, 8192), (40, 70, 8192), (56, 70, 8192), (20, 150, 8192), (128, 2, 1024), (130, 2, 1040),
+                                          (200, 1, 2048)])
 @pytest.mark.parametrize("group", [0, 32, 64, 128, 1024])
 def test_pair_distances(ctx, n, pages, page, group):
     import torch
