@@ -37,18 +37,6 @@ lib.lb_keyswitch_workspace_bytes.restype = C.c_size_t
 lib.lb_keyswitch_workspace_bytes.argtypes = [C.c_void_p, C.c_int]
 lib.lb_context_destroy.restype = None
 lib.lb_context_destroy.argtypes = [C.c_void_p]
-_i64, _ptr = C.c_int64, C.c_void_p
-lib.lb_quantize_rows_workspace_bytes.restype = C.c_size_t
-lib.lb_quantize_rows_workspace_bytes.argtypes = [_i64] * 4
-lib.lb_quantize_rows.argtypes = [_ptr, _ptr, C.c_int, _i64, _i64, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64,
-                                 _ptr, C.c_size_t, _ptr]
-lib.lb_dequantize_rows.argtypes = [_ptr, _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, C.c_int, _i64, _ptr]
-lib.lb_int8_matmul_workspace_bytes.restype = C.c_size_t
-lib.lb_int8_matmul_workspace_bytes.argtypes = [_i64, _i64, _i64, _ptr, _i64, _ptr, _i64]
-lib.lb_int8_matmul.argtypes = [_ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _i64, _ptr, _ptr, C.c_int, _i64, _ptr, C.c_size_t, _ptr]
-lib.lb_int8_distances_workspace_bytes.restype = C.c_size_t
-lib.lb_int8_distances_workspace_bytes.argtypes = [_ptr, _i64, _i64, _i64]
-lib.lb_int8_distances.argtypes = [_ptr, _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, C.c_size_t, _ptr]
 
 
 def check(code):

@@ -5,11 +5,12 @@ bit patterns of the ``uint64`` residues; torch only provides the memory and the 
 Every method forwards to exactly one ``lb_*`` entry point.
 """
 import ctypes as C
+import functools
 
 import numpy as np
 import torch
 
-from ._lib import LB_ERR_INVALID_ARG, InvalidArgument, check, lib
+from ._lib import check, lib
 
 _u64p = C.POINTER(C.c_uint64)
 
@@ -34,11 +35,13 @@ def to_host(t):
 
 
 VALUE_TYPES = {torch.float32: 1, torch.bfloat16: 3, torch.float16: 4}  # the value types of the 8-bit cache as the C ABI numbers them
-_INT8, _INT32, _FLOAT32 = (torch.int8,), (torch.int32,), (torch.float32,)
 
 
-def _invalid(message):
-    return InvalidArgument(LB_ERR_INVALID_ARG, message)
+@functools.lru_cache(None)
+def _updates8():
+    from .pybind import _updates8 as module  # built beside the library; there is no other path for these calls
+
+    return module
 
 
 def coeff_modulus_create(n, bit_sizes):
@@ -409,140 +412,27 @@ class Context:
         check(lib.lb_mask_accumulate(self.h, size_l, n, n_chunks, ptrs, C.c_size_t(2 * size_l * self.N), _p(masks), _p(out), self._stream()))
         return out
 
-    # -- 8-bit updates (the cache: codes [n_slots][page] int8, scales [n_slots][groups] float32).  Messages are put together only
-    # where a check fails: these calls may take less time on the GPU than formatting them takes on the host
-    def _on_device(self, t, dtypes, dims, what):
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == self.device):
-            raise _invalid("%s must be a tensor on cuda:%d" % (what, self.device))
-        if t.dtype not in dtypes or t.dim() != dims:
-            raise _invalid("%s must have %d dimension(s) and one of the types %s" % (what, dims, ", ".join(map(str, dtypes))))
-        if t.stride(-1) != 1 and t.shape[-1] > 1:
-            raise _invalid("%s must be dense along its rows" % what)
-
-    @staticmethod
-    def _row_stride(t):
-        """elements from one row to the next; a single row has none of its own"""
-        n, cols = t.shape
-        return t.stride(0) if n > 1 else max(t.stride(0), cols)
-
-    def _cache(self, codes, scales, group):
-        self._on_device(codes, _INT8, 2, "codes")
-        self._on_device(scales, _FLOAT32, 2, "scales")
-        n_slots, page = codes.shape
-        groups = -(-page // group) if 0 < group < page else 1
-        rows, cols = scales.shape
-        if rows < n_slots or cols < groups:
-            raise _invalid("scales must hold %d scale(s) for each of the %d slots" % (groups, n_slots))
-        return n_slots, page
-
-    def _pages(self, slots, n_rows, n_cols, page):
-        """address of the slots of n_rows rows"""
-        if slots is None:
-            return None
-        if not (isinstance(slots, torch.Tensor) and slots.is_cuda and slots.get_device() == self.device and slots.dtype == torch.int32
-                and slots.is_contiguous()):
-            raise _invalid("slots must be a contiguous int32 tensor on cuda:%d" % self.device)
-        pages = -(-n_cols // page) if page else 0
-        if slots.numel() != n_rows * pages:
-            raise _invalid("slots must name %d page(s) for each of the %d row(s)" % (pages, n_rows))
-        return slots.data_ptr()
-
-    def _result(self, out, rows, cols, dtype, device):
-        if out is None:
-            if dtype not in VALUE_TYPES:
-                raise _invalid("dtype must be one of %s" % ", ".join(map(str, VALUE_TYPES)))
-            return torch.empty((rows, cols), dtype=dtype, device=device)
-        self._on_device(out, VALUE_TYPES, 2, "out")
-        if tuple(out.shape) != (rows, cols):
-            raise _invalid("out must be [%d][%d]" % (rows, cols))
-        return out
-
-    def _raw_stream(self):
-        return torch._C._cuda_getCurrentRawStream(self.device)
-
+    # -- 8-bit updates (the cache: codes [n_slots][page] int8, scales [n_slots][groups] float32); arguments are checked by the
+    # extension module, see pybind/updates8.cpp
     def quantize_rows(self, values, codes, scales, group=0, slots=None, lengths=None, residual=None, residual_out=None):
         """values [n][cols] (float32, bfloat16, float16; rows may be strided) -> the cache's codes and scales (updated in place).
         A row covers ceil(cols / page) slots, page = codes.shape[1]; slots [n][pages] int32 names them (None: in order; one outside the
         cache is skipped; no slot may occur twice).  lengths [n] int32: columns of each row that count.  residual [n][cols] float32 is added
         first, residual_out (may be residual) gets what the rounding lost.  group: columns with one scale, 0 = the whole page"""
-        self._on_device(values, VALUE_TYPES, 2, "values")
-        n, cols = values.shape
-        n_slots, page = self._cache(codes, scales, group)
-        table = self._pages(slots, n, cols, page)
-        p_lengths = p_res = p_out = None
-        if lengths is not None:
-            self._on_device(lengths, _INT32, 1, "lengths")
-            if lengths.numel() != n:
-                raise _invalid("lengths must have one entry for each row")
-            p_lengths = lengths.data_ptr()
-        stride = 0
-        if residual is not None:
-            self._on_device(residual, _FLOAT32, 2, "residual")
-            stride, p_res = self._row_stride(residual), residual.data_ptr()
-        if residual_out is not None:
-            self._on_device(residual_out, _FLOAT32, 2, "residual_out")
-            if residual is not None and stride != self._row_stride(residual_out):
-                raise _invalid("residual and residual_out must have the same row stride")
-            stride, p_out = self._row_stride(residual_out), residual_out.data_ptr()
-        for t in (residual, residual_out):
-            if t is not None and t.shape != values.shape:
-                raise _invalid("a residual must have the shape of values")
-        need = lib.lb_quantize_rows_workspace_bytes(n, cols, page, group) if page > 32768 else 0
-        ws = torch.empty(need, dtype=torch.uint8, device=values.device) if need else None
-        check(lib.lb_quantize_rows(self.h, values.data_ptr(), VALUE_TYPES[values.dtype], n, cols, self._row_stride(values), p_lengths, p_res, p_out,
-                                   stride, table, n_slots, page, group, codes.data_ptr(), self._row_stride(codes), scales.data_ptr(),
-                                   self._row_stride(scales), None if ws is None else ws.data_ptr(), need, self._raw_stream()))
+        _updates8().quantize_rows(self.h.value, self.device, values, codes, scales, group, slots, lengths, residual, residual_out)
 
     def dequantize_rows(self, codes, scales, n_cols, group=0, slots=None, n_rows=None, dtype=torch.float32, out=None):
         """rows of n_cols values read back from the cache -> [n][n_cols] of dtype; slots as in quantize_rows (pages that are not in the
-        cache read as zeros).  n: the rows that slots names, else n_rows, else as many as the cache holds in order"""
-        n_slots, page = self._cache(codes, scales, group)
-        if n_rows is None:
-            if out is not None:
-                n_rows = out.shape[0]
-            else:
-                n_rows = (n_slots if slots is None else slots.numel()) // max(-(-n_cols // page) if page else 0, 1)
-        table = self._pages(slots, n_rows, n_cols, page)
-        out = self._result(out, n_rows, n_cols, dtype, codes.device)
-        check(lib.lb_dequantize_rows(self.h, codes.data_ptr(), self._row_stride(codes), scales.data_ptr(), self._row_stride(scales), n_slots,
-                                     page, group, table, n_rows, n_cols, out.data_ptr(), VALUE_TYPES[out.dtype], self._row_stride(out),
-                                     self._raw_stream()))
-        return out
+        cache read as zeros).  n: n_rows, else the rows of out, else those that slots names, else as many as the cache holds in order"""
+        return _updates8().dequantize_rows(self.h.value, self.device, codes, scales, n_cols, group, slots, n_rows, VALUE_TYPES.get(dtype, 0), out)
 
     def int8_matmul(self, a, b, a_scale, b_scale, dtype=torch.bfloat16, out=None):
         """a [m][k], b [n][k] int8, a_scale [m], b_scale [n] float32 -> [m][n]: (a b^T) * a_scale[:, None] * b_scale, the sum an exact integer"""
-        self._on_device(a, _INT8, 2, "a")
-        self._on_device(b, _INT8, 2, "b")
-        (m, k), (n, kb) = a.shape, b.shape
-        if k != kb:
-            raise _invalid("a and b must have rows of the same length")
-        self._on_device(a_scale, _FLOAT32, 1, "a_scale")
-        self._on_device(b_scale, _FLOAT32, 1, "b_scale")
-        if a_scale.numel() != m or b_scale.numel() != n:
-            raise _invalid("a scale must have one entry for each row of its operand")
-        out = self._result(out, m, n, dtype, a.device)
-        pa, pb, sa, sb = a.data_ptr(), b.data_ptr(), self._row_stride(a), self._row_stride(b)
-        need = lib.lb_int8_matmul_workspace_bytes(m, n, k, pa, sa, pb, sb)
-        ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
-        check(lib.lb_int8_matmul(self.h, m, n, k, pa, sa, a_scale.data_ptr(), pb, sb, b_scale.data_ptr(), out.data_ptr(), VALUE_TYPES[out.dtype],
-                                 self._row_stride(out), None if ws is None else ws.data_ptr(), need, self._raw_stream()))
-        return out
+        return _updates8().int8_matmul(self.h.value, self.device, a, b, a_scale, b_scale, VALUE_TYPES.get(dtype, 0), out)
 
     def int8_distances(self, codes, scales, slots, group=0):
         """squared distances between all pairs of cached rows: slots [n][pages] int32 -> [n][n] float64 (0 on the diagonal)"""
-        n_slots, page = self._cache(codes, scales, group)
-        self._on_device(slots, _INT32, 2, "slots")
-        if not slots.is_contiguous():
-            raise _invalid("slots must be contiguous")
-        n, pages = slots.shape
-        device = codes.device
-        out = torch.empty((n, n), dtype=torch.float64, device=device)
-        need = lib.lb_int8_distances_workspace_bytes(self.h, n, pages, page)
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        check(lib.lb_int8_distances(self.h, codes.data_ptr(), self._row_stride(codes), scales.data_ptr(), self._row_stride(scales), n_slots,
-                                    page, group, slots.data_ptr(), n, pages, out.data_ptr(), None if ws is None else ws.data_ptr(), need,
-                                    self._raw_stream()))
-        return out
+        return _updates8().int8_distances(self.h.value, self.device, codes, scales, slots, group)
 
     def check_status(self):
         check(lib.lb_check_status(self.h, self._stream()))

@@ -1,7 +1,8 @@
-"""Builds the ``pyCAHEL`` extension module (binding.cpp) in this folder with the host compiler.
+"""Builds the extension modules in this folder with the host compiler.
 
-The module is what lancelot-main-GPU imports (``import pyCAHEL as cahel``): put this folder on PYTHONPATH.
-It links ``../liblancelot_b200.so`` (found at run time relative to the module) and the CUDA runtime."""
+``pyCAHEL`` (binding.cpp) is what lancelot-main-GPU imports (``import pyCAHEL as cahel``): put this folder on PYTHONPATH.
+It links ``../liblancelot_b200.so`` (found at run time relative to the module) and the CUDA runtime.
+``_updates8`` (updates8.cpp) holds the 8-bit update calls of ``cabi.Context``; it links torch's C++ libraries as well."""
 import os
 import subprocess
 import sys
@@ -12,28 +13,41 @@ PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 
 
-def target():
-    return os.path.join(HERE, "pyCAHEL" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+def target(module="pyCAHEL"):
+    return os.path.join(HERE, module + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
-def build(force=False):
-    import pybind11
-
-    out = target()
-    deps = [os.path.join(HERE, "binding.cpp"), os.path.join(ROOT, "include", "cahel_b200.hpp"), os.path.join(ROOT, "include", "lancelot_b200.h")]
+def _compile(module, deps, flags, force):
+    out = target(module)
     if not force and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in deps):
         return out
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cxx = os.environ.get("CXX", "g++")
     cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           "-I" + pybind11.get_include(), "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(ROOT, "include"),
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(ROOT, "include"),
            "-I" + os.path.join(cuda, "include"), deps[0], "-o", out + ".tmp",
            "-L" + PKG, "-llancelot_b200", "-L" + os.path.join(cuda, "lib64"), "-lcudart",
-           "-Wl,-rpath,$ORIGIN/..", "-Wl,-rpath," + os.path.join(cuda, "lib64")]
+           "-Wl,-rpath,$ORIGIN/..", "-Wl,-rpath," + os.path.join(cuda, "lib64")] + flags
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("building pyCAHEL failed: %s\n%s" % (" ".join(cmd), r.stderr))
+        raise RuntimeError("building %s failed: %s\n%s" % (module, " ".join(cmd), r.stderr))
     os.replace(out + ".tmp", out)
+    return out
+
+
+def build(force=False):
+    import pybind11
+    import torch
+
+    header = os.path.join(ROOT, "include", "lancelot_b200.h")
+    out = _compile("pyCAHEL", [os.path.join(HERE, "binding.cpp"), os.path.join(ROOT, "include", "cahel_b200.hpp"), header],
+                   ["-I" + pybind11.get_include()], force)
+    site = os.path.dirname(torch.__file__)
+    lib = os.path.join(site, "lib")
+    _compile("_updates8", [os.path.join(HERE, "updates8.cpp"), header],
+             ["-I" + os.path.join(site, "include"), "-I" + os.path.join(site, "include", "torch", "csrc", "api", "include"),
+              "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-L" + lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+              "-ltorch_python", "-Wl,-rpath," + lib], force)
     return out
 
 
