@@ -6,12 +6,13 @@
 // The reference has no 8-bit form of an update: its driver holds every client's values in the clear as lists of doubles
 // (lancelot-main-GPU/utils/byzantine_fl.py:478-490).
 //
-// The nearest integer is found without a division.  q0 = rint(t * (1 / s)) is off by at most one, and only next to a border
+// The nearest integer is found without a division.  q0 = t * (1 / s), rounded, is off by at most one, and only next to a border
 // between two codes; r = fma(-q0, s, t) is exact there (both terms are multiples of the smaller of their units in the last
 // place, and |r| is about s / 2, so it has at most 24 bits), and comparing 2 |r| with s settles the border, ties included.
 // The same r is what the rounding lost, exactly: error feedback adds no error of its own.
 //
 // All kernels stream: bound by HBM at (value bytes + 1 + 8 with a residual) per value.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -23,10 +24,8 @@ namespace {
 
 constexpr unsigned kInfBits = 0x7f800000u;
 
-__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
 // Four consecutive values as 32-bit floats.  `valid`: how many of them lie inside the row (<= 0: none)
-template <bool VEC> __device__ __forceinline__ float4 load4(const float *p, long valid)
+template <bool VEC> __device__ __forceinline__ float4 load4(const float *p, int valid)
 {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (VEC && valid >= 4) return __ldcs(reinterpret_cast<const float4 *>(p));
@@ -36,7 +35,7 @@ template <bool VEC> __device__ __forceinline__ float4 load4(const float *p, long
     if (valid > 3) v.w = __ldcs(p + 3);
     return v;
 }
-template <bool VEC> __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p, long valid)
+template <bool VEC> __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p, int valid)
 {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (VEC && valid >= 4) {
@@ -50,7 +49,7 @@ template <bool VEC> __device__ __forceinline__ float4 load4(const __nv_bfloat16 
     if (valid > 3) v.w = __bfloat162float(p[3]);
     return v;
 }
-template <bool VEC> __device__ __forceinline__ float4 load4(const __half *p, long valid)
+template <bool VEC> __device__ __forceinline__ float4 load4(const __half *p, int valid)
 {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (VEC && valid >= 4) {
@@ -66,7 +65,7 @@ template <bool VEC> __device__ __forceinline__ float4 load4(const __half *p, lon
     return v;
 }
 
-template <bool VEC> __device__ __forceinline__ void store4(float *p, float4 v, long valid)
+template <bool VEC> __device__ __forceinline__ void store4(float *p, float4 v, int valid)
 {
     if (VEC && valid >= 4) {
         __stcs(reinterpret_cast<float4 *>(p), v);
@@ -77,7 +76,7 @@ template <bool VEC> __device__ __forceinline__ void store4(float *p, float4 v, l
     if (valid > 2) p[2] = v.z;
     if (valid > 3) p[3] = v.w;
 }
-template <bool VEC> __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v, long valid)
+template <bool VEC> __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v, int valid)
 {
     if (VEC && valid >= 4) {
         __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
@@ -89,7 +88,7 @@ template <bool VEC> __device__ __forceinline__ void store4(__nv_bfloat16 *p, flo
     if (valid > 2) p[2] = __float2bfloat16_rn(v.z);
     if (valid > 3) p[3] = __float2bfloat16_rn(v.w);
 }
-template <bool VEC> __device__ __forceinline__ void store4(__half *p, float4 v, long valid)
+template <bool VEC> __device__ __forceinline__ void store4(__half *p, float4 v, int valid)
 {
     if (VEC && valid >= 4) {
         __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
@@ -102,51 +101,35 @@ template <bool VEC> __device__ __forceinline__ void store4(__half *p, float4 v, 
     if (valid > 3) p[3] = __float2half_rn(v.w);
 }
 
-// Rows that start off a 16-byte boundary (an odd number of values a row is the rule for updates).  The warp's run of columns
-// is still contiguous, so it moves in aligned pieces and the lanes hand the values on to where they belong: `off` values of a piece
-// belong to the lane before.  All 32 lanes take part; lane l stands for columns col .. col + 3, col = (lane 0's) + 4 l.  Only values with
-// 0 <= column < limit are touched.
-template <typename T> __device__ __forceinline__ float4 load_piece(const T *row, long at, long limit)
+// Four values at positions at .. at + 3 of a run, of which only [lo, hi) exist or are wanted
+template <bool VEC, typename T> __device__ __forceinline__ float4 load_piece(const T *p, int at, int lo, int hi)
 {
-    if (at >= 0 && at + 4 <= limit) return load4<true>(row + at, 4);
+    if (VEC && at >= lo && at + 4 <= hi) return load4<true>(p + at, 4);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (at >= 0 && at < limit) v.x = (float)row[at];
-    if (at + 1 >= 0 && at + 1 < limit) v.y = (float)row[at + 1];
-    if (at + 2 >= 0 && at + 2 < limit) v.z = (float)row[at + 2];
-    if (at + 3 >= 0 && at + 3 < limit) v.w = (float)row[at + 3];
+    if (at >= lo && at < hi) v.x = (float)p[at];
+    if (at + 1 >= lo && at + 1 < hi) v.y = (float)p[at + 1];
+    if (at + 2 >= lo && at + 2 < hi) v.z = (float)p[at + 2];
+    if (at + 3 >= lo && at + 3 < hi) v.w = (float)p[at + 3];
     return v;
 }
-template <typename T> __device__ __forceinline__ float4 load_shifted(const T *row, long col, long limit)
+__device__ __forceinline__ void set(float *p, float v) { *p = v; }
+__device__ __forceinline__ void set(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void set(__half *p, float v) { *p = __float2half_rn(v); }
+template <bool VEC, typename T> __device__ __forceinline__ void store_piece(T *p, int at, const float4 &v, int lo, int hi)
 {
-    const int off = (int)((uintptr_t)(row + col) / sizeof(T)) & 3;
-    const float4 a = load_piece(row, col - off, limit);
-    if (off == 0) return a;
-    float4 next = make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool last = (threadIdx.x & 31) == 31;
-    if (last) next = load_piece(row, col - off + 4, limit);
-    const float x = __shfl_down_sync(0xffffffffu, a.x, 1), y = __shfl_down_sync(0xffffffffu, a.y, 1), z = __shfl_down_sync(0xffffffffu, a.z, 1);
-    if (!last) next = make_float4(x, y, z, 0.f);
-    if (off == 1) return make_float4(a.y, a.z, a.w, next.x);
-    if (off == 2) return make_float4(a.z, a.w, next.x, next.y);
-    return make_float4(a.w, next.x, next.y, next.z);
-}
-template <typename T> __device__ __forceinline__ void store_shifted(T *row, long col, float4 v, long limit)
-{
-    const int off = (int)((uintptr_t)(row + col) / sizeof(T)) & 3;
-    if (off == 0) {
-        store4<true>(row + col, v, limit - col);
+    if (VEC && at >= lo && at + 4 <= hi) {
+        store4<true>(p + at, v, 4);
         return;
     }
-    const float y = __shfl_up_sync(0xffffffffu, v.y, 1), z = __shfl_up_sync(0xffffffffu, v.z, 1), w = __shfl_up_sync(0xffffffffu, v.w, 1);
-    const int lane = threadIdx.x & 31;
-    const float4 piece = off == 1 ? make_float4(w, v.x, v.y, v.z) : off == 2 ? make_float4(z, w, v.x, v.y) : make_float4(y, z, w, v.x);
-    if (lane == 0) store4<false>(row + col, v, min(limit - col, 4L - off)); // the rest of the piece is not this warp's
-    else store4<true>(row + col - off, piece, limit - col + off);
-    if (lane == 31) {
-        const float4 rest = off == 1 ? make_float4(v.w, 0.f, 0.f, 0.f) : off == 2 ? make_float4(v.z, v.w, 0.f, 0.f) : make_float4(v.y, v.z, v.w, 0.f);
-        store4<false>(row + col + 4 - off, rest, min(limit - col - 4 + off, (long)off));
-    }
+    if (at >= lo && at < hi) set(p + at, v.x);
+    if (at + 1 >= lo && at + 1 < hi) set(p + at + 1, v.y);
+    if (at + 2 >= lo && at + 2 < hi) set(p + at + 2, v.z);
+    if (at + 3 >= lo && at + 3 < hi) set(p + at + 3, v.w);
 }
+template <typename T> __device__ __forceinline__ int offset_of(const T *p) { return (int)((uintptr_t)p / sizeof(T)) & 3; }
+// the first n elements, or those from n on; the others 0
+__device__ __forceinline__ float4 first_of(const float4 &v, int n) { return make_float4(n > 0 ? v.x : 0.f, n > 1 ? v.y : 0.f, n > 2 ? v.z : 0.f, n > 3 ? v.w : 0.f); }
+__device__ __forceinline__ float4 from_of(const float4 &v, int n) { return make_float4(n > 0 ? 0.f : v.x, n > 1 ? 0.f : v.y, n > 2 ? 0.f : v.z, n > 3 ? 0.f : v.w); }
 
 // The scale of a group from the bits of its largest magnitude.  The bit patterns of magnitudes are ordered like the magnitudes
 // with infinities and NaN above all numbers, so an integer maximum carries them along: such a group gets NaN
@@ -155,53 +138,78 @@ __device__ __forceinline__ float scale_of(unsigned most)
     return most >= kInfBits ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(most), 127.0f);
 }
 
-// the code of t in a group of scale s (inv = 1 / s); t <- what the rounding lost
-__device__ __forceinline__ int code_of(float &t, float s, float inv)
+// Codes of four values in a group of scale s (inv = 1 / s), packed; v <- what the rounding lost.  Adding 1.5 * 2^23 rounds a
+// product to an integer, ties to even, and leaves its last eight bits as the code.
+constexpr float kMagic = 12582912.0f;
+__device__ __forceinline__ void settle(float &y, float &t, float r, float s) // the neighbour on the side of r, past the border, or on it from an odd code
 {
-    float q = rintf(t * inv);
-    float r = fmaf(-q, s, t);
     const float twice = fabsf(r + r);
-    // past the border, or on it with an odd code: the neighbour on the side of r
-    if (twice > s || (twice == s && ((int)q & 1))) {
-        q += copysignf(1.0f, r);
-        r = fmaf(-q, s, t);
+    if (twice > s || (twice == s && (__float_as_int(y) & 1))) {
+        y += copysignf(1.0f, r);
+        r = fmaf(-(y - kMagic), s, t);
     }
     t = r;
-    return (int)q;
 }
-// Groups without a normal scale: empty (0), not finite (NaN), or so small that 1 / s overflows and the rounding of s itself
-// moves codes past 127; a quotient of 64 bits decides a border between 32-bit numbers rightly
-__device__ __noinline__ float2 code_of_odd(float t, float s) // (code, what was lost)
+__device__ __forceinline__ unsigned codes4_normal(float4 &v, const float4 &s, const float4 &inv)
 {
-    if (!(s > 0.0f)) return make_float2(0.0f, s == s ? t : 0.0f);
+    float a = fmaf(v.x, inv.x, kMagic), b = fmaf(v.y, inv.y, kMagic), c = fmaf(v.z, inv.z, kMagic), d = fmaf(v.w, inv.w, kMagic);
+    const float p = fmaf(kMagic - a, s.x, v.x), q = fmaf(kMagic - b, s.y, v.y), r = fmaf(kMagic - c, s.z, v.z), u = fmaf(kMagic - d, s.w, v.w);
+    if (fabsf(p + p) >= s.x || fabsf(q + q) >= s.y || fabsf(r + r) >= s.z || fabsf(u + u) >= s.w) { // seldom: one of the four lies next to a border
+        settle(a, v.x, p, s.x);
+        settle(b, v.y, q, s.y);
+        settle(c, v.z, r, s.z);
+        settle(d, v.w, u, s.w);
+    } else {
+        v = make_float4(p, q, r, u);
+    }
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+}
+// Groups whose scale is below the normal numbers: 1 / s overflows, and the rounding of s itself moves codes past 127.  A quotient of
+// 64 bits decides a border between 32-bit numbers rightly
+__device__ __noinline__ float2 code_of_tiny(float t, float s) // (code, what was lost)
+{
     const double q = fmin(fmax(rint((double)t / (double)s), -127.0), 127.0);
     return make_float2((float)q, (float)((double)t - q * (double)s));
 }
-
-// codes of four values, packed; v <- what was lost
 __device__ __forceinline__ unsigned codes4(float4 &v, float s)
 {
-    int a, b, c, d;
     if (s >= 1.17549435e-38f) {
         const float inv = __frcp_rn(s);
-        a = code_of(v.x, s, inv);
-        b = code_of(v.y, s, inv);
-        c = code_of(v.z, s, inv);
-        d = code_of(v.w, s, inv);
-    } else {
-        const float2 x = code_of_odd(v.x, s), y = code_of_odd(v.y, s), z = code_of_odd(v.z, s), w = code_of_odd(v.w, s);
-        v = make_float4(x.y, y.y, z.y, w.y);
-        a = (int)x.x;
-        b = (int)y.x;
-        c = (int)z.x;
-        d = (int)w.x;
+        return codes4_normal(v, make_float4(s, s, s, s), make_float4(inv, inv, inv, inv));
     }
-    return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)d << 24;
+    if (!(s > 0.0f)) { // an empty group, or one that is not finite
+        if (s != s) v = make_float4(0.f, 0.f, 0.f, 0.f);
+        return 0;
+    }
+    const float2 x = code_of_tiny(v.x, s), y = code_of_tiny(v.y, s), z = code_of_tiny(v.z, s), w = code_of_tiny(v.w, s);
+    v = make_float4(x.y, y.y, z.y, w.y);
+    return ((unsigned)(int)x.x & 255) | ((unsigned)(int)y.x & 255) << 8 | ((unsigned)(int)z.x & 255) << 16 | (unsigned)(int)w.x << 24;
+}
+// the first `off` of the four belong to the group before, of scale `before`
+__device__ __forceinline__ unsigned codes4_across(float4 &v, float before, float s, int off)
+{
+    if (before >= 1.17549435e-38f && s >= 1.17549435e-38f) {
+        const float i = __frcp_rn(before), j = __frcp_rn(s);
+        return codes4_normal(v, make_float4(off > 0 ? before : s, off > 1 ? before : s, off > 2 ? before : s, s),
+                             make_float4(off > 0 ? i : j, off > 1 ? i : j, off > 2 ? i : j, j));
+    }
+    float4 head = first_of(v, off);
+    v = from_of(v, off);
+    const unsigned mask = (1u << 8 * off) - 1, q = codes4(head, before) & mask, r = codes4(v, s) & ~mask;
+    v = make_float4(off > 0 ? head.x : v.x, off > 1 ? head.y : v.y, off > 2 ? head.z : v.z, v.w);
+    return q | r;
 }
 
+// the largest magnitude, NaN if one is NaN
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
 __device__ __forceinline__ unsigned most4(const float4 &v)
 {
-    return max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
+    return __float_as_uint(max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)))) & 0x7fffffffu;
 }
 
 struct QuantizeArgs {
@@ -233,52 +241,77 @@ __device__ __forceinline__ long row_limit(const QuantizeArgs &a, long row)
     return a.lengths ? min((long)max(a.lengths[row], 0), a.n_cols) : a.n_cols;
 }
 
-// t for columns col .. col + 3 of a row, 0 from column `limit` on.  VEC: all rows start on the boundary of a vector
-template <typename T, bool VEC> __device__ __forceinline__ float4 load_sum(const QuantizeArgs &a, long row, long col, long limit)
+// A run of columns of one row, as its warps see it.  Rows seldom start on a 16-byte boundary (an update has an odd number of values as
+// often as not), so the values move in aligned pieces of four that begin `off` columns early: piece i holds the columns 4 i - off to
+// 4 i + 3 - off of the run.  A piece across the border of two groups is rounded with both scales, and the codes, which are aligned to
+// the columns, are put together from two pieces.  VEC: values and residuals have the same offset; otherwise off is 0 and everything
+// moves value by value.
+template <typename T> struct Run {
+    const T *values;
+    const float *residual;
+    float *lost;
+    int off;
+    int hi;    // columns [0, hi) exist
+    bool full; // the whole run does, and the row goes on by a piece on either side
+};
+template <typename T, bool VEC> __device__ __forceinline__ Run<T> run_of(const QuantizeArgs &a, long row, long col, long limit, int length)
 {
-    const T *values = reinterpret_cast<const T *>(a.values) + row * a.value_stride;
-    float4 v = VEC ? load4<true>(values + col, limit - col) : load_shifted(values, col, limit);
-    if (a.residual) {
-        const float *res = a.residual + row * a.residual_stride;
-        const float4 r = VEC ? load4<true>(res + col, limit - col) : load_shifted(res, col, limit);
-        v.x += r.x;
-        v.y += r.y;
-        v.z += r.z;
-        v.w += r.w;
+    Run<T> r;
+    r.values = reinterpret_cast<const T *>(a.values) + row * a.value_stride + col;
+    r.residual = a.residual ? a.residual + row * a.residual_stride + col : nullptr;
+    r.lost = a.residual_out ? a.residual_out + row * a.residual_stride + col : nullptr;
+    r.off = VEC ? offset_of(r.values) : 0;
+    r.hi = (int)max(0l, min(limit - col, 1l << 30));
+    r.full = VEC && r.hi >= length && (r.off == 0 || (col >= 4 && col + length + 4 <= a.n_cols));
+    return r;
+}
+template <bool FULL, bool VEC, typename T> __device__ __forceinline__ float4 load_sum(const Run<T> &r, int at)
+{
+    float4 v = FULL ? load4<true>(r.values + at, 4) : load_piece<VEC>(r.values, at, 0, r.hi);
+    if (r.residual) {
+        const float4 w = FULL ? load4<true>(r.residual + at, 4) : load_piece<VEC>(r.residual, at, 0, r.hi);
+        v.x += w.x;
+        v.y += w.y;
+        v.z += w.z;
+        v.w += w.w;
     }
     return v;
 }
-template <bool VEC> __device__ __forceinline__ void store_lost(const QuantizeArgs &a, long row, long col, const float4 &v, long limit)
-{
-    if (!a.residual_out) return;
-    float *out = a.residual_out + row * a.residual_stride;
-    if (VEC) store4<true>(out + col, v, limit - col);
-    else store_shifted(out, col, v, limit);
-}
 
-// ---- groups of 32 to 512 columns: a warp takes 512 columns, four of each lane's values side by side -------------------
-// Every load and store of a warp is one contiguous run (512 bytes of 32-bit values, 128 bytes of codes); a group's maximum
-// never leaves the warp.
-template <typename T, bool VEC, int LOG_G>
-__global__ void __launch_bounds__(256) quantize_warp_kernel(const QuantizeArgs a, const unsigned tiles, const unsigned total)
+// ---- groups of 32 to 512 columns: a warp takes 512 columns ------------------------------------------------------------
+// Every load and store of a warp is one contiguous run (512 bytes of 32-bit values, 128 bytes of codes); a group's maximum never
+// leaves the warp.
+template <typename T, bool VEC, int LOG_G, bool FULL>
+__device__ __forceinline__ void quantize_tile(const Run<T> &r, signed char *codes, float *scales, int in_page, int page)
 {
-    const unsigned w = blockIdx.x * 8u + (threadIdx.x >> 5);
-    if (w >= total) return;
-    const int lane = threadIdx.x & 31;
-    const unsigned page_index = w / tiles, tile = w - page_index * tiles;
-    const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
-    long slot;
-    if (!page_slot(a, page_index, slot)) return;
-    const long limit = min(row_limit(a, row), (long)(page + 1) * a.page);
-    const int in_page = tile * 512 + lane * 4;
-    const long col = (long)page * a.page + in_page;
-    float4 v[4];
-    unsigned m[4];
+    const int lane = threadIdx.x & 31, off = r.off, first = lane * 4 - off;
+    float4 v[4], last = make_float4(0.f, 0.f, 0.f, 0.f); // of lane 0: the end of the run
+    unsigned m[4], q[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = load_sum<T, VEC>(a, row, col + j * 128, limit);
+    for (int j = 0; j < 4; ++j) v[j] = load_sum<FULL, VEC>(r, first + j * 128);
+    if (off) {
+        if (lane == 0) {
+            last = first_of(load_sum<FULL, VEC>(r, 512 - off), off);
+            v[0] = from_of(v[0], off);
+        }
+        unsigned head[5];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            head[j] = most4(first_of(v[j], off));
+            m[j] = most4(from_of(v[j], off));
+        }
+        head[4] = most4(last);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { // the columns of a lane: the rest of its piece and the head of the next lane's
+            const unsigned next = __shfl_down_sync(0xffffffffu, head[j], 1), wrap = __shfl_sync(0xffffffffu, head[j + 1], 0);
+            m[j] = max(m[j], lane == 31 ? wrap : next);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] = most4(v[j]);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        m[j] = most4(v[j]);
         if (LOG_G >= 7) {
             m[j] = __reduce_max_sync(0xffffffffu, m[j]);
         } else {
@@ -293,52 +326,145 @@ __global__ void __launch_bounds__(256) quantize_warp_kernel(const QuantizeArgs a
         m[2] = m[3] = max(m[2], m[3]);
     }
     if (LOG_G >= 9) m[0] = m[1] = m[2] = m[3] = max(m[0], m[2]);
+    float s[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int c = in_page + j * 128;
-        const float s = scale_of(m[j]);
-        const unsigned q = codes4(v[j], s);
-        if (c < a.page) {
-            if ((c & ((1 << LOG_G) - 1)) == 0) a.scales[slot * a.scale_stride + (c >> LOG_G)] = s;
-            *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
-        }
-        store_lost<VEC>(a, row, col + j * 128, v[j], limit);
+        s[j] = scale_of(m[j]);
+        const int c = in_page + lane * 4 + j * 128;
+        if (c < page && (c & ((1 << LOG_G) - 1)) == 0) scales[c >> LOG_G] = s[j];
     }
+    if (off) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float before = __shfl_up_sync(0xffffffffu, s[j], 1);
+            const float wrap = __shfl_sync(0xffffffffu, s[j > 0 ? j - 1 : 0], 31);
+            if (lane == 0) before = wrap;
+            q[j] = codes4_across(v[j], before, s[j], off);
+        }
+        const float end = __shfl_sync(0xffffffffu, s[3], 31);
+        unsigned tail = 0;
+        if (lane == 0) tail = codes4(last, end);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned next = __shfl_down_sync(0xffffffffu, q[j], 1), wrap = __shfl_sync(0xffffffffu, j < 3 ? q[j < 3 ? j + 1 : 3] : tail, 0);
+            q[j] = __funnelshift_r(q[j], lane == 31 ? wrap : next, 8 * off);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = codes4(v[j], s[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int c = lane * 4 + j * 128;
+        if (in_page + c < page) *reinterpret_cast<unsigned *>(codes + c) = q[j];
+    }
+    if (!r.lost) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (FULL && (j > 0 || off == 0 || lane > 0)) store4<true>(r.lost + first + j * 128, v[j], 4);
+        else store_piece<VEC>(r.lost, first + j * 128, v[j], 0, r.hi);
+    }
+    if (off && lane == 0) store_piece<false>(r.lost, 512 - off, last, 0, min(r.hi, 512));
 }
 
-// ---- groups of up to 32768 columns: a block holds the group in registers ----------------------------------------------
-template <typename T, bool VEC, int THREADS, int V>
-__global__ void __launch_bounds__(THREADS) quantize_block_kernel(const QuantizeArgs a)
+template <typename T, bool VEC, int LOG_G>
+__global__ void __launch_bounds__(256) quantize_warp_kernel(const QuantizeArgs a, const unsigned tiles, const unsigned total)
 {
-    __shared__ unsigned warp_most[32];
-    const unsigned page_index = blockIdx.x / (unsigned)a.groups, g = blockIdx.x - page_index * (unsigned)a.groups;
+    const unsigned w = blockIdx.x * 8u + (threadIdx.x >> 5);
+    if (w >= total) return;
+    const unsigned page_index = w / tiles, tile = w - page_index * tiles;
     const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
     long slot;
     if (!page_slot(a, page_index, slot)) return;
-    const int first = g * a.group, end = min(a.page, first + a.group); // columns of the group inside the page
-    const long limit = min(row_limit(a, row), (long)page * a.page + end);
-    const int in_page = first + threadIdx.x * 4;
-    const long col = (long)page * a.page + in_page;
-    float4 v[V];
-    unsigned m = 0;
+    const long limit = min(row_limit(a, row), (long)(page + 1) * a.page), col = (long)page * a.page + tile * 512;
+    const Run<T> r = run_of<T, VEC>(a, row, col, limit, 512);
+    signed char *codes = a.codes + slot * a.code_stride + tile * 512;
+    float *scales = a.scales + slot * a.scale_stride;
+    if (r.full) quantize_tile<T, VEC, LOG_G, true>(r, codes, scales, tile * 512, a.page);
+    else quantize_tile<T, VEC, LOG_G, false>(r, codes, scales, tile * 512, a.page);
+}
+
+// ---- groups of up to 65536 columns: a block, or a cluster of blocks, holds the group in registers ---------------------
+// A block of 256 threads holds 8192 columns.  One of 1024 threads for 32768 columns would be alone on its SM, and all of it would wait for
+// its loads, then compute, then store; the blocks of a cluster do these at different times from those of others on the SM.
+template <int V> struct GroupShared {
+    unsigned most[32 + 8]; // of the warps; of the cluster's blocks
+    unsigned heads[V * 8 + 1]; // the first codes of every warp's pieces, in the order of their columns
+};
+template <typename T, bool VEC, int V, bool FULL>
+__device__ __forceinline__ void quantize_group(const Run<T> &r, signed char *codes, float *scale, int length, GroupShared<V> &shared, bool leader, int peers)
+{
+    constexpr int kThreads = 256, kRun = kThreads * V * 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, off = r.off, first = threadIdx.x * 4 - off;
+    float4 v[V], last = make_float4(0.f, 0.f, 0.f, 0.f); // of thread 0: the end of the run
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = load_sum<T, VEC>(a, row, col + j * THREADS * 4, limit);
+    for (int j = 0; j < V; ++j) v[j] = load_sum<FULL, VEC>(r, first + j * kThreads * 4);
+    if (off && threadIdx.x == 0) {
+        last = first_of(load_sum<FULL, VEC>(r, kRun - off), off);
+        v[0] = from_of(v[0], off);
+    }
+    unsigned m = most4(last);
 #pragma unroll
     for (int j = 0; j < V; ++j) m = max(m, most4(v[j]));
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = m;
+    if (lane == 0) shared.most[warp] = m;
     __syncthreads();
-    m = (threadIdx.x & 31) < THREADS / 32 ? warp_most[threadIdx.x & 31] : 0;
-    m = __reduce_max_sync(0xffffffffu, m);
+    m = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? shared.most[lane] : 0);
+    if (peers > 1) { // the other blocks' maxima, by way of their shared memory
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // all of them have begun
+        if (threadIdx.x < (unsigned)peers) *cluster.map_shared_rank(shared.most + 32 + cluster.block_rank(), threadIdx.x) = m;
+        cluster.sync();
+        m = __reduce_max_sync(0xffffffffu, lane < peers ? shared.most[32 + lane] : 0);
+    }
     const float s = scale_of(m);
-    if (threadIdx.x == 0) a.scales[slot * a.scale_stride + g] = s;
+    if (leader && threadIdx.x == 0) *scale = s;
+    unsigned q[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) q[j] = codes4(v[j], s);
+    if (off) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (lane == 0) shared.heads[j * 8 + warp] = q[j];
+        if (threadIdx.x == 0) shared.heads[V * 8] = codes4(last, s);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const unsigned next = __shfl_down_sync(0xffffffffu, q[j], 1);
+            q[j] = __funnelshift_r(q[j], lane == 31 ? shared.heads[j * 8 + warp + 1] : next, 8 * off);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = in_page + j * THREADS * 4;
-        const unsigned q = codes4(v[j], s);
-        if (c < end) *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
-        store_lost<VEC>(a, row, col + j * THREADS * 4, v[j], limit);
+        const int c = threadIdx.x * 4 + j * kThreads * 4;
+        if (c < length) *reinterpret_cast<unsigned *>(codes + c) = q[j];
     }
+    if (!r.lost) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (FULL && (j > 0 || off == 0 || threadIdx.x > 0)) store4<true>(r.lost + first + j * kThreads * 4, v[j], 4);
+        else store_piece<VEC>(r.lost, first + j * kThreads * 4, v[j], 0, r.hi);
+    }
+    if (off && threadIdx.x == 0) store_piece<false>(r.lost, kRun - off, last, 0, min(r.hi, kRun));
+}
+
+template <typename T, bool VEC, int V> __global__ void __launch_bounds__(256, V == 4 ? 4 : 2) quantize_block_kernel(const QuantizeArgs a, const int peers)
+{
+    __shared__ GroupShared<V> shared;
+    const unsigned group_index = blockIdx.x / peers, peer = blockIdx.x - group_index * peers;
+    const unsigned page_index = group_index / (unsigned)a.groups, g = group_index - page_index * (unsigned)a.groups;
+    const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
+    long slot;
+    if (!page_slot(a, page_index, slot)) return; // all blocks of a cluster alike
+    if (peers > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); // nothing has been written yet
+    constexpr int kRun = 256 * V * 4;
+    const int first = g * a.group + peer * kRun, end = min(a.page, (int)(g + 1) * a.group); // columns inside the page
+    const long limit = min(row_limit(a, row), (long)page * a.page + end), col = (long)page * a.page + first;
+    const Run<T> r = run_of<T, VEC>(a, row, col, limit, kRun);
+    signed char *codes = a.codes + slot * a.code_stride + first;
+    float *scale = a.scales + slot * a.scale_stride + g;
+    if (r.full) quantize_group<T, VEC, V, true>(r, codes, scale, end - first, shared, peer == 0, peers);
+    else quantize_group<T, VEC, V, false>(r, codes, scale, end - first, shared, peer == 0, peers);
 }
 
 // ---- longer groups: the maxima of parts of 32768 columns first, then the codes -----------------------------------------
@@ -353,11 +479,10 @@ __global__ void __launch_bounds__(1024) quantize_part_kernel(const QuantizeArgs 
     const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
     long slot;
     if (!page_slot(a, page_index, slot)) return;
-    const long first = (long)g * a.group;
-    const long end = min((long)a.page, first + a.group);
-    const long limit = min(row_limit(a, row), (long)page * a.page + end);
-    const long in_page = first + (long)part * kPart + threadIdx.x * 4;
-    const long col = (long)page * a.page + in_page;
+    const long first = (long)g * a.group + (long)part * kPart, end = min((long)a.page, (long)(g + 1) * a.group);
+    const long limit = min(row_limit(a, row), (long)page * a.page + end), col = (long)page * a.page + first;
+    Run<T> r = run_of<T, VEC>(a, row, col, limit, kPart);
+    const bool vec = VEC && r.off == 0; // other rows value by value: such groups are rare
     unsigned m = 0;
     if (WRITE) {
         for (unsigned p = threadIdx.x & 31; p < parts; p += 32) m = max(m, part_most[(size_t)group_index * parts + p]);
@@ -367,12 +492,13 @@ __global__ void __launch_bounds__(1024) quantize_part_kernel(const QuantizeArgs 
     if (WRITE && part == 0 && threadIdx.x == 0) a.scales[slot * a.scale_stride + g] = s;
 #pragma unroll 4
     for (int j = 0; j < kPart / 4096; ++j) {
-        const long c = in_page + j * 4096;
-        float4 v = load_sum<T, VEC>(a, row, col + j * 4096, limit);
+        const int c = threadIdx.x * 4 + j * 4096;
+        float4 v = vec ? load_sum<false, true>(r, c) : load_sum<false, false>(r, c);
         if (WRITE) {
             const unsigned q = codes4(v, s);
-            if (c < end) *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + c) = q;
-            store_lost<VEC>(a, row, col + j * 4096, v, limit);
+            if (first + c < end) *reinterpret_cast<unsigned *>(a.codes + slot * a.code_stride + first + c) = q;
+            if (r.lost && vec) store_piece<true>(r.lost, c, v, 0, r.hi);
+            else if (r.lost) store_piece<false>(r.lost, c, v, 0, r.hi);
         } else {
             m = max(m, most4(v));
         }
@@ -384,6 +510,23 @@ __global__ void __launch_bounds__(1024) quantize_part_kernel(const QuantizeArgs 
         m = __reduce_max_sync(0xffffffffu, warp_most[threadIdx.x & 31]);
         if (threadIdx.x == 0) part_most[(size_t)group_index * parts + part] = m;
     }
+}
+
+constexpr int kBlock = 8192, kCluster = 8; // columns that a block holds; blocks of a cluster, at most
+
+template <typename T, bool VEC, int V> int launch_block(const QuantizeArgs &a, long groups, int peers, cudaStream_t stream)
+{
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(groups * peers));
+    config.blockDim = dim3(256);
+    config.stream = stream;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim = {(unsigned)peers, 1, 1};
+    config.attrs = &cluster;
+    config.numAttrs = peers > 1 ? 1 : 0;
+    LB_CUDA(cudaLaunchKernelEx(&config, quantize_block_kernel<T, VEC, V>, a, peers));
+    return LB_OK;
 }
 
 template <typename T, bool VEC>
@@ -402,13 +545,12 @@ int quantize_typed(const QuantizeArgs &a, long n_rows, void *workspace, double b
         case 256: quantize_warp_kernel<T, VEC, 8><<<grid, 256, 0, stream>>>(a, tiles, total); break;
         default: quantize_warp_kernel<T, VEC, 9><<<grid, 256, 0, stream>>>(a, tiles, total); break; // 512, or one group in a page of at most 512
         }
-    } else if (longest <= kPart) {
-        const unsigned grid = (unsigned)(n_pages * a.groups);
-        if (longest <= 1024) quantize_block_kernel<T, VEC, 256, 1><<<grid, 256, 0, stream>>>(a);
-        else if (longest <= 4096) quantize_block_kernel<T, VEC, 256, 4><<<grid, 256, 0, stream>>>(a);
-        else if (longest <= 8192) quantize_block_kernel<T, VEC, 512, 4><<<grid, 512, 0, stream>>>(a);
-        else if (longest <= 16384) quantize_block_kernel<T, VEC, 1024, 4><<<grid, 1024, 0, stream>>>(a);
-        else quantize_block_kernel<T, VEC, 1024, 8><<<grid, 1024, 0, stream>>>(a);
+    } else if (longest <= kBlock * kCluster) {
+        const long groups = n_pages * a.groups;
+        if (longest <= 1024) return launch_block<T, VEC, 1>(a, groups, 1, stream);
+        if (longest <= 4096) return launch_block<T, VEC, 4>(a, groups, 1, stream);
+        if (longest <= kBlock / 2 * kCluster) return launch_block<T, VEC, 4>(a, groups, (longest + kBlock / 2 - 1) / (kBlock / 2), stream);
+        return launch_block<T, VEC, 8>(a, groups, (longest + kBlock - 1) / kBlock, stream);
     } else {
         const unsigned parts = (unsigned)((longest + kPart - 1) / kPart);
         const unsigned grid = (unsigned)(n_pages * a.groups * parts);
@@ -435,7 +577,17 @@ struct DequantizeArgs {
     long out_stride;
 };
 
-template <typename T, bool VEC>
+// Four codes as floats: a byte below the exponent of 2^23 is 2^23 + the byte
+__device__ __forceinline__ float4 floats_of(unsigned x)
+{
+    const unsigned u = x ^ 0x80808080u; // code + 128
+    return make_float4(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)) - 8388736.0f, __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)) - 8388736.0f,
+                       __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.0f, __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.0f);
+}
+
+// A warp takes 512 columns of a page.  The results are written in aligned pieces of four (see Run), whose codes are put together from two
+// words.  ONE: one scale in a page
+template <typename T, bool ONE>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a, const unsigned tiles, const unsigned total)
 {
     const unsigned w = blockIdx.x * 8u + (threadIdx.x >> 5);
@@ -445,37 +597,69 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a,
     const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
     const long slot = a.slots ? (long)a.slots[page_index] : (long)page_index;
     const bool there = slot >= 0 && slot < a.n_slots; // a page that is not in the cache reads as zeros
-    const int in_page = tile * 512 + lane * 4;
-    const long col = (long)page * a.page + in_page;
-    unsigned q[4] = {0, 0, 0, 0};
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const long col = (long)page * a.page + tile * 512;
+    T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride + col;
+    const int off = offset_of(out), hi = (int)max(0l, min(min(a.n_cols - col, 512l), (long)a.page - tile * 512));
+    const signed char *codes = a.codes + (there ? slot : 0) * a.code_stride + tile * 512 + lane * 4;
+    const float *scales = a.scales + (there ? slot : 0) * a.scale_stride;
+    const int end = there ? hi : 0; // columns whose codes are read, in words
+    unsigned q[4];
+    float s[4];
+    if (ONE) s[0] = s[1] = s[2] = s[3] = end ? __ldg(scales) : 0.f;
+    if (end == 512) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int c = in_page + j * 128;
-        if (there && c < a.page && col + j * 128 < a.n_cols) {
-            q[j] = __ldcs(reinterpret_cast<const unsigned *>(a.codes + slot * a.code_stride + c));
-            s[j] = __ldg(a.scales + slot * a.scale_stride + (c >> a.log_group));
+        for (int j = 0; j < 4; ++j) {
+            q[j] = __ldcs(reinterpret_cast<const unsigned *>(codes + j * 128));
+            if (!ONE) s[j] = __ldg(scales + ((int)(tile * 512 + lane * 4 + j * 128) >> a.log_group));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool inside = lane * 4 + j * 128 < end;
+            q[j] = 0;
+            if (inside) q[j] = __ldcs(reinterpret_cast<const unsigned *>(codes + j * 128));
+            if (!ONE) {
+                s[j] = 0.f;
+                if (inside) s[j] = __ldg(scales + ((int)(tile * 512 + lane * 4 + j * 128) >> a.log_group));
+            }
         }
     }
-    T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride;
-    const long limit = min(a.n_cols, (long)(page + 1) * a.page);
+    if (off == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float4 f = floats_of(q[j]);
+            store_piece<true>(out, lane * 4 + j * 128, make_float4(s[j] * f.x, s[j] * f.y, s[j] * f.z, s[j] * f.w), 0, hi);
+        }
+        return;
+    }
+    // the words and scales of the lane before; lane 0's are of the run before, or of the j before
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float4 v = make_float4(s[j] * (float)(signed char)(q[j] & 255), s[j] * (float)(signed char)(q[j] >> 8 & 255),
-                                     s[j] * (float)(signed char)(q[j] >> 16 & 255), s[j] * (float)(signed char)(q[j] >> 24));
-        if (VEC) store4<true>(out + col + j * 128, v, limit - col - j * 128);
-        else store_shifted(out, col + j * 128, v, limit);
+        const unsigned before = __shfl_up_sync(0xffffffffu, q[j], 1), wrap = __shfl_sync(0xffffffffu, q[j > 0 ? j - 1 : 0], 31);
+        const float4 f = floats_of(__funnelshift_r(lane ? before : wrap, q[j], 32 - 8 * off));
+        float b = s[j];
+        if (!ONE) {
+            const float up = __shfl_up_sync(0xffffffffu, s[j], 1), down = __shfl_sync(0xffffffffu, s[j > 0 ? j - 1 : 0], 31);
+            b = lane ? up : down;
+        }
+        const float4 v = make_float4(b * f.x, (off > 1 ? b : s[j]) * f.y, (off > 2 ? b : s[j]) * f.z, s[j] * f.w);
+        if (hi == 512 && (j > 0 || lane > 0)) store4<true>(out + lane * 4 + j * 128 - off, v, 4);
+        else store_piece<true>(out, lane * 4 + j * 128 - off, v, 0, hi);
+    }
+    if (hi == 512 && lane == 31) { // the columns before the next run's first piece
+        const float4 f = floats_of(q[3] >> (32 - 8 * off));
+        store_piece<false>(out, 512 - off, make_float4(s[3] * f.x, s[3] * f.y, s[3] * f.z, 0.f), 0, 512);
     }
 }
 
-template <typename T> bool aligned4(const void *p, long stride) { return (uintptr_t)p % (4 * sizeof(T)) == 0 && stride % 4 == 0; }
+template <typename T> int phase_of(const void *p) { return (int)((uintptr_t)p / sizeof(T)) & 3; }
 
 } // namespace
 
 size_t quantize_workspace_bytes(long n_rows, long n_cols, int page, int group)
 {
     const int longest = group == 0 || group > page ? page : group;
-    if (longest <= kPart) return 0;
+    if (longest <= kBlock * kCluster) return 0;
     const long pages = (n_cols + page - 1) / page, groups = (page + longest - 1) / longest;
     return sizeof(unsigned) * (size_t)(n_rows * pages * groups * ((longest + kPart - 1) / kPart));
 }
@@ -503,17 +687,21 @@ int quantize_rows(const void *values, int dtype, long n_rows, long n_cols, long 
     // one group in a page: a power of two that covers it, as far as the warp kernel goes
     a.group = group == 0 || group >= page ? (page <= 512 ? 512 : page) : group;
     a.groups = (page + a.group - 1) / a.group;
-    const bool res = (!residual || aligned4<float>(residual, residual_stride)) && (!residual_out || aligned4<float>(residual_out, residual_stride));
+    // whether values and residuals lie at the same offset from an aligned piece in every row
+    auto same = [&](int phase) {
+        const bool strides = n_rows == 1 || (value_stride - residual_stride) % 4 == 0;
+        return (!residual && !residual_out) || (strides && (!residual || phase_of<float>(residual) == phase) && (!residual_out || phase_of<float>(residual_out) == phase));
+    };
     const double bytes = (double)n_rows * n_cols * ((dtype == 1 ? 4 : 2) + 1 + (residual ? 4 : 0) + (residual_out ? 4 : 0));
     switch (dtype) {
     case 1:
-        return res && aligned4<float>(values, value_stride) ? quantize_typed<float, true>(a, n_rows, workspace, bytes, stream)
+        return same(phase_of<float>(values)) ? quantize_typed<float, true>(a, n_rows, workspace, bytes, stream)
                                                             : quantize_typed<float, false>(a, n_rows, workspace, bytes, stream);
     case 3:
-        return res && aligned4<__nv_bfloat16>(values, value_stride) ? quantize_typed<__nv_bfloat16, true>(a, n_rows, workspace, bytes, stream)
+        return same(phase_of<__nv_bfloat16>(values)) ? quantize_typed<__nv_bfloat16, true>(a, n_rows, workspace, bytes, stream)
                                                                     : quantize_typed<__nv_bfloat16, false>(a, n_rows, workspace, bytes, stream);
     default:
-        return res && aligned4<__half>(values, value_stride) ? quantize_typed<__half, true>(a, n_rows, workspace, bytes, stream)
+        return same(phase_of<__half>(values)) ? quantize_typed<__half, true>(a, n_rows, workspace, bytes, stream)
                                                              : quantize_typed<__half, false>(a, n_rows, workspace, bytes, stream);
     }
 }
@@ -537,16 +725,10 @@ int dequantize_rows(const signed char *codes, long code_stride, const float *sca
     a.out_stride = out_stride;
     const unsigned tiles = (page + 511) / 512, total = (unsigned)(n_rows * a.pages * tiles), grid = (total + 7) / 8;
     count_launch("dequantize", stream, (double)n_rows * n_cols * (1 + (dtype == 1 ? 4 : 2)));
-    if (dtype == 1) {
-        if (aligned4<float>(out, out_stride)) dequantize_kernel<float, true><<<grid, 256, 0, stream>>>(a, tiles, total);
-        else dequantize_kernel<float, false><<<grid, 256, 0, stream>>>(a, tiles, total);
-    } else if (dtype == 3) {
-        if (aligned4<__nv_bfloat16>(out, out_stride)) dequantize_kernel<__nv_bfloat16, true><<<grid, 256, 0, stream>>>(a, tiles, total);
-        else dequantize_kernel<__nv_bfloat16, false><<<grid, 256, 0, stream>>>(a, tiles, total);
-    } else {
-        if (aligned4<__half>(out, out_stride)) dequantize_kernel<__half, true><<<grid, 256, 0, stream>>>(a, tiles, total);
-        else dequantize_kernel<__half, false><<<grid, 256, 0, stream>>>(a, tiles, total);
-    }
+    const bool one = a.log_group == 31;
+    if (dtype == 1) (one ? dequantize_kernel<float, true> : dequantize_kernel<float, false>)<<<grid, 256, 0, stream>>>(a, tiles, total);
+    else if (dtype == 3) (one ? dequantize_kernel<__nv_bfloat16, true> : dequantize_kernel<__nv_bfloat16, false>)<<<grid, 256, 0, stream>>>(a, tiles, total);
+    else (one ? dequantize_kernel<__half, true> : dequantize_kernel<__half, false>)<<<grid, 256, 0, stream>>>(a, tiles, total);
     LB_CUDA(cudaGetLastError());
     return LB_OK;
 }
