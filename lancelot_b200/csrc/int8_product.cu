@@ -26,27 +26,33 @@ __device__ __forceinline__ float scaled(int sum, float sa, float sb) { return __
 // ---- rows copied to a 16-byte pitch --------------------------------------------------------------------------------------
 // Operands whose rows start off a 16-byte boundary are copied once, zeros up to the pitch: a TMA row and a 16-byte load have to
 // start on such a boundary.
-__global__ void __launch_bounds__(256) pack_kernel(const signed char *__restrict__ src, const long stride, const long rows, const int cols,
-                                                   signed char *__restrict__ dst, const int pitch)
+struct Packed {
+    const signed char *src;
+    long stride, rows;
+    signed char *dst;
+};
+__global__ void __launch_bounds__(256) pack_kernel(const Packed one, const Packed two, const int cols, const int pitch)
 {
-    const long per_row = pitch / 4, total = rows * per_row;
+    const long per_row = pitch / 4, total = (one.rows + two.rows) * per_row;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long r = i / per_row;
+        long r = i / per_row;
         const int c = (int)(i - r * per_row) * 4;
-        const signed char *p = src + r * stride + c;
+        const bool first = r < one.rows;
+        if (!first) r -= one.rows;
+        const signed char *p = (first ? one.src : two.src) + r * (first ? one.stride : two.stride) + c;
         unsigned v = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (c + e < cols) v |= (unsigned)(unsigned char)p[e] << (8 * e);
-        *reinterpret_cast<unsigned *>(dst + r * pitch + c) = v;
+        *reinterpret_cast<unsigned *>((first ? one.dst : two.dst) + r * pitch + c) = v;
     }
 }
 
 // ---- few rows on one side -------------------------------------------------------------------------------------------------
-// A block forms 16 rows of the long side (the rows of A of m16n8k32) against up to 32 rows of the short side; its eight warps
-// split k and add up through shared memory.  As in the pair distances, the order of k inside a product is free, so lane (g, t) loads
+// A block forms 16 rows of the long side (the rows of A of m16n8k32) against up to 32 rows of the short side; its 16 warps split k
+// and add up through shared memory (so many, because a round of loads is what a small call waits for: k = 4096 takes one).  As in the pair distances, the order of k inside a product is free, so lane (g, t) loads
 // 16 consecutive bytes of a row and uses them as four k-slots on either side.
-constexpr int kSkinnyWarps = 8;
+constexpr int kSkinnyWarps = 16;
 
 struct SkinnyArgs {
     const signed char *w, *x; // long side [rows][k], short side [cols][k]
@@ -57,7 +63,7 @@ struct SkinnyArgs {
     long row_step, col_step; // of the result
 };
 
-template <typename T, int NB> __global__ void __launch_bounds__(kSkinnyWarps * 32) skinny_kernel(const SkinnyArgs a)
+template <typename T, int NB> __global__ void __launch_bounds__(kSkinnyWarps * 32, 2) skinny_kernel(const SkinnyArgs a)
 {
     __shared__ int part[kSkinnyWarps][16][NB * 8 + 1];
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
@@ -111,11 +117,16 @@ template <typename T> int launch_skinny(const SkinnyArgs &a, cudaStream_t stream
 // One CTA per SM walks over tiles of 128 x BN.  Warp 0 brings 128-byte wide blocks of k by TMA into a ring of stages, warp 1
 // issues the products (four of k = 32 a stage), warps 2 to 5 take a finished tile out of TMEM.  TMEM holds two tiles, so
 // a tile leaves while the next one is being formed.
-constexpr int kTileM = 128, kTileK = 128, kTileThreads = 192;
-template <int BN> struct Tile {
+constexpr int kTileM = 128, kTileK = 128;
+
+// SHORT: few blocks of k, so that the results are what takes time: eight warps instead of four take them out, and fewer stages leave
+// shared memory for them to leave by TMA
+template <int BN, bool SHORT> struct Tile {
+    static constexpr int kOutWarps = SHORT ? 8 : 4, kThreads = 64 + kOutWarps * 32;
     static constexpr int kStageBytes = (kTileM + BN) * kTileK;
-    static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr int kSmem = kStages * kStageBytes + 1024 + 4 * 256 * 4 + 256;
+    static constexpr int kStages = SHORT ? 3 : BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int kOutBytes = SHORT ? 2 * 4096 : 0; // of a warp: two boxes of 32 rows of 128 bytes
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kOutWarps * (kOutBytes + BN * 4) + 256;
     // D 32-bit signed, A and B 8-bit signed, both k-major
     static constexpr unsigned kDesc = 2u << 4 | 1u << 7 | 1u << 10 | (unsigned)(BN >> 3) << 17 | (unsigned)(kTileM >> 4) << 24;
 };
@@ -126,7 +137,7 @@ struct ProductArgs {
     const float *a_scale, *b_scale;
     void *out;
     long out_stride;
-    int align; // 32, 16: the result's rows start on such a boundary; 0: on none
+    int align; // 32, 16: the result's rows start on such a boundary; 0: on none; 1: the results leave by TMA
     int *status;
 };
 
@@ -190,15 +201,22 @@ template <typename T> __device__ __forceinline__ void put32(T *p, const float (&
     }
 }
 
-template <typename T, int BN>
-__global__ void __launch_bounds__(kTileThreads, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                                                                  const ProductArgs a)
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, int x, int y, unsigned src)
 {
-    using C = Tile<BN>;
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+template <typename T, int BN, bool SHORT>
+__global__ void __launch_bounds__(Tile<BN, SHORT>::kThreads, 1) product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                                                                               const __grid_constant__ CUtensorMap map_out, const ProductArgs a)
+{
+    using C = Tile<BN, SHORT>;
     extern __shared__ unsigned char raw[];
     unsigned char *stages = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    float *scales = reinterpret_cast<float *>(stages + C::kStages * C::kStageBytes); // [4][256], one set per warp that takes results out
-    unsigned char *tail = reinterpret_cast<unsigned char *>(scales + 1024);
+    unsigned char *boxes = stages + C::kStages * C::kStageBytes;                           // [warp][2][32][128]
+    float *scales = reinterpret_cast<float *>(boxes + C::kOutWarps * C::kOutBytes);        // [warp][BN]
+    unsigned char *tail = reinterpret_cast<unsigned char *>(scales + C::kOutWarps * BN);
     unsigned long long *bars = reinterpret_cast<unsigned long long *>(tail); // full[stages], empty[stages], done[2], freed[2], drained
     unsigned *tmem_at = reinterpret_cast<unsigned *>(bars + 2 * C::kStages + 5);
     volatile int *failed = reinterpret_cast<volatile int *>(tmem_at + 1);
@@ -213,7 +231,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) product_kernel(const __grid_c
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(done + 8 * i, 1);
-            mbar_init(freed + 8 * i, 128);
+            mbar_init(freed + 8 * i, C::kOutWarps * 32);
         }
         mbar_init(drained, 1);
         *failed = 0;
@@ -281,42 +299,99 @@ __global__ void __launch_bounds__(kTileThreads, 1) product_kernel(const __grid_c
                 if (mbar_try(drained, 0)) break;
         }
     } else {
-        const int quarter = warp & 3;
-        float *sb = scales + quarter * 256;
-        int done_tiles = 0;
+        // a warp sees the 32 lanes of TMEM of its quarter; the warps of a quarter take their runs of 32 columns by turns
+        constexpr int kTurns = C::kOutWarps / 4, kCols = SHORT && sizeof(T) == 2 ? 64 : 32; // columns of a run: a box of 128 bytes
+        const int quarter = warp & 3, turn = (warp - 2) / 4;
+        float *sb = scales + (warp - 2) * BN;
+        unsigned char *box = boxes + (warp - 2) * C::kOutBytes;
+        int done_tiles = 0, sent = 0;
         bool ok = true;
+        float next_a, next_b[BN / 32]; // the scales of the next tile, on their way while this one is taken out
+        auto fetch = [&](int t) {
+            int tm, tn;
+            tile_at(a, min(t, tiles - 1), tm, tn);
+            const int row = tm * kTileM + quarter * 32 + lane;
+            next_a = row < a.m ? __ldg(a.a_scale + row) : 0.f;
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) next_b[c] = tn * BN + c * 32 + lane < a.n ? __ldg(a.b_scale + tn * BN + c * 32 + lane) : 0.f;
+        };
+        fetch(blockIdx.x);
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++done_tiles) {
             const int buf = done_tiles & 1;
             int tm, tn;
             tile_at(a, t, tm, tn);
-            __syncwarp();
-            for (int c = lane; c < BN; c += 32) sb[c] = tn * BN + c < a.n ? a.b_scale[tn * BN + c] : 0.f;
-            __syncwarp();
             const int row = tm * kTileM + quarter * 32 + lane;
-            const float sa = row < a.m ? a.a_scale[row] : 0.f;
+            const float sa = next_a;
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) sb[c * 32 + lane] = next_b[c];
+            __syncwarp();
+            fetch(t + gridDim.x);
             ok = mbar_wait(done + 8 * buf, (done_tiles / 2) & 1, failed);
             if (!__all_sync(0xffffffffu, ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride + tn * BN;
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 32) {
-                if (tn * BN + c >= a.n) break;
-                int v[32];
-                tmem_load32(tmem + buf * BN + c + ((unsigned)quarter << 21), v);
-                float f[32];
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    const float4 s4 = *reinterpret_cast<const float4 *>(sb + c + e);
-                    f[e] = scaled(v[e], sa, s4.x);
-                    f[e + 1] = scaled(v[e + 1], sa, s4.y);
-                    f[e + 2] = scaled(v[e + 2], sa, s4.z);
-                    f[e + 3] = scaled(v[e + 3], sa, s4.w);
+            for (int c0 = turn * kCols; c0 < BN; c0 += kTurns * kCols) {
+                if (tn * BN + c0 >= a.n) break;
+                const bool by_tma = SHORT && a.align == 1;
+                unsigned char *to = box + (sent & 1) * 4096;
+                if (by_tma) { // the box has been read out
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    __syncwarp();
                 }
-                if (row < a.m) put32(out + c, f, a.n - tn * BN - c, a.align);
+#pragma unroll
+                for (int c = c0; c < c0 + kCols; c += 32) {
+                    int v[32];
+                    tmem_load32(tmem + buf * BN + c + ((unsigned)quarter << 21), v);
+                    float f[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(sb + c + e);
+                        f[e] = scaled(v[e], sa, s4.x);
+                        f[e + 1] = scaled(v[e + 1], sa, s4.y);
+                        f[e + 2] = scaled(v[e + 2], sa, s4.z);
+                        f[e + 3] = scaled(v[e + 3], sa, s4.w);
+                    }
+                    if (by_tma) { // 16-byte pieces where the 128-byte swizzle wants them
+                        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                *reinterpret_cast<float4 *>(to + lane * 128 + ((e / 4 ^ (lane & 7)) << 4)) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8)
+                                *reinterpret_cast<uint4 *>(to + lane * 128 + ((((c - c0) / 8 + e / 8) ^ (lane & 7)) << 4)) =
+                                    make_uint4(pack2((T *)nullptr, f[e], f[e + 1]), pack2((T *)nullptr, f[e + 2], f[e + 3]), pack2((T *)nullptr, f[e + 4], f[e + 5]),
+                                               pack2((T *)nullptr, f[e + 6], f[e + 7]));
+                        }
+                    } else if (SHORT && a.align == 0) { // rows off their alignment: a row of the run at a time
+                        // (through the box, 32 rows of 32 floats with the columns turned by the row, so that neither side meets a bank twice)
+                        float *turned = reinterpret_cast<float *>(box);
+                        __syncwarp();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) turned[lane * 32 + ((e + lane) & 31)] = f[e];
+                        __syncwarp();
+                        const int first = tm * kTileM + quarter * 32, rows = min(32, a.m - first), col = tn * BN + c + lane;
+                        T *p = reinterpret_cast<T *>(a.out) + (long)first * a.out_stride + col;
+                        if (col < a.n)
+                            for (int i = 0; i < rows; ++i) put(p + i * a.out_stride, turned[i * 32 + ((lane + i) & 31)]);
+                    } else if (row < a.m) {
+                        put32(out + c, f, a.n - tn * BN - c, a.align);
+                    }
+                }
+                if (by_tma) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0 && tm * kTileM + quarter * 32 < a.m) tma_store(&map_out, tn * BN + c0, tm * kTileM + quarter * 32, smem_u32(to));
+                    ++sent;
+                }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             mbar_arrive(freed + 8 * buf);
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -325,20 +400,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) product_kernel(const __grid_c
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * BN) : "memory");
 }
 
-template <typename T, int BN> int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const ProductArgs &a, cudaStream_t stream)
+template <typename T, int BN, bool SHORT>
+int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const ProductArgs &a, cudaStream_t stream)
 {
-    using C = Tile<BN>;
+    using C = Tile<BN, SHORT>;
     static bool set[64] = {};
-    if (ctx->device < 64 && !set[ctx->device]) {
-        LB_CUDA(cudaFuncSetAttribute(product_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-        set[ctx->device] = true;
+    if (ctx->device >= 64 || !set[ctx->device]) {
+        LB_CUDA(cudaFuncSetAttribute(product_kernel<T, BN, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        if (ctx->device < 64) set[ctx->device] = true;
     }
     const int tiles = a.tiles_m * a.tiles_n;
-    product_kernel<T, BN><<<tiles < ctx->sm_count ? tiles : ctx->sm_count, kTileThreads, C::kSmem, stream>>>(ma, mb, a);
+    product_kernel<T, BN, SHORT><<<tiles < ctx->sm_count ? tiles : ctx->sm_count, C::kThreads, C::kSmem, stream>>>(ma, mb, mo, a);
     LB_CUDA(cudaGetLastError());
     return LB_OK;
 }
 
+constexpr int kShort = 8;   // blocks of k up to which the results are what takes time
 constexpr int kSkinny = 32; // rows on the short side up to which the long side is streamed
 
 struct ProductPlan {
@@ -395,17 +472,27 @@ int product_typed(Context *ctx, int m, int n, int k, const signed char *a, long 
     p.align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
     p.status = ctx->d_status;
     p.band = 8;
-    // the widest tile that still gives every SM one
-    const int bn = (long)p.tiles_m * ((n + 255) / 256) >= ctx->sm_count ? 256 : (long)p.tiles_m * ((n + 127) / 128) >= ctx->sm_count ? 128 : 64;
+    // The widest tile that still gives every SM one.  Up to kShort blocks of k, and where rows are off their alignment, the form that takes
+    // results out faster
+    const bool quick = p.k_blocks <= kShort || p.align == 0;
+    const int widest = quick ? 128 : 256;
+    int bn = 64;
+    while (bn < widest && (long)p.tiles_m * ((n + 2 * bn - 1) / (2 * bn)) >= ctx->sm_count) bn *= 2;
     p.tiles_n = (n + bn - 1) / bn;
-    CUtensorMap ma, mb;
+    CUtensorMap ma, mb, mo;
     int rc = encode_map(&ma, a, m, k, a_stride, kTileK, kTileM);
     if (rc) return rc;
     if ((rc = encode_map(&mb, b, n, k, b_stride, kTileK, bn))) return rc;
+    mo = ma; // not used unless
+    if (quick && p.align >= 16) {
+        if ((rc = encode_map(&mo, out, m, (long)n * (long)sizeof(T), out_stride * (long)sizeof(T), 128, 32, sizeof(T)))) return rc;
+        p.align = 1;
+    }
     count_launch("int8_tiles", stream, bytes);
-    if (bn == 256) return launch_tiles<T, 256>(ctx, ma, mb, p, stream);
-    if (bn == 128) return launch_tiles<T, 128>(ctx, ma, mb, p, stream);
-    return launch_tiles<T, 64>(ctx, ma, mb, p, stream);
+    if (quick) return bn == 128 ? launch_tiles<T, 128, true>(ctx, ma, mb, mo, p, stream) : launch_tiles<T, 64, true>(ctx, ma, mb, mo, p, stream);
+    if (bn == 256) return launch_tiles<T, 256, false>(ctx, ma, mb, mo, p, stream);
+    if (bn == 128) return launch_tiles<T, 128, false>(ctx, ma, mb, mo, p, stream);
+    return launch_tiles<T, 64, false>(ctx, ma, mb, mo, p, stream);
 }
 
 } // namespace
@@ -419,19 +506,16 @@ int int8_matmul(Context *ctx, int m, int n, int k, const signed char *a, long a_
                 const float *b_scale, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream)
 {
     const ProductPlan p = product_plan(m, n, k, a, a_stride, b, b_stride);
-    auto pack = [&](const signed char *&x, long &stride, long rows, signed char *to) -> int {
-        const long total = rows * (p.pitch / 4), blocks = (total + 255) / 256, most = (long)ctx->sm_count * 16;
-        count_launch("int8_pack", stream, 2.0 * rows * k);
-        pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(x, stride, rows, k, to, p.pitch);
-        LB_CUDA(cudaGetLastError());
-        x = to;
-        stride = p.pitch;
-        return LB_OK;
-    };
     signed char *ws = reinterpret_cast<signed char *>(workspace);
-    int rc;
-    if (p.pack_a && (rc = pack(a, a_stride, m, ws))) return rc;
-    if (p.pack_b && (rc = pack(b, b_stride, n, ws + p.a_bytes))) return rc;
+    if (p.pack_a || p.pack_b) {
+        const Packed one = {a, a_stride, p.pack_a ? m : 0, ws}, two = {b, b_stride, p.pack_b ? n : 0, ws + p.a_bytes};
+        const long blocks = ((one.rows + two.rows) * (p.pitch / 4) + 255) / 256, most = (long)ctx->sm_count * 16;
+        count_launch("int8_pack", stream, 2.0 * (one.rows + two.rows) * k);
+        pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(one, two, k, p.pitch);
+        LB_CUDA(cudaGetLastError());
+        if (p.pack_a) a = one.dst, a_stride = p.pitch;
+        if (p.pack_b) b = two.dst, b_stride = p.pitch;
+    }
     k = p.pitch; // k itself where a side is not packed: a ragged k packs both
     switch (dtype) {
     case 1: return product_typed<float>(ctx, m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);

@@ -118,8 +118,9 @@ __device__ __forceinline__ void tmem_load32(unsigned addr, int (&v)[32])
 typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// rows of `cols` bytes, `stride` apart, in boxes of box_cols x box_rows with a 128-byte swizzle; outside the matrix lie zeros
-inline int encode_map(CUtensorMap *map, const void *base, long rows, int cols, long stride, int box_cols, int box_rows)
+// Rows of `cols` bytes, `stride` apart, in boxes of box_cols bytes x box_rows with a 128-byte swizzle; outside the matrix lie zeros.
+// size: bytes of an element, which coordinates count in
+inline int encode_map(CUtensorMap *map, const void *base, long rows, long cols, long stride, int box_cols, int box_rows, int size = 1)
 {
     static EncodeTiled encode = nullptr;
     if (!encode) {
@@ -132,9 +133,9 @@ inline int encode_map(CUtensorMap *map, const void *base, long rows, int cols, l
         }
         encode = reinterpret_cast<EncodeTiled>(f);
     }
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
-    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, steps[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const cuuint64_t dims[2] = {(cuuint64_t)(cols / size), (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+    const cuuint32_t box[2] = {(cuuint32_t)(box_cols / size), (cuuint32_t)box_rows}, steps[2] = {1, 1};
+    const CUresult r = encode(map, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
