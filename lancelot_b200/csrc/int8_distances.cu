@@ -7,10 +7,16 @@
 // floats, so that the three terms of D_ij may cancel by nine digits before a 32-bit result would suffer.  Two equal updates
 // give exactly 0: the same warps add the same numbers in the same order for ii, ij and jj.
 //
-// Bound by reading the codes once.  The rows of a tile of clients go from memory straight into the registers of the matrix
-// instruction: a row of A and a column of B are both "a client's codes along k", and the order of k inside the product does not
-// matter as long as both sides agree, so lane (g, t) loads 16 consecutive bytes of client g and uses them as four k-slots of A and
-// of B at once.  No shared memory, no transposition, one load per code.
+// A row of A and a column of B are both "a client's codes along k", and the order of k inside a product does not matter as long as
+// both sides agree: lane (g, t) of the matrix instruction takes 16 consecutive bytes of client g and uses them as four k-slots of A
+// and of B at once, without a transposition.
+//
+// What was measured on the way (20 x 11 M, groups of 128; 36 us at the copy rate).  m16n8k32 takes 8 cycles of a quarter of the SM, so
+// that 20 clients keep it busy for a fifth of the time that their codes take to come in: the warp's own instruction is the right
+// one.  tcgen05 took 148 us: one thread issues for all, its results leave TMEM group by group, and a product of few columns costs as
+// much as a wide one.  A ring of shared memory filled by a warp of its own took 123 us (a bulk copy or a gathered TMA load of four rows
+// holds its warp up for 70 cycles), filled by all warps 96 us (instructions); registers 61 us.  Beyond 32 clients the registers of a
+// warp do not hold what it would have to read, and the ring is used after all.
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -195,11 +201,10 @@ template <int BYTES> __global__ void __launch_bounds__(kWarps * 32) gram_kernel(
 
 // ---- pieces of the kernels for up to 128 clients ----------------------------------------------------------------------------------
 constexpr int kRingBytes = 216 * 1024;
-constexpr int kMaxScales = 4; // copies of scales that a thread makes for one stage
+constexpr int kSlotStages = 16; // stages whose slots are held; at least twice the ring's
 
 // An integer sum as a 64-bit float, without the conversion unit (which takes 8 cycles for what the FP64 pipe does in 2): sums start
-// from -2^31 instead of 0, and 2^52 + 2^31 + x has just those bits below an exponent of 52.  Where there is time, every
-// fourth sum goes through the conversion unit all the same, beside the others.
+// from -2^31 instead of 0, and 2^52 + 2^31 + x has just those bits below an exponent of 52.
 constexpr int kBias = (int)0x80000000;
 __device__ __forceinline__ double unbiased(int x) { return __hiloint2double(0x43300000, x) - 4503601774854144.0; }
 
@@ -250,53 +255,18 @@ template <> struct Cover<2> : Tiles<2, 0x00, 0xf1, 0x01> {};
 template <> struct Cover<3> : Tiles<3, 0x100, 0x212, 0x210> {};
 template <> struct Cover<4> : Tiles<6, 0x103210, 0xff0321, 0x320321> {};
 
-// all pairs of 32 clients, columns [begin, end) of the rows from `codes` on, one scale each from `scales` on
+// 16 clients (`codes`, `scales` at the first) with the first `blocks` x 8 of 32 clients `apart` rows further down: columns [begin, end), one
+// scale each
 template <int BYTES>
-__device__ __forceinline__ void triangle(double (&total)[8][4], const unsigned char *codes, const double *scales, int pitch, int begin, int end)
-{
-    using V = Cover<4>;
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const unsigned char *at = codes + g * pitch + t * BYTES;
-    int acc[V::kTiles][4];
-    auto step = [&](int c, auto first) {
-        unsigned w[5][BYTES / 4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) load_rows<BYTES>(w[r], at + r * 8 * pitch + c);
-#pragma unroll
-        for (int k = 0; k < BYTES / 4; ++k) w[4][k] = 0;
-#pragma unroll
-        for (int k = 0; k < BYTES / 4; k += 2)
-#pragma unroll
-            for (int v = 0; v < V::kTiles; ++v) {
-                const int lo = V::lo(v), hi = V::hi(v) >= 0 ? V::hi(v) : 4, col = V::col(v);
-                if (decltype(first)::value && k == 0) mma_s8_from(acc[v], kBias, w[lo][k], w[hi][k], w[lo][k + 1], w[hi][k + 1], w[col][k], w[col][k + 1]);
-                else mma_s8(acc[v], w[lo][k], w[hi][k], w[lo][k + 1], w[hi][k + 1], w[col][k], w[col][k + 1]);
-            }
-    };
-    step(begin, std::true_type());
-    for (int c = begin + 4 * BYTES; c < end; c += 4 * BYTES) step(c, std::false_type());
-    double row[4];
-    double2 col[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        row[r] = scales[r * 8 + g];
-        col[r] = *reinterpret_cast<const double2 *>(scales + r * 8 + t * 2);
-    }
-#pragma unroll
-    for (int v = 0; v < V::kTiles; ++v) apply_scales(total[v], acc[v], row[V::lo(v)], V::hi(v) >= 0 ? row[V::hi(v) >= 0 ? V::hi(v) : 0] : 0.0, col[V::col(v)]);
-}
-
-// 32 clients with the first `blocks` x 8 of 32 others, `apart` rows further down
-template <int BYTES>
-__device__ __forceinline__ void square(double (&total)[8][4], const unsigned char *codes, const double *scales, int apart, int blocks, int pitch, int begin, int end)
+__device__ __forceinline__ void strip(double (&total)[4][4], const unsigned char *codes, const double *scales, int apart, int blocks, int pitch, int begin, int end)
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const unsigned char *at = codes + g * pitch + t * BYTES, *other = at + apart * pitch;
-    int acc[8][4];
+    int acc[4][4];
     auto step = [&](int c, auto first) {
-        unsigned a[4][BYTES / 4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) load_rows<BYTES>(a[r], at + r * 8 * pitch + c);
+        unsigned lo[BYTES / 4], hi[BYTES / 4];
+        load_rows<BYTES>(lo, at + c);
+        load_rows<BYTES>(hi, at + 8 * pitch + c);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j >= blocks) break;
@@ -304,33 +274,25 @@ __device__ __forceinline__ void square(double (&total)[8][4], const unsigned cha
             load_rows<BYTES>(b, other + j * 8 * pitch + c);
 #pragma unroll
             for (int k = 0; k < BYTES / 4; k += 2) {
-                if (decltype(first)::value && k == 0) {
-                    mma_s8_from(acc[2 * j], kBias, a[0][k], a[1][k], a[0][k + 1], a[1][k + 1], b[k], b[k + 1]);
-                    mma_s8_from(acc[2 * j + 1], kBias, a[2][k], a[3][k], a[2][k + 1], a[3][k + 1], b[k], b[k + 1]);
-                } else {
-                    mma_s8(acc[2 * j], a[0][k], a[1][k], a[0][k + 1], a[1][k + 1], b[k], b[k + 1]);
-                    mma_s8(acc[2 * j + 1], a[2][k], a[3][k], a[2][k + 1], a[3][k + 1], b[k], b[k + 1]);
-                }
+                if (decltype(first)::value && k == 0) mma_s8_from(acc[j], kBias, lo[k], hi[k], lo[k + 1], hi[k + 1], b[k], b[k + 1]);
+                else mma_s8(acc[j], lo[k], hi[k], lo[k + 1], hi[k + 1], b[k], b[k + 1]);
             }
         }
     };
     step(begin, std::true_type());
     for (int c = begin + 4 * BYTES; c < end; c += 4 * BYTES) step(c, std::false_type());
-    double row[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) row[r] = scales[r * 8 + g];
+    const double lo = scales[g], hi = scales[8 + g];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (j >= blocks) break;
-        const double2 col = *reinterpret_cast<const double2 *>(scales + apart + j * 8 + t * 2);
-        apply_scales(total[2 * j], acc[2 * j], row[0], row[1], col);
-        apply_scales(total[2 * j + 1], acc[2 * j + 1], row[2], row[3], col);
+        apply_scales(total[j], acc[j], lo, hi, *reinterpret_cast<const double2 *>(scales + apart + j * 8 + t * 2));
     }
 }
 
 // ---- up to 32 clients: no shared memory ----------------------------------------------------------------------------------------
-// A warp takes a unit of a page's columns, kChunk columns at a time, the next ones on their way in registers while these are multiplied.
-// 16 warps an SM, none of which waits for another.  A client that is not there (or a page of one) is read as the cache's first
+// A warp takes a unit of a page's columns, CHUNK columns at a time, the next ones on their way in registers while these are multiplied.
+// 16 warps an SM, none of which waits for another: 20 x 11 M in 61 us (3.8 TB/s), of which some 8 us are the first loads, the sums of the
+// blocks and the second kernel.  A client that is not there (or a page of one) is read as the cache's first
 // slot with scales of 0, so that no load needs a condition.
 template <int NB, int BYTES, int CHUNK, int GROUPS> // GROUPS: scales of a chunk
 __global__ void __launch_bounds__(kWarps * 32, NB == 4 ? 1 : 2) gram_direct_kernel(const DistanceArgs a)
@@ -492,11 +454,15 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 4 ? 1 : 2) gram_direct_kern
 
 // ---- up to 128 clients: a ring of shared memory --------------------------------------------------------------------------------
 // One CTA per SM.  All its warps together copy the codes and scales of some hundred columns of all clients into the ring, several stages
-// ahead (cp.async; one barrier a stage), and each warp multiplies two groups of 32 clients, or one with itself.  Rows lie 64 bytes off
-// a multiple of 128 apart, so that the 16-byte loads of eight rows fall on different banks.
+// ahead (cp.async; one barrier a stage), and each warp multiplies 16 clients with 32.  Rows lie 64 bytes off a multiple of 128 apart, so
+// that the 16-byte loads of eight rows fall on different banks.
 //
-// NB: blocks of eight clients: 8, 12 or 16.  SETS warps split the columns of a stage, 2^LOG_UNIT, for the same pairs.  (Sizes are constants because instructions are what this kernel runs short of: with
-// divisions by a unit of run-time size it took 870 a warp and stage, four times what follows.)
+// Bound by instructions and by shared memory, which every warp reads six 512-byte rows from for four products: 100 x 1.6 M takes 142 us
+// with one scale a page, 185 us with groups of 64 (26 us at the copy rate).  32 by 32 clients a warp, which read less, left too few warps
+// (162, 219 us); slots looked up by every thread for itself instead of by way of shared memory took 180, 224 us.
+//
+// NB: blocks of eight clients: 8, 12 or 16.  SETS warps split the columns of a stage, 2^LOG_UNIT, for the same pairs.  Sizes are constants
+// because divisions by a unit of run-time size took more instructions than all the rest.
 template <int NB, int LOG_UNIT, int BYTES, int WARPS, int SETS>
 __global__ void __launch_bounds__(WARPS * 32, 1) gram_ring_kernel(const DistanceArgs a, const Ring r)
 {
@@ -527,84 +493,89 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gram_ring_kernel(const Distance
     Place now = {(int)(blockIdx.x / a.units_per_page), (int)(blockIdx.x % a.units_per_page) << LOG_UNIT};
     Place ahead = now; // the next unit to be copied
 
-    // What this thread copies of every stage: 16 bytes of the same columns of every kRowsApart-th row, and some scales.  The slots are
-    // looked up a stage ahead; none of these loads is behind a branch, and nothing looks at the slots before fill does
+    // What this thread copies of every stage: 16 bytes of the same columns of every kRowsApart-th row, some scales, and the slots of a stage
+    // further on, so that these are in shared memory when that stage is copied
     static_assert(WARPS % kCopiesARow == 0, "a warp's copies are of the same columns");
     constexpr int kRowsApart = WARPS / kCopiesARow * kRowsACopy;
     const int first_row = warp / kCopiesARow * kRowsACopy + lane / kLanes, column = warp % kCopiesARow * 512 + lane % kLanes * 16;
     const unsigned first_to = smem_u32(ring) + first_row * kPitch + column;
     const int n_slots = (int)a.n_slots, code_stride = (int)a.code_stride, scale_stride = (int)a.scale_stride;
-    int code_entry[kFill], scale_entry[kMaxScales], code_slot[kFill], scale_slot[kMaxScales];
-#pragma unroll
-    for (int k = 0; k < kFill; ++k) code_entry[k] = min(first_row + k * kRowsApart, a.n - 1) * a.pages;
-#pragma unroll
-    for (int k = 0; k < kMaxScales; ++k) scale_entry[k] = min((int)(threadIdx.x + k * kThreads) >> log_groups, a.n - 1) * a.pages;
-    auto look_up = [&](int page) {
-        const int at = min(page, a.pages - 1);
-        if (a.slots) { // (not a choice for each slot: that would wait for it)
-#pragma unroll
-            for (int k = 0; k < kFill; ++k) code_slot[k] = __ldg(a.slots + code_entry[k] + at);
-#pragma unroll
-            for (int k = 0; k < kMaxScales; ++k)
-                if (k * kThreads < scales_a_stage) scale_slot[k] = __ldg(a.slots + scale_entry[k] + at);
-        } else {
-#pragma unroll
-            for (int k = 0; k < kFill; ++k) code_slot[k] = code_entry[k] + at;
-#pragma unroll
-            for (int k = 0; k < kMaxScales; ++k) scale_slot[k] = scale_entry[k] + at;
+    int *slots = reinterpret_cast<int *>(wide_scales + 2 * r.groups * kWide); // [kSlotStages][kWide]
+    auto look_up = [&](int page, int at) { // entry `at` of the slots
+        const int i = (int)threadIdx.x * a.pages + min(page, a.pages - 1);
+        if ((int)threadIdx.x < a.n) {
+            if (a.slots) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(slots + at * kWide + threadIdx.x)), "l"(a.slots + i));
+            else slots[at * kWide + threadIdx.x] = i;
         }
     };
-    auto fill = [&](const Place &p, int stage) { // a page that is not there leaves old codes, and scales of 0
+    auto fill = [&](const Place &p, int stage, int at) { // a page that is not there leaves old codes, and scales of 0
         if (p.page < a.pages) {
+            const int *slot = slots + at * kWide;
             const unsigned to = first_to + stage * r.stage_bytes;
             const signed char *from = a.codes + p.begin + column;
             const bool inside = p.begin + column < a.page;
 #pragma unroll
-            for (int k = 0; k < kFill; ++k)
-                if (first_row + k * kRowsApart < a.n && (unsigned)code_slot[k] < (unsigned)n_slots) // zeros behind the page's end
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + k * kRowsApart * kPitch), "l"(inside ? from + (long)code_slot[k] * code_stride : a.codes),
-                                 "r"(inside ? 16 : 0));
-            const unsigned scales_to = smem_u32(ring) + stage * r.stage_bytes + code_bytes;
-#pragma unroll
-            for (int k = 0; k < kMaxScales; ++k) {
-                const int i = threadIdx.x + k * kThreads;
-                if (i < scales_a_stage) {
-                    const int q = (p.begin >> log_group) + (i & (r.groups - 1));
-                    const bool there = (unsigned)scale_slot[k] < (unsigned)n_slots && (long)q << log_group < a.page;
-                    const float *src = there ? a.scales + (long)scale_slot[k] * scale_stride + q : a.scales;
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scales_to + i * 4), "l"(src), "r"(there ? 4 : 0));
+            for (int k = 0; k < kFill; ++k) {
+                const int row = first_row + k * kRowsApart;
+                if (row >= a.n) break;
+                const int here = slot[row];
+                if ((unsigned)here < (unsigned)n_slots) {
+                    if (inside) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + k * kRowsApart * kPitch), "l"(from + (long)here * code_stride));
+                    else asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to + k * kRowsApart * kPitch), "r"(0) : "memory"); // behind the page's end
                 }
             }
+            const unsigned scales_to = smem_u32(ring) + stage * r.stage_bytes + code_bytes;
+            for (int i = threadIdx.x; i < scales_a_stage; i += kThreads) {
+                const int q = (p.begin >> log_group) + (i & (r.groups - 1)), here = slot[i >> log_groups];
+                const bool there = (unsigned)here < (unsigned)n_slots && (long)q << log_group < a.page;
+                const float *src = there ? a.scales + (long)here * scale_stride + q : a.scales;
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(scales_to + i * 4), "l"(src), "r"(there ? 4 : 0));
+            }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto commit = [&]() { asm volatile("cp.async.commit_group;" ::: "memory"); };
     auto widen = [&](int stage, int parity) { // a stage's scales as 64-bit floats, [group][client]
         const float *from = reinterpret_cast<const float *>(ring + (size_t)stage * r.stage_bytes + code_bytes);
         double *to = wide_scales + parity * r.groups * kWide;
         for (int i = threadIdx.x; i < scales_a_stage; i += kThreads) to[(i & (r.groups - 1)) * kWide + (i >> log_groups)] = from[i];
     };
 
-    // the pairs of this warp: rows from row0 on with rows from col0 on
-    const int set = warp % SETS;
-    int row0 = 0, col0 = warp / SETS;
+    // the pairs of this warp: 16 rows from row0 on with up to 32 from col0 on; two warps make a pair of groups
+    const int set = warp % SETS, half = warp / SETS & 1;
+    int row0 = 0, col0 = warp / SETS / 2;
     constexpr int kGroups = NB / 4;
     while (col0 >= kGroups - row0) col0 -= kGroups - row0++;
-    col0 = (row0 + col0) * 32;
-    row0 *= 32;
-    const int col_blocks = min(4, (a.n - col0 + 7) / 8);
+    const bool same = col0 == 0; // a group with itself: the lower half has nothing to do with the upper
+    col0 = (row0 + col0) * 32 + (same ? half * 16 : 0);
+    row0 = row0 * 32 + half * 16;
+    const int col_blocks = min(same && half ? 2 : 4, (a.n - col0 + 7) / 8);
     constexpr int kPer = kUnit / SETS; // columns of a warp
     const int step = min(a.group, kPer);
-    double total[8][4];
+    double total[4][4];
 #pragma unroll
-    for (int v = 0; v < 8; ++v)
+    for (int v = 0; v < 4; ++v)
 #pragma unroll
         for (int e = 0; e < 4; ++e) total[v][e] = 0.0;
 
-    look_up(ahead.page);
+    // The slots of unit u stand at u % kSlotStages.  They come with the copies of unit u - (stages - 1), which are complete when
+    // unit u is copied; those of the first units are waited for here
+    Place looked = now;
+    int look_at = 0, fill_at = 0;
+    auto look_further = [&]() {
+        look_up(looked.page, look_at);
+        advance(looked);
+        look_at = (look_at + 1) % kSlotStages;
+    };
+    for (int u = 0; u < r.stages - 1; ++u) look_further();
+    commit();
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
     for (int s = 0; s < r.stages - 1; ++s) {
-        fill(ahead, s);
+        fill(ahead, s, fill_at);
+        fill_at = (fill_at + 1) % kSlotStages;
         advance(ahead);
-        look_up(ahead.page);
+        look_further();
+        commit();
     }
     // a stage and the next one have come in when all but the last stages - 3 copies have
     auto wait = [&]() {
@@ -625,9 +596,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gram_ring_kernel(const Distance
         wait();
         __syncthreads(); // this stage and the next have come in, the last one has been read
         const int next = s + 1 == r.stages ? 0 : s + 1;
-        fill(ahead, s ? s - 1 : r.stages - 1);
+        fill(ahead, s ? s - 1 : r.stages - 1, fill_at);
+        fill_at = (fill_at + 1) % kSlotStages;
         advance(ahead);
-        look_up(ahead.page);
+        look_further();
+        commit();
         widen(next, parity ^ 1); // (behind the last unit: old scales, and nobody reads them)
         const int columns = min(kUnit, a.page - now.begin);
         const unsigned char *codes = ring + (size_t)s * r.stage_bytes;
@@ -635,8 +608,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gram_ring_kernel(const Distance
         const double *scales = wide_scales + parity * r.groups * kWide;
         for (int c = set * kPer; c < to; c += step) {
             const double *sc = scales + (c >> log_group) * kWide; // a stage begins where a group does, or has only one
-            if (row0 == col0) triangle<BYTES>(total, codes + row0 * kPitch, sc + row0, kPitch, c, c + step);
-            else square<BYTES>(total, codes + row0 * kPitch, sc + row0, col0 - row0, col_blocks, kPitch, c, c + step);
+            strip<BYTES>(total, codes + row0 * kPitch, sc + row0, col0 - row0, col_blocks, kPitch, c, c + step);
         }
         s = next;
         parity ^= 1;
@@ -648,27 +620,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gram_ring_kernel(const Distance
     for (int k = 0; k < SETS; ++k) {
         __syncthreads();
         if (set != k) continue;
-        auto put = [&](int x, int y, double v) {
-            double *at = sums + min(x, y) * kWide + max(x, y);
-            *at = k ? *at + v : v;
-        };
-        if (row0 == col0) {
-            using V = Cover<4>;
 #pragma unroll
-            for (int v = 0; v < V::kTiles; ++v)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int block = e < 2 ? V::lo(v) : V::hi(v);
-                    if (block < 0) continue;
-                    const int x = block * 8 + g, y = V::col(v) * 8 + t * 2 + (e & 1);
-                    if (block != V::col(v) || x <= y) put(row0 + x, row0 + y, total[v][e]);
-                }
-        } else {
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) put(row0 + (v & 1) * 16 + (e >> 1) * 8 + g, col0 + (v >> 1) * 8 + t * 2 + (e & 1), total[v][e]);
-        }
+            for (int e = 0; e < 4; ++e) {
+                const int x = row0 + (e >> 1) * 8 + g, y = col0 + j * 8 + t * 2 + (e & 1);
+                if (j >= col_blocks || x > y) continue;
+                double *at = sums + x * kWide + y;
+                *at = k ? *at + total[j][e] : total[j][e];
+            }
     }
     __syncthreads();
     double *out = a.partial + (size_t)blockIdx.x * (kWide * kWide + kWide);
@@ -787,7 +747,7 @@ template <int NB, int LOG_UNIT, int BYTES, int WARPS, int SETS> int launch_ring(
     r.groups = a.group < kUnit ? kUnit / a.group : 1;
     r.stage_bytes = (r.rows * kPitch + r.rows * r.groups * 4 + 127) / 128 * 128;
     r.spare = (NB * 8 - r.rows) * kPitch;
-    const int wide = 2 * r.groups * NB * 8 * 8;
+    const int wide = 2 * r.groups * NB * 8 * 8 + kSlotStages * NB * 8 * 4; // 64-bit scales, slots
     r.stages = (kRingBytes - r.spare - wide) / r.stage_bytes;
     if (r.stages > 8) r.stages = 8;
     static bool set[64] = {};
@@ -824,9 +784,9 @@ template <int BYTES> int launch_gram(Context *ctx, const DistanceArgs &a, const 
     case 2: return launch_direct<2, BYTES, BYTES == 8 ? 128 : 256>(a, p, stream);
     case 3: return launch_direct<3, BYTES, 128>(a, p, stream);
     case 4: return launch_direct<4, BYTES, 64>(a, p, stream);
-    case 8: return small ? launch_ring<8, 8, BYTES, 12, 4>(ctx, a, p, stream) : launch_ring<8, 9, BYTES, 12, 4>(ctx, a, p, stream); // three pairs of groups of 32
-    case 12: return launch_ring<12, 8, BYTES, 12, 2>(ctx, a, p, stream); // six
-    case 16: return launch_ring<16, 8, BYTES, 10, 1>(ctx, a, p, stream); // ten
+    case 8: return small ? launch_ring<8, 8, BYTES, 12, 2>(ctx, a, p, stream) : launch_ring<8, 9, BYTES, 12, 2>(ctx, a, p, stream); // three pairs of groups of 32, two warps each
+    case 12: return launch_ring<12, 8, BYTES, 12, 1>(ctx, a, p, stream); // six
+    case 16: return launch_ring<16, 8, BYTES, 20, 1>(ctx, a, p, stream); // ten
     }
     gram_kernel<BYTES><<<dim3((unsigned)p.tiles, (unsigned)p.blocks), kWarps * 32, 0, stream>>>(a, p.n_blocks);
     return LB_OK;

@@ -26,6 +26,7 @@ import numpy as np
 import torch
 
 from . import pycahel as cahel
+from .updates import UpdateCache, low_rank_update
 
 # module constants of the reference driver (byzantine_fl.py:23-34)
 lazy_relin_flag = 1
@@ -489,10 +490,23 @@ class EncryptedKrum:
         v = self._as_chunks(update)
         return self.encrypt_chunks(v, self.client_seeds(client, v.shape[0]), out=out)
 
+    def encrypt_low_rank(self, factors, client=0, out=None):
+        """An update of low rank, given by 8-bit factors (see ``updates.low_rank_update``) -> ciphertexts [chunks][2][3][N], the same as
+        ``encrypt_client`` of the update that the factors stand for."""
+        return self.encrypt_client(low_rank_update(self.lb, factors), client=client, out=out)
+
+    def update_cache(self, n_clients, dim, group=128):
+        """An empty 8-bit cache for the updates of n_clients clients, in pages that ``round`` and ``encrypt_slices`` read chunk by chunk"""
+        return UpdateCache(self.lb, n_clients, dim, page=self.slots, group=group)
+
     def staged(self, updates, clients):
         """Yields (client, update on the device) for the given clients.  Updates that live in host
         memory are copied on a side stream one client ahead of the encryption that consumes them (two
         device buffers), so a pinned host tensor streams in behind the encode + encrypt kernels."""
+        if isinstance(updates, UpdateCache):
+            for c in clients:
+                yield c, updates.read(c)[0]
+            return
         if updates.is_cuda:
             for c in clients:
                 yield c, updates[c]
@@ -523,7 +537,7 @@ class EncryptedKrum:
 
     def encrypt_slices(self, updates, c_lo, c_hi):
         """Encodes and encrypts chunks [c_lo, c_hi) of EVERY client: updates [n_clients][dim] (CUDA, pinned or pageable
-        host) -> ciphertexts [n_clients][c_hi - c_lo][2][3][N].  Several clients' slices share one fused encode + encrypt
+        host, or an ``UpdateCache``) -> ciphertexts [n_clients][c_hi - c_lo][2][3][N].  Several clients' slices share one fused encode + encrypt
         call so that a launch fills the GPU in whole waves even when a rank only holds a few dozen chunks per client;
         rows are copied into a zero-padded staging buffer (on a side stream, one group ahead, when they come from
         host memory)."""
@@ -537,6 +551,8 @@ class EncryptedKrum:
         if k == 0:
             return cts
         groups = [list(range(g, min(g + per_call, n_clients))) for g in range(0, n_clients, per_call)]
+        if isinstance(updates, UpdateCache):
+            return self._encrypt_cached(updates, c_lo, c_hi, groups, cts)
         dtype = updates.dtype if updates.dtype in (torch.float32, torch.float64) else torch.float64
         n_buf = 2 if len(groups) > 1 else 1
         bufs = [torch.zeros(per_call, k * self.slots, dtype=dtype, device=dev) for _ in range(n_buf)]
@@ -572,6 +588,19 @@ class EncryptedKrum:
                 free[b].record(main)
             elif i + 1 < len(groups):
                 start(i + 1)
+        return cts
+
+    def _encrypt_cached(self, cache, c_lo, c_hi, groups, cts):
+        """encrypt_slices of an 8-bit cache: the chunks of a group of clients are read back into one staging buffer and encrypted from there"""
+        if self.slots % cache.page:
+            raise ValueError("the cache's pages must divide a chunk of %d slots" % self.slots)
+        k, per_chunk = c_hi - c_lo, self.slots // cache.page
+        p_lo, p_hi = c_lo * per_chunk, min(c_hi * per_chunk, cache.pages)
+        buf = torch.zeros(len(groups[0]), k * self.slots, device=cache.device)
+        for grp in groups:
+            cache.read(slice(grp[0], grp[-1] + 1), p_lo, p_hi - p_lo, out=buf[: len(grp), : (p_hi - p_lo) * cache.page])
+            seeds = np.concatenate([self.client_seeds(c, k, first_chunk=c_lo) for c in grp])
+            self.encrypt_chunks(buf[: len(grp)].view(len(grp) * k, self.slots), seeds, out=cts[grp[0]: grp[-1] + 1].view(len(grp) * k, 2, 3, self.N))
         return cts
 
     # -- server side ---------------------------------------------------------------------------
@@ -698,7 +727,7 @@ class EncryptedKrum:
 
     # -- one round ---------------------------------------------------------------------------------
     def round(self, updates, rank=0, world_size=1, group=None, keep=None, timing=None, exchange="chunks"):
-        """updates: [n_clients][dim] tensor (CUDA, pinned or pageable host).  Every rank runs this; rank 0 returns
+        """updates: [n_clients][dim] tensor (CUDA, pinned or pageable host) or ``UpdateCache``.  Every rank runs this; rank 0 returns
         (distances, order), the others (None, None).
         exchange: how several ranks share the work.
         "chunks" (default): the pair sum is linear in the chunk axis, so rank r encrypts chunks
@@ -837,7 +866,10 @@ def gather_scores(local, schedule, rank, world_size, group=None):
 
 def plaintext_krum(updates):
     """float64 reference of the selection rule as Lancelot applies it (byzantine_fl.py:527-536:
-    sum of squared distances to ALL other clients, argmin)."""
+    sum of squared distances to ALL other clients, argmin).  For an ``UpdateCache`` the distances come from its codes, on the GPU."""
+    if isinstance(updates, UpdateCache):
+        d = updates.distances().sum(1).cpu()
+        return d.tolist(), np.argsort(d.numpy())
     x = updates.to(torch.float64)
     n = x.shape[0]
     d = torch.zeros(n, dtype=torch.float64)

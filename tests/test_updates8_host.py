@@ -1,0 +1,62 @@
+"""8-bit updates without a GPU: what the calls refuse before they touch a device."""
+import pytest
+import torch
+
+
+def test_the_extension_refuses_tensors_that_are_not_on_the_device():
+    from lancelot_b200._lib import InvalidArgument
+    from lancelot_b200.pybind import _updates8 as m
+
+    v, codes, scales = torch.zeros(2, 64), torch.zeros(2, 64, dtype=torch.int8), torch.zeros(2, 1)
+    for call in (lambda: m.quantize_rows(0, 0, v, codes, scales, 0, None, None, None, None),
+                 lambda: m.dequantize_rows(0, 0, codes, scales, 64, 0, None, None, 1, None),
+                 lambda: m.int8_matmul(0, 0, codes, codes, v[0, :2], v[0, :2], 3, None),
+                 lambda: m.int8_distances(0, 0, codes, scales, torch.zeros(2, 1, dtype=torch.int32), 0)):
+        with pytest.raises(InvalidArgument, match="cuda:0"):
+            call()
+    with pytest.raises(TypeError):
+        m.int8_matmul(0, 0, [[1]], codes, v, v, 3, None)
+
+
+def test_the_c_entries_refuse_a_null_context():
+    import ctypes as C
+
+    from lancelot_b200 import lib
+
+    z, n, f = C.c_int64(0), None, C.c_size_t(0)
+    assert lib.lb_quantize_rows(n, n, 1, z, z, z, n, n, n, z, n, z, C.c_int64(64), z, n, z, n, z, n, f, n) == 1
+    assert lib.lb_dequantize_rows(n, n, z, n, z, z, C.c_int64(64), z, n, z, z, n, 1, z, n) == 1
+    assert lib.lb_int8_matmul(n, z, z, z, n, z, n, n, z, n, n, 1, z, n, f, n) == 1
+    assert lib.lb_int8_distances(n, n, z, n, z, z, C.c_int64(64), z, n, z, z, n, n, f, n) == 1
+    assert b"context" in lib.lb_last_error()
+
+
+def test_workspaces_are_asked_for_only_where_they_are_needed():
+    import ctypes as C
+
+    from lancelot_b200 import lib
+
+    q, m, d = lib.lb_quantize_rows_workspace_bytes, lib.lb_int8_matmul_workspace_bytes, lib.lb_int8_distances_workspace_bytes
+    for f in (q, m, d):
+        f.restype = C.c_size_t
+    i = C.c_int64
+    assert q(i(5), i(1000), i(1008), i(0)) == 0 and q(i(5), i(1 << 20), i(1 << 20), i(128)) == 0
+    assert q(i(2), i(1 << 20), i(1 << 20), i(0)) == 2 * 32 * 4  # the maxima of parts of 32768 columns
+    assert q(i(0), i(5), i(16), i(0)) == 0 and q(i(1), i(1), i(15), i(0)) == 0
+    a, b = C.c_void_p(4096), C.c_void_p(8192)
+    assert m(i(8), i(8), i(64), a, i(64), b, i(64)) == 0
+    assert m(i(8), i(9), i(33), a, i(33), b, i(33)) == 512 + 9 * 48   # both packed to 48 bytes a row
+    assert m(i(8), i(9), i(64), C.c_void_p(4097), i(64), b, i(64)) == 512
+    assert m(i(8), i(9), i(131072), a, i(131072), b, i(131072)) == 0
+    assert d(None, i(4), i(4), i(64)) == 0
+
+
+def test_a_cache_checks_its_sizes():
+    from lancelot_b200.updates import UpdateCache
+
+    class Device:
+        device = 0
+
+    for args in ((0, 5), (3, 0), (3, 5, 24), (3, 5, 8), (3, 5, 32, 48), (3, 5, 32, 16)):
+        with pytest.raises(ValueError):
+            UpdateCache(Device(), *args)
