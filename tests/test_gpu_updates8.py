@@ -63,7 +63,8 @@ GROUPS = [0, 32, 64, 128, 256, 512, 1024, 4096, 65536]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
-@pytest.mark.parametrize("rows,cols,page", [(1, 1, 16), (3, 33, 48), (5, 1000, 1008), (2, 5000, 2048), (1, 70001, 32768), (2, 100000, 98304)])
+@pytest.mark.parametrize("rows,cols,page", [(1, 1, 16), (3, 33, 48), (5, 1000, 1008), (2, 5000, 2048), (3, 70001, 32768), (2, 100000, 98304), (3, 140003, 65536),
+                                            (2, 3001, 4096), (2, 20005, 16384)])
 def test_rows_written_and_read_back(ctx, dtype, rows, cols, page):
     import torch
 
@@ -302,6 +303,58 @@ def test_pair_distances(ctx, n, pages, page, group):
     assert torch.equal(got, got.T) and bool((got.diagonal() == 0).all())
     if n > 2:
         assert float(got[1, 2]) == 0.0 and torch.equal(got[1], got[2])
+
+
+def test_the_c_entry_takes_pages_in_order_where_no_slots_are_given(ctx):
+    import ctypes as C
+
+    import torch
+
+    from lancelot_b200._lib import check, lib
+
+    for n in (3, 40, 130):
+        pages, page = 3, 1024
+        codes = torch.randint(-127, 128, (n * pages, page), generator=gen(n), device="cuda", dtype=torch.int8)
+        scales = torch.rand(n * pages, 8, generator=gen(n + 1), device="cuda")
+        out, i, p = torch.empty(n, n, dtype=torch.float64, device="cuda"), C.c_int64, C.c_void_p
+        lib.lb_int8_distances_workspace_bytes.restype = C.c_size_t
+        need = lib.lb_int8_distances_workspace_bytes(ctx.h, i(n), i(pages), i(page))
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        call = lambda size: lib.lb_int8_distances(ctx.h, p(codes.data_ptr()), i(page), p(scales.data_ptr()), i(8), i(n * pages), i(page), i(128), None, i(n),  # noqa: E731
+                                                  i(pages), p(out.data_ptr()), p(ws.data_ptr()), C.c_size_t(size), ctx._stream())
+        check(call(need))
+        slots = torch.arange(n * pages, dtype=torch.int32, device="cuda").view(n, pages)
+        assert torch.equal(out, ctx.int8_distances(codes, scales, slots, group=128))
+        assert call(need - 1) == 1 and b"workspace" in lib.lb_last_error()
+
+
+def test_two_streams_at_once(ctx):
+    """calls of one context on two streams share no scratch: each gives what it gives alone"""
+    import torch
+
+    n, page = 40, 4096
+    sets = []
+    for k in range(2):
+        codes = torch.randint(-127, 128, (n, page), generator=gen(k), device="cuda", dtype=torch.int8)
+        sets.append((codes, torch.rand(n, 32, generator=gen(9 + k), device="cuda"), torch.rand(n, generator=gen(20 + k), device="cuda")))
+    slots = torch.arange(n, dtype=torch.int32, device="cuda").view(n, 1)
+    odd = [c[:, :1001] for c, _, _ in sets]
+
+    def work(k):
+        codes, scales, s = sets[k]
+        return ctx.int8_distances(codes, scales, slots, group=128), ctx.int8_matmul(odd[k], odd[k], s, s, dtype=torch.float32)
+
+    alone = [work(k) for k in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        got = []
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append(work(k))
+        torch.cuda.synchronize()
+        for x, y in zip(got, alone):
+            assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
 
 
 def test_distances_of_a_row_that_is_not_a_number(ctx):
