@@ -472,12 +472,21 @@ int product_typed(Context *ctx, int m, int n, int k, const signed char *a, long 
     p.align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
     p.status = ctx->d_status;
     p.band = 8;
-    // The widest tile that still gives every SM one.  Up to kShort blocks of k, and where rows are off their alignment, the form that takes
-    // results out faster
+    // Up to kShort blocks of k, and where rows are off their alignment, the form that takes results out faster (4096 x 4096 x 1024 in bf16:
+    // 19.0 us instead of 24.6; from k = 2048 on its three stages cost more: 8192 x 8192 x 4096 205 us instead of 188).
     const bool quick = p.k_blocks <= kShort || p.align == 0;
-    const int widest = quick ? 128 : 256;
+    // The tile whose waves over the SMs take least: a block of k costs what its (128 + bn) x 128 bytes take from L2 to the SM, some
+    // 58 bytes a cycle (0.22, 0.29, 0.43 us), a tile about a microsecond and the time of its results beside that.
     int bn = 64;
-    while (bn < widest && (long)p.tiles_m * ((n + 2 * bn - 1) / (2 * bn)) >= ctx->sm_count) bn *= 2;
+    double least = 0.0;
+    for (int b = 64; b <= 256; b *= 2) {
+        const long tiles = (long)p.tiles_m * ((n + b - 1) / b), waves = (tiles + ctx->sm_count - 1) / ctx->sm_count;
+        const double us = (double)waves * ((double)p.k_blocks * (128 + b) * 1.15e-3 + 0.7 + b * 6e-3);
+        if (least == 0.0 || us < least) {
+            least = us;
+            bn = b;
+        }
+    }
     p.tiles_n = (n + bn - 1) / bn;
     CUtensorMap ma, mb, mo;
     int rc = encode_map(&ma, a, m, k, a_stride, kTileK, kTileM);
@@ -489,6 +498,7 @@ int product_typed(Context *ctx, int m, int n, int k, const signed char *a, long 
         p.align = 1;
     }
     count_launch("int8_tiles", stream, bytes);
+    if (quick && bn == 256) return launch_tiles<T, 256, true>(ctx, ma, mb, mo, p, stream);
     if (quick) return bn == 128 ? launch_tiles<T, 128, true>(ctx, ma, mb, mo, p, stream) : launch_tiles<T, 64, true>(ctx, ma, mb, mo, p, stream);
     if (bn == 256) return launch_tiles<T, 256, false>(ctx, ma, mb, mo, p, stream);
     if (bn == 128) return launch_tiles<T, 128, false>(ctx, ma, mb, mo, p, stream);
