@@ -255,38 +255,33 @@ template <> struct Cover<2> : Tiles<2, 0x00, 0xf1, 0x01> {};
 template <> struct Cover<3> : Tiles<3, 0x100, 0x212, 0x210> {};
 template <> struct Cover<4> : Tiles<6, 0x103210, 0xff0321, 0x320321> {};
 
-// 16 clients (`codes`, `scales` at the first) with the first `blocks` x 8 of 32 clients `apart` rows further down: columns [begin, end), one
-// scale each
-template <int BYTES>
-__device__ __forceinline__ void strip(double (&total)[4][4], const unsigned char *codes, const double *scales, int apart, int blocks, int pitch, int begin, int end)
+// 16 clients (`codes`, `scales` at the first) with BLOCKS x 8 clients `apart` rows further down: columns [begin, end), one scale each.
+// BLOCKS is a constant so that all loads of a step are on their way before its first product.
+template <int BYTES, int BLOCKS>
+__device__ __forceinline__ void strip(double (&total)[4][4], const unsigned char *codes, const double *scales, int apart, int pitch, int begin, int end)
 {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const unsigned char *at = codes + g * pitch + t * BYTES, *other = at + apart * pitch;
-    int acc[4][4];
+    int acc[BLOCKS][4];
     auto step = [&](int c, auto first) {
-        unsigned lo[BYTES / 4], hi[BYTES / 4];
+        unsigned lo[BYTES / 4], hi[BYTES / 4], b[BLOCKS][BYTES / 4];
         load_rows<BYTES>(lo, at + c);
         load_rows<BYTES>(hi, at + 8 * pitch + c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j >= blocks) break;
-            unsigned b[BYTES / 4];
-            load_rows<BYTES>(b, other + j * 8 * pitch + c);
+        for (int j = 0; j < BLOCKS; ++j) load_rows<BYTES>(b[j], other + j * 8 * pitch + c);
 #pragma unroll
-            for (int k = 0; k < BYTES / 4; k += 2) {
-                if (decltype(first)::value && k == 0) mma_s8_from(acc[j], kBias, lo[k], hi[k], lo[k + 1], hi[k + 1], b[k], b[k + 1]);
-                else mma_s8(acc[j], lo[k], hi[k], lo[k + 1], hi[k + 1], b[k], b[k + 1]);
+        for (int k = 0; k < BYTES / 4; k += 2)
+#pragma unroll
+            for (int j = 0; j < BLOCKS; ++j) {
+                if (decltype(first)::value && k == 0) mma_s8_from(acc[j], kBias, lo[k], hi[k], lo[k + 1], hi[k + 1], b[j][k], b[j][k + 1]);
+                else mma_s8(acc[j], lo[k], hi[k], lo[k + 1], hi[k + 1], b[j][k], b[j][k + 1]);
             }
-        }
     };
     step(begin, std::true_type());
     for (int c = begin + 4 * BYTES; c < end; c += 4 * BYTES) step(c, std::false_type());
     const double lo = scales[g], hi = scales[8 + g];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (j >= blocks) break;
-        apply_scales(total[j], acc[j], lo, hi, *reinterpret_cast<const double2 *>(scales + apart + j * 8 + t * 2));
-    }
+    for (int j = 0; j < BLOCKS; ++j) apply_scales(total[j], acc[j], lo, hi, *reinterpret_cast<const double2 *>(scales + apart + j * 8 + t * 2));
 }
 
 // ---- up to 32 clients: no shared memory ----------------------------------------------------------------------------------------
@@ -606,9 +601,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gram_ring_kernel(const Distance
         const unsigned char *codes = ring + (size_t)s * r.stage_bytes;
         const int to = min((set + 1) * kPer, columns);
         const double *scales = wide_scales + parity * r.groups * kWide;
-        for (int c = set * kPer; c < to; c += step) {
-            const double *sc = scales + (c >> log_group) * kWide; // a stage begins where a group does, or has only one
-            strip<BYTES>(total, codes + row0 * kPitch, sc + row0, col0 - row0, col_blocks, kPitch, c, c + step);
+        auto all = [&](auto blocks) {
+            for (int c = set * kPer; c < to; c += step) {
+                const double *sc = scales + (c >> log_group) * kWide; // a stage begins where a group does, or has only one
+                strip<BYTES, decltype(blocks)::value>(total, codes + row0 * kPitch, sc + row0, col0 - row0, kPitch, c, c + step);
+            }
+        };
+        switch (col_blocks) {
+        case 4: all(std::integral_constant<int, 4>()); break;
+        case 3: all(std::integral_constant<int, 3>()); break;
+        case 2: all(std::integral_constant<int, 2>()); break;
+        case 1: all(std::integral_constant<int, 1>()); break;
         }
         s = next;
         parity ^= 1;
