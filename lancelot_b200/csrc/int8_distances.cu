@@ -200,7 +200,7 @@ template <int BYTES> __global__ void __launch_bounds__(kWarps * 32) gram_kernel(
 }
 
 // ---- pieces of the kernels for up to 128 clients ----------------------------------------------------------------------------------
-constexpr int kRingBytes = 216 * 1024;
+constexpr int kRingBytes = 226 * 1024;
 constexpr int kSlotStages = 16; // stages whose slots are held; at least twice the ring's
 
 // An integer sum as a 64-bit float, without the conversion unit (which takes 8 cycles for what the FP64 pipe does in 2): sums start
@@ -214,6 +214,7 @@ struct Ring {
     int stage_bytes; // codes [rows][pitch], then scales [rows][groups] in 32 bits
     int stages;
     int spare;       // bytes behind the ring that a read of rows beyond `rows` may reach
+    int wide;        // bytes of the scales in 64 bits and of the slots
 };
 
 // Eight rows of codes at columns `at` of a stage, as four (two) k-slots of the matrix instruction
@@ -452,9 +453,11 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 4 ? 1 : 2) gram_direct_kern
 // ahead (cp.async; one barrier a stage), and each warp multiplies 16 clients with 32.  Rows lie 64 bytes off a multiple of 128 apart, so
 // that the 16-byte loads of eight rows fall on different banks.
 //
-// Bound by instructions and by shared memory, which every warp reads six 512-byte rows from for four products: 100 x 1.6 M takes 142 us
-// with one scale a page, 185 us with groups of 64 (26 us at the copy rate).  32 by 32 clients a warp, which read less, left too few warps
-// (162, 219 us); slots looked up by every thread for itself instead of by way of shared memory took 180, 224 us.
+// Bound by the warps' own work, which is most of the time even without the copies: 100 x 1.6 M takes 94 us with one scale a page, 147 us
+// with groups of 64 (26 us at the copy rate).  Each group costs three 64-bit operations a pair and group, 50 us at their rate; a step's six
+// 512-byte rows of loads and up to eight products wait for one another.  Stages of 256 columns took 124, 161 us, loads next to their products
+// 142, 186 us; 32 by 32 clients a warp, which read less, left too few warps (162, 219 us); a barrier for each stage and warp instead of one
+// for all took 152, 245 us.
 //
 // NB: blocks of eight clients: 8, 12 or 16.  SETS warps split the columns of a stage, 2^LOG_UNIT, for the same pairs.  Sizes are constants
 // because divisions by a unit of run-time size took more instructions than all the rest.
@@ -536,8 +539,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) gram_ring_kernel(const Distance
     };
 
     // the pairs of this warp: 16 rows from row0 on with up to 32 from col0 on; two warps make a pair of groups
-    const int set = warp % SETS, half = warp / SETS & 1;
-    int row0 = 0, col0 = warp / SETS / 2;
+    const int set = warp % SETS, pair = warp / SETS / 2, half = (warp / SETS & 1) ^ (NB == 8 ? pair >> 1 & 1 : pair >> 2 & 1); // (the quarters of
+    int row0 = 0, col0 = pair;                                                    // an SM, warps modulo 4, get equal numbers of products this way)
     constexpr int kGroups = NB / 4;
     while (col0 >= kGroups - row0) col0 -= kGroups - row0++;
     const bool same = col0 == 0; // a group with itself: the lower half has nothing to do with the upper
@@ -714,7 +717,21 @@ struct DistancePlan {
     size_t bytes;
 };
 
-DistancePlan distance_plan(int sm_count, int n, long pages, int page)
+Ring ring_shape(int blocks, int unit, int n, int group) // blocks of eight clients
+{
+    Ring r;
+    r.rows = (n + 7) / 8 * 8;
+    r.groups = group < unit ? unit / group : 1;
+    r.stage_bytes = (r.rows * (unit + 64) + r.rows * r.groups * 4 + 127) / 128 * 128;
+    r.spare = r.rows % 16 * (unit + 64); // a warp reads 16 rows from a multiple of 16 below n on
+    r.wide = 2 * r.groups * blocks * 8 * 8 + kSlotStages * blocks * 8 * 4;
+    r.stages = (kRingBytes - r.spare - r.wide) / r.stage_bytes;
+    if (r.stages > 8) r.stages = 8;
+    return r;
+}
+
+// A smaller group never takes larger units, nor fewer blocks
+DistancePlan distance_plan(int sm_count, int n, long pages, int page, int group)
 {
     DistancePlan p;
     p.n_blocks = (n + 31) / 32;
@@ -724,7 +741,7 @@ DistancePlan distance_plan(int sm_count, int n, long pages, int page)
     const bool ring = n > 32 && n <= 128;
     const int warp_blocks = p.rows ? (p.rows == 32 ? 1 : 2) * sm_count : (2 * sm_count + p.tiles - 1) / p.tiles;
     const long takers = ring ? sm_count : (long)warp_blocks * kWarps;
-    p.unit = !ring ? 1024 : p.rows > 64 ? 256 : 512;
+    p.unit = !ring ? 1024 : ring_shape(p.rows / 8, 512, n, group).stages >= 3 ? 512 : 256; // of 100 x 1.6 M: 153 us with 512, 161 us with 256
     p.least_unit = !ring ? 128 : 256;
     while (p.unit > p.least_unit && pages * ((page + p.unit - 1) / p.unit) < takers) p.unit >>= 1;
     p.units = pages * ((page + p.unit - 1) / p.unit);
@@ -744,21 +761,13 @@ DistancePlan distance_plan(int sm_count, int n, long pages, int page)
 
 template <int NB, int LOG_UNIT, int BYTES, int WARPS, int SETS> int launch_ring(Context *ctx, const DistanceArgs &a, const DistancePlan &p, cudaStream_t stream)
 {
-    constexpr int kUnit = 1 << LOG_UNIT, kPitch = kUnit + 64;
-    Ring r;
-    r.rows = (a.n + 7) / 8 * 8;
-    r.groups = a.group < kUnit ? kUnit / a.group : 1;
-    r.stage_bytes = (r.rows * kPitch + r.rows * r.groups * 4 + 127) / 128 * 128;
-    r.spare = (NB * 8 - r.rows) * kPitch;
-    const int wide = 2 * r.groups * NB * 8 * 8 + kSlotStages * NB * 8 * 4; // 64-bit scales, slots
-    r.stages = (kRingBytes - r.spare - wide) / r.stage_bytes;
-    if (r.stages > 8) r.stages = 8;
+    const Ring r = ring_shape(NB, 1 << LOG_UNIT, a.n, a.group);
     static bool set[64] = {};
     if (ctx->device >= 64 || !set[ctx->device]) {
         LB_CUDA(cudaFuncSetAttribute(gram_ring_kernel<NB, LOG_UNIT, BYTES, WARPS, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
         if (ctx->device < 64) set[ctx->device] = true;
     }
-    gram_ring_kernel<NB, LOG_UNIT, BYTES, WARPS, SETS><<<p.blocks, WARPS * 32, r.stages * r.stage_bytes + r.spare + wide, stream>>>(a, r);
+    gram_ring_kernel<NB, LOG_UNIT, BYTES, WARPS, SETS><<<p.blocks, WARPS * 32, r.stages * r.stage_bytes + r.spare + r.wide, stream>>>(a, r);
     return LB_OK;
 }
 
@@ -788,8 +797,8 @@ template <int BYTES> int launch_gram(Context *ctx, const DistanceArgs &a, const 
     case 3: return launch_direct<3, BYTES, 128>(a, p, stream);
     case 4: return launch_direct<4, BYTES, 64>(a, p, stream);
     case 8: return small ? launch_ring<8, 8, BYTES, 12, 2>(ctx, a, p, stream) : launch_ring<8, 9, BYTES, 12, 2>(ctx, a, p, stream); // three pairs of groups of 32, two warps each
-    case 12: return launch_ring<12, 8, BYTES, 12, 1>(ctx, a, p, stream); // six
-    case 16: return launch_ring<16, 8, BYTES, 20, 1>(ctx, a, p, stream); // ten
+    case 12: return small ? launch_ring<12, 8, BYTES, 12, 1>(ctx, a, p, stream) : launch_ring<12, 9, BYTES, 12, 1>(ctx, a, p, stream); // six
+    case 16: return small ? launch_ring<16, 8, BYTES, 20, 1>(ctx, a, p, stream) : launch_ring<16, 9, BYTES, 20, 1>(ctx, a, p, stream); // ten
     }
     gram_kernel<BYTES><<<dim3((unsigned)p.tiles, (unsigned)p.blocks), kWarps * 32, 0, stream>>>(a, p.n_blocks);
     return LB_OK;
@@ -797,7 +806,7 @@ template <int BYTES> int launch_gram(Context *ctx, const DistanceArgs &a, const 
 
 } // namespace
 
-size_t int8_distances_workspace_bytes(const Context *ctx, int n, long pages, int page) { return distance_plan(ctx->sm_count, n, pages, page).bytes; }
+size_t int8_distances_workspace_bytes(const Context *ctx, int n, long pages, int page) { return distance_plan(ctx->sm_count, n, pages, page, 32).bytes; }
 
 int int8_distances(Context *ctx, const signed char *codes, long code_stride, const float *scales, long scale_stride, long n_slots, int page,
                    int group, const int *slots, int n, int pages, double *out, void *workspace, cudaStream_t stream)
@@ -807,7 +816,8 @@ int int8_distances(Context *ctx, const signed char *codes, long code_stride, con
         LB_CUDA(cudaMemsetAsync(out, 0, (size_t)n * n * sizeof(double), stream));
         return LB_OK;
     }
-    const DistancePlan p = distance_plan(ctx->sm_count, n, pages, page);
+    if (group == 0 || group >= page) group = 1 << 30;
+    const DistancePlan p = distance_plan(ctx->sm_count, n, pages, page, group);
     DistanceArgs a;
     a.codes = codes;
     a.code_stride = code_stride;
@@ -818,7 +828,7 @@ int int8_distances(Context *ctx, const signed char *codes, long code_stride, con
     a.n = n;
     a.pages = pages;
     a.page = page;
-    a.group = group == 0 || group >= page ? 1 << 30 : group;
+    a.group = group;
     a.unit = p.unit;
     a.units_per_page = (unsigned)((page + p.unit - 1) / p.unit);
     a.units = (unsigned)p.units;
