@@ -795,7 +795,7 @@ int lb_quantize_rows(lb_context *h, const void *values, int dtype, int64_t n_row
     if ((rc = workspace_ok(workspace, workspace_bytes, lb_quantize_rows_workspace_bytes(n_rows, n_cols, page, group)))) return rc;
     return quantize_rows(values, dtype, n_rows, n_cols, value_stride, lengths, residual, residual_out, residual_stride, slots, n_slots, (int)page,
                          (int)(group > page ? page : group), reinterpret_cast<signed char *>(codes), code_stride, scales, scale_stride, workspace,
-                         S(stream));
+                         C(h)->d_status, S(stream));
 }
 
 int lb_dequantize_rows(lb_context *h, const int8_t *codes, int64_t code_stride, const float *scales, int64_t scale_stride, int64_t n_slots,

@@ -200,7 +200,7 @@ int encrypt_asymmetric(Context *ctx, const u64 *pk, const u64 *pt, int pt_is_coe
 size_t quantize_workspace_bytes(long n_rows, long n_cols, int page, int group);
 int quantize_rows(const void *values, int dtype, long n_rows, long n_cols, long value_stride, const int *lengths, const float *residual,
                   float *residual_out, long residual_stride, const int *slots, long n_slots, int page, int group, signed char *codes,
-                  long code_stride, float *scales, long scale_stride, void *workspace, cudaStream_t stream);
+                  long code_stride, float *scales, long scale_stride, void *workspace, int *status, cudaStream_t stream);
 int dequantize_rows(const signed char *codes, long code_stride, const float *scales, long scale_stride, long n_slots, int page, int group,
                     const int *slots, long n_rows, long n_cols, void *out, int dtype, long out_stride, cudaStream_t stream);
 size_t int8_matmul_workspace_bytes(int m, int n, int k, const void *a, long a_stride, const void *b, long b_stride);

@@ -12,11 +12,11 @@
 // The same r is what the rounding lost, exactly: error feedback adds no error of its own.
 //
 // All kernels stream: bound by HBM at (value bytes + 1 + 8 with a residual) per value.
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "context.h"
+#include "tcgen05.cuh"
 
 namespace lb {
 
@@ -228,6 +228,7 @@ struct QuantizeArgs {
     float *scales;
     long scale_stride;
     int group, groups; // columns of a group, groups of a page
+    int *status;
 };
 
 // where a page's codes go; false: the page is skipped
@@ -385,14 +386,22 @@ __global__ void __launch_bounds__(256) quantize_warp_kernel(const QuantizeArgs a
 }
 
 // ---- groups of up to 65536 columns: a block, or a cluster of blocks, holds the group in registers ---------------------
-// A block of 256 threads holds 8192 columns.  One of 1024 threads for 32768 columns would be alone on its SM, and all of it would wait for
-// its loads, then compute, then store; the blocks of a cluster do these at different times from those of others on the SM.
+// A block of 256 threads holds up to 8192 columns.  One of 1024 threads for 32768 columns would be alone on its SM, and all of it would
+// wait for its loads, then compute, then store; the blocks of a cluster do these at different times from those of others on the SM.  They
+// send their maxima to one another, each to an mbarrier of its own, so that nobody waits for stores or for a barrier of the whole cluster.
+//
+// Bound by HBM, less what the wait for the slowest block costs: 20 x 11 M with one scale for 32768 columns takes 479 us with residuals (6.1
+// of 6.5 TB/s), 271 us without (4.1 TB/s; four loads of 16 bytes a thread, or as many blocks as 64 registers allow, gave 287 and 271,
+// and 497 and 520 with residuals; a barrier of the cluster instead of the messages 592 and 317); 100 x 1.6 M with groups of 4096, which
+// one block holds, 345 us (6.3 TB/s).
 template <int V> struct GroupShared {
     unsigned most[32 + 8]; // of the warps; of the cluster's blocks
     unsigned heads[V * 8 + 1]; // the first codes of every warp's pieces, in the order of their columns
+    unsigned long long arrived; // the cluster's maxima
+    int failed;
 };
 template <typename T, bool VEC, int V, bool FULL>
-__device__ __forceinline__ void quantize_group(const Run<T> &r, signed char *codes, float *scale, int length, GroupShared<V> &shared, bool leader, int peers)
+__device__ __forceinline__ void quantize_group(const Run<T> &r, signed char *codes, float *scale, int length, GroupShared<V> &shared, int peer, int peers, int *status)
 {
     constexpr int kThreads = 256, kRun = kThreads * V * 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, off = r.off, first = threadIdx.x * 4 - off;
@@ -411,14 +420,19 @@ __device__ __forceinline__ void quantize_group(const Run<T> &r, signed char *cod
     __syncthreads();
     m = __reduce_max_sync(0xffffffffu, lane < kThreads / 32 ? shared.most[lane] : 0);
     if (peers > 1) { // the other blocks' maxima, by way of their shared memory
-        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); // all of them have begun
-        if (threadIdx.x < (unsigned)peers) *cluster.map_shared_rank(shared.most + 32 + cluster.block_rank(), threadIdx.x) = m;
-        cluster.sync();
+        const unsigned arrived = smem_u32(&shared.arrived);
+        if (threadIdx.x < (unsigned)peers)
+            asm volatile("{\n\t.reg .b32 to, bar;\n\tmapa.shared::cluster.u32 to, %0, %2;\n\tmapa.shared::cluster.u32 bar, %1, %2;\n\t"
+                         "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [to], %3, [bar];\n\t}" ::"r"(smem_u32(shared.most + 32 + peer)),
+                         "r"(arrived), "r"(threadIdx.x), "r"(m)
+                         : "memory");
+        if (!mbar_wait(arrived, 0, &shared.failed)) atomicOr(status, 2); // a block leaves when all maxima are there: none is sent to one that has left
+        __syncwarp();
         m = __reduce_max_sync(0xffffffffu, lane < peers ? shared.most[32 + lane] : 0);
     }
     const float s = scale_of(m);
-    if (leader && threadIdx.x == 0) *scale = s;
+    if (peer == 0 && threadIdx.x == 0) *scale = s;
     unsigned q[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) q[j] = codes4(v[j], s);
@@ -448,7 +462,7 @@ __device__ __forceinline__ void quantize_group(const Run<T> &r, signed char *cod
     if (off && threadIdx.x == 0) store_piece<false>(r.lost, kRun - off, last, 0, min(r.hi, kRun));
 }
 
-template <typename T, bool VEC, int V> __global__ void __launch_bounds__(256, V == 4 ? 4 : 2) quantize_block_kernel(const QuantizeArgs a, const int peers)
+template <typename T, bool VEC, int V> __global__ void __launch_bounds__(256, V == 8 ? 3 : 5) quantize_block_kernel(const QuantizeArgs a, const int peers)
 {
     __shared__ GroupShared<V> shared;
     const unsigned group_index = blockIdx.x / peers, peer = blockIdx.x - group_index * peers;
@@ -456,15 +470,24 @@ template <typename T, bool VEC, int V> __global__ void __launch_bounds__(256, V 
     const unsigned row = page_index / (unsigned)a.pages, page = page_index - row * (unsigned)a.pages;
     long slot;
     if (!page_slot(a, page_index, slot)) return; // all blocks of a cluster alike
-    if (peers > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); // nothing has been written yet
+    if (peers > 1) {
+        if (threadIdx.x == 0) {
+            mbar_init(smem_u32(&shared.arrived), 1);
+            mbar_expect(smem_u32(&shared.arrived), peers * 4);
+            shared.failed = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    }
     constexpr int kRun = 256 * V * 4;
     const int first = g * a.group + peer * kRun, end = min(a.page, (int)(g + 1) * a.group); // columns inside the page
     const long limit = min(row_limit(a, row), (long)page * a.page + end), col = (long)page * a.page + first;
     const Run<T> r = run_of<T, VEC>(a, row, col, limit, kRun);
     signed char *codes = a.codes + slot * a.code_stride + first;
     float *scale = a.scales + slot * a.scale_stride + g;
-    if (r.full) quantize_group<T, VEC, V, true>(r, codes, scale, end - first, shared, peer == 0, peers);
-    else quantize_group<T, VEC, V, false>(r, codes, scale, end - first, shared, peer == 0, peers);
+    if (r.full) quantize_group<T, VEC, V, true>(r, codes, scale, end - first, shared, (int)peer, peers, a.status);
+    else quantize_group<T, VEC, V, false>(r, codes, scale, end - first, shared, (int)peer, peers, a.status);
 }
 
 // ---- longer groups: the maxima of parts of 32768 columns first, then the codes -----------------------------------------
@@ -549,7 +572,6 @@ int quantize_typed(const QuantizeArgs &a, long n_rows, void *workspace, double b
         const long groups = n_pages * a.groups;
         if (longest <= 1024) return launch_block<T, VEC, 1>(a, groups, 1, stream);
         if (longest <= 4096) return launch_block<T, VEC, 4>(a, groups, 1, stream);
-        if (longest <= kBlock / 2 * kCluster) return launch_block<T, VEC, 4>(a, groups, (longest + kBlock / 2 - 1) / (kBlock / 2), stream);
         return launch_block<T, VEC, 8>(a, groups, (longest + kBlock - 1) / kBlock, stream);
     } else {
         const unsigned parts = (unsigned)((longest + kPart - 1) / kPart);
@@ -666,9 +688,10 @@ size_t quantize_workspace_bytes(long n_rows, long n_cols, int page, int group)
 
 int quantize_rows(const void *values, int dtype, long n_rows, long n_cols, long value_stride, const int *lengths, const float *residual,
                   float *residual_out, long residual_stride, const int *slots, long n_slots, int page, int group, signed char *codes,
-                  long code_stride, float *scales, long scale_stride, void *workspace, cudaStream_t stream)
+                  long code_stride, float *scales, long scale_stride, void *workspace, int *status, cudaStream_t stream)
 {
     QuantizeArgs a;
+    a.status = status;
     a.values = values;
     a.value_stride = value_stride;
     a.lengths = lengths;
