@@ -287,9 +287,20 @@ __device__ __forceinline__ void strip(double (&total)[4][4], const unsigned char
 
 // ---- up to 32 clients: no shared memory ----------------------------------------------------------------------------------------
 // A warp takes a unit of a page's columns, CHUNK columns at a time, the next ones on their way in registers while these are multiplied.
-// 16 warps an SM, none of which waits for another: 20 x 11 M in 61 us (3.8 TB/s), of which some 8 us are the first loads, the sums of the
-// blocks and the second kernel.  A client that is not there (or a page of one) is read as the cache's first
-// slot with scales of 0, so that no load needs a condition.
+// 16 warps an SM, none of which waits for another: 20 x 11 M in 56 us (4.2 TB/s), of which some 8 us are the first loads, the sums of the
+// blocks and the second kernel.  More bytes on their way would take more registers; loads that also bring the next chunk into L2 gained
+// 6 us of the 62.  Above 24 clients the sums leave room for 8 warps: 32 x 11 M in 136 us, 156 us with half the columns a chunk; scales
+// applied at the end of a group of several chunks gained 12 us there with one scale a page and cost up to 12 us below.  A client
+// that is not there (or a page of one) is read as the cache's first slot with scales of 0, so that no load needs a condition.
+
+// 16 bytes of codes; the 256 bytes around them are brought into L2, for the next chunk
+__device__ __forceinline__ uint4 load_and_next(const signed char *at)
+{
+    uint4 x;
+    asm volatile("ld.global.nc.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(at));
+    return x;
+}
+
 template <int NB, int BYTES, int CHUNK, int GROUPS> // GROUPS: scales of a chunk
 __global__ void __launch_bounds__(kWarps * 32, NB == 4 ? 1 : 2) gram_direct_kernel(const DistanceArgs a)
 {
@@ -351,7 +362,7 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 4 ? 1 : 2) gram_direct_kern
                 const bool inside = whole || at + i * STEP + t * BYTES < end;
                 if constexpr (BYTES == 16) {
                     uint4 x = make_uint4(0, 0, 0, 0);
-                    if (inside) x = __ldg(reinterpret_cast<const uint4 *>(src[r] + at + i * STEP));
+                    if (inside) x = load_and_next(src[r] + at + i * STEP);
                     k.w[r][i][0] = x.x;
                     k.w[r][i][1] = x.y;
                     k.w[r][i][2] = x.z;
@@ -779,11 +790,9 @@ template <int NB, int BYTES, int CHUNK> int launch_direct(const DistanceArgs &a,
         if (a.group < 128) gram_direct_kernel<NB, 16, CHUNK, 4><<<p.blocks, kWarps * 32, 0, stream>>>(a);
         else if (a.group < CHUNK) gram_direct_kernel<NB, 16, CHUNK, 2><<<p.blocks, kWarps * 32, 0, stream>>>(a);
         else gram_direct_kernel<NB, 16, CHUNK, 1><<<p.blocks, kWarps * 32, 0, stream>>>(a);
-    } else if constexpr (CHUNK == 128) {
+    } else {
         if (a.group < CHUNK) gram_direct_kernel<NB, 16, CHUNK, 2><<<p.blocks, kWarps * 32, 0, stream>>>(a);
         else gram_direct_kernel<NB, 16, CHUNK, 1><<<p.blocks, kWarps * 32, 0, stream>>>(a);
-    } else {
-        gram_direct_kernel<NB, 16, CHUNK, 1><<<p.blocks, kWarps * 32, 0, stream>>>(a);
     }
     return LB_OK;
 }
@@ -795,7 +804,7 @@ template <int BYTES> int launch_gram(Context *ctx, const DistanceArgs &a, const 
     case 1: return launch_direct<1, BYTES, 256>(a, p, stream);
     case 2: return launch_direct<2, BYTES, BYTES == 8 ? 128 : 256>(a, p, stream);
     case 3: return launch_direct<3, BYTES, 128>(a, p, stream);
-    case 4: return launch_direct<4, BYTES, 64>(a, p, stream);
+    case 4: return launch_direct<4, BYTES, BYTES == 8 ? 64 : 128>(a, p, stream);
     case 8: return small ? launch_ring<8, 8, BYTES, 12, 2>(ctx, a, p, stream) : launch_ring<8, 9, BYTES, 12, 2>(ctx, a, p, stream); // three pairs of groups of 32, two warps each
     case 12: return small ? launch_ring<12, 8, BYTES, 12, 1>(ctx, a, p, stream) : launch_ring<12, 9, BYTES, 12, 1>(ctx, a, p, stream); // six
     case 16: return small ? launch_ring<16, 8, BYTES, 20, 1>(ctx, a, p, stream) : launch_ring<16, 9, BYTES, 20, 1>(ctx, a, p, stream); // ten
