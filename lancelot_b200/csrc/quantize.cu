@@ -610,8 +610,8 @@ __device__ __forceinline__ float4 floats_of(unsigned x)
                        __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.0f, __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.0f);
 }
 
-// A warp takes 512 columns of a page: 20 x 11 M in 179 us (6.3 TB/s) as 32-bit floats, 132 us (5.1 TB/s) as bf16.  The results are written in aligned pieces of four (see Run), whose codes are put together from two
-// words.  ONE: one scale in a page
+// A warp takes 512 columns of a page: 20 x 11 M in 179 us (6.3 TB/s) as 32-bit floats, 132 us (5.1 TB/s) as bf16.  The results are
+// written in aligned pieces of four (see Run), whose codes are put together from two words.  ONE: one scale in a page
 template <typename T, bool ONE>
 __global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a, const unsigned tiles, const unsigned total)
 {
@@ -671,9 +671,9 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a,
         if (hi == 512 && (j > 0 || lane > 0)) store4<true>(out + lane * 4 + j * 128 - off, v, 4);
         else store_piece<true>(out, lane * 4 + j * 128 - off, v, 0, hi);
     }
-    if (hi == 512 && lane == 31) { // the columns before the next run's first piece
+    if (hi > 512 - off && lane == 31) { // the columns before the next run's first piece
         const float4 f = floats_of(q[3] >> (32 - 8 * off));
-        store_piece<false>(out, 512 - off, make_float4(s[3] * f.x, s[3] * f.y, s[3] * f.z, 0.f), 0, 512);
+        store_piece<false>(out, 512 - off, make_float4(s[3] * f.x, s[3] * f.y, s[3] * f.z, 0.f), 0, hi);
     }
 }
 

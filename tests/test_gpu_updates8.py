@@ -188,6 +188,32 @@ def test_lengths_slots_residual_and_strides(ctx, group):
     assert bool((out[:, :3] == 5).all()) and bool((out[:, 3 + cols:] == 5).all())
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("cols", [509, 510, 511, 512, 513, 1021, 1022, 1023])
+def test_rows_that_end_next_to_a_run_of_512_columns(ctx, dtype, cols):
+    """at every offset from an aligned piece, written and read back, with nothing touched beside the rows"""
+    import torch
+
+    dt = getattr(torch, dtype)
+    for group in (0, 32, 256):
+        for shift in range(4):
+            g = gen(cols * 4 + shift)
+            wide = torch.randn(3, cols + 1 + shift, generator=g, device="cuda").to(dt)
+            base = torch.full((3, cols + 5), 7.0, device="cuda")
+            v, lost = wide[:, shift:shift + cols], base[:, shift:shift + cols]
+            codes = torch.empty(6, 1008, dtype=torch.int8, device="cuda")[: 3 * -(-cols // 1008)]
+            scales = torch.empty(codes.shape[0], -(-1008 // group) if group else 1, device="cuda")
+            ctx.quantize_rows(v, codes, scales, group=group, residual_out=lost)
+            want_codes, want_scales, want_lost = quantized(v.float(), 1008, group)
+            assert torch.equal(codes, want_codes) and torch.equal(scales, want_scales) and torch.equal(lost, want_lost), (group, shift)
+            out = torch.full((3, cols + 5), 7.0, dtype=dt, device="cuda")
+            ctx.dequantize_rows(codes, scales, cols, group=group, out=out[:, shift:shift + cols])
+            want = torch.full_like(out, 7.0)
+            want[:, shift:shift + cols] = expanded(codes, scales, group).view(3, -1)[:, :cols].to(dt)
+            assert torch.equal(out, want), (group, shift)
+            assert (base[:, :shift] == 7).all() and (base[:, shift + cols:] == 7).all()
+
+
 def test_error_feedback_over_rounds_loses_nothing(ctx):
     """sum of what was sent plus the residual left = sum of the updates (to the roundings of the 32-bit sums t)"""
     import torch
