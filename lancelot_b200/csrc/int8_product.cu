@@ -499,8 +499,12 @@ int product_typed(Context *ctx, int m, int n, int k, const signed char *a, long 
     if ((rc = encode_map(&mb, b, n, k, b_stride, kTileK, bn))) return rc;
     mo = ma; // not used unless
     if (quick && p.align >= 16) {
-        if ((rc = encode_map(&mo, out, m, (long)n * (long)sizeof(T), out_stride * (long)sizeof(T), 128, 32, sizeof(T)))) return rc;
-        p.align = 1;
+        if ((long)n * (long)sizeof(T) % 16 != 0) { // a TMA store would write the rest of a row's last 16 bytes, which is not the result's
+            p.align = 0;
+        } else {
+            if ((rc = encode_map(&mo, out, m, (long)n * (long)sizeof(T), out_stride * (long)sizeof(T), 128, 32, sizeof(T)))) return rc;
+            p.align = 1;
+        }
     }
     count_launch("int8_tiles", stream, bytes);
     if (quick && bn == 256) return launch_tiles<T, 256, true>(ctx, ma, mb, mo, p, stream);

@@ -292,6 +292,23 @@ def test_product_of_strided_rows(ctx, m, n, k):
             assert bool((wide[:, :off] == 7).all()) and bool((wide[:, off + n:] == 7).all())
 
 
+@pytest.mark.parametrize("k", [16, 240, 2048])
+@pytest.mark.parametrize("n", [33, 36, 41, 44, 45, 130, 257, 260, 300])
+def test_product_into_aligned_rows_with_room_behind_them(ctx, n, k):
+    """rows of the result start on 16-byte boundaries and end between two: what lies behind their ends stays as it was"""
+    import torch
+
+    g = gen(n + k)
+    m = 70
+    a = torch.randint(-127, 128, (m, k), generator=g, device="cuda", dtype=torch.int8)
+    b = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    sa, sb = torch.rand(m, generator=g, device="cuda") * 1e-3, torch.rand(n, generator=g, device="cuda")
+    for dt in (torch.float32, torch.bfloat16, torch.float16):
+        wide = torch.full((m + 1, -(-n // 16) * 16 + 16), 7.0, dtype=dt, device="cuda")
+        check_product(ctx.int8_matmul(a, b, sa, sb, out=wide[:m, :n]), a, b, sa, sb)
+        assert bool((wide[:m, n:] == 7).all()) and bool((wide[m] == 7).all())
+
+
 def distances(codes, scales, slots, group):
     """from differences, in 64 bits, and how far sums of 64-bit floats may be off"""
     import torch
