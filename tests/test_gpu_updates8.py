@@ -371,6 +371,43 @@ def test_the_c_entry_takes_pages_in_order_where_no_slots_are_given(ctx):
         assert call(need - 1) == 1 and b"workspace" in lib.lb_last_error()
 
 
+def test_offsets_past_32_bits(ctx):
+    """slots, rows and results more than 2^32 bytes or elements from the start of their memory"""
+    import torch
+
+    g = gen(11)
+    page, cols = 32768, 40001
+    codes = torch.empty(140000, page, dtype=torch.int8, device="cuda")
+    scales = torch.empty(140000, page // 128, device="cuda")
+    slots = (torch.randperm(2000, generator=g, device="cuda")[:80] + 138000).int()
+    for n in (3, 40):
+        t = slots[: n * 2].view(n, 2)
+        v = torch.randn(n, cols, generator=g, device="cuda")
+        ctx.quantize_rows(v, codes, scales, group=128, slots=t)
+        want_codes, want_scales, _ = quantized(v, page, 128)
+        at = t.view(-1).long()
+        assert torch.equal(codes[at], want_codes) and torch.equal(scales[at], want_scales)
+        x = expanded(want_codes, want_scales, 128).view(n, -1)[:, :cols]
+        assert torch.equal(ctx.dequantize_rows(codes, scales, cols, group=128, slots=t), x)
+        want, tol = distances(want_codes, want_scales, torch.arange(2 * n, device="cuda", dtype=torch.int32).view(n, 2), 128)
+        assert bool(((ctx.int8_distances(codes, scales, t, group=128) - want).abs() <= tol).all())
+    del codes, scales
+    wide = torch.empty(40, 1 << 27, dtype=torch.bfloat16, device="cuda")
+    v = wide[::39, -cols:]
+    v.copy_(torch.randn(2, cols, generator=g, device="cuda"))
+    codes, scales = torch.empty(4, page, dtype=torch.int8, device="cuda"), torch.empty(4, 1, device="cuda")
+    ctx.quantize_rows(v, codes, scales)
+    want_codes, want_scales, _ = quantized(v.float(), page, 0)
+    assert torch.equal(codes, want_codes) and torch.equal(scales, want_scales)
+    ctx.dequantize_rows(codes, scales, cols, out=v)
+    assert torch.equal(v, expanded(codes, scales, 0).view(2, -1)[:, :cols].to(torch.bfloat16))
+    a = torch.randint(-127, 128, (40, 64), generator=g, device="cuda", dtype=torch.int8)
+    b = torch.randint(-127, 128, (301, 64), generator=g, device="cuda", dtype=torch.int8)
+    sa, sb = torch.rand(40, generator=g, device="cuda"), torch.rand(301, generator=g, device="cuda")
+    check_product(ctx.int8_matmul(a, b, sa, sb, out=wide[:, -304:-3]), a, b, sa, sb)
+    check_product(ctx.int8_matmul(a[:9], b, sa[:9], sb, out=wide[-9:, -304:-3]), a[:9], b, sa[:9], sb)
+
+
 def test_two_streams_at_once(ctx):
     """calls of one context on two streams share no scratch: each gives what it gives alone"""
     import torch
