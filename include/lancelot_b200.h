@@ -275,8 +275,8 @@ LB_API int lb_dequantize_rows(lb_context *ctx, const int8_t *codes, int64_t code
                        int64_t n_slots, int64_t page, int64_t group, const int32_t *slots, int64_t n_rows, int64_t n_cols, void *out,
                        int dtype, int64_t out_stride, void *stream);
 /* out[i][j] = (sum over k of a[i][k] b[j][k]) * a_scale[i] * b_scale[j]: an exact integer sum (k <= 131071), scaled in 32 bits, rounded to
- * dtype.  a [m][k], b [n][k], any alignment of their rows (rows off a 16-byte boundary are copied into the workspace first).
- * a_scale [m], b_scale [n]; out must not overlap an operand. */
+ * dtype.  a [m][k], b [n][k], any alignment of their rows (where m and n are above 32, rows off a 16-byte boundary
+ * are copied into the workspace first).  a_scale [m], b_scale [n]; out must not overlap an operand. */
 LB_API size_t lb_int8_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t a_stride, const int8_t *b, int64_t b_stride);
 LB_API int lb_int8_matmul(lb_context *ctx, int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t a_stride, const float *a_scale,
                    const int8_t *b, int64_t b_stride, const float *b_scale, void *out, int dtype, int64_t out_stride, void *workspace,

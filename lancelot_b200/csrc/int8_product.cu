@@ -23,28 +23,50 @@ __device__ __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v
 
 __device__ __forceinline__ float scaled(int sum, float sa, float sb) { return __int2float_rn(sum) * sa * sb; }
 
-// ---- rows copied to a 16-byte pitch --------------------------------------------------------------------------------------
-// Operands whose rows start off a 16-byte boundary are copied once, zeros up to the pitch: a TMA row and a 16-byte load have to
-// start on such a boundary.  Both operands go in one launch.
+// ---- rows off a 16-byte boundary --------------------------------------------------------------------------------------------
+// 16 codes from p on, zeros from `left` codes on.  Not aligned: out of the two aligned lines that they lie in, the second one only where it
+// holds one of them.
+template <bool ALIGNED> __device__ __forceinline__ uint4 load16(const signed char *p, int left)
+{
+    if (left <= 0) return make_uint4(0, 0, 0, 0);
+    if (ALIGNED) return __ldg(reinterpret_cast<const uint4 *>(p));
+    const unsigned shift = (unsigned)(uintptr_t)p & 15;
+    const uint4 *line = reinterpret_cast<const uint4 *>(p - shift);
+    const uint4 x = __ldg(line);
+    uint4 y = make_uint4(0, 0, 0, 0);
+    if ((int)shift + min(left, 16) > 16) y = __ldg(line + 1);
+    unsigned v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) v[i] = shift & 8 ? v[i + 2] : v[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) v[i] = shift & 4 ? v[i + 1] : v[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = __funnelshift_r(v[i], v[i + 1], 8 * (shift & 3));
+        const int keep = left - 4 * i;
+        if (keep < 4) v[i] = keep <= 0 ? 0 : v[i] & ((1u << 8 * keep) - 1);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// Operands of the tiles whose rows start off a 16-byte boundary are copied once, zeros up to the pitch: a TMA row has to start on such a
+// boundary.  Both operands go in one launch; 2^log_lanes threads take a row together.  333 x 1111 x 2047 takes 10.6 us with it, 8.0 us with
+// k = 2048 (13.0 us where each thread put four bytes together one by one).
 struct Packed {
     const signed char *src;
     long stride, rows;
     signed char *dst;
 };
-__global__ void __launch_bounds__(256) pack_kernel(const Packed one, const Packed two, const int cols, const int pitch)
+__global__ void __launch_bounds__(256) pack_kernel(const Packed one, const Packed two, const int cols, const int pitch, const int log_lanes)
 {
-    const long per_row = pitch / 4, total = (one.rows + two.rows) * per_row;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        long r = i / per_row;
-        const int c = (int)(i - r * per_row) * 4;
-        const bool first = r < one.rows;
-        if (!first) r -= one.rows;
-        const signed char *p = (first ? one.src : two.src) + r * (first ? one.stride : two.stride) + c;
-        unsigned v = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (c + e < cols) v |= (unsigned)(unsigned char)p[e] << (8 * e);
-        *reinterpret_cast<unsigned *>((first ? one.dst : two.dst) + r * pitch + c) = v;
+    const int lane = threadIdx.x & ((1 << log_lanes) - 1);
+    const long step = (long)gridDim.x << (8 - log_lanes);
+    for (long i = ((long)blockIdx.x << (8 - log_lanes)) + (threadIdx.x >> log_lanes); i < one.rows + two.rows; i += step) {
+        const bool first = i < one.rows;
+        const long r = first ? i : i - one.rows;
+        const signed char *p = first ? one.src + r * one.stride : two.src + r * two.stride;
+        signed char *to = (first ? one.dst : two.dst) + r * pitch;
+        for (int c = lane * 16; c < pitch; c += 16 << log_lanes) *reinterpret_cast<uint4 *>(to + c) = load16<false>(p + c, cols - c);
     }
 }
 
@@ -52,20 +74,21 @@ __global__ void __launch_bounds__(256) pack_kernel(const Packed one, const Packe
 // A block forms 16 rows of the long side (the rows of A of m16n8k32) against up to 32 rows of the short side; its 16 warps split k
 // and add up through shared memory (so many, because a round of loads is what a small call waits for: k = 4096 takes one).  As in the
 // pair distances, the order of k inside a product is free, so lane (g, t) loads 16 consecutive bytes of a row and uses them as four
-// k-slots on either side.  Bound by the latency of its loads: 1 x 4096 x 4096 in 4.6 us (2.6 us at the copy rate, and the launch; 7.6 us
-// with 8 warps), 16 x 11008 x 4096 in 12.8 us (3.5 TB/s).
+// k-slots on either side.  Bound by the latency of its loads: 1 x 4096 x 4096 in 4.5 us, 3.4 us where L2 still holds the long side
+// (2.6 us at the copy rate; 7.6 us with 8 warps), 1 x 4096 x 4095, whose rows are taken off their alignment, in 7.1 us (18.5 us where they
+// were copied to aligned ones first), 16 x 11008 x 4096 in 13.5 us (3.3 TB/s).
 constexpr int kSkinnyWarps = 16;
 
 struct SkinnyArgs {
     const signed char *w, *x; // long side [rows][k], short side [cols][k]
     long w_stride, x_stride;
     const float *w_scale, *x_scale;
-    int rows, cols, k; // k a multiple of 16
+    int rows, cols, k;
     void *out;
     long row_step, col_step; // of the result
 };
 
-template <typename T, int NB> __global__ void __launch_bounds__(kSkinnyWarps * 32, 2) skinny_kernel(const SkinnyArgs a)
+template <typename T, int NB, bool ALIGNED> __global__ void __launch_bounds__(kSkinnyWarps * 32, 2) skinny_kernel(const SkinnyArgs a)
 {
     __shared__ int part[kSkinnyWarps][16][NB * 8 + 1];
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
@@ -77,15 +100,14 @@ template <typename T, int NB> __global__ void __launch_bounds__(kSkinnyWarps * 3
     for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = 0;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 4
+#pragma unroll(ALIGNED ? 4 : 1)
     for (int k = warp * 64 + t * 16; k < a.k + t * 16; k += kSkinnyWarps * 64) { // the warp stays together: mma.sync wants all lanes
-        const bool in = k < a.k;
-        const uint4 u = in && in0 ? __ldcs(reinterpret_cast<const uint4 *>(w0 + k)) : zero;
-        const uint4 v = in && in1 ? __ldcs(reinterpret_cast<const uint4 *>(w1 + k)) : zero;
+        const int left = a.k - k;
+        const uint4 u = load16<ALIGNED>(w0 + k, in0 ? left : 0);
+        const uint4 v = load16<ALIGNED>(w1 + k, in1 ? left : 0);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-            const uint4 x = in && j * 8 + g < a.cols ? __ldg(reinterpret_cast<const uint4 *>(a.x + (j * 8 + g) * a.x_stride + k)) : zero;
+            const uint4 x = load16<ALIGNED>(a.x + (j * 8 + g) * a.x_stride + k, j * 8 + g < a.cols ? left : 0);
             mma_s8(acc[j], u.x, v.x, u.y, v.y, x.x, x.y);
             mma_s8(acc[j], u.z, v.z, u.w, v.w, x.z, x.w);
         }
@@ -105,12 +127,12 @@ template <typename T, int NB> __global__ void __launch_bounds__(kSkinnyWarps * 3
     }
 }
 
-template <typename T> int launch_skinny(const SkinnyArgs &a, cudaStream_t stream)
+template <typename T, bool ALIGNED> int launch_skinny(const SkinnyArgs &a, cudaStream_t stream)
 {
     const unsigned grid = (unsigned)((a.rows + 15) / 16);
-    if (a.cols <= 8) skinny_kernel<T, 1><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
-    else if (a.cols <= 16) skinny_kernel<T, 2><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
-    else skinny_kernel<T, 4><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
+    if (a.cols <= 8) skinny_kernel<T, 1, ALIGNED><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
+    else if (a.cols <= 16) skinny_kernel<T, 2, ALIGNED><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
+    else skinny_kernel<T, 4, ALIGNED><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
     LB_CUDA(cudaGetLastError());
     return LB_OK;
 }
@@ -424,6 +446,7 @@ constexpr int kShort = 8;   // blocks of k up to which the results are what take
 constexpr int kSkinny = 32; // rows on the short side up to which the long side is streamed
 
 struct ProductPlan {
+    bool off_a, off_b;   // rows off a 16-byte boundary
     bool pack_a, pack_b;
     int pitch;      // of packed rows
     size_t a_bytes; // of packed a
@@ -433,8 +456,11 @@ ProductPlan product_plan(int m, int n, int k, const void *a, long a_stride, cons
 {
     ProductPlan p;
     auto off = [&](const void *x, long stride, int rows) { return (uintptr_t)x % 16 != 0 || (rows > 1 && stride % 16 != 0) || k % 16 != 0 || k == 0; };
-    p.pack_a = off(a, a_stride, m);
-    p.pack_b = off(b, b_stride, n);
+    p.off_a = off(a, a_stride, m);
+    p.off_b = off(b, b_stride, n);
+    const bool skinny = m <= kSkinny || n <= kSkinny;
+    p.pack_a = p.off_a && !skinny;
+    p.pack_b = p.off_b && !skinny;
     p.pitch = k ? (k + 15) / 16 * 16 : 16;
     p.a_bytes = p.pack_a ? ((size_t)m * p.pitch + 255) / 256 * 256 : 0;
     p.bytes = p.a_bytes + (p.pack_b ? (size_t)n * p.pitch : 0);
@@ -442,7 +468,7 @@ ProductPlan product_plan(int m, int n, int k, const void *a, long a_stride, cons
 }
 
 template <typename T>
-int product_typed(Context *ctx, int m, int n, int k, const signed char *a, long a_stride, const float *a_scale, const signed char *b, long b_stride,
+int product_typed(Context *ctx, int m, int n, int k, bool aligned, const signed char *a, long a_stride, const float *a_scale, const signed char *b, long b_stride,
                   const float *b_scale, void *out, long out_stride, cudaStream_t stream)
 {
     const double bytes = (double)m * k + (double)n * k + (double)m * n * sizeof(T);
@@ -462,7 +488,7 @@ int product_typed(Context *ctx, int m, int n, int k, const signed char *a, long 
         s.row_step = turned ? out_stride : 1;
         s.col_step = turned ? 1 : out_stride;
         count_launch("int8_skinny", stream, bytes);
-        return launch_skinny<T>(s, stream);
+        return aligned ? launch_skinny<T, true>(s, stream) : launch_skinny<T, false>(s, stream);
     }
     ProductArgs p;
     p.m = m;
@@ -528,18 +554,21 @@ int int8_matmul(Context *ctx, int m, int n, int k, const signed char *a, long a_
     signed char *ws = reinterpret_cast<signed char *>(workspace);
     if (p.pack_a || p.pack_b) {
         const Packed one = {a, a_stride, p.pack_a ? m : 0, ws}, two = {b, b_stride, p.pack_b ? n : 0, ws + p.a_bytes};
-        const long blocks = ((one.rows + two.rows) * (p.pitch / 4) + 255) / 256, most = (long)ctx->sm_count * 16;
+        int log_lanes = 0;
+        while (log_lanes < 8 && 16 << log_lanes < p.pitch) ++log_lanes;
+        const long blocks = (one.rows + two.rows + (256 >> log_lanes) - 1) >> (8 - log_lanes), most = (long)ctx->sm_count * 32;
         count_launch("int8_pack", stream, 2.0 * (one.rows + two.rows) * k);
-        pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(one, two, k, p.pitch);
+        pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(one, two, k, p.pitch, log_lanes);
         LB_CUDA(cudaGetLastError());
         if (p.pack_a) a = one.dst, a_stride = p.pitch;
         if (p.pack_b) b = two.dst, b_stride = p.pitch;
     }
-    k = p.pitch; // k itself where a side is not packed: a ragged k packs both
+    const bool aligned = !p.off_a && !p.off_b;
+    if (p.pack_a || p.pack_b) k = p.pitch; // k itself where only one side is packed: a ragged k packs both
     switch (dtype) {
-    case 1: return product_typed<float>(ctx, m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
-    case 3: return product_typed<__nv_bfloat16>(ctx, m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
-    default: return product_typed<__half>(ctx, m, n, k, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
+    case 1: return product_typed<float>(ctx, m, n, k, aligned, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
+    case 3: return product_typed<__nv_bfloat16>(ctx, m, n, k, aligned, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
+    default: return product_typed<__half>(ctx, m, n, k, aligned, a, a_stride, a_scale, b, b_stride, b_scale, out, out_stride, stream);
     }
 }
 

@@ -45,8 +45,9 @@ def test_workspaces_are_asked_for_only_where_they_are_needed():
     assert q(i(0), i(5), i(16), i(0)) == 0 and q(i(1), i(1), i(15), i(0)) == 0
     a, b = C.c_void_p(4096), C.c_void_p(8192)
     assert m(i(8), i(8), i(64), a, i(64), b, i(64)) == 0
-    assert m(i(8), i(9), i(33), a, i(33), b, i(33)) == 512 + 9 * 48   # both packed to 48 bytes a row
-    assert m(i(8), i(9), i(64), C.c_void_p(4097), i(64), b, i(64)) == 512
+    assert m(i(40), i(41), i(33), a, i(33), b, i(33)) == 2048 + 41 * 48  # both packed to 48 bytes a row
+    assert m(i(40), i(41), i(64), C.c_void_p(4097), i(64), b, i(64)) == 2560
+    assert m(i(8), i(900), i(33), a, i(33), b, i(33)) == 0  # few rows on one side: read as they lie
     assert m(i(8), i(9), i(131072), a, i(131072), b, i(131072)) == 0
     assert d(None, i(4), i(4), i(64)) == 0
 
