@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const Packed one, const Packe
 // and add up through shared memory (so many, because a round of loads is what a small call waits for: k = 4096 takes one).  As in the
 // pair distances, the order of k inside a product is free, so lane (g, t) loads 16 consecutive bytes of a row and uses them as four
 // k-slots on either side.  Bound by the latency of its loads: 1 x 4096 x 4096 in 4.5 us, 3.4 us where L2 still holds the long side
-// (2.6 us at the copy rate; 7.6 us with 8 warps), 1 x 4096 x 4095, whose rows are taken off their alignment, in 7.1 us (18.5 us where they
+// (2.6 us at the copy rate; 7.6 us with 8 warps), 1 x 4096 x 4095, whose rows are taken off their alignment, in 6.7 us (18.5 us where they
 // were copied to aligned ones first), 16 x 11008 x 4096 in 13.5 us (3.3 TB/s).
 constexpr int kSkinnyWarps = 16;
 
@@ -100,7 +100,7 @@ template <typename T, int NB, bool ALIGNED> __global__ void __launch_bounds__(kS
     for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = 0;
-#pragma unroll(ALIGNED ? 4 : 1)
+#pragma unroll(ALIGNED ? 4 : 2)
     for (int k = warp * 64 + t * 16; k < a.k + t * 16; k += kSkinnyWarps * 64) { // the warp stays together: mma.sync wants all lanes
         const int left = a.k - k;
         const uint4 u = load16<ALIGNED>(w0 + k, in0 ? left : 0);
