@@ -523,7 +523,7 @@ int product_typed(Context *ctx, int m, int n, int k, bool aligned, const signed 
     int rc = encode_map(&ma, a, m, k, a_stride, kTileK, kTileM);
     if (rc) return rc;
     if ((rc = encode_map(&mb, b, n, k, b_stride, kTileK, bn))) return rc;
-    mo = ma; // not used unless
+    mo = ma; // not used where results do not leave by TMA
     if (quick && p.align >= 16) {
         if ((long)n * (long)sizeof(T) % 16 != 0) { // a TMA store would write the rest of a row's last 16 bytes, which is not the result's
             p.align = 0;
