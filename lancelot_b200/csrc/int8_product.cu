@@ -358,12 +358,14 @@ __global__ void __launch_bounds__(Tile<BN, SHORT>::kThreads, 1) product_kernel(c
             if (!__all_sync(0xffffffffu, ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride + tn * BN;
+            // A quarter wholly behind the last row has nothing to send.  It must not walk the boxes either: one that is passed without a store
+            // leaves the wait below one store short of the box that it is about to write
+            const int columns = tm * kTileM + quarter * 32 < a.m ? min(BN, a.n - tn * BN) : 0;
 #pragma unroll 1
-            for (int c0 = turn * kCols; c0 < BN; c0 += kTurns * kCols) {
-                if (tn * BN + c0 >= a.n) break;
+            for (int c0 = turn * kCols; c0 < columns; c0 += kTurns * kCols) {
                 const bool by_tma = SHORT && a.align == 1;
                 unsigned char *to = box + (sent & 1) * 4096;
-                if (by_tma) { // the box has been read out
+                if (by_tma) { // all stores but the last one have been read out of their boxes
                     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                     __syncwarp();
                 }
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(Tile<BN, SHORT>::kThreads, 1) product_kernel(c
                 if (by_tma) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0 && tm * kTileM + quarter * 32 < a.m) tma_store(&map_out, tn * BN + c0, tm * kTileM + quarter * 32, smem_u32(to));
+                    if (lane == 0) tma_store(&map_out, tn * BN + c0, tm * kTileM + quarter * 32, smem_u32(to));
                     ++sent;
                 }
             }

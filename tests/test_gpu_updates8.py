@@ -530,3 +530,23 @@ def test_refusals(ctx):
     assert ctx.dequantize_rows(codes, scales, 0, n_rows=2).shape == (2, 0)
     assert ctx.int8_matmul(codes[:0], codes, v[0, :0], v[0, :2]).shape == (0, 2)
     assert ctx.int8_distances(codes, scales, torch.zeros(0, 1, dtype=torch.int32, device="cuda")).shape == (0, 0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("m,n,k", [(4000, 4096, 16), (4001, 4096, 128), (2337, 4104, 48), (300, 40000, 16), (1100, 20000, 1024)])
+def test_product_whose_last_rows_fill_part_of_a_tile(ctx, m, n, k, dtype):
+    """several tiles a block, of which some lie partly behind the last row: no result that is still on its way out is written over"""
+    import torch
+
+    g = gen(m + n + k)
+    a = torch.randint(-127, 128, (m, k), generator=g, device="cuda", dtype=torch.int8)
+    b = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    sa, sb = torch.rand(m, generator=g, device="cuda") * 1e-3 + 1e-4, torch.rand(n, generator=g, device="cuda") + 0.1
+    out = torch.empty(m, n, dtype=getattr(torch, dtype), device="cuda")
+    first = ctx.int8_matmul(a, b, sa, sb, out=out).clone()
+    check_product(first, a, b, sa, sb)
+    for _ in range(30):
+        out.fill_(math.nan)
+        ctx.int8_matmul(a, b, sa, sb, out=out)
+        assert torch.equal(out, first)
+    ctx.check_status()
