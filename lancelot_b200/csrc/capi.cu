@@ -874,18 +874,11 @@ int lb_check_status(lb_context *h, void *stream)
     LB_CUDA(cudaStreamSynchronize(S(stream)));
     if (flags) {
         LB_CUDA(cudaMemsetAsync(C(h)->d_status, 0, sizeof(int), S(stream)));
-        if (flags & 1) {
-            set_error("encoded values are too large");
-            return LB_ERR_INVALID_ARG;
-        }
-        if (flags & 2) {
-            set_error("a wait inside a kernel ran out: the results of the calls before this one are not complete");
-            return LB_ERR_LOGIC;
-        }
-        set_error("device-side status flag raised");
-        return LB_ERR_LOGIC;
+        std::string message;
+        rc = status_of(flags, message);
+        set_error(message);
     }
-    return LB_OK;
+    return rc;
 }
 
 } // extern "C"

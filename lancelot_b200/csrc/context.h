@@ -38,7 +38,7 @@ struct Context {
     // inverse-FFT twiddles of the encoder in the order its stages use them, one table per log2(slots), each built
     // on first use: entry (n - (n >> u)) + k is the twiddle of butterfly group k at stage u
     double2 *d_ifft_tw[20] = {};
-    int *d_status = nullptr;         // sticky device-side condition flags (bit 0: encoded values are too large)
+    int *d_status = nullptr;         // sticky device-side condition flags, see status_of
     // scratch owned by the context, grown on demand between operations
     void *ws = nullptr;
     size_t ws_bytes = 0;
@@ -46,6 +46,18 @@ struct Context {
 
     int ensure_workspace(size_t bytes);
 };
+
+// What the flags of Context::d_status report.  Several may stand at once: lb_check_status clears all of them, so it has to name them all.
+//   1  the encoder met values that are too large for its modulus
+//   2  a bounded wait inside a kernel ran out
+inline int status_of(int flags, std::string &message)
+{
+    message.clear();
+    if (flags & 2) message = "a wait inside a kernel ran out: the results of the calls before this one are not complete";
+    if (flags & 1) message += std::string(message.empty() ? "" : "; ") + "encoded values are too large";
+    if (flags & ~3) message += std::string(message.empty() ? "" : "; ") + "device-side status flag raised";
+    return flags == 0 ? LB_OK : flags == 1 ? LB_ERR_INVALID_ARG : LB_ERR_LOGIC;
+}
 
 void set_error(const std::string &msg);
 // every kernel launch of this library goes through this (diag.cu): counted always, timed per kernel name while

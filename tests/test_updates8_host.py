@@ -61,3 +61,35 @@ def test_a_cache_checks_its_sizes():
     for args in ((0, 5), (3, 0), (3, 5, 24), (3, 5, 8), (3, 5, 32, 48), (3, 5, 32, 16)):
         with pytest.raises(ValueError):
             UpdateCache(Device(), *args)
+
+
+def test_the_status_names_every_condition_that_it_clears(tmp_path):
+    """a wait that ran out beside values that are too large: the check clears both, so it reports both, the graver one as its code"""
+    import os
+    import subprocess
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    source, program = tmp_path / "status.cpp", tmp_path / "status"
+    source.write_text("""
+#include <cstdio>
+#include "context.h"
+int main()
+{
+    for (int flags : {0, 1, 2, 3, 4, 7}) {
+        std::string message;
+        const int code = lb::status_of(flags, message);
+        std::printf("%d %d %s\\n", flags, code, message.c_str());
+    }
+}
+""")
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    subprocess.check_call([os.environ.get("CXX", "g++"), "-std=c++17", "-I" + os.path.join(root, "lancelot_b200", "csrc"), "-I" + os.path.join(cuda, "include"),
+                           str(source), "-o", str(program)])
+    large, wait, other = "encoded values are too large", "a wait inside a kernel ran out", "device-side status flag raised"
+    lines = subprocess.check_output([str(program)], text=True).splitlines()
+    got = {int(f): (int(c), m) for f, c, m in (line.split(" ", 2) for line in lines)}
+    invalid, logic = 1, 2
+    assert got[0] == (0, "")
+    for flags, code, named in ((1, invalid, [large]), (2, logic, [wait]), (3, logic, [large, wait]), (4, logic, [other]), (7, logic, [large, wait, other])):
+        assert got[flags][0] == code
+        assert [m for m in (large, wait, other) if m in got[flags][1]] == named
