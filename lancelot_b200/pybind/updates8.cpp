@@ -62,8 +62,8 @@ struct Call {
     Tensor workspace(size_t bytes) const { return bytes ? empty({(int64_t)bytes}, at::kByte) : Tensor(); }
 };
 
-// elements from one row to the next; a single row has none of its own
-int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+// elements from one row to the next; a single row has no next one, and counts as dense wherever it was taken from
+int64_t row_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 template <typename T> T *address(const Tensor &t) { return t.defined() && t.numel() ? static_cast<T *>(t.data_ptr()) : nullptr; }
 template <typename T> T *address(const Maybe &t) { return t ? address<T>(*t) : nullptr; }
 

@@ -550,3 +550,28 @@ def test_product_whose_last_rows_fill_part_of_a_tile(ctx, m, n, k, dtype):
         ctx.int8_matmul(a, b, sa, sb, out=out)
         assert torch.equal(out, first)
     ctx.check_status()
+
+
+def test_a_single_row_or_slot_has_no_stride(ctx):
+    """one row of a wider matrix beside a dense one, one slot of wider slots: how far the next row would lie does not matter"""
+    import torch
+
+    g = gen(6)
+    cols = 1003
+    v = torch.randn(1, cols + 7, generator=g, device="cuda")[:, 3:3 + cols]
+    res = torch.randn(1, 1050, generator=g, device="cuda")[:, :cols] * 0.01
+    res = torch.cat([res, torch.zeros(1, 47, device="cuda")], 1)[:, :cols]
+    assert res.stride(0) == 1050
+    lost = torch.empty(1, cols, device="cuda")
+    wide = torch.full((3, 1025), 9, dtype=torch.int8, device="cuda")
+    codes, scales = wide[:1, :1008], torch.empty(1, 9, device="cuda")[:, :8]
+    ctx.quantize_rows(v, codes, scales, group=128, residual=res, residual_out=lost)
+    want_codes, want_scales, want_lost = quantized(v + res, 1008, 128)
+    assert torch.equal(codes, want_codes) and torch.equal(scales, want_scales) and torch.equal(lost, want_lost)
+    assert bool((wide[0, 1008:] == 9).all()) and bool((wide[1:] == 9).all())
+    assert torch.equal(ctx.dequantize_rows(codes, scales, cols, group=128), expanded(codes, scales, 128)[:, :cols])
+    assert float(ctx.int8_distances(codes, scales, torch.zeros(2, 1, dtype=torch.int32, device="cuda"), group=128).abs().max()) == 0
+    # the residual that is kept in a row of another width, the other way round
+    kept = torch.full((2, 1050), 5.0, device="cuda")
+    ctx.quantize_rows(v, codes, scales, group=128, residual=res.contiguous(), residual_out=kept[1:, :cols])
+    assert torch.equal(kept[1:, :cols], want_lost) and bool((kept[0] == 5).all()) and bool((kept[1, cols:] == 5).all())
