@@ -262,7 +262,7 @@ LB_API int lb_decode_batch(lb_context *ctx, int size_l, int batch, const uint64_
 /* t = values + residual (residual NULL: 0) in 32 bits, 0 from lengths[i] columns of row i on (lengths DEVICE; NULL: n_cols; clamped to
  * [0, n_cols]).  Per group: m = max|t|, scale = m / 127 rounded to 32 bits, code = the integer nearest to t / scale, ties to
  * even.  A group of zeros has scale 0; one that holds an infinity or NaN has scale NaN and codes 0, so that it reads as NaN.
- * residual_out (NULL, residual itself, or memory apart from it) gets t - code * scale, exactly, for the columns below the row's
+ * residual_out (NULL, residual itself, or apart from it: behind it or in the gaps of its rows) gets t - code * scale, exactly, for the columns below the row's
  * length (0 in a group whose scale is NaN); the columns from there on are left as they are.  A page is always written whole, with
  * zeros behind the row's end. */
 LB_API size_t lb_quantize_rows_workspace_bytes(int64_t n_rows, int64_t n_cols, int64_t page, int64_t group);

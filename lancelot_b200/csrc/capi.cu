@@ -751,6 +751,17 @@ static int rows_ok(const void *p, int64_t rows, int64_t cols, int64_t stride, in
     return LB_OK;
 }
 
+// whether two operands of the same shape and stride have no element in common: one lies behind the other, or the rows of one lie in the gaps
+// of the other
+static bool rows_apart(const float *x, const float *y, int64_t rows, int64_t cols, int64_t stride)
+{
+    const int64_t span = (rows - 1) * stride + cols, d = ((int64_t)(intptr_t)y - (int64_t)(intptr_t)x) / 4;
+    if (d >= span || d <= -span) return true;
+    if (rows == 1) return false;
+    const int64_t in = d >= 0 ? d % stride : (stride - -d % stride) % stride; // of y's row in the room of a row of x
+    return in >= cols && in + cols <= stride;
+}
+
 // warps that a call over `pages` pages launches at most: their number has to fit the grid's arithmetic
 static int pages_ok(int64_t n_rows, int64_t n_cols, int64_t page)
 {
@@ -787,8 +798,7 @@ int lb_quantize_rows(lb_context *h, const void *values, int dtype, int64_t n_row
     if ((rc = rows_ok(values, n_rows, n_cols, value_stride, value_size(dtype)))) return rc;
     if (residual && (rc = rows_ok(residual, n_rows, n_cols, residual_stride, 4))) return rc;
     if (residual_out && (rc = rows_ok(residual_out, n_rows, n_cols, residual_stride, 4))) return rc;
-    const int64_t span = (n_rows - 1) * residual_stride + n_cols;
-    REQUIRE(!residual || !residual_out || residual == residual_out || residual + span <= residual_out || residual_out + span <= residual,
+    REQUIRE(!residual || !residual_out || residual == residual_out || rows_apart(residual, residual_out, n_rows, n_cols, residual_stride),
             "residual_out is residual itself or apart from it");
     REQUIRE((uintptr_t)lengths % 4 == 0 && (uintptr_t)slots % 4 == 0, "an operand is not aligned to its type");
     REQUIRE(slots || n_rows * ((n_cols + page - 1) / page) <= n_slots, "the cache has too few slots");

@@ -575,3 +575,32 @@ def test_a_single_row_or_slot_has_no_stride(ctx):
     kept = torch.full((2, 1050), 5.0, device="cuda")
     ctx.quantize_rows(v, codes, scales, group=128, residual=res.contiguous(), residual_out=kept[1:, :cols])
     assert torch.equal(kept[1:, :cols], want_lost) and bool((kept[0] == 5).all()) and bool((kept[1, cols:] == 5).all())
+
+
+@pytest.mark.parametrize("group", [32, 0])
+def test_residuals_in_the_gaps_of_one_another(ctx, group):
+    """residual and residual_out are memory apart where their rows take turns; rows that share an element are refused"""
+    import torch
+
+    from lancelot_b200._lib import InvalidArgument
+
+    g = gen(12)
+    n, cols = 5, 1003
+    v = torch.randn(n, cols, generator=g, device="cuda")
+    codes, scales = torch.empty(n, 1008, dtype=torch.int8, device="cuda"), torch.empty(n, -(-1008 // group) if group else 1, device="cuda")
+    for gap in (0, 1, 5):
+        both = torch.randn(n, 2 * cols + gap, generator=g, device="cuda") * 0.01
+        for x, y in ((0, cols + gap), (cols + gap, 0)):
+            before = both.clone()
+            res, lost = both[:, x:x + cols], both[:, y:y + cols]
+            ctx.quantize_rows(v, codes, scales, group=group, residual=res, residual_out=lost)
+            want_codes, want_scales, want_lost = quantized(v + before[:, x:x + cols], 1008, group)
+            assert torch.equal(codes, want_codes) and torch.equal(scales, want_scales) and torch.equal(lost, want_lost)
+            before[:, y:y + cols] = want_lost
+            assert torch.equal(both, before)
+    wide = torch.zeros(n + 1, 2 * cols, device="cuda")
+    for res, lost in ((wide[:n, :cols], wide[:n, 1:1 + cols]), (wide[:n, :cols], wide[:n, cols - 1:-1]), (wide[:n, :cols], wide[1:, :cols]),
+                      (wide[1:, 2:2 + cols], wide[:n, :cols]), (wide[:n, 1:1 + cols], wide[:n, :cols]), (wide[:1, :cols], wide[:1, 1:1 + cols])):
+        with pytest.raises(InvalidArgument, match="apart"):
+            ctx.quantize_rows(v[: len(res)], codes, scales, group=group, residual=res, residual_out=lost)
+    assert not wide.any()
