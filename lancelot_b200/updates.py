@@ -77,7 +77,7 @@ def quantize_matrix(lb, x):
     codes start on 16-byte boundaries whatever cols is."""
     rows, cols = x.shape
     codes = torch.empty(rows, max(16, -(-cols // 16) * 16), dtype=torch.int8, device=x.device)
-    scales = torch.empty(rows, 1, device=x.device)
+    scales = (torch.empty if cols else torch.zeros)(rows, 1, device=x.device)  # a row of no columns has no page to be written: scale 0
     lb.quantize_rows(x, codes, scales)
     return codes[:, :cols], scales.view(-1)
 

@@ -109,3 +109,20 @@ def test_low_rank_updates_are_formed_and_encrypted(ek, rank):
     ek.lb.check_status()
     with pytest.raises(ValueError):
         low_rank_update(ek.lb, factors, out=torch.empty(3, device="cuda"))
+
+
+def test_factors_without_columns(ek):
+    """rank 0: rows of zeros, whatever their memory held before"""
+    import torch
+
+    from lancelot_b200.updates import low_rank_update, quantize_matrix
+
+    for dtype in (torch.float32, torch.bfloat16):
+        stale = torch.full((1 << 16,), float("nan"), device="cuda")
+        del stale
+        (qb, sb), (qa, sa) = [quantize_matrix(ek.lb, torch.empty(rows, 0, dtype=dtype, device="cuda")) for rows in (70, 300)]
+        assert qb.shape == (70, 0) and qa.shape == (300, 0) and not sb.any() and not sa.any()
+        update = low_rank_update(ek.lb, [(qb, sb, qa, sa)])
+        assert update.shape == (70 * 300,) and not update.any()
+    codes, scales = quantize_matrix(ek.lb, torch.empty(0, 8, device="cuda"))
+    assert codes.shape == (0, 8) and scales.shape == (0,)
