@@ -92,6 +92,10 @@ class Context:
         """the current torch stream of THIS context's device (not of whatever device is current)"""
         return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
 
+    def _handle(self):
+        """the context's address for the extension module; 0, which the C entries refuse, once it is closed"""
+        return self.h.value if self.h else 0
+
     def reserve_workspace(self, nbytes):
         check(lib.lb_context_reserve_workspace(self.h, C.c_size_t(int(nbytes))))
 
@@ -419,20 +423,20 @@ class Context:
         A row covers ceil(cols / page) slots, page = codes.shape[1]; slots [n][pages] int32 names them (None: in order; one outside the
         cache is skipped; no slot may occur twice).  lengths [n] int32: columns of each row that count.  residual [n][cols] float32 is added
         first, residual_out (may be residual) gets what the rounding lost.  group: columns with one scale, 0 = the whole page"""
-        _updates8().quantize_rows(self.h.value, self.device, values, codes, scales, group, slots, lengths, residual, residual_out)
+        _updates8().quantize_rows(self._handle(), self.device, values, codes, scales, group, slots, lengths, residual, residual_out)
 
     def dequantize_rows(self, codes, scales, n_cols, group=0, slots=None, n_rows=None, dtype=torch.float32, out=None):
         """rows of n_cols values read back from the cache -> [n][n_cols] of dtype; slots as in quantize_rows (pages that are not in the
         cache read as zeros).  n: n_rows, else the rows of out, else those that slots names, else as many as the cache holds in order"""
-        return _updates8().dequantize_rows(self.h.value, self.device, codes, scales, n_cols, group, slots, n_rows, VALUE_TYPES.get(dtype, 0), out)
+        return _updates8().dequantize_rows(self._handle(), self.device, codes, scales, n_cols, group, slots, n_rows, VALUE_TYPES.get(dtype, 0), out)
 
     def int8_matmul(self, a, b, a_scale, b_scale, dtype=torch.bfloat16, out=None):
         """a [m][k], b [n][k] int8, a_scale [m], b_scale [n] float32 -> [m][n]: (a b^T) * a_scale[:, None] * b_scale, the sum an exact integer"""
-        return _updates8().int8_matmul(self.h.value, self.device, a, b, a_scale, b_scale, VALUE_TYPES.get(dtype, 0), out)
+        return _updates8().int8_matmul(self._handle(), self.device, a, b, a_scale, b_scale, VALUE_TYPES.get(dtype, 0), out)
 
     def int8_distances(self, codes, scales, slots, group=0):
         """squared distances between all pairs of cached rows: slots [n][pages] int32 -> [n][n] float64 (0 on the diagonal)"""
-        return _updates8().int8_distances(self.h.value, self.device, codes, scales, slots, group)
+        return _updates8().int8_distances(self._handle(), self.device, codes, scales, slots, group)
 
     def check_status(self):
         check(lib.lb_check_status(self.h, self._stream()))

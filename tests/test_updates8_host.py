@@ -93,3 +93,19 @@ int main()
     for flags, code, named in ((1, invalid, [large]), (2, logic, [wait]), (3, logic, [large, wait]), (4, logic, [other]), (7, logic, [large, wait, other])):
         assert got[flags][0] == code
         assert [m for m in (large, wait, other) if m in got[flags][1]] == named
+
+
+def test_a_closed_context_is_refused_like_a_null_one():
+    from lancelot_b200._lib import InvalidArgument
+    from lancelot_b200.cabi import Context
+
+    closed = Context.__new__(Context)
+    closed.h, closed.device = None, 0
+    v, codes, scales = torch.zeros(2, 64), torch.zeros(2, 64, dtype=torch.int8), torch.zeros(2, 1)
+    on = "cuda" if torch.cuda.is_available() else "cpu"
+    v, codes, scales = v.to(on), codes.to(on), scales.to(on)
+    for call in (lambda: closed.quantize_rows(v, codes, scales), lambda: closed.dequantize_rows(codes, scales, 64),
+                 lambda: closed.int8_matmul(codes, codes, v[0, :2], v[0, :2]),
+                 lambda: closed.int8_distances(codes, scales, torch.zeros(2, 1, dtype=torch.int32, device=on))):
+        with pytest.raises(InvalidArgument, match="context is null" if on == "cuda" else "cuda:0"):
+            call()
