@@ -2,7 +2,8 @@
 
 ``pyCAHEL`` (binding.cpp) is what lancelot-main-GPU imports (``import pyCAHEL as cahel``): put this folder on PYTHONPATH.
 It links ``../liblancelot_b200.so`` (found at run time relative to the module) and the CUDA runtime.
-``_updates8`` (updates8.cpp) holds the 8-bit update calls of ``cabi.Context``; it links torch's C++ libraries as well."""
+``_updates8`` (updates8.cpp) holds the 8-bit update calls of ``cabi.Context``; it links torch's C++ libraries as well, and is left out, with a
+note, where torch or its CUDA part is not installed."""
 import os
 import subprocess
 import sys
@@ -36,14 +37,21 @@ def _compile(module, deps, flags, force):
 
 
 def build(force=False):
+    """Returns the path of ``pyCAHEL``, which needs no torch."""
     import pybind11
-    import torch
 
     header = os.path.join(ROOT, "include", "lancelot_b200.h")
     out = _compile("pyCAHEL", [os.path.join(HERE, "binding.cpp"), os.path.join(ROOT, "include", "cahel_b200.hpp"), header],
                    ["-I" + pybind11.get_include()], force)
-    site = os.path.dirname(torch.__file__)
+    try:
+        import torch
+    except ImportError:
+        torch = None
+    site = os.path.dirname(torch.__file__) if torch else ""
     lib = os.path.join(site, "lib")
+    if not torch or not os.path.exists(os.path.join(lib, "libc10_cuda.so")):
+        sys.stderr.write("no torch with CUDA: _updates8 is not built, the 8-bit update calls of cabi.Context will not import\n")
+        return out
     _compile("_updates8", [os.path.join(HERE, "updates8.cpp"), header],
              ["-I" + os.path.join(site, "include"), "-I" + os.path.join(site, "include", "torch", "csrc", "api", "include"),
               "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-L" + lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",

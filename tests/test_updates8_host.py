@@ -109,3 +109,19 @@ def test_a_closed_context_is_refused_like_a_null_one():
                  lambda: closed.int8_distances(codes, scales, torch.zeros(2, 1, dtype=torch.int32, device=on))):
         with pytest.raises(InvalidArgument, match="context is null" if on == "cuda" else "cuda:0"):
             call()
+
+
+def test_the_module_of_the_reference_builds_without_torch(monkeypatch, tmp_path, capsys):
+    import sys
+
+    from lancelot_b200.pybind import build
+
+    compiled = []
+    monkeypatch.setattr(build, "_compile", lambda module, *args: compiled.append(module) or module)
+    assert build.build() == "pyCAHEL" and compiled == ["pyCAHEL", "_updates8"]
+    compiled.clear()
+    monkeypatch.setattr(torch, "__file__", str(tmp_path / "__init__.py"))  # one that has no CUDA part
+    assert build.build() == "pyCAHEL" and compiled == ["pyCAHEL"] and "_updates8" in capsys.readouterr().err
+    compiled.clear()
+    monkeypatch.setitem(sys.modules, "torch", None)  # none at all
+    assert build.build() == "pyCAHEL" and compiled == ["pyCAHEL"] and "_updates8" in capsys.readouterr().err
