@@ -18,9 +18,15 @@ def target(module="pyCAHEL"):
     return os.path.join(HERE, module + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
-def _compile(module, deps, flags, force):
+def _compile(module, deps, flags, force, against=""):
+    """against: what a module was linked to that its sources do not show; it is built anew when that changes"""
     out = target(module)
-    if not force and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in deps):
+    record = os.path.join(PKG, "build", module + ".against")
+    built = ""
+    if os.path.exists(record):
+        with open(record) as f:
+            built = f.read()
+    if not force and built == against and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in deps):
         return out
     cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     cxx = os.environ.get("CXX", "g++")
@@ -33,6 +39,9 @@ def _compile(module, deps, flags, force):
     if r.returncode != 0:
         raise RuntimeError("building %s failed: %s\n%s" % (module, " ".join(cmd), r.stderr))
     os.replace(out + ".tmp", out)
+    os.makedirs(os.path.dirname(record), exist_ok=True)
+    with open(record, "w") as f:
+        f.write(against)
     return out
 
 
@@ -55,7 +64,7 @@ def build(force=False):
     _compile("_updates8", [os.path.join(HERE, "updates8.cpp"), header],
              ["-I" + os.path.join(site, "include"), "-I" + os.path.join(site, "include", "torch", "csrc", "api", "include"),
               "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-L" + lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
-              "-ltorch_python", "-Wl,-rpath," + lib], force)
+              "-ltorch_python", "-Wl,-rpath," + lib], force, "torch %s %s in %s" % (torch.__version__, torch.version.git_version, site))
     return out
 
 

@@ -125,3 +125,31 @@ def test_the_module_of_the_reference_builds_without_torch(monkeypatch, tmp_path,
     compiled.clear()
     monkeypatch.setitem(sys.modules, "torch", None)  # none at all
     assert build.build() == "pyCAHEL" and compiled == ["pyCAHEL"] and "_updates8" in capsys.readouterr().err
+
+
+def test_a_module_is_built_anew_when_torch_was_replaced(monkeypatch, tmp_path):
+    import os
+    import types
+
+    from lancelot_b200.pybind import build
+
+    commands = []
+
+    def run(cmd, **_):
+        commands.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w"):
+            pass
+        return types.SimpleNamespace(returncode=0, stderr="")
+
+    monkeypatch.setattr(build, "PKG", str(tmp_path))
+    monkeypatch.setattr(build, "target", lambda module="pyCAHEL": str(tmp_path / (module + ".so")))
+    monkeypatch.setattr(build.subprocess, "run", run)
+    build.build()
+    assert [os.path.basename(c[c.index("-o") + 1]) for c in commands] == ["pyCAHEL.so.tmp", "_updates8.so.tmp"]
+    build.build()
+    assert len(commands) == 2  # nothing has changed
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    build.build()
+    assert len(commands) == 3 and "_updates8.so.tmp" in commands[2][commands[2].index("-o") + 1]
+    build.build()
+    assert len(commands) == 3
