@@ -5,6 +5,8 @@ and ``plaintext_krum``: a quarter of the memory (20 clients of 11 M values: 0.22
 error feedback of 8-bit uploads, and read back a range of pages at a time.  ``low_rank_update`` forms an update from 8-bit factors.
 The reference keeps every update as a list of doubles (lancelot-main-GPU/utils/byzantine_fl.py:478-490) and has neither.
 """
+import operator
+
 import torch
 
 
@@ -37,7 +39,10 @@ class UpdateCache:
             if not rows.is_contiguous():
                 raise ValueError("clients is a contiguous range")
             return rows
-        c = int(clients)
+        try:
+            c = operator.index(clients)
+        except TypeError:
+            raise ValueError("clients is None, an integer or a contiguous range") from None
         if not 0 <= c < self.shape[0]:
             raise ValueError("client %d is not in the cache" % c)
         return self.table[c:c + 1]

@@ -153,3 +153,17 @@ def test_a_module_is_built_anew_when_torch_was_replaced(monkeypatch, tmp_path):
     assert len(commands) == 3 and "_updates8.so.tmp" in commands[2][commands[2].index("-o") + 1]
     build.build()
     assert len(commands) == 3
+
+
+def test_a_cache_takes_no_fraction_of_a_client():
+    import numpy as np
+
+    from lancelot_b200.updates import UpdateCache
+
+    cache = UpdateCache.__new__(UpdateCache)
+    cache.shape, cache.table = torch.Size((3, 40)), torch.arange(6, dtype=torch.int32).view(3, 2)
+    for one in (1, np.int64(1), torch.tensor(1)):
+        assert cache._rows(one).tolist() == [[2, 3]]
+    for bad in (1.7, 1.0, "1", [1], torch.tensor(1.5), 3, -1):
+        with pytest.raises(ValueError):
+            cache._rows(bad)
