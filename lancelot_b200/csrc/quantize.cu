@@ -27,87 +27,37 @@ namespace {
 
 constexpr unsigned kInfBits = 0x7f800000u;
 
-// Four consecutive values as 32-bit floats.  `valid`: how many of them lie inside the row (<= 0: none)
-template <bool VEC> __device__ __forceinline__ float4 load4(const float *p, int valid)
+// Four consecutive values on their piece's boundary, as 32-bit floats
+__device__ __forceinline__ float4 load4(const float *p) { return __ldcs(reinterpret_cast<const float4 *>(p)); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16 *p)
 {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (VEC && valid >= 4) return __ldcs(reinterpret_cast<const float4 *>(p));
-    if (valid > 0) v.x = __ldcs(p);
-    if (valid > 1) v.y = __ldcs(p + 1);
-    if (valid > 2) v.z = __ldcs(p + 2);
-    if (valid > 3) v.w = __ldcs(p + 3);
-    return v;
+    const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(p));
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
 }
-template <bool VEC> __device__ __forceinline__ float4 load4(const __nv_bfloat16 *p, int valid)
+__device__ __forceinline__ float4 load4(const __half *p)
 {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (VEC && valid >= 4) {
-        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(p));
-        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                           __uint_as_float(w.y & 0xffff0000u));
-    }
-    if (valid > 0) v.x = __bfloat162float(p[0]);
-    if (valid > 1) v.y = __bfloat162float(p[1]);
-    if (valid > 2) v.z = __bfloat162float(p[2]);
-    if (valid > 3) v.w = __bfloat162float(p[3]);
-    return v;
-}
-template <bool VEC> __device__ __forceinline__ float4 load4(const __half *p, int valid)
-{
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (VEC && valid >= 4) {
-        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(p));
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
-        return make_float4(a.x, a.y, b.x, b.y);
-    }
-    if (valid > 0) v.x = __half2float(p[0]);
-    if (valid > 1) v.y = __half2float(p[1]);
-    if (valid > 2) v.z = __half2float(p[2]);
-    if (valid > 3) v.w = __half2float(p[3]);
-    return v;
+    const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(p));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
 }
 
-template <bool VEC> __device__ __forceinline__ void store4(float *p, float4 v, int valid)
+__device__ __forceinline__ void store4(float *p, float4 v) { __stcs(reinterpret_cast<float4 *>(p), v); }
+__device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v)
 {
-    if (VEC && valid >= 4) {
-        __stcs(reinterpret_cast<float4 *>(p), v);
-        return;
-    }
-    if (valid > 0) p[0] = v.x;
-    if (valid > 1) p[1] = v.y;
-    if (valid > 2) p[2] = v.z;
-    if (valid > 3) p[3] = v.w;
+    __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    __stcs(reinterpret_cast<uint2 *>(p), make_uint2(*reinterpret_cast<unsigned *>(&a), *reinterpret_cast<unsigned *>(&b)));
 }
-template <bool VEC> __device__ __forceinline__ void store4(__nv_bfloat16 *p, float4 v, int valid)
+__device__ __forceinline__ void store4(__half *p, float4 v)
 {
-    if (VEC && valid >= 4) {
-        __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-        __stcs(reinterpret_cast<uint2 *>(p), make_uint2(*reinterpret_cast<unsigned *>(&a), *reinterpret_cast<unsigned *>(&b)));
-        return;
-    }
-    if (valid > 0) p[0] = __float2bfloat16_rn(v.x);
-    if (valid > 1) p[1] = __float2bfloat16_rn(v.y);
-    if (valid > 2) p[2] = __float2bfloat16_rn(v.z);
-    if (valid > 3) p[3] = __float2bfloat16_rn(v.w);
-}
-template <bool VEC> __device__ __forceinline__ void store4(__half *p, float4 v, int valid)
-{
-    if (VEC && valid >= 4) {
-        __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
-        __stcs(reinterpret_cast<uint2 *>(p), make_uint2(*reinterpret_cast<unsigned *>(&a), *reinterpret_cast<unsigned *>(&b)));
-        return;
-    }
-    if (valid > 0) p[0] = __float2half_rn(v.x);
-    if (valid > 1) p[1] = __float2half_rn(v.y);
-    if (valid > 2) p[2] = __float2half_rn(v.z);
-    if (valid > 3) p[3] = __float2half_rn(v.w);
+    __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    __stcs(reinterpret_cast<uint2 *>(p), make_uint2(*reinterpret_cast<unsigned *>(&a), *reinterpret_cast<unsigned *>(&b)));
 }
 
 // Four values at positions at .. at + 3 of a run, of which only [lo, hi) exist or are wanted
 template <bool VEC, typename T> __device__ __forceinline__ float4 load_piece(const T *p, int at, int lo, int hi)
 {
-    if (VEC && at >= lo && at + 4 <= hi) return load4<true>(p + at, 4);
+    if (VEC && at >= lo && at + 4 <= hi) return load4(p + at);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     if (at >= lo && at < hi) v.x = (float)p[at];
     if (at + 1 >= lo && at + 1 < hi) v.y = (float)p[at + 1];
@@ -121,7 +71,7 @@ __device__ __forceinline__ void set(__half *p, float v) { *p = __float2half_rn(v
 template <bool VEC, typename T> __device__ __forceinline__ void store_piece(T *p, int at, const float4 &v, int lo, int hi)
 {
     if (VEC && at >= lo && at + 4 <= hi) {
-        store4<true>(p + at, v, 4);
+        store4(p + at, v);
         return;
     }
     if (at >= lo && at < hi) set(p + at, v.x);
@@ -271,9 +221,9 @@ template <typename T, bool VEC> __device__ __forceinline__ Run<T> run_of(const Q
 }
 template <bool FULL, bool VEC, typename T> __device__ __forceinline__ float4 load_sum(const Run<T> &r, int at)
 {
-    float4 v = FULL ? load4<true>(r.values + at, 4) : load_piece<VEC>(r.values, at, 0, r.hi);
+    float4 v = FULL ? load4(r.values + at) : load_piece<VEC>(r.values, at, 0, r.hi);
     if (r.residual) {
-        const float4 w = FULL ? load4<true>(r.residual + at, 4) : load_piece<VEC>(r.residual, at, 0, r.hi);
+        const float4 w = FULL ? load4(r.residual + at) : load_piece<VEC>(r.residual, at, 0, r.hi);
         v.x += w.x;
         v.y += w.y;
         v.z += w.z;
@@ -365,7 +315,7 @@ __device__ __forceinline__ void quantize_tile(const Run<T> &r, signed char *code
     if (!r.lost) return;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if (FULL && (j > 0 || off == 0 || lane > 0)) store4<true>(r.lost + first + j * 128, v[j], 4);
+        if (FULL && (j > 0 || off == 0 || lane > 0)) store4(r.lost + first + j * 128, v[j]);
         else store_piece<VEC>(r.lost, first + j * 128, v[j], 0, r.hi);
     }
     if (off && lane == 0) store_piece<false>(r.lost, 512 - off, last, 0, min(r.hi, 512));
@@ -459,7 +409,7 @@ __device__ __forceinline__ void quantize_group(const Run<T> &r, signed char *cod
     if (!r.lost) return;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        if (FULL && (j > 0 || off == 0 || threadIdx.x > 0)) store4<true>(r.lost + first + j * kThreads * 4, v[j], 4);
+        if (FULL && (j > 0 || off == 0 || threadIdx.x > 0)) store4(r.lost + first + j * kThreads * 4, v[j]);
         else store_piece<VEC>(r.lost, first + j * kThreads * 4, v[j], 0, r.hi);
     }
     if (off && threadIdx.x == 0) store_piece<false>(r.lost, kRun - off, last, 0, min(r.hi, kRun));
@@ -668,7 +618,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const DequantizeArgs a,
             b = lane ? up : down;
         }
         const float4 v = make_float4(b * f.x, (off > 1 ? b : s[j]) * f.y, (off > 2 ? b : s[j]) * f.z, s[j] * f.w);
-        if (hi == 512 && (j > 0 || lane > 0)) store4<true>(out + lane * 4 + j * 128 - off, v, 4);
+        if (hi == 512 && (j > 0 || lane > 0)) store4(out + lane * 4 + j * 128 - off, v);
         else store_piece<true>(out, lane * 4 + j * 128 - off, v, 0, hi);
     }
     if (hi > 512 - off && lane == 31) { // the columns before the next run's first piece
