@@ -17,6 +17,7 @@
 // much as a wide one.  A ring of shared memory filled by a warp of its own took 123 us (a bulk copy or a gathered TMA load of four rows
 // holds its warp up for 70 cycles), filled by all warps 96 us (instructions); registers 56 us.  Beyond 32 clients the registers of a
 // warp do not hold what it would have to read, and the ring is used after all.
+#include <atomic>
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -777,7 +778,7 @@ DistancePlan distance_plan(int sm_count, int n, long pages, int page, int group)
 template <int NB, int LOG_UNIT, int BYTES, int WARPS, int SETS> int launch_ring(Context *ctx, const DistanceArgs &a, const DistancePlan &p, cudaStream_t stream)
 {
     const Ring r = ring_shape(NB, 1 << LOG_UNIT, a.n, a.group);
-    static bool set[64] = {};
+    static std::atomic<bool> set[64]; // host threads that come here first at once all set the same attribute
     if (ctx->device >= 64 || !set[ctx->device]) {
         LB_CUDA(cudaFuncSetAttribute(gram_ring_kernel<NB, LOG_UNIT, BYTES, WARPS, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes));
         if (ctx->device < 64) set[ctx->device] = true;

@@ -10,6 +10,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "tcgen05.cuh"
 
 namespace lb {
@@ -433,7 +435,7 @@ template <typename T, int BN, bool SHORT>
 int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &mo, const ProductArgs &a, cudaStream_t stream)
 {
     using C = Tile<BN, SHORT>;
-    static bool set[64] = {};
+    static std::atomic<bool> set[64]; // host threads that come here first at once all set the same attribute
     if (ctx->device >= 64 || !set[ctx->device]) {
         LB_CUDA(cudaFuncSetAttribute(product_kernel<T, BN, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
         if (ctx->device < 64) set[ctx->device] = true;

@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda.h>
 
+#include <atomic>
+
 #include "context.h"
 
 namespace lb {
@@ -122,7 +124,8 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
 // size: bytes of an element, which coordinates count in
 inline int encode_map(CUtensorMap *map, const void *base, long rows, long cols, long stride, int box_cols, int box_rows, int size = 1)
 {
-    static EncodeTiled encode = nullptr;
+    static std::atomic<EncodeTiled> known; // host threads that come here first at once all find the same function
+    EncodeTiled encode = known;
     if (!encode) {
         void *f = nullptr;
         cudaDriverEntryPointQueryResult found;
@@ -131,7 +134,7 @@ inline int encode_map(CUtensorMap *map, const void *base, long rows, long cols, 
             set_error("the driver has no cuTensorMapEncodeTiled");
             return LB_ERR_CUDA;
         }
-        encode = reinterpret_cast<EncodeTiled>(f);
+        known = encode = reinterpret_cast<EncodeTiled>(f);
     }
     const cuuint64_t dims[2] = {(cuuint64_t)(cols / size), (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
     const cuuint32_t box[2] = {(cuuint32_t)(box_cols / size), (cuuint32_t)box_rows}, steps[2] = {1, 1};

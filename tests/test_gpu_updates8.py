@@ -604,3 +604,49 @@ def test_residuals_in_the_gaps_of_one_another(ctx, group):
         with pytest.raises(InvalidArgument, match="apart"):
             ctx.quantize_rows(v[: len(res)], codes, scales, group=group, residual=res, residual_out=lost)
     assert not wide.any()
+
+
+THREADS = """
+import ctypes as C, threading, torch
+from lancelot_b200 import cabi
+from lancelot_b200._lib import lib
+ctx = cabi.Context(12, cabi.coeff_modulus_create(1 << 12, [40, 40]), 1)
+lib.lb_int8_distances_workspace_bytes.restype = C.c_size_t
+i, p = C.c_int64, lambda t: C.c_void_p(t.data_ptr())
+g = torch.Generator("cuda").manual_seed(1)
+codes = torch.randint(-127, 128, (40, 1024), generator=g, device="cuda", dtype=torch.int8)
+scale = torch.rand(40, generator=g, device="cuda")
+want = (codes.double() @ codes.double().T) * scale.double()[:, None] * scale.double()
+need = lib.lb_int8_distances_workspace_bytes(ctx.h, i(40), i(1), i(1024))
+n, results = 8, []
+for _ in range(n):
+    results.append((torch.empty(40, 40, device="cuda"), torch.empty(40, 40, dtype=torch.float64, device="cuda"), torch.empty(need, dtype=torch.uint8, device="cuda"),
+                    torch.cuda.Stream(), [None, None]))
+torch.cuda.synchronize()
+start = threading.Barrier(n)
+def call(product, distances, ws, stream, codes_of):  # the C entries themselves: ctypes lets the threads run side by side
+    start.wait()
+    s = C.c_void_p(stream.cuda_stream)
+    codes_of[0] = lib.lb_int8_matmul(ctx.h, i(40), i(40), i(1024), p(codes), i(1024), p(scale), p(codes), i(1024), p(scale), p(product), 1, i(40), None, C.c_size_t(0), s)
+    codes_of[1] = lib.lb_int8_distances(ctx.h, p(codes), i(1024), p(scale), i(1), i(40), i(1024), i(0), None, i(40), i(1), p(distances), p(ws), C.c_size_t(need), s)
+threads = [threading.Thread(target=call, args=r) for r in results]
+for t in threads: t.start()
+for t in threads: t.join()
+torch.cuda.synchronize()
+d = want.diagonal()[:, None] + want.diagonal() - 2 * want
+for product, distances, _, _, codes_of in results:
+    assert codes_of == [0, 0]
+    assert bool(((product.double() - want).abs() <= want.abs() * 3.1 * 2.0 ** -24).all())
+    assert bool(((distances - d).abs() <= (want.diagonal()[:, None] + want.diagonal()) * 2.0 ** -53 * 1032 * 2).all())
+print("threads agree")
+"""
+
+
+def test_threads_that_make_the_first_calls_at_once():
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", THREADS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "threads agree" in r.stdout, r.stderr
