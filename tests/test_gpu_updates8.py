@@ -650,3 +650,63 @@ def test_threads_that_make_the_first_calls_at_once():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", THREADS], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "threads agree" in r.stdout, r.stderr
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("m,n,k", [(3, 200, 64), (20, 70, 1001), (140, 300, 128), (140, 301, 2048), (200, 256, 100)])
+def test_product_with_scales_that_are_not_finite(ctx, m, n, k, dtype):
+    """they reach their own row or column of the result and no other: a sum of 0 times an infinity is NaN, any other one infinite"""
+    import torch
+
+    g = gen(m + k)
+    a = torch.randint(-127, 128, (m, k), generator=g, device="cuda", dtype=torch.int8)
+    b = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    a[m // 2] = 0  # a row of sums that are 0
+    sa, sb = torch.rand(m, generator=g, device="cuda") + 0.5, torch.rand(n, generator=g, device="cuda") + 0.5
+    clean = ctx.int8_matmul(a, b, sa, sb, dtype=getattr(torch, dtype))
+    sa[0], sa[m - 1], sb[1], sb[n - 1] = math.inf, math.nan, -math.inf, math.nan
+    got = ctx.int8_matmul(a, b, sa, sb, dtype=getattr(torch, dtype))
+    total = (a.double() @ b.double().T).float()  # 64 bits hold the sum exactly; rounded once, as defined
+    want = (total * sa[:, None] * sb).to(got.dtype)
+    fine = torch.ones(m, n, dtype=torch.bool, device="cuda")
+    fine[0] = fine[m - 1] = False
+    fine[:, 1] = fine[:, n - 1] = False
+    assert torch.equal(got[fine], clean[fine]) and bool(got[fine].isfinite().all())
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~fine].nan_to_num(0.0), want[~fine].nan_to_num(0.0))
+    assert bool(got[m // 2, 1].isnan()) and bool(got[m - 1].isnan().all()) and bool(got[:, n - 1].isnan().all())
+    assert got[0].isinf().any()
+
+
+@pytest.mark.parametrize("n", [5, 20, 40, 130])
+def test_distances_of_a_row_with_an_infinite_scale(ctx, n):
+    """they are not finite (64-bit terms that are infinite cancel to NaN); those of all other pairs are what they were"""
+    import torch
+
+    codes = torch.randint(1, 128, (n, 512), generator=gen(n), device="cuda", dtype=torch.int8)
+    scales = torch.rand(n, 4, generator=gen(n + 1), device="cuda") + 0.5
+    slots = torch.arange(n, dtype=torch.int32, device="cuda").view(n, 1)
+    before = ctx.int8_distances(codes, scales, slots, group=128)
+    scales[2, 1] = math.inf
+    got = ctx.int8_distances(codes, scales, slots, group=128)
+    others = [i for i in range(n) if i != 2]
+    assert torch.equal(got[others][:, others], before[others][:, others])
+    assert not bool(got[2, others].isfinite().any()) and torch.equal(got[2].isnan(), got[:, 2].isnan()) and float(got[2, 2]) == 0.0
+
+
+@pytest.mark.parametrize("n,pages,page", [(129, 5, 1040), (160, 3, 4096), (200, 6, 2048), (257, 2, 1008)])
+@pytest.mark.parametrize("group", [0, 32, 128])
+def test_pair_distances_of_many_clients_over_several_pages(ctx, n, pages, page, group):
+    import torch
+
+    g = gen(n * pages + group)
+    groups = -(-page // group) if 0 < group < page else 1
+    codes = torch.randint(-127, 128, (n * pages + 2, page), generator=g, device="cuda", dtype=torch.int8)
+    scales = torch.rand(n * pages + 2, groups, generator=g, device="cuda")
+    slots = torch.randperm(n * pages + 2, generator=g, device="cuda")[: n * pages].to(torch.int32).view(n, pages)
+    slots[n - 1] = slots[0]                        # two rows that are the same, in blocks of clients far apart
+    slots[1, pages - 1], slots[40, 0] = -1, 1 << 30  # pages that are not there
+    got = ctx.int8_distances(codes, scales, slots, group=group)
+    want, slack = distances(codes, scales, slots, group)
+    assert bool(((got - want).abs() <= slack).all())
+    assert torch.equal(got, got.T) and bool((got.diagonal() == 0).all()) and float(got[0, n - 1]) == 0.0
+    assert torch.equal(got, ctx.int8_distances(codes, scales, slots, group=group))
