@@ -262,9 +262,9 @@ LB_API int lb_decode_batch(lb_context *ctx, int size_l, int batch, const uint64_
 /* t = values + residual (residual NULL: 0) in 32 bits, 0 from lengths[i] columns of row i on (lengths DEVICE; NULL: n_cols; clamped to
  * [0, n_cols]).  Per group: m = max|t|, scale = m / 127 rounded to 32 bits, code = the integer nearest to t / scale, ties to
  * even.  A group of zeros has scale 0; one that holds an infinity or NaN has scale NaN and codes 0, so that it reads as NaN.
- * residual_out (NULL, residual itself, or apart from it: behind it or in the gaps of its rows) gets t - code * scale, exactly, for the columns below the row's
- * length (0 in a group whose scale is NaN); the columns from there on are left as they are.  A page is always written whole, with
- * zeros behind the row's end. */
+ * residual_out (NULL, residual itself, or apart from it, in the gaps of its rows too) gets t - code * scale, exactly, for the
+ * columns below the row's length (0 in a group whose scale is NaN); the columns from there on are left as they are.  A page is
+ * always written whole, with zeros behind the row's end. */
 LB_API size_t lb_quantize_rows_workspace_bytes(int64_t n_rows, int64_t n_cols, int64_t page, int64_t group);
 LB_API int lb_quantize_rows(lb_context *ctx, const void *values, int dtype, int64_t n_rows, int64_t n_cols, int64_t value_stride,
                      const int32_t *lengths, const float *residual, float *residual_out, int64_t residual_stride, const int32_t *slots,
@@ -276,14 +276,16 @@ LB_API int lb_dequantize_rows(lb_context *ctx, const int8_t *codes, int64_t code
                        int dtype, int64_t out_stride, void *stream);
 /* out[i][j] = (sum over k of a[i][k] b[j][k]) * a_scale[i] * b_scale[j]: an exact integer sum (k <= 131071), scaled in 32 bits, rounded to
  * dtype.  a [m][k], b [n][k], any alignment of their rows (where m and n are above 32, rows off a 16-byte boundary
- * are copied into the workspace first).  a_scale [m], b_scale [n]; out must not overlap an operand. */
+ * are copied into the workspace first).  Such rows are read in whole aligned pieces of 16 bytes: up to 15 bytes on either side of a
+ * row's codes are read along and dropped.  a_scale [m], b_scale [n]; out must not overlap an operand. */
 LB_API size_t lb_int8_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t a_stride, const int8_t *b, int64_t b_stride);
 LB_API int lb_int8_matmul(lb_context *ctx, int64_t m, int64_t n, int64_t k, const int8_t *a, int64_t a_stride, const float *a_scale,
                    const int8_t *b, int64_t b_stride, const float *b_scale, void *out, int dtype, int64_t out_stride, void *workspace,
                    size_t workspace_bytes, void *stream);
 /* The selection rule's pair distances in the clear (lancelot-main-GPU/utils/byzantine_fl.py:162-171,527-536) over cached updates:
- * out[i][j] (DEVICE, n x n doubles) = the squared distance of rows i and j of the cache, 0 for i == j.  slots [n][n_pages]; the
- * pages of a row count whole (what lb_quantize_rows wrote behind a row's end are zeros).  n <= 4096. */
+ * out[i][j] (DEVICE, n x n doubles) = the squared distance of rows i and j of the cache, 0 for i == j; not finite where a scale
+ * of i or j is not.  slots [n][n_pages]; the pages of a row count whole (what lb_quantize_rows wrote behind a row's end are zeros).
+ * n <= 4096. */
 LB_API size_t lb_int8_distances_workspace_bytes(const lb_context *ctx, int64_t n, int64_t n_pages, int64_t page);
 LB_API int lb_int8_distances(lb_context *ctx, const int8_t *codes, int64_t code_stride, const float *scales, int64_t scale_stride,
                       int64_t n_slots, int64_t page, int64_t group, const int32_t *slots, int64_t n, int64_t n_pages, double *out,

@@ -191,9 +191,11 @@ __device__ void gram_tile(const DistanceArgs &a, const int row_a, const int row_
     }
 }
 
-// More than 128 clients: 32 by 32 of them a block, whose codes come from L2 once for each of the n / 32 blocks they meet.  Bound by
-// instructions and the latency of loads with two warps a quarter: 200 x 1.6 M takes 605 us with one scale a page, 1.6 ms with groups of 64
-// (64-bit operations of all pairs; 52 us at the copy rate).
+// More than 128 clients: 32 by 32 of them a block, whose codes come from L2 once for each of the n / 32 blocks they meet.  (The ring below
+// keeps the 64-bit sums of all pairs in one block's registers: 20 warps for 128 clients; 160 would take 30 of 64 registers, half of them
+// sums.)  Bound by instructions and the latency of loads with two warps a quarter: 200 x 1.6 M takes 605 us with one scale a page, 1.6 ms with
+// groups of 64 (64-bit operations of all pairs; 52 us at the copy rate).  At the border, 1.67 M values with one scale a page and with groups
+// of 64: 129 clients 305 and 780 us here, 128 clients 142 and 202 us in the ring.
 template <int BYTES> __global__ void __launch_bounds__(kWarps * 32) gram_kernel(const DistanceArgs a, const int n_blocks)
 {
     __shared__ double sum[32 * 32];

@@ -27,7 +27,7 @@ __device__ __forceinline__ float scaled(int sum, float sa, float sb) { return __
 
 // ---- rows off a 16-byte boundary --------------------------------------------------------------------------------------------
 // 16 codes from p on, zeros from `left` codes on.  Not aligned: out of the two aligned lines that they lie in, the second one only where it
-// holds one of them.
+// holds one of them.  What else such a line holds is dropped; it lies in the same 16 bytes as a code of the operand, so it can be read.
 template <bool ALIGNED> __device__ __forceinline__ uint4 load16(const signed char *p, int left)
 {
     if (left <= 0) return make_uint4(0, 0, 0, 0);
@@ -143,7 +143,8 @@ template <typename T, bool ALIGNED> int launch_skinny(const SkinnyArgs &a, cudaS
 // One CTA per SM walks over tiles of 128 x BN.  Warp 0 brings 128-byte wide blocks of k by TMA into a ring of stages, warp 1
 // issues the products (four of k = 32 a stage), warps 2 to 5 take a finished tile out of TMEM.  TMEM holds two tiles, so
 // a tile leaves while the next one is being formed.  Bound by the tensor cores where k is long: 8192 x 8192 x 8192 in 372 us, 2.95 P
-// operations a second (0.91 of twice the rate that bf16 products reach), and by the results where it is short: 4096 x 4096 x 16 in 18 us
+// operations a second (0.91 of twice the rate that bf16 products reach), in a burst; one such product after the other takes some 430 us (2.56 P)
+// under the power cap.  Bound by the results where it is short: 4096 x 4096 x 16 in 18 us
 // (67 MB).  All of warp 1 comes to the instruction and one lane is elected, instead of a branch for lane 0: the operands are then in
 // uniform registers (64 x 64 x 131056: 230 us, 300 us before).
 constexpr int kTileM = 128, kTileK = 128;

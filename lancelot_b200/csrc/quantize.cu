@@ -11,9 +11,10 @@
 // place, and |r| is about s / 2, so it has at most 24 bits), and comparing 2 |r| with s settles the border, ties included.
 // The same r is what the rounding lost, exactly: error feedback adds no error of its own.
 //
-// All kernels stream: bound by HBM at (value bytes + 1 + 8 with a residual) per value.  20 rows of 11 M 32-bit values with residuals, one
+// All kernels stream, (value bytes + 1 + 8 with a residual) per value.  Bound by HBM with 32-bit values and residuals: 20 rows of 11 M, one
 // B200 that copies at 6.5 TB/s: groups of 128 in 496 us (5.9 TB/s), one scale for 32768 columns in 479 us (6.1), for 131072 columns in
-// 856 us, where every value is read twice; read back in 179 us (6.3 TB/s).  Moves of 16 bytes are what it takes, for rows off
+// 856 us, where every value is read twice; read back in 179 us (6.3 TB/s).  With fewer bytes a value the instructions and waits of a group show:
+// 32-bit values without residuals 271 us (one scale for 32768 columns), 338 us (groups of 128), 16-bit ones 266 and 341 us (2.5, 2.0 TB/s).  Moves of 16 bytes are what it takes, for rows off
 // their alignment too: these are taken in the values' aligned pieces and the codes are shifted, not the values.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
