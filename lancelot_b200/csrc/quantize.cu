@@ -13,9 +13,10 @@
 //
 // All kernels stream, (value bytes + 1 + 8 with a residual) per value.  Bound by HBM with 32-bit values and residuals: 20 rows of 11 M, one
 // B200 that copies at 6.5 TB/s: groups of 128 in 496 us (5.9 TB/s), one scale for 32768 columns in 479 us (6.1), for 131072 columns in
-// 856 us, where every value is read twice; read back in 179 us (6.3 TB/s).  With fewer bytes a value the instructions and waits of a group show:
-// 32-bit values without residuals 271 us (one scale for 32768 columns), 338 us (groups of 128), 16-bit ones 266 and 341 us (2.5, 2.0 TB/s).  Moves of 16 bytes are what it takes, for rows off
-// their alignment too: these are taken in the values' aligned pieces and the codes are shifted, not the values.
+// 856 us, where every value is read twice; read back in 179 us (6.3 TB/s).  With fewer bytes a value the instructions bound
+// it: 32-bit values without residuals 271 us (one scale for 32768 columns), 338 us (groups of 128), 16-bit ones 266 and 341 us (2.5 and 2.0
+// TB/s, with instructions issued in 65 and 81 % of the cycles).  Moves of 16 bytes are what it takes, for rows off their alignment too:
+// these are taken in the values' aligned pieces and the codes are shifted, not the values.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
