@@ -291,6 +291,53 @@ LB_API int lb_int8_distances(lb_context *ctx, const int8_t *codes, int64_t code_
                       int64_t n_slots, int64_t page, int64_t group, const int32_t *slots, int64_t n, int64_t n_pages, double *out,
                       void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- 8-bit floating point, clipping (no counterpart in the reference) ----------------------------
+ * Matrices in 8-bit floating point (code_type 5 = e4m3, largest value M = 448; 6 = e5m2, M = 57344) with a scale for each block of
+ * 128 values.  blocks: 1 = 128 columns of a row, scales [n_rows][ceil(n_cols / 128)]; 2 = 128 rows of a column,
+ * scales [ceil(n_rows / 128)][n_cols]; 4 = 128 x 128, scales [ceil(n_rows / 128)][ceil(n_cols / 128)]; the last block of an axis may be
+ * shorter.  dtype, strides and workspaces as in the calls above. */
+
+/* m = max|v| of a block, scale = m / M rounded to 32 bits, code = the type's value nearest to v / scale, ties to even, at most M in
+ * magnitude.  A block of zeros has scale 0; one that holds an infinity or NaN has scale NaN and codes 0, so that it reads as NaN.
+ * blocks 1 and 4 fill codes and scales, 2 codes_down and scales_down, 3 all four, with the blocks of 1 and of 2.  Results must not overlap
+ * values or one another. */
+LB_API int lb_quantize_fp8(lb_context *ctx, const void *values, int dtype, int64_t n_rows, int64_t n_cols, int64_t value_stride, int blocks,
+                    int code_type, uint8_t *codes, int64_t code_stride, float *scales, int64_t scale_stride, uint8_t *codes_down,
+                    int64_t code_down_stride, float *scales_down, int64_t scale_down_stride, void *stream);
+/* out = code * scale (32 bits, then rounded to dtype); blocks is 1, 2 or 4 */
+LB_API int lb_dequantize_fp8(lb_context *ctx, const uint8_t *codes, int code_type, int64_t code_stride, const float *scales, int64_t scale_stride,
+                      int blocks, int64_t n_rows, int64_t n_cols, void *out, int dtype, int64_t out_stride, void *stream);
+
+/* An operand X [rows][k] of a product over k.  across 0: stored as it is, row r at codes + r * stride; across 1: its transpose is
+ * stored, the rows' entries of place q of k at codes + q * stride.  The scale of row r in block p of k (128 places of k) is
+ * scales[(r / scale_rows) * scale_row + p * scale_block], scale_rows 1 or 128. */
+typedef struct lb_fp8_operand {
+    const uint8_t *codes;
+    int64_t stride;
+    int across, code_type;
+    const float *scales;
+    int64_t scale_row, scale_block;
+    int scale_rows;
+} lb_fp8_operand;
+
+/* out[i][j] = sum over blocks p of ((sum over k in p of a[i][k] b[j][k]) * a's scale) * b's scale: sums and products in 32-bit floats, one rounding to
+ * dtype.  The scales are multiplied in that order: their product with a block's sum has to stay in the range of 32 bits.
+ * Any alignment of the codes' rows: those off a 16-byte boundary may be copied into the workspace first, and are read in whole
+ * aligned pieces of 16 bytes (up to 15 bytes on either side are read along and dropped).  out must not overlap an operand. */
+LB_API size_t lb_fp8_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, const lb_fp8_operand *a, const lb_fp8_operand *b);
+LB_API int lb_fp8_matmul(lb_context *ctx, int64_t m, int64_t n, int64_t k, const lb_fp8_operand *a, const lb_fp8_operand *b, void *out, int dtype,
+                  int64_t out_stride, void *workspace, size_t workspace_bytes, void *stream);
+
+/* norms[c] (DEVICE, n_clients doubles) = sqrt of the sum of squares, in 64 bits, over all tensors of client c (0 if it has none).
+ * outs (HOST array, NULL: norms only): out = v * f, in 32 bits, then rounded to its type, with f = 1 where norms[c] <= max_norm,
+ * max_norm / norms[c] rounded to 32 bits where it is larger, NaN where it is not finite.  tensors, outs: HOST arrays of n_tensors device
+ * pointers to sizes[i] contiguous values of type dtypes[i], out_dtypes[i]; clients[i], not decreasing: whose tensor it is.
+ * outs[i] is tensors[i] itself or apart from all tensors and all other results. */
+LB_API size_t lb_clip_updates_workspace_bytes(const lb_context *ctx, int n_clients, int n_tensors, const int *clients, const int64_t *sizes);
+LB_API int lb_clip_updates(lb_context *ctx, int n_clients, int n_tensors, const int *clients, const void *const *tensors, const int *dtypes,
+                    const int64_t *sizes, double max_norm, void *const *outs, const int *out_dtypes, double *norms, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
 /* Synchronises the stream and reports (then clears) conditions kernels could only flag. */
 LB_API int lb_check_status(lb_context *ctx, void *stream);
 

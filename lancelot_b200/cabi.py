@@ -35,6 +35,8 @@ def to_host(t):
 
 
 VALUE_TYPES = {torch.float32: 1, torch.bfloat16: 3, torch.float16: 4}  # the value types of the 8-bit cache as the C ABI numbers them
+FP8_TYPES = {torch.float8_e4m3fn: 5, torch.float8_e5m2: 6}
+FP8_BLOCKS = {(1, 128): 1, (128, 1): 2, (128, 128): 4}
 
 
 @functools.lru_cache(None)
@@ -437,6 +439,41 @@ class Context:
     def int8_distances(self, codes, scales, slots, group=0):
         """squared distances between all pairs of cached rows: slots [n][pages] int32 -> [n][n] float64 (0 on the diagonal)"""
         return _updates8().int8_distances(self._handle(), self.device, codes, scales, slots, group)
+
+    # -- 8-bit floating point (codes float8_e4m3fn or float8_e5m2 with a float32 scale for each block of 128 values), clipping
+    def quantize_fp8(self, values, block=(1, 128), dtype=torch.float8_e4m3fn, codes=None, scales=None):
+        """values [n][cols] (float32, bfloat16, float16; rows may be strided) -> (codes [n][cols] of dtype, scales).  block: (1, 128), 128 columns of a
+        row, scales [n][ceil(cols / 128)]; (128, 1), 128 rows of a column, scales [ceil(n / 128)][cols]; (128, 128).  scale = the block's largest
+        magnitude / the largest value of dtype; a code is the value nearest to value / scale, ties to even.  A block that holds an infinity or
+        NaN reads as NaN.  codes, scales: where the results go (made here if not given, the codes' rows on 16-byte boundaries)"""
+        blocks = FP8_BLOCKS.get(tuple(block) if isinstance(block, (tuple, list)) else block, 0)
+        if blocks == 2:
+            return _updates8().quantize_fp8(self._handle(), self.device, values, blocks, FP8_TYPES.get(dtype, 0), None, None, codes, scales)
+        return _updates8().quantize_fp8(self._handle(), self.device, values, blocks, FP8_TYPES.get(dtype, 0), codes, scales, None, None)
+
+    def quantize_fp8_both(self, values, dtype=torch.float8_e4m3fn):
+        """quantize_fp8 with blocks (1, 128) and (128, 1) in one pass -> (codes, scales, codes_down, scales_down): the operands of a product over the
+        columns and of one over the rows"""
+        return _updates8().quantize_fp8(self._handle(), self.device, values, 3, FP8_TYPES.get(dtype, 0), None, None, None, None)
+
+    def dequantize_fp8(self, codes, scales, dtype=torch.float32, out=None):
+        """code * scale in 32 bits -> [n][cols] of dtype (or of out); the shape of scales says which blocks they belong to"""
+        return _updates8().dequantize_fp8(self._handle(), self.device, codes, scales, VALUE_TYPES.get(dtype, 0), out)
+
+    def fp8_matmul(self, a, a_scale, b, b_scale, dtype=torch.bfloat16, out=None):
+        """a [m][k], b [n][k] of 8-bit floats -> [m][n]: for each block of 128 of k, the sum of products times a's and b's scales, added up in 32
+        bits.  a_scale [m][ceil(k / 128)] or [ceil(m / 128)][ceil(k / 128)], b_scale likewise.  An operand is dense along either
+        axis: transposed views (of codes and scales) give the gradients of a product without a copy.  With x8, xs = quantize_fp8(x), w8, ws =
+        quantize_fp8(w, (128, 128)) and y = fp8_matmul(x8, xs, w8, ws), the gradient of x is fp8_matmul(g8, gs, w8.t(), ws.t()), that of w
+        fp8_matmul(gd.t(), gds.t(), xd.t(), xds.t()) from the codes in blocks (128, 1)"""
+        return _updates8().fp8_matmul(self._handle(), self.device, a, a_scale, b, b_scale, VALUE_TYPES.get(dtype, 0), out)
+
+    def clip_updates(self, updates, max_norm=None, out=None):
+        """The norm of each client's update over all its tensors -> [n_clients] float64, on the device.  updates: for each client a list of tensors
+        (float32, bfloat16, float16, also mixed), or a matrix with a row for each client.  With max_norm, updates of a larger norm are
+        scaled down to it, in place; one whose norm is not finite becomes NaN throughout.  out [n_clients][values] (float32, bfloat16,
+        float16): the (scaled) values of each client, tensor by tensor, go there instead, and the tensors stay as they are"""
+        return _updates8().clip_updates(self._handle(), self.device, updates, max_norm, out)
 
     def check_status(self):
         check(lib.lb_check_status(self.h, self._stream()))

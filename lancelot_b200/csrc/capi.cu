@@ -875,6 +875,237 @@ int lb_int8_distances(lb_context *h, const int8_t *codes, int64_t code_stride, c
                           (int)(group > page ? 0 : group), slots, (int)n, (int)n_pages, out, workspace, S(stream));
 }
 
+// ---- 8-bit floating point, clipping -----------------------------------------------------------------------
+
+static int code_type_ok(int code_type)
+{
+    REQUIRE(code_type == 5 || code_type == 6, "code_type is 5 (e4m3) or 6 (e5m2)");
+    return LB_OK;
+}
+static int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+int lb_quantize_fp8(lb_context *h, const void *values, int dtype, int64_t n_rows, int64_t n_cols, int64_t value_stride, int blocks, int code_type,
+                    uint8_t *codes, int64_t code_stride, float *scales, int64_t scale_stride, uint8_t *codes_down, int64_t code_down_stride,
+                    float *scales_down, int64_t scale_down_stride, void *stream)
+{
+    int rc = bind(h);
+    if (rc) return rc;
+    REQUIRE(value_size(dtype), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+    REQUIRE(blocks >= 1 && blocks <= 4, "blocks is 1 (rows), 2 (columns), 3 (both) or 4 (square)");
+    if ((rc = code_type_ok(code_type))) return rc;
+    REQUIRE(n_rows >= 0 && n_cols >= 0 && n_rows <= (int64_t)1 << 31 && n_cols <= (1 << 30), "n_rows or n_cols is out of range");
+    if (n_rows == 0 || n_cols == 0) return LB_OK;
+    REQUIRE(blocks_of(n_rows) * blocks_of(n_cols) < (int64_t)1 << 31, "too many blocks for one call");
+    if ((rc = rows_ok(values, n_rows, n_cols, value_stride, value_size(dtype)))) return rc;
+    if (blocks != 2) {
+        if ((rc = rows_ok(codes, n_rows, n_cols, code_stride, 1))) return rc;
+        if ((rc = rows_ok(scales, blocks == 4 ? blocks_of(n_rows) : n_rows, blocks_of(n_cols), scale_stride, 4))) return rc;
+    }
+    if (blocks == 2 || blocks == 3) {
+        if ((rc = rows_ok(codes_down, n_rows, n_cols, code_down_stride, 1))) return rc;
+        if ((rc = rows_ok(scales_down, blocks_of(n_rows), n_cols, scale_down_stride, 4))) return rc;
+    }
+    return quantize_fp8(values, dtype, n_rows, (int)n_cols, value_stride, blocks, code_type, codes, code_stride, scales, scale_stride, codes_down,
+                        code_down_stride, scales_down, scale_down_stride, S(stream));
+}
+
+int lb_dequantize_fp8(lb_context *h, const uint8_t *codes, int code_type, int64_t code_stride, const float *scales, int64_t scale_stride, int blocks,
+                      int64_t n_rows, int64_t n_cols, void *out, int dtype, int64_t out_stride, void *stream)
+{
+    int rc = bind(h);
+    if (rc) return rc;
+    REQUIRE(value_size(dtype), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+    REQUIRE(blocks == 1 || blocks == 2 || blocks == 4, "blocks is 1 (rows), 2 (columns) or 4 (square)");
+    if ((rc = code_type_ok(code_type))) return rc;
+    REQUIRE(n_rows >= 0 && n_cols >= 0 && n_rows <= (int64_t)1 << 31 && n_cols <= (1 << 30), "n_rows or n_cols is out of range");
+    if (n_rows == 0 || n_cols == 0) return LB_OK;
+    if ((rc = rows_ok(codes, n_rows, n_cols, code_stride, 1))) return rc;
+    if ((rc = rows_ok(scales, blocks == 1 ? n_rows : blocks_of(n_rows), blocks == 2 ? n_cols : blocks_of(n_cols), scale_stride, 4))) return rc;
+    if ((rc = rows_ok(out, n_rows, n_cols, out_stride, value_size(dtype)))) return rc;
+    return dequantize_fp8(C(h), codes, code_type, code_stride, scales, scale_stride, blocks, n_rows, (int)n_cols, out, dtype, out_stride, S(stream));
+}
+
+static Fp8Operand operand_of(const lb_fp8_operand *o)
+{
+    return Fp8Operand{o->codes, o->stride, o->across, o->code_type, o->scales, o->scale_row, o->scale_block, o->scale_rows == 128 ? 7 : 0};
+}
+static int operand_ok(const lb_fp8_operand *o, int64_t rows, int64_t k)
+{
+    REQUIRE(o, "operand is null");
+    int rc = code_type_ok(o->code_type);
+    if (rc) return rc;
+    REQUIRE(o->across == 0 || o->across == 1, "across is 0 or 1");
+    REQUIRE(o->scale_rows == 1 || o->scale_rows == 128, "a scale is for 1 row or for 128");
+    if (k == 0 || rows == 0) return LB_OK;
+    if ((rc = rows_ok(o->codes, o->across ? k : rows, o->across ? rows : k, o->stride, 1))) return rc;
+    REQUIRE(o->scales && (uintptr_t)o->scales % 4 == 0, "the scales are null or not aligned to their type");
+    const int64_t n = o->scale_rows == 128 ? blocks_of(rows) : rows;
+    REQUIRE((n <= 1 || (o->scale_row >= 0 && o->scale_row <= (int64_t)1 << 40)) && (k <= 128 || (o->scale_block >= 0 && o->scale_block <= (int64_t)1 << 40)),
+            "a stride of the scales is out of range");
+    return LB_OK;
+}
+
+size_t lb_fp8_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, const lb_fp8_operand *a, const lb_fp8_operand *b)
+{
+    if (m < 1 || n < 1 || k < 1 || m > (1 << 30) || n > (1 << 30) || k > (1 << 30) || !a || !b) return 0;
+    return fp8_matmul_workspace_bytes((int)m, (int)n, (int)k, operand_of(a), operand_of(b));
+}
+
+int lb_fp8_matmul(lb_context *h, int64_t m, int64_t n, int64_t k, const lb_fp8_operand *a, const lb_fp8_operand *b, void *out, int dtype,
+                  int64_t out_stride, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = bind(h);
+    if (rc) return rc;
+    REQUIRE(value_size(dtype), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+    REQUIRE(m >= 0 && n >= 0 && k >= 0 && m <= (1 << 30) && n <= (1 << 30) && k <= (1 << 30), "m, n or k is out of range");
+    if ((rc = operand_ok(a, m, k)) || (rc = operand_ok(b, n, k))) return rc;
+    if (m == 0 || n == 0) return LB_OK;
+    REQUIRE(blocks_of(m) * ((n + 63) / 64) < (int64_t)1 << 31, "too many tiles for one call");
+    if ((rc = rows_ok(out, m, n, out_stride, value_size(dtype)))) return rc;
+    if (k == 0) { // an empty sum
+        LB_CUDA(cudaMemset2DAsync(out, (size_t)(m > 1 ? out_stride : n) * value_size(dtype), 0, (size_t)n * value_size(dtype), (size_t)m, S(stream)));
+        return LB_OK;
+    }
+    if ((rc = workspace_ok(workspace, workspace_bytes, lb_fp8_matmul_workspace_bytes(m, n, k, a, b)))) return rc;
+    return fp8_matmul(C(h), (int)m, (int)n, (int)k, operand_of(a), operand_of(b), out, dtype, out_stride, workspace, S(stream));
+}
+
+// The pieces of a call: as many of each tensor as its elements take, one (of no elements) for a client that has none
+static int64_t clip_parts(const Context *c, int n_clients, int n_tensors, const int *clients, const int64_t *sizes, int &piece, std::vector<ClipPart> *parts)
+{
+    double all = 0.0;
+    for (int i = 0; i < n_tensors; ++i) all += (double)sizes[i];
+    piece = clip_piece(c, all);
+    int64_t at = 0;
+    int i = 0;
+    for (int k = 0; k < n_clients; ++k) {
+        const int64_t begin = at;
+        const size_t first = parts ? parts->size() : 0;
+        for (; i < n_tensors && clients[i] == k; ++i) {
+            if (sizes[i] == 0) continue;
+            if (parts) {
+                ClipPart p = {};
+                p.n = sizes[i];
+                p.first = (int)at;
+                p.client = k;
+                p.in_type = i; // the tensor, for the caller to fill in
+                parts->push_back(p);
+            }
+            at += (sizes[i] + piece - 1) / piece;
+        }
+        if (at == begin) {
+            if (parts) {
+                ClipPart p = {};
+                p.first = (int)at;
+                p.client = k;
+                p.in_type = -1;
+                parts->push_back(p);
+            }
+            ++at;
+        }
+        if (parts)
+            for (size_t j = first; j < parts->size(); ++j) (*parts)[j].begin = (int)begin, (*parts)[j].end = (int)at;
+    }
+    return at;
+}
+
+static int clip_ok(int n_clients, int n_tensors, const int *clients, const int64_t *sizes)
+{
+    REQUIRE(n_clients >= 0 && n_clients < 1 << 23 && n_tensors >= 0, "n_clients or n_tensors is out of range");
+    REQUIRE(n_tensors == 0 || (clients && sizes), "operand is null");
+    double all = 0.0;
+    for (int i = 0; i < n_tensors; ++i) {
+        REQUIRE(clients[i] >= (i ? clients[i - 1] : 0) && clients[i] < n_clients, "the tensors are in the order of their clients");
+        REQUIRE(sizes[i] >= 0 && sizes[i] <= (int64_t)1 << 40, "a tensor's size is out of range");
+        all += (double)sizes[i] / 1024 + 1;
+    }
+    REQUIRE(all + n_clients < (double)(1 << 30), "too many values for one call");
+    return LB_OK;
+}
+
+// No result may lie on another one, or on what is still to be read: in place, a tensor's result is the tensor itself
+static int clip_apart(const std::vector<ClipPart> &parts)
+{
+    struct Span {
+        uintptr_t begin, end;
+        bool out;
+    };
+    std::vector<Span> spans;
+    spans.reserve(2 * parts.size());
+    uintptr_t low = UINTPTR_MAX, high = 0, last = 0;
+    bool in_order = true;
+    for (const ClipPart &p : parts)
+        if (p.out) {
+            const uintptr_t b = (uintptr_t)p.out, e = b + (uintptr_t)p.n * (uintptr_t)value_size(p.out_type);
+            in_order = in_order && b >= last;
+            last = e;
+            low = b < low ? b : low;
+            high = e > high ? e : high;
+            spans.push_back({b, e, true});
+        }
+    if (spans.empty()) return LB_OK;
+    bool clear = in_order;
+    for (const ClipPart &p : parts)
+        if (p.n && p.in != p.out) {
+            const uintptr_t b = (uintptr_t)p.in, e = b + (uintptr_t)p.n * (uintptr_t)value_size(p.in_type);
+            clear = clear && (e <= low || b >= high);
+            spans.push_back({b, e, false});
+        }
+    if (clear) return LB_OK;
+    std::sort(spans.begin(), spans.end(), [](const Span &x, const Span &y) { return x.begin < y.begin; });
+    uintptr_t any = 0, out = 0;
+    for (const Span &s : spans) {
+        REQUIRE(s.begin >= (s.out ? any : out), "a result overlaps another one, or a tensor that is not its own");
+        any = s.end > any ? s.end : any;
+        if (s.out) out = s.end > out ? s.end : out;
+    }
+    return LB_OK;
+}
+
+size_t lb_clip_updates_workspace_bytes(const lb_context *h, int n_clients, int n_tensors, const int *clients, const int64_t *sizes)
+{
+    if (!h || !h->c || n_clients < 1 || clip_ok(n_clients, n_tensors, clients, sizes)) return 0;
+    int piece = 0;
+    return (size_t)clip_parts(h->c, n_clients, n_tensors, clients, sizes, piece, nullptr) * 8;
+}
+
+int lb_clip_updates(lb_context *h, int n_clients, int n_tensors, const int *clients, const void *const *tensors, const int *dtypes,
+                    const int64_t *sizes, double max_norm, void *const *outs, const int *out_dtypes, double *norms, void *workspace,
+                    size_t workspace_bytes, void *stream)
+try {
+    int rc = bind(h);
+    if (rc) return rc;
+    if ((rc = clip_ok(n_clients, n_tensors, clients, sizes))) return rc;
+    REQUIRE(max_norm >= 0.0, "max_norm is a number that is not negative");
+    if (n_clients == 0) return LB_OK;
+    REQUIRE(norms && (n_tensors == 0 || (tensors && dtypes)) && (!outs || out_dtypes), "operand is null");
+    REQUIRE((uintptr_t)norms % 8 == 0, "an operand is not aligned to its type");
+    std::vector<ClipPart> parts;
+    int piece = 0;
+    const int64_t pieces = clip_parts(C(h), n_clients, n_tensors, clients, sizes, piece, &parts);
+    for (ClipPart &p : parts) {
+        const int i = p.in_type;
+        p.in_type = p.out_type = 1;
+        if (i < 0) continue;
+        REQUIRE(value_size(dtypes[i]), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+        REQUIRE(tensors[i] && (uintptr_t)tensors[i] % value_size(dtypes[i]) == 0, "a tensor is null or not aligned to its type");
+        p.in = tensors[i];
+        p.in_type = dtypes[i];
+        if (!outs) continue;
+        REQUIRE(value_size(out_dtypes[i]), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+        REQUIRE(outs[i] && (uintptr_t)outs[i] % value_size(out_dtypes[i]) == 0, "a result is null or not aligned to its type");
+        REQUIRE(outs[i] != tensors[i] || out_dtypes[i] == dtypes[i], "a result in place has the type of its tensor");
+        p.out = outs[i];
+        p.out_type = out_dtypes[i];
+    }
+    if ((rc = clip_apart(parts))) return rc;
+    if ((rc = workspace_ok(workspace, workspace_bytes, (size_t)pieces * 8))) return rc;
+    return clip_updates(C(h), parts.data(), (int)parts.size(), piece, max_norm, reinterpret_cast<double *>(workspace), norms, S(stream));
+} catch (const std::bad_alloc &) {
+    set_error("out of host memory");
+    return LB_ERR_NO_MEMORY;
+}
+
 int lb_check_status(lb_context *h, void *stream)
 {
     int rc = bind(h);

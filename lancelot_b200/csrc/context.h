@@ -222,4 +222,32 @@ size_t int8_distances_workspace_bytes(const Context *ctx, int n, long pages, int
 int int8_distances(Context *ctx, const signed char *codes, long code_stride, const float *scales, long scale_stride, long n_slots, int page,
                    int group, const int *slots, int n, int pages, double *out, void *workspace, cudaStream_t stream);
 
+// 8-bit floating point by blocks of 128 (fp8_quantize.cu, fp8_product.cu).  Code types: 5 = e4m3, 6 = e5m2; blocks: 1 = 128 columns of a row,
+// 2 = 128 rows of a column, 3 = both, 4 = 128 x 128
+struct Fp8Operand {
+    const unsigned char *codes;
+    long stride; // bytes between stored rows
+    int across;  // 1: the summed axis lies across the stored rows
+    int type;
+    const float *scales;
+    long scale_row, scale_block; // from one row (of 128 rows where scale_shift is 7) to the next, from one block of the summed axis to the next
+    int scale_shift;
+};
+int quantize_fp8(const void *values, int dtype, long rows, int cols, long stride, int blocks, int code_type, unsigned char *codes, long code_stride,
+                 float *scales, long scale_stride, unsigned char *down, long down_stride, float *down_scales, long down_scale_stride, cudaStream_t stream);
+int dequantize_fp8(const Context *ctx, const unsigned char *codes, int code_type, long code_stride, const float *scales, long scale_stride, int blocks,
+                   long rows, int cols, void *out, int dtype, long out_stride, cudaStream_t stream);
+size_t fp8_matmul_workspace_bytes(int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b);
+int fp8_matmul(Context *ctx, int m, int n, int k, Fp8Operand a, Fp8Operand b, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream);
+
+// norms and clipping (clip.cu): a tensor of a client, in pieces of `piece` elements; first: of the call's pieces, begin and end: its client's
+struct ClipPart {
+    const void *in;
+    void *out;
+    long n;
+    int first, begin, end, client, in_type, out_type;
+};
+int clip_piece(const Context *ctx, double elements);
+int clip_updates(const Context *ctx, const ClipPart *parts, int n_parts, int piece, double most, double *partial, double *norms, cudaStream_t stream);
+
 } // namespace lb

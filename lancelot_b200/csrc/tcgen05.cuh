@@ -1,4 +1,4 @@
-// What the kernels on Blackwell's tensor memory share: bounded mbarrier waits, TMA loads, tcgen05 in its 8-bit integer form.
+// What the kernels on Blackwell's tensor memory share: bounded mbarrier waits, TMA loads, tcgen05 in its 8-bit integer and 8-bit floating-point forms.
 #pragma once
 #include <cuda.h>
 
@@ -82,10 +82,21 @@ __device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, i
                  "r"(x), "r"(y), "r"(bar)
                  : "memory");
 }
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, int x, int y, unsigned src)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 // rows of 128 bytes, 128-byte swizzle: groups of eight rows 1024 bytes apart
 __device__ __forceinline__ unsigned long long operand_desc(unsigned addr)
 {
     return (unsigned long long)((addr & 0x3ffff) >> 4) | 1ull << 16 | (unsigned long long)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// The same bytes with the summed axis across the rows: a row holds 128 places along the other axis, eight rows (of the summed axis) lie 1024 bytes
+// before the next eight; runs of 128 places are `run` bytes apart
+__device__ __forceinline__ unsigned long long operand_desc_across(unsigned addr, unsigned run)
+{
+    return (unsigned long long)((addr & 0x3ffff) >> 4) | (unsigned long long)(run >> 4) << 16 | (unsigned long long)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 // One lane issues (`elected`, from elect_one), but the whole warp comes here, and without divergence: the operands are uniform
 // registers, which the compiler only uses where the warp provably stays together.
@@ -98,6 +109,12 @@ __device__ __forceinline__ unsigned elect_one()
 __device__ __forceinline__ void mma_i8(unsigned elected, unsigned d, unsigned long long a, unsigned long long b, unsigned desc, bool add)
 {
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(desc), "r"((unsigned)add), "r"(elected)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_f8(unsigned elected, unsigned d, unsigned long long a, unsigned long long b, unsigned desc, bool add)
+{
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
                  "l"(a), "l"(b), "r"(desc), "r"((unsigned)add), "r"(elected)
                  : "memory");
 }

@@ -1,14 +1,18 @@
-// The 8-bit update calls of cabi.Context on torch tensors: argument checks, results and workspaces, then one lb_* call each.  These
+// The 8-bit update calls of cabi.Context (integers, floating point) and its clipping on torch tensors: argument checks, results and workspaces, then one lb_* call each.  These
 // kernels run in a few microseconds where operands are small; the same checks in Python took longer than the kernels.
 // Built by lancelot_b200/pybind/build.py; links liblancelot_b200.so and torch's C++ libraries and launches nothing itself.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_strided.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cmath>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "lancelot_b200.h"
 
@@ -182,6 +186,179 @@ Tensor int8_distances(int64_t context, int device, const Tensor &codes, const Te
     return out;
 }
 
+// ---- 8-bit floating point -------------------------------------------------------------------------------------------------------
+int code_type(const Tensor &t, const char *what) // as the C ABI numbers them
+{
+    if (t.scalar_type() == at::kFloat8_e4m3fn) return 5;
+    if (t.scalar_type() == at::kFloat8_e5m2) return 6;
+    refuse(std::string(what) + " must be of type float8_e4m3fn or float8_e5m2");
+}
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// codes and scales of one kind of blocks: given ones are checked, missing ones made, with rows of codes on 16-byte boundaries
+void blocks_into(const Call &c, Maybe &codes, Maybe &scales, int64_t rows, int64_t cols, int64_t scale_rows, int64_t scale_cols, int type)
+{
+    const at::ScalarType t = type == 5 ? at::kFloat8_e4m3fn : at::kFloat8_e5m2;
+    if (!codes) codes = at::empty_strided({rows, cols}, {std::max<int64_t>((cols + 15) / 16 * 16, 16), 1}, at::TensorOptions().dtype(t).device(at::kCUDA, (c10::DeviceIndex)c.device));
+    if (!scales) scales = c.empty({scale_rows, scale_cols}, at::kFloat);
+    c.tensor(*codes, 2, t, "codes");
+    c.tensor(*scales, 2, at::kFloat, "scales");
+    if (codes->size(0) != rows || codes->size(1) != cols) refuse("codes must have the shape of values");
+    if (scales->size(0) != scale_rows || scales->size(1) != scale_cols)
+        refuse("scales must be [" + std::to_string(scale_rows) + "][" + std::to_string(scale_cols) + "]");
+}
+
+py::tuple quantize_fp8(int64_t context, int device, const Tensor &values, int blocks, int type, Maybe codes, Maybe scales, Maybe codes_down, Maybe scales_down)
+{
+    const Call c = call_of(context, device);
+    c.tensor(values, 2, "values");
+    const int dtype = value_type(values.scalar_type());
+    if (!dtype) refuse("values must be float32, bfloat16 or float16");
+    if (blocks < 1 || blocks > 4) refuse("block must be (1, 128), (128, 1) or (128, 128)");
+    if (type != 5 && type != 6) refuse("dtype must be float8_e4m3fn or float8_e5m2");
+    const int64_t n = values.size(0), cols = values.size(1);
+    if (blocks != 2) blocks_into(c, codes, scales, n, cols, blocks == 4 ? blocks_of(n) : n, blocks_of(cols), type);
+    if (blocks == 2 || blocks == 3) blocks_into(c, codes_down, scales_down, n, cols, blocks_of(n), cols, type);
+    auto stride = [](const Maybe &t) { return t ? row_stride(*t) : 0; };
+    check(lb_quantize_fp8(c.context, address<void>(values), dtype, n, cols, row_stride(values), blocks, type, address<uint8_t>(codes), stride(codes),
+                          address<float>(scales), stride(scales), address<uint8_t>(codes_down), stride(codes_down), address<float>(scales_down),
+                          stride(scales_down), c.stream()));
+    if (blocks == 3) return py::make_tuple(*codes, *scales, *codes_down, *scales_down);
+    return blocks == 2 ? py::make_tuple(*codes_down, *scales_down) : py::make_tuple(*codes, *scales);
+}
+
+Tensor dequantize_fp8(int64_t context, int device, const Tensor &codes, const Tensor &scales, int dtype, const Maybe &out)
+{
+    const Call c = call_of(context, device);
+    c.tensor(codes, 2, "codes");
+    const int type = code_type(codes, "codes");
+    c.tensor(scales, 2, at::kFloat, "scales");
+    const int64_t n = codes.size(0), cols = codes.size(1), r = scales.size(0), q = scales.size(1);
+    // where two kinds of blocks have scales of the same shape they are the same blocks
+    const int blocks = r == n && q == blocks_of(cols) ? 1 : r == blocks_of(n) && q == cols ? 2 : r == blocks_of(n) && q == blocks_of(cols) ? 4 : 0;
+    if (!blocks) refuse("scales must have one entry for each block of 128 columns, 128 rows or 128 x 128");
+    const Tensor to = result(c, out, n, cols, dtype);
+    check(lb_dequantize_fp8(c.context, address<uint8_t>(codes), type, row_stride(codes), address<float>(scales), row_stride(scales), blocks, n, cols,
+                            address<void>(to), value_type(to.scalar_type()), row_stride(to), c.stream()));
+    return to;
+}
+
+// [rows][k] with its scales; dense along either axis
+lb_fp8_operand operand(const Call &c, const Tensor &t, const Tensor &scales, const char *what)
+{
+    if (!t.is_cuda() || t.get_device() != c.device) refuse(std::string(what) + " must be a tensor on cuda:" + std::to_string(c.device));
+    if (t.dim() != 2) refuse(std::string(what) + " must have 2 dimension(s)");
+    lb_fp8_operand o = {};
+    o.code_type = code_type(t, what);
+    const int64_t rows = t.size(0), k = t.size(1);
+    const bool along = k <= 1 || t.stride(1) == 1, across = rows <= 1 || t.stride(0) == 1;
+    if (!along && !across) refuse(std::string(what) + " must be dense along one of its axes");
+    // a single column that is dense as a row: the row
+    o.across = !along || (across && k == 1 && rows > 1);
+    o.codes = address<uint8_t>(t);
+    o.stride = o.across ? (k > 1 ? t.stride(1) : rows) : (rows > 1 ? t.stride(0) : k);
+    if (!scales.is_cuda() || scales.get_device() != c.device || scales.scalar_type() != at::kFloat || scales.dim() != 2)
+        refuse(std::string("the scales of ") + what + " must be a float32 tensor of 2 dimensions on cuda:" + std::to_string(c.device));
+    if (scales.size(1) != blocks_of(k) || (scales.size(0) != rows && scales.size(0) != blocks_of(rows)))
+        refuse(std::string("the scales of ") + what + " must be [" + std::to_string(rows) + "][" + std::to_string(blocks_of(k)) + "] or [" +
+               std::to_string(blocks_of(rows)) + "][" + std::to_string(blocks_of(k)) + "]");
+    o.scales = address<float>(scales);
+    o.scale_row = scales.stride(0);
+    o.scale_block = scales.stride(1);
+    o.scale_rows = scales.size(0) == rows ? 1 : 128;
+    return o;
+}
+
+Tensor fp8_matmul(int64_t context, int device, const Tensor &a, const Tensor &a_scale, const Tensor &b, const Tensor &b_scale, int dtype, const Maybe &out)
+{
+    const Call c = call_of(context, device);
+    const lb_fp8_operand x = operand(c, a, a_scale, "a"), y = operand(c, b, b_scale, "b");
+    const int64_t m = a.size(0), n = b.size(0), k = a.size(1);
+    if (b.size(1) != k) refuse("a and b must have rows of the same length");
+    const Tensor to = result(c, out, m, n, dtype);
+    const size_t need = lb_fp8_matmul_workspace_bytes(m, n, k, &x, &y);
+    const Tensor ws = c.workspace(need);
+    check(lb_fp8_matmul(c.context, m, n, k, &x, &y, address<void>(to), value_type(to.scalar_type()), row_stride(to), address<void>(ws), need, c.stream()));
+    return to;
+}
+
+// ---- clipping -------------------------------------------------------------------------------------------------------------------
+Tensor clip_updates(int64_t context, int device, const py::object &updates, std::optional<double> max_norm, const Maybe &out)
+{
+    const Call c = call_of(context, device);
+    std::vector<int> clients, dtypes, out_dtypes;
+    std::vector<const void *> tensors;
+    std::vector<void *> outs;
+    std::vector<int64_t> sizes;
+    std::vector<Tensor> held;
+    const bool in_place = max_norm && !out;
+    int n = 0;
+    auto add = [&](const Tensor &t, int64_t size, int64_t offset) {
+        clients.push_back(n);
+        dtypes.push_back(value_type(t.scalar_type()));
+        tensors.push_back(size ? static_cast<char *>(t.data_ptr()) + offset * t.element_size() : nullptr);
+        sizes.push_back(size);
+    };
+    if (THPVariable_Check(updates.ptr())) { // [clients][values]
+        const Tensor t = THPVariable_Unpack(updates.ptr());
+        c.tensor(t, 2, "updates");
+        if (!value_type(t.scalar_type())) refuse("updates must be float32, bfloat16 or float16");
+        if (t.size(0) > 1 && t.stride(0) < t.size(1)) refuse("the rows of updates overlap");
+        for (; n < t.size(0); ++n) add(t, t.size(1), n * t.stride(0));
+        held.push_back(t);
+    } else {
+        if (!py::isinstance<py::sequence>(updates)) refuse("updates must be a matrix, or for each client a list of tensors");
+        for (const py::handle client : py::reinterpret_borrow<py::sequence>(updates)) {
+            if (THPVariable_Check(client.ptr()) || !py::isinstance<py::sequence>(client)) refuse("updates must be a matrix, or for each client a list of tensors");
+            for (const py::handle item : py::reinterpret_borrow<py::sequence>(client)) {
+                if (!THPVariable_Check(item.ptr())) refuse("updates must be a matrix, or for each client a list of tensors");
+                const Tensor t = THPVariable_Unpack(item.ptr());
+                if (!t.is_cuda() || t.get_device() != c.device || t.layout() != at::kStrided) refuse("an update's tensors must be on cuda:" + std::to_string(device));
+                if (!value_type(t.scalar_type())) refuse("an update's tensors must be float32, bfloat16 or float16");
+                // the order of the values is the result's where they are copied
+                if (out ? !t.is_contiguous() : !t.is_non_overlapping_and_dense()) refuse(out ? "an update's tensors must be contiguous" : "an update's tensors must be dense");
+                add(t, t.numel(), 0);
+                held.push_back(t);
+            }
+            ++n;
+        }
+    }
+    if (max_norm && !(*max_norm >= 0.0)) refuse("max_norm is a number that is not negative");
+    if (out) {
+        c.tensor(*out, 2, "out");
+        const int type = value_type(out->scalar_type());
+        if (!type) refuse("out must be float32, bfloat16 or float16");
+        if (out->size(0) != n) refuse("out must have a row for each of the " + std::to_string(n) + " client(s)");
+        if (n > 1 && out->stride(0) < out->size(1)) refuse("the rows of out overlap");
+        int64_t at = 0;
+        for (size_t i = 0; i <= sizes.size(); ++i) {
+            const bool next = i == sizes.size() || (i > 0 && clients[i] != clients[i - 1]);
+            if (next && i > 0 && at != out->size(1)) refuse("an update does not have the " + std::to_string(out->size(1)) + " values of a row of out");
+            if (i == sizes.size()) break;
+            if (next || i == 0) at = 0;
+            outs.push_back(sizes[i] ? static_cast<char *>(out->data_ptr()) + (clients[i] * (n > 1 ? out->stride(0) : 0) + at) * out->element_size() : nullptr);
+            at += sizes[i];
+        }
+        std::vector<bool> some(n);
+        for (const int k : clients) some[k] = true;
+        for (int k = 0; k < n; ++k)
+            if (!some[k] && out->size(1)) refuse("an update does not have the " + std::to_string(out->size(1)) + " values of a row of out");
+        out_dtypes.assign(sizes.size(), type);
+    } else if (in_place) {
+        for (const void *p : tensors) outs.push_back(const_cast<void *>(p));
+        out_dtypes = dtypes;
+        for (const Tensor &t : held)
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    const Tensor norms = c.empty({n}, at::kDouble);
+    const int count = (int)sizes.size();
+    const size_t need = n ? lb_clip_updates_workspace_bytes(c.context, n, count, clients.data(), sizes.data()) : 0;
+    const Tensor ws = c.workspace(need);
+    check(lb_clip_updates(c.context, n, count, clients.data(), tensors.data(), dtypes.data(), sizes.data(), max_norm ? *max_norm : HUGE_VAL,
+                          out || in_place ? outs.data() : nullptr, out_dtypes.data(), address<double>(norms), address<void>(ws), need, c.stream()));
+    return norms;
+}
+
 } // namespace
 
 PYBIND11_MODULE(_updates8, m)
@@ -200,4 +377,8 @@ PYBIND11_MODULE(_updates8, m)
     m.def("dequantize_rows", &dequantize_rows);
     m.def("int8_matmul", &int8_matmul);
     m.def("int8_distances", &int8_distances);
+    m.def("quantize_fp8", &quantize_fp8);
+    m.def("dequantize_fp8", &dequantize_fp8);
+    m.def("fp8_matmul", &fp8_matmul);
+    m.def("clip_updates", &clip_updates);
 }

@@ -1,13 +1,16 @@
-"""Clients' updates held as 8-bit integers with scales.
+"""Clients' updates: held as 8-bit integers with scales, formed in 8 bits, bounded.
 
 ``UpdateCache`` takes the place of the ``[n_clients][dim]`` tensor of updates in ``EncryptedKrum.round``, ``EncryptedKrum.encrypt_slices``
 and ``plaintext_krum``: a quarter of the memory (20 clients of 11 M values: 0.22 GB instead of 0.9), written as updates arrive, with the
-error feedback of 8-bit uploads, and read back a range of pages at a time.  ``low_rank_update`` forms an update from 8-bit factors.
-The reference keeps every update as a list of doubles (lancelot-main-GPU/utils/byzantine_fl.py:478-490) and has neither.
+error feedback of 8-bit uploads, and read back a range of pages at a time.  ``low_rank_update`` forms an update from 8-bit factors,
+``fp8_linear`` trains a client's layer with products in 8-bit floating point, ``flat_updates`` bounds what came of it and lays it out as rows.
+The reference keeps every update as a list of doubles (lancelot-main-GPU/utils/byzantine_fl.py:478-490) and has none of these.
 """
 import operator
 
 import torch
+
+from .cabi import FP8_TYPES
 
 
 class UpdateCache:
@@ -88,9 +91,10 @@ def quantize_matrix(lb, x):
 
 
 def low_rank_update(lb, factors, out=None):
-    """The flat float32 update of matrices given by 8-bit factors.  factors: for every matrix W = B A^T a tuple (b [rows][rank] int8, b_scale [rows],
-    a [cols][rank] int8, a_scale [cols]), see ``quantize_matrix``; the matrices follow one another row by row.  Clients' factors cannot be
-    averaged for the update (the mean of products is not the product of means), so the product is formed before the encryption."""
+    """The flat float32 update of matrices given by 8-bit factors.  factors: for every matrix W = B A^T a tuple (b [rows][rank], b_scale, a [cols][rank],
+    a_scale), either int8 with a scale per row (``quantize_matrix``) or 8-bit floats with scales for blocks of 128
+    (``cabi.Context.quantize_fp8``); the matrices follow one another row by row.  Clients' factors cannot be averaged for the update (the
+    mean of products is not the product of means), so the product is formed before the encryption."""
     sizes = [b.shape[0] * a.shape[0] for b, _, a, _ in factors]
     if out is None:
         out = torch.empty(sum(sizes), device="cuda:%d" % lb.device)
@@ -98,6 +102,74 @@ def low_rank_update(lb, factors, out=None):
         raise ValueError("out must be a contiguous float32 vector of %d values" % sum(sizes))
     at = 0
     for (b, b_scale, a, a_scale), size in zip(factors, sizes):
-        lb.int8_matmul(b, a, b_scale, a_scale, out=out[at:at + size].view(b.shape[0], a.shape[0]))
+        to = out[at:at + size].view(b.shape[0], a.shape[0])
+        if b.dtype in FP8_TYPES:
+            lb.fp8_matmul(b, b_scale, a, a_scale, out=to)
+        else:
+            lb.int8_matmul(b, a, b_scale, a_scale, out=to)
         at += size
     return out
+
+
+def _matrix(t):
+    """t [..., k] as a matrix whose rows are dense and apart: not so are transposed ones, and the gradient of a sum, one value for all"""
+    rows = t.reshape(t.shape[:-1].numel(), t.shape[-1])
+    return rows if rows.stride(1) == 1 and (rows.shape[0] < 2 or rows.stride(0) >= rows.shape[1]) else rows.contiguous()
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lb, x, w, grad_dtype):
+        need_x, need_w = ctx.needs_input_grad[1:3]
+        rows = _matrix(x)
+        if need_w:
+            x8, xs, xd, xds = lb.quantize_fp8_both(rows)
+        else:
+            (x8, xs), xd, xds = lb.quantize_fp8(rows), None, None
+        w8, ws = lb.quantize_fp8(_matrix(w), (128, 128))
+        ctx.lb, ctx.grad_dtype, ctx.dtypes = lb, grad_dtype, (x.dtype, w.dtype)
+        ctx.save_for_backward(xd, xds, *((w8, ws) if need_x else (None, None)))
+        return lb.fp8_matmul(x8, xs, w8, ws, dtype=x.dtype).view(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        lb = ctx.lb
+        xd, xds, w8, ws = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[1:3]
+        rows = _matrix(g)
+        dx = dw = None
+        if need_x and need_w:
+            g8, gs, gd, gds = lb.quantize_fp8_both(rows, dtype=ctx.grad_dtype)
+        elif need_x:
+            g8, gs = lb.quantize_fp8(rows, dtype=ctx.grad_dtype)
+        else:
+            gd, gds = lb.quantize_fp8(rows, (128, 1), dtype=ctx.grad_dtype)
+        if need_x:
+            dx = lb.fp8_matmul(g8, gs, w8.t(), ws.t(), dtype=ctx.dtypes[0]).view(*g.shape[:-1], w8.shape[1])
+        if need_w:
+            dw = lb.fp8_matmul(gd.t(), gds.t(), xd.t(), xds.t(), dtype=ctx.dtypes[1])
+        return None, dx, dw, None
+
+
+def fp8_linear(lb, x, w, grad_dtype=torch.float8_e4m3fn):
+    """y = x w^T with gradients, x [..., k], w [n][k] (float32, bfloat16, float16, on the device of lb): the three products of a training step in
+    8-bit floating point.  x is quantised in blocks of 128 values along what a product sums over, w in blocks of 128 x 128; the gradient of y as x,
+    to grad_dtype.  y and the gradients have the types of x and of their tensors.  What is kept for the backward pass are the codes"""
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ValueError("x must be [..., k] and w [n][k]")
+    if grad_dtype not in FP8_TYPES:
+        raise ValueError("grad_dtype must be float8_e4m3fn or float8_e5m2")
+    return _Fp8Linear.apply(lb, x, w, grad_dtype)
+
+
+def flat_updates(lb, updates, max_norm=None, out=None, dtype=torch.float32):
+    """Clients' updates, for each a list of tensors (the parameters' differences or gradients of its model), as the matrix [n_clients][dim] that
+    ``EncryptedKrum.round``, ``plaintext_krum`` and ``UpdateCache.write`` take, scaled down to max_norm where their norm over all tensors is larger
+    -> (matrix, norms [n_clients] float64)"""
+    if out is None:
+        dims = {sum(t.numel() for t in tensors) for tensors in updates}
+        if len(dims) > 1:
+            raise ValueError("the updates have different numbers of values")
+        out = torch.empty(len(updates), dims.pop() if dims else 0, dtype=dtype, device="cuda:%d" % lb.device)
+    return out, lb.clip_updates(updates, max_norm, out=out)
