@@ -970,56 +970,34 @@ int lb_fp8_matmul(lb_context *h, int64_t m, int64_t n, int64_t k, const lb_fp8_o
     return fp8_matmul(C(h), (int)m, (int)n, (int)k, operand_of(a), operand_of(b), out, dtype, out_stride, workspace, S(stream));
 }
 
-// The pieces of a call: as many of each tensor as its elements take, one (of no elements) for a client that has none
-static int64_t clip_parts(const Context *c, int n_clients, int n_tensors, const int *clients, const int64_t *sizes, int &piece, std::vector<ClipPart> *parts)
+// The tensors of a call that hold values, and for a client that has none one of no values
+static std::vector<ClipPart> clip_parts(int n_clients, int n_tensors, const int *clients, const int *dtypes, const int64_t *sizes, const int *out_dtypes)
 {
-    double all = 0.0;
-    for (int i = 0; i < n_tensors; ++i) all += (double)sizes[i];
-    piece = clip_piece(c, all);
-    int64_t at = 0;
+    std::vector<ClipPart> parts;
+    parts.reserve((size_t)n_tensors + n_clients);
+    auto type = [&](const int *types, int i) { return types && n_tensors ? types[i] : 1; };
     int i = 0;
     for (int k = 0; k < n_clients; ++k) {
-        const int64_t begin = at;
-        const size_t first = parts ? parts->size() : 0;
-        for (; i < n_tensors && clients[i] == k; ++i) {
-            if (sizes[i] == 0) continue;
-            if (parts) {
-                ClipPart p = {};
-                p.n = sizes[i];
-                p.first = (int)at;
-                p.client = k;
-                p.in_type = i; // the tensor, for the caller to fill in
-                parts->push_back(p);
-            }
-            at += (sizes[i] + piece - 1) / piece;
-        }
-        if (at == begin) {
-            if (parts) {
-                ClipPart p = {};
-                p.first = (int)at;
-                p.client = k;
-                p.in_type = -1;
-                parts->push_back(p);
-            }
-            ++at;
-        }
-        if (parts)
-            for (size_t j = first; j < parts->size(); ++j) (*parts)[j].begin = (int)begin, (*parts)[j].end = (int)at;
+        const size_t begin = parts.size();
+        for (; i < n_tensors && clients[i] == k; ++i)
+            if (sizes[i]) parts.push_back({nullptr, nullptr, (long)sizes[i], k, type(dtypes, i), type(out_dtypes, i), i});
+        if (parts.size() == begin) parts.push_back({nullptr, nullptr, 0, k, type(dtypes, 0), type(out_dtypes, 0), -1});
     }
-    return at;
+    return parts;
 }
 
-static int clip_ok(int n_clients, int n_tensors, const int *clients, const int64_t *sizes)
+static int clip_ok(int n_clients, int n_tensors, const int *clients, const int *dtypes, const int64_t *sizes, const int *out_dtypes)
 {
     REQUIRE(n_clients >= 0 && n_clients < 1 << 23 && n_tensors >= 0, "n_clients or n_tensors is out of range");
-    REQUIRE(n_tensors == 0 || (clients && sizes), "operand is null");
+    REQUIRE(n_tensors == 0 || (clients && dtypes && sizes), "operand is null");
     double all = 0.0;
     for (int i = 0; i < n_tensors; ++i) {
         REQUIRE(clients[i] >= (i ? clients[i - 1] : 0) && clients[i] < n_clients, "the tensors are in the order of their clients");
         REQUIRE(sizes[i] >= 0 && sizes[i] <= (int64_t)1 << 40, "a tensor's size is out of range");
-        all += (double)sizes[i] / 1024 + 1;
+        REQUIRE(value_size(dtypes[i]) && (!out_dtypes || value_size(out_dtypes[i])), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
+        all += (double)sizes[i];
     }
-    REQUIRE(all + n_clients < (double)(1 << 30), "too many values for one call");
+    REQUIRE(all <= (double)((int64_t)1 << 40), "too many values for one call");
     return LB_OK;
 }
 
@@ -1062,11 +1040,14 @@ static int clip_apart(const std::vector<ClipPart> &parts)
     return LB_OK;
 }
 
-size_t lb_clip_updates_workspace_bytes(const lb_context *h, int n_clients, int n_tensors, const int *clients, const int64_t *sizes)
-{
-    if (!h || !h->c || n_clients < 1 || clip_ok(n_clients, n_tensors, clients, sizes)) return 0;
-    int piece = 0;
-    return (size_t)clip_parts(h->c, n_clients, n_tensors, clients, sizes, piece, nullptr) * 8;
+size_t lb_clip_updates_workspace_bytes(const lb_context *h, int n_clients, int n_tensors, const int *clients, const int *dtypes, const int64_t *sizes,
+                                       const int *out_dtypes)
+try {
+    if (!h || !h->c || n_clients < 1 || clip_ok(n_clients, n_tensors, clients, dtypes, sizes, out_dtypes)) return 0;
+    const std::vector<ClipPart> parts = clip_parts(n_clients, n_tensors, clients, dtypes, sizes, out_dtypes);
+    return clip_workspace_bytes(h->c, parts.data(), (int)parts.size(), out_dtypes != nullptr);
+} catch (const std::bad_alloc &) {
+    return 0;
 }
 
 int lb_clip_updates(lb_context *h, int n_clients, int n_tensors, const int *clients, const void *const *tensors, const int *dtypes,
@@ -1075,32 +1056,27 @@ int lb_clip_updates(lb_context *h, int n_clients, int n_tensors, const int *clie
 try {
     int rc = bind(h);
     if (rc) return rc;
-    if ((rc = clip_ok(n_clients, n_tensors, clients, sizes))) return rc;
+    if (!outs) out_dtypes = nullptr;
+    if ((rc = clip_ok(n_clients, n_tensors, clients, dtypes, sizes, out_dtypes))) return rc;
     REQUIRE(max_norm >= 0.0, "max_norm is a number that is not negative");
     if (n_clients == 0) return LB_OK;
-    REQUIRE(norms && (n_tensors == 0 || (tensors && dtypes)) && (!outs || out_dtypes), "operand is null");
+    REQUIRE(norms && (n_tensors == 0 || (tensors && (!outs || out_dtypes))), "operand is null");
     REQUIRE((uintptr_t)norms % 8 == 0, "an operand is not aligned to its type");
-    std::vector<ClipPart> parts;
-    int piece = 0;
-    const int64_t pieces = clip_parts(C(h), n_clients, n_tensors, clients, sizes, piece, &parts);
+    std::vector<ClipPart> parts = clip_parts(n_clients, n_tensors, clients, dtypes, sizes, out_dtypes);
+    const size_t need = clip_workspace_bytes(C(h), parts.data(), (int)parts.size(), outs != nullptr);
     for (ClipPart &p : parts) {
-        const int i = p.in_type;
-        p.in_type = p.out_type = 1;
+        const int i = p.index;
         if (i < 0) continue;
-        REQUIRE(value_size(dtypes[i]), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
-        REQUIRE(tensors[i] && (uintptr_t)tensors[i] % value_size(dtypes[i]) == 0, "a tensor is null or not aligned to its type");
+        REQUIRE(tensors[i] && (uintptr_t)tensors[i] % value_size(p.in_type) == 0, "a tensor is null or not aligned to its type");
         p.in = tensors[i];
-        p.in_type = dtypes[i];
         if (!outs) continue;
-        REQUIRE(value_size(out_dtypes[i]), "dtype is 1 (float), 3 (bfloat16) or 4 (half)");
-        REQUIRE(outs[i] && (uintptr_t)outs[i] % value_size(out_dtypes[i]) == 0, "a result is null or not aligned to its type");
-        REQUIRE(outs[i] != tensors[i] || out_dtypes[i] == dtypes[i], "a result in place has the type of its tensor");
+        REQUIRE(outs[i] && (uintptr_t)outs[i] % value_size(p.out_type) == 0, "a result is null or not aligned to its type");
+        REQUIRE(outs[i] != tensors[i] || p.in_type == p.out_type, "a result in place has the type of its tensor");
         p.out = outs[i];
-        p.out_type = out_dtypes[i];
     }
     if ((rc = clip_apart(parts))) return rc;
-    if ((rc = workspace_ok(workspace, workspace_bytes, (size_t)pieces * 8))) return rc;
-    return clip_updates(C(h), parts.data(), (int)parts.size(), piece, max_norm, reinterpret_cast<double *>(workspace), norms, S(stream));
+    if ((rc = workspace_ok(workspace, workspace_bytes, need))) return rc;
+    return clip_updates(C(h), parts.data(), (int)parts.size(), outs != nullptr, max_norm, reinterpret_cast<double *>(workspace), norms, S(stream));
 } catch (const std::bad_alloc &) {
     set_error("out of host memory");
     return LB_ERR_NO_MEMORY;

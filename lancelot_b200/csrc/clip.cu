@@ -6,13 +6,18 @@
 // (lancelot-main-GPU/utils/byzantine_fl.py:162-171,527-536); the reference has none.
 //
 // Squares of 32-bit floats are exact in 64 bits, and so are summed there: no sum passes the range, and small entries are not lost behind
-// large ones.  The tensors are cut into pieces; a piece's sum goes to its own place, and every block that needs a client's norm adds
-// its pieces up in the same order, so that results do not depend on which block was first.
-#include <cooperative_groups.h>
+// large ones.  The tensors are cut into pieces, dealt out to the blocks; a block's sum for a client goes to its own slot, and every block that needs a
+// client's norm adds its slots up in the same order, so that results do not depend on which block was first.
+//
+// Two kernels, for some clients at a time (a round): the values are read for their sums, and read again, out of L2, the last ones first, and
+// written.  The sums of a round start while the results of the one before are still being written (programmatic launches).
+// Bound by HBM: TIMES
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <atomic>
+#include <algorithm>
+#include <type_traits>
+#include <vector>
 
 #include "product.cuh"
 
@@ -21,24 +26,26 @@ namespace lb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMostTensors = 800; // of one launch: they travel as its argument
+constexpr int kMostTensors = 640;    // of one launch: they travel as its argument
+constexpr double kRoundBytes = 48e6; // of values: what stays in L2 until they are read again, beside the results
 
 struct Part {
     const void *in;
     void *out; // NULL: nothing is written
     long n;
-    int first;      // of the call's pieces
-    int begin, end; // the client's pieces
-    int client : 24, in_type : 4, out_type : 4;
+    int first;            // of the launch's pieces
+    int slot;             // of that piece's sum
+    int slots, slots_end; // of all sums of the client
+    int client, begins;   // begins: whether it is the client's first tensor
 };
 template <int MOST> struct ClipArgs {
     Part tensor[MOST];
-    int n_tensors, n_pieces; // of this launch
-    int piece;               // elements of a piece, a multiple of 64
-    bool sums, writes;       // whether this launch forms the pieces' sums, and whether it goes on to norms and results
+    int n_tensors, piece; // piece: elements of a piece
     double most;
     double *partial, *norms;
 };
+
+static_assert(sizeof(ClipArgs<kMostTensors>) <= 31 * 1024, "arguments and what the driver puts before them share 32 KB");
 
 template <typename T> struct Pack; // values in 16 bytes
 template <> struct Pack<float> {
@@ -88,7 +95,7 @@ __device__ __forceinline__ double block_sum(double v, double *shared)
 }
 
 // the tensor that holds a piece
-template <int MOST> __device__ __forceinline__ int tensor_of(const ClipArgs<MOST> &a, int piece)
+template <int MOST> __device__ __forceinline__ const Part &tensor_of(const ClipArgs<MOST> &a, int piece)
 {
     int lo = 0, hi = a.n_tensors - 1;
     while (lo < hi) {
@@ -96,166 +103,386 @@ template <int MOST> __device__ __forceinline__ int tensor_of(const ClipArgs<MOST
         if (a.tensor[mid].first <= piece) lo = mid;
         else hi = mid - 1;
     }
-    return lo;
+    return a.tensor[lo];
+}
+
+// The sum of squares of values from 16 bytes.  16-bit types: conversions to 64 bits come slowly (16 a cycle), so a value that is part of 20 bits is
+// moved to its place in a double's upper half by hand; that is not right for zeros and for what is below 2^-126 (they come out as 2^-126 at
+// most), which does not matter beside a value from 2^-60 on, nor for what is not finite.
+__device__ __forceinline__ double add_squares(double sum, const float (&v)[4])
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = fma((double)v[e], (double)v[e], sum);
+    return sum;
+}
+__device__ __forceinline__ double add_squares(double sum, const float (&v)[8])
+{
+    unsigned u[8], most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        u[e] = __float_as_uint(v[e]) & 0x7fffffffu;
+        most = max(most, u[e]);
+    }
+    if (most - 0x21800000u < 0x7f800000u - 0x21800000u) { // 2^-60 and infinity
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double d = __hiloint2double((int)((u[e] >> 3) + 0x38000000u), 0);
+            sum = fma(d, d, sum);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fma((double)v[e], (double)v[e], sum);
+    }
+    return sum;
 }
 
 template <typename T> __device__ __forceinline__ double squares(const T *p, int n)
 {
     constexpr int N = Pack<T>::kN;
     double sum = 0.0;
-    int done = 0;
-    if ((uintptr_t)p % 16 == 0) {
-        done = n / N * N;
-#pragma unroll 4
-        for (int i = threadIdx.x * N; i < done; i += kThreads * N) {
-            float v[N];
-            Pack<T>::open(__ldg(reinterpret_cast<const uint4 *>(p + i)), v);
+    const int head = min((int)((16 - (unsigned)(uintptr_t)p % 16) % 16 / sizeof(T)), n), body = (n - head) / N * N;
+    const T *q = p + head;
+    for (int i = threadIdx.x * N; i < body; i += 4 * kThreads * N) {
+        uint4 w[4];
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum = fma((double)v[e], (double)v[e], sum);
+        for (int j = 0; j < 4; ++j) w[j] = i + j * kThreads * N < body ? __ldg(reinterpret_cast<const uint4 *>(q + i + j * kThreads * N)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float v[N];
+            Pack<T>::open(w[j], v);
+            sum = add_squares(sum, v);
         }
     }
-#pragma unroll 4
-    for (int i = done + threadIdx.x; i < n; i += kThreads) {
-        const double v = Pack<T>::one(p[i]);
+    for (int i = threadIdx.x; i < n - body; i += kThreads) { // what lies before the first boundary and behind the last one
+        const double v = Pack<T>::one(p[i < head ? i : i + body]);
         sum = fma(v, v, sum);
     }
     return sum;
 }
-
-template <typename T, typename O> __device__ __forceinline__ void scaled(const T *p, O *out, int n, float f)
-{
-    constexpr int N = Pack<T>::kN;
-    int done = 0;
-    if ((uintptr_t)p % 16 == 0 && (uintptr_t)out % 16 == 0) {
-        done = n / N * N;
-#pragma unroll 4
-        for (int i = threadIdx.x * N; i < done; i += kThreads * N) {
-            float v[N];
-            Pack<T>::open(__ldcs(reinterpret_cast<const uint4 *>(p + i)), v);
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[e] *= f;
-            if constexpr (sizeof(O) == 4) {
-#pragma unroll
-                for (int e = 0; e < N; e += 4) __stcs(reinterpret_cast<float4 *>(out + i + e), make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
-            } else if constexpr (N == 8) {
-                __stcs(reinterpret_cast<uint4 *>(out + i), make_uint4(pack2(out, v[0], v[1]), pack2(out, v[2], v[3]), pack2(out, v[4], v[5]), pack2(out, v[6], v[7])));
-            } else {
-                __stcs(reinterpret_cast<uint2 *>(out + i), make_uint2(pack2(out, v[0], v[1]), pack2(out, v[2], v[3])));
-            }
+// N values from `off` elements on behind a boundary of kAlign elements, out of the aligned pieces that they lie in: the pieces, and the values
+template <typename T, int N> struct Raw { // 16-bit types
+    static constexpr int kAlign = N, kSteps = N == 8 ? 3 : 4; // kSteps: of a thread, whose loads are on their way together
+    unsigned w[N];
+    __device__ __forceinline__ void part(const T *q, int at)
+    {
+        if constexpr (N == 8) {
+            const uint4 x = __ldcs(reinterpret_cast<const uint4 *>(q));
+            w[at] = x.x, w[at + 1] = x.y, w[at + 2] = x.z, w[at + 3] = x.w;
+        } else {
+            const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(q));
+            w[at] = x.x, w[at + 1] = x.y;
         }
     }
-#pragma unroll 8
-    for (int i = done + threadIdx.x; i < n; i += kThreads) put(out + i, Pack<T>::one(p[i]) * f);
+    __device__ __forceinline__ void load(const T *q, int off)
+    {
+        part(q, 0);
+        if (off) part(q + N, N / 2);
+    }
+    __device__ __forceinline__ void open(int off, float (&v)[N])
+    {
+        if (off) {
+            if constexpr (N == 8) {
+#pragma unroll
+                for (int e = 0; e < 6; ++e) w[e] = off & 4 ? w[e + 2] : w[e];
+            }
+#pragma unroll
+            for (int e = 0; e <= N / 2; ++e)
+                if (e + 1 < N) w[e] = off & 2 ? w[e + 1] : w[e];
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) w[e] = __funnelshift_r(w[e], w[e + 1], off & 1 ? 16 : 0);
+        }
+        float u[8];
+        Pack<T>::open(make_uint4(w[0], w[1], N == 8 ? w[N - 6] : 0, N == 8 ? w[N - 5] : 0), u);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = u[e];
+    }
+};
+template <int N> struct Raw<float, N> {
+    static constexpr int kAlign = 4, kSteps = N == 4 ? 4 : 2;
+    uint4 r[N / 4 + 1];
+    __device__ __forceinline__ void load(const float *q, int off)
+    {
+#pragma unroll
+        for (int j = 0; j < N / 4; ++j) r[j] = __ldcs(reinterpret_cast<const uint4 *>(q) + j);
+        if (off) r[N / 4] = __ldcs(reinterpret_cast<const uint4 *>(q) + N / 4);
+    }
+    __device__ __forceinline__ void open(int off, float (&v)[N])
+    {
+        float w[N + 4];
+#pragma unroll
+        for (int j = 0; j <= N / 4; ++j) Pack<float>::open(r[j], w + 4 * j);
+        if (off) {
+#pragma unroll
+            for (int e = 0; e < N + 2; ++e) w[e] = off & 2 ? w[e + 2] : w[e];
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = off & 1 ? w[e + 1] : w[e];
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = w[e];
+    }
+};
+__device__ __forceinline__ void store(float *p, const float (&v)[4]) { __stcs(reinterpret_cast<float4 *>(p), make_float4(v[0], v[1], v[2], v[3])); }
+template <typename O> __device__ __forceinline__ void store(O *p, const float (&v)[8])
+{
+    __stcs(reinterpret_cast<uint4 *>(p), make_uint4(pack2(p, v[0], v[1]), pack2(p, v[2], v[3]), pack2(p, v[4], v[5]), pack2(p, v[6], v[7])));
 }
 
-__device__ __forceinline__ double squares(const void *in, int type, long at, int n)
-{
-    return type == 1 ? squares(reinterpret_cast<const float *>(in) + at, n)
-         : type == 3 ? squares(reinterpret_cast<const __nv_bfloat16 *>(in) + at, n)
-                     : squares(reinterpret_cast<const __half *>(in) + at, n);
-}
-template <typename T> __device__ __forceinline__ void scaled(const T *in, void *out, int type, long at, int n, float f)
-{
-    if (type == 1) scaled(in, reinterpret_cast<float *>(out) + at, n, f);
-    else if (type == 3) scaled(in, reinterpret_cast<__nv_bfloat16 *>(out) + at, n, f);
-    else scaled(in, reinterpret_cast<__half *>(out) + at, n, f);
-}
+// out = p * f, 16 bytes of results a thread and step.  A tensor seldom starts at the same place between two 16-byte boundaries as its run of the
+// flat row: the results of a step are put together from the two or three aligned pieces that their values lie in.
+template <typename T, typename O> struct Scaling {
+    using R = Raw<T, 16 / sizeof(O)>;
+    static constexpr int N = 16 / sizeof(O), A = R::kAlign, kStep = kThreads * N, kBatch = R::kSteps * kStep;
+    const T *p;
+    O *out;
+    int n, off, first, from, body;
+    R r[R::kSteps];
 
-template <int MOST> __global__ void __launch_bounds__(kThreads, 4) clip_kernel(const __grid_constant__ ClipArgs<MOST> a)
+    __device__ __forceinline__ Scaling(const T *p_, O *out_, int n_) : p(p_), out(out_), n(n_)
+    {
+        const int head = min((int)((16 - (unsigned)(uintptr_t)out % 16) % 16 / sizeof(O)), n);
+        off = (int)((unsigned)((uintptr_t)(p + head) / sizeof(T)) % A); // of the values of the first step
+        first = off <= head ? head : head + N;                          // pieces that begin before p are not read
+        int steps = max((n - first) / N, 0);
+        if (off && steps > 0 && first + N * steps - off + A > n) --steps; // nor those that end behind its end
+        body = steps * N;
+        from = min(first, n);
+    }
+    __device__ __forceinline__ void load(int i) // all loads of a batch before its first store: none may pass one that might lie in its way
+    {
+#pragma unroll
+        for (int j = 0; j < R::kSteps; ++j)
+            if (i + j * kStep < body) r[j].load(p + first - off + i + j * kStep, off);
+    }
+    __device__ __forceinline__ void finish(int i, float f) // with the batch from i on loaded
+    {
+        while (true) {
+#pragma unroll
+            for (int j = 0; j < R::kSteps; ++j)
+                if (i + j * kStep < body) {
+                    float v[N];
+                    r[j].open(off, v);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[e] *= f;
+                    store(out + first + i + j * kStep, v);
+                }
+            i += kBatch;
+            if (i >= body) break;
+            load(i);
+        }
+        for (int k = threadIdx.x; k < n - body; k += kThreads) {
+            const int j = k < from ? k : k + body;
+            put(out + j, Pack<T>::one(p[j]) * f);
+        }
+    }
+};
+
+// what the kernel before this one wrote is there
+__device__ __forceinline__ void predecessor_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// the next kernel's blocks may come as soon as there is room
+__device__ __forceinline__ void successor_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename T, int MOST> __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ ClipArgs<MOST> a)
 {
     __shared__ double shared[kThreads / 32];
-    const int piece0 = a.tensor[0].first;
-    if (a.sums)
-        for (int i = piece0 + blockIdx.x; i < piece0 + a.n_pieces; i += gridDim.x) {
-            const Part &t = a.tensor[tensor_of(a, i)];
-            const long at = (long)(i - t.first) * a.piece;
-            const double sum = block_sum(squares(t.in, t.in_type, at, (int)min((long)a.piece, t.n - at)), shared);
-            if (threadIdx.x == 0) a.partial[i] = sum;
-        }
-    if (!a.writes) return;
-    if (a.sums) cooperative_groups::this_grid().sync();
-    int client = -1;
-    float f = 1.0f;
-    for (int i = piece0 + blockIdx.x; i < piece0 + a.n_pieces; i += gridDim.x) {
-        const Part &t = a.tensor[tensor_of(a, i)];
-        if (t.client != client) {
-            client = t.client;
-            double sum = 0.0;
-            for (int j = t.begin + (int)threadIdx.x; j < t.end; j += kThreads) sum += __ldcg(a.partial + j);
-            const double norm = sqrt(block_sum(sum, shared));
-            f = !isfinite(norm) ? __int_as_float(0x7fc00000) : norm > a.most ? (float)(a.most / norm) : 1.0f;
-            if (i == t.begin && threadIdx.x == 0) a.norms[client] = norm;
-        }
-        if (!t.out || (f == 1.0f && t.out == t.in)) continue;
-        const long at = (long)(i - t.first) * a.piece;
-        const int n = (int)min((long)a.piece, t.n - at);
-        if (t.in_type == 1) scaled(reinterpret_cast<const float *>(t.in) + at, t.out, t.out_type, at, n, f);
-        else if (t.in_type == 3) scaled(reinterpret_cast<const __nv_bfloat16 *>(t.in) + at, t.out, t.out_type, at, n, f);
-        else scaled(reinterpret_cast<const __half *>(t.in) + at, t.out, t.out_type, at, n, f);
-    }
+    successor_may_start();
+    const int i = (int)blockIdx.x;
+    const Part &t = tensor_of(a, i);
+    const long e = (long)(i - t.first) * a.piece;
+    const double sum = block_sum(squares(reinterpret_cast<const T *>(t.in) + e, (int)min((long)a.piece, t.n - e)), shared);
+    if (threadIdx.x == 0) a.partial[t.slot + (i - t.first)] = sum;
+    predecessor_done(); // nothing of it is used: whoever waits for this kernel has then waited for that one too
 }
 
-template <int MOST> int launch_clip(const Context *ctx, const ClipPart *parts, int n_tensors, int n_pieces, int piece, bool sums, bool writes, double most,
-                                    double *partial, double *norms, cudaStream_t stream)
+__device__ __forceinline__ double norm_of(const double *partial, int from, int to, double *shared)
 {
-    static std::atomic<int> known{0};
-    int per_sm = known;
-    if (!per_sm) {
-        LB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, clip_kernel<MOST>, kThreads, 0));
-        known = per_sm;
+    double sum = 0.0;
+    for (int j = from + (int)threadIdx.x; j < to; j += kThreads) sum += __ldcg(partial + j);
+    return sqrt(block_sum(sum, shared));
+}
+
+template <typename T, typename O, int MOST> __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ ClipArgs<MOST> a)
+{
+    __shared__ double shared[kThreads / 32];
+    successor_may_start();
+    const int i = (int)(gridDim.x - 1 - blockIdx.x); // what was read last is read first
+    const Part &t = tensor_of(a, i);
+    const long e = (long)(i - t.first) * a.piece;
+    // values on their way while the norm is found: no kernel before this one that may still run writes them
+    Scaling<T, O> s(reinterpret_cast<const T *>(t.in) + e, t.out ? reinterpret_cast<O *>(t.out) + e : nullptr, (int)min((long)a.piece, t.n - e));
+    s.load(threadIdx.x * s.N);
+    predecessor_done();
+    const double norm = norm_of(a.partial, t.slots, t.slots_end, shared);
+    if (threadIdx.x == 0 && t.begins && i == t.first) a.norms[t.client] = norm;
+    const float f = !isfinite(norm) ? __int_as_float(0x7fc00000) : norm > a.most ? (float)(a.most / norm) : 1.0f;
+    if (!t.out || (f == 1.0f && t.out == t.in)) return;
+    s.finish(threadIdx.x * s.N, f);
+}
+
+// norms alone: a block for a client
+struct Client {
+    int client, slots, slots_end;
+};
+constexpr int kMostClients = 2000;
+struct NormArgs {
+    Client client[kMostClients];
+    const double *partial;
+    double *norms;
+};
+__global__ void __launch_bounds__(kThreads) norms_kernel(const __grid_constant__ NormArgs a)
+{
+    __shared__ double shared[kThreads / 32];
+    const Client c = a.client[blockIdx.x];
+    predecessor_done();
+    const double norm = norm_of(a.partial, c.slots, c.slots_end, shared);
+    if (threadIdx.x == 0) a.norms[c.client] = norm;
+}
+
+// A launch: tensors of the same types; whole clients where a client's tensors fit and are of the same types
+struct Launch {
+    int first, count; // of the tensors
+    int piece, pieces;
+    bool writes; // a launch of sums, or of results
+};
+
+double part_bytes(const ClipPart &p) { return (double)p.n * (p.in_type == 1 ? 4 : 2); }
+
+// The launches of a call, and (with `parts`) their tables; returns the number of sums
+long plan(const Context *ctx, const ClipPart *in, int n, bool writes, std::vector<Launch> &launches, std::vector<Part> *parts)
+{
+    long slots = 0;
+    auto pieces_of = [](long size, int piece) { return size ? (int)((size + piece - 1) / piece) : 1; };
+    auto add = [&](int i, int end) { // the sums of some tensors
+        double all = 0.0;
+        for (int j = i; j < end; ++j) all += (double)in[j].n;
+        // some eight pieces an SM, of 64 KB of 32-bit values at most: every block of the second kernel reads the sums of all pieces of its client
+        const double even = all / (8.0 * ctx->sm_count);
+        const int piece = even <= 1024 ? 1024 : even >= 16384 && all < 16384.0 * (1 << 20) ? 16384 : ((int)(even / 1024) + 1) * 1024;
+        Launch l = {i, end - i, piece, 0, false};
+        for (int j = i; j < end; ++j) {
+            const int pieces = pieces_of(in[j].n, piece);
+            if (parts) (*parts)[j] = {in[j].in, in[j].out, in[j].n, l.pieces, (int)slots, 0, (int)slots + pieces, in[j].client, j == 0 || in[j].client != in[j - 1].client};
+            l.pieces += pieces;
+            slots += pieces;
+        }
+        launches.push_back(l);
+    };
+    auto alike = [&](int i, int j) { return in[i].in_type == in[j].in_type && in[i].out_type == in[j].out_type; };
+    bool same = true;
+    for (int i = 1; i < n; ++i) same = same && alike(i - 1, i);
+    for (int i = 0; i < n;) {
+        // as many whole clients as one launch holds and L2 keeps; where there is none, because a client has more tensors or types differ, all tensors
+        int whole = i;
+        double bytes = 0.0;
+        for (int end = i; same && end < n && end - i < kMostTensors; ++end) {
+            bytes += part_bytes(in[end]);
+            if (end + 1 < n && in[end + 1].client == in[end].client) continue;
+            if (writes && whole > i && bytes > kRoundBytes) break;
+            whole = end + 1;
+        }
+        const size_t first = launches.size();
+        if (whole > i) {
+            add(i, whole);
+        } else {
+            whole = n;
+            for (int j = i, end; j < n; j = end) {
+                for (end = j; end < n && end - j < kMostTensors && alike(end, j);) ++end;
+                add(j, end);
+            }
+        }
+        if (writes)
+            for (size_t j = first, last = launches.size(); j < last; ++j) {
+                const Launch sums = launches[j];
+                launches.push_back(sums);
+                launches.back().writes = true;
+            }
+        i = whole;
     }
+    if (parts)
+        for (int i = 0; i < n;) { // a client's sums lie together, those of several launches too
+            int end = i;
+            while (end < n && in[end].client == in[i].client) ++end;
+            for (int j = i; j < end; ++j) (*parts)[j].slots = (*parts)[i].slot, (*parts)[j].slots_end = (*parts)[end - 1].slots_end;
+            i = end;
+        }
+    return slots;
+}
+
+// The first kernel of a call waits for what came before it; the others are set up, and those of sums begin, while their predecessor ends
+int start(const void *kernel, int grid, void *args, bool first, cudaStream_t stream)
+{
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)grid);
+    c.blockDim = dim3(kThreads);
+    c.stream = stream;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &early;
+    c.numAttrs = first ? 0 : 1;
+    void *list[] = {args};
+    LB_CUDA(cudaLaunchKernelExC(&c, kernel, list));
+    return LB_OK;
+}
+template <int MOST> int launch(const std::vector<Part> &parts, const Launch &l, const void *kernel, double most, double *partial, double *norms, bool first, cudaStream_t stream)
+{
     ClipArgs<MOST> a;
-    for (int i = 0; i < n_tensors; ++i) {
-        const ClipPart &p = parts[i];
-        Part &t = a.tensor[i];
-        t.in = p.in;
-        t.out = p.out;
-        t.n = p.n;
-        t.first = p.first;
-        t.begin = p.begin;
-        t.end = p.end;
-        t.client = p.client;
-        t.in_type = p.in_type;
-        t.out_type = p.out_type;
-    }
-    a.n_tensors = n_tensors;
-    a.n_pieces = n_pieces;
-    a.piece = piece;
-    a.sums = sums;
-    a.writes = writes;
+    std::copy(parts.begin() + l.first, parts.begin() + l.first + l.count, a.tensor);
+    a.n_tensors = l.count;
+    a.piece = l.piece;
     a.most = most;
     a.partial = partial;
     a.norms = norms;
-    const int blocks = per_sm * ctx->sm_count;
-    void *args[] = {&a};
-    LB_CUDA(cudaLaunchCooperativeKernel(reinterpret_cast<const void *>(clip_kernel<MOST>), dim3((unsigned)(n_pieces < blocks ? n_pieces : blocks)), dim3(kThreads), args, 0,
-                                        stream));
-    return LB_OK;
+    return start(kernel, l.pieces, &a, first, stream);
+}
+template <typename T, int MOST> const void *kernel_of(int out_type)
+{
+    return out_type == 0   ? reinterpret_cast<const void *>(norm_kernel<T, MOST>)
+           : out_type == 1 ? reinterpret_cast<const void *>(clip_kernel<T, float, MOST>)
+           : out_type == 3 ? reinterpret_cast<const void *>(clip_kernel<T, __nv_bfloat16, MOST>)
+                           : reinterpret_cast<const void *>(clip_kernel<T, __half, MOST>);
+}
+template <int MOST> const void *kernel_of(int in_type, int out_type)
+{
+    return in_type == 1 ? kernel_of<float, MOST>(out_type) : in_type == 3 ? kernel_of<__nv_bfloat16, MOST>(out_type) : kernel_of<__half, MOST>(out_type);
 }
 
 } // namespace
 
-int clip_piece(const Context *ctx, double elements)
+size_t clip_workspace_bytes(const Context *ctx, const ClipPart *parts, int n, bool writes)
 {
-    const double even = elements / (8.0 * ctx->sm_count);
-    return even <= 1024 ? 1024 : even >= 32768 ? 32768 : ((int)even + 63) / 64 * 64;
+    std::vector<Launch> launches;
+    return (size_t)plan(ctx, parts, n, writes, launches, nullptr) * 8;
 }
 
-int clip_updates(const Context *ctx, const ClipPart *parts, int n_parts, int piece, double most, double *partial, double *norms, cudaStream_t stream)
+int clip_updates(const Context *ctx, const ClipPart *in, int n, bool writes, double most, double *partial, double *norms, cudaStream_t stream)
 {
-    double bytes = 0.0;
-    for (int i = 0; i < n_parts; ++i) bytes += (double)parts[i].n * ((parts[i].in_type == 1 ? 4 : 2) + (!parts[i].out ? 0 : parts[i].out_type == 1 ? 4 : 2));
-    const bool one = n_parts <= kMostTensors;
-    for (int pass = one ? 1 : 0; pass < 2; ++pass) // more tensors than one launch holds: all sums first
-        for (int i = 0; i < n_parts; i += kMostTensors) {
-            const int n = n_parts - i < kMostTensors ? n_parts - i : kMostTensors;
-            const ClipPart &last = parts[i + n - 1];
-            const int pieces = last.first + (last.n > piece ? (int)((last.n + piece - 1) / piece) : 1) - parts[i].first;
-            count_launch("clip_updates", stream, i ? 0.0 : bytes);
-            const auto launch = n <= 16 ? launch_clip<16> : n <= 96 ? launch_clip<96> : launch_clip<kMostTensors>;
-            const int rc = launch(ctx, parts + i, n, pieces, piece, one || pass == 0, pass == 1, most, partial, norms, stream);
-            if (rc) return rc;
-        }
+    std::vector<Launch> launches;
+    std::vector<Part> parts(n);
+    plan(ctx, in, n, writes, launches, &parts);
+    int rc = LB_OK;
+    for (const Launch &l : launches) {
+        double bytes = 0.0;
+        for (int i = l.first; i < l.first + l.count; ++i) bytes += !l.writes ? part_bytes(in[i]) : in[i].out ? (double)in[i].n * (in[i].out_type == 1 ? 4 : 2) : 0.0;
+        count_launch(l.writes ? "clip_scale" : "clip_norm", stream, bytes);
+        const int in_type = in[l.first].in_type, out_type = l.writes ? in[l.first].out_type : 0;
+        const bool first = &l == launches.data();
+        if (l.count <= 16) rc = launch<16>(parts, l, kernel_of<16>(in_type, out_type), most, partial, norms, first, stream);
+        else if (l.count <= 96) rc = launch<96>(parts, l, kernel_of<96>(in_type, out_type), most, partial, norms, first, stream);
+        else rc = launch<kMostTensors>(parts, l, kernel_of<kMostTensors>(in_type, out_type), most, partial, norms, first, stream);
+        if (rc) return rc;
+    }
+    if (writes) return LB_OK;
+    NormArgs a;
+    a.partial = partial;
+    a.norms = norms;
+    int held = 0;
+    for (int i = 0; i < n; ++i) {
+        if (parts[i].begins) a.client[held++] = {parts[i].client, parts[i].slots, parts[i].slots_end};
+        if (held < kMostClients && (i + 1 < n || held == 0)) continue;
+        count_launch("clip_norms", stream, 0.0);
+        if ((rc = start(reinterpret_cast<const void *>(norms_kernel), held, &a, false, stream))) return rc;
+        held = 0;
+    }
     return LB_OK;
 }
 

@@ -240,14 +240,15 @@ int dequantize_fp8(const Context *ctx, const unsigned char *codes, int code_type
 size_t fp8_matmul_workspace_bytes(int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b);
 int fp8_matmul(Context *ctx, int m, int n, int k, Fp8Operand a, Fp8Operand b, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream);
 
-// norms and clipping (clip.cu): a tensor of a client, in pieces of `piece` elements; first: of the call's pieces, begin and end: its client's
+// norms and clipping (clip.cu): the tensors of the clients, in their order; every client has one at least, of no values if it has none
 struct ClipPart {
     const void *in;
     void *out;
     long n;
-    int first, begin, end, client, in_type, out_type;
+    int client, in_type, out_type;
+    int index; // of the call's tensors; -1: none of them
 };
-int clip_piece(const Context *ctx, double elements);
-int clip_updates(const Context *ctx, const ClipPart *parts, int n_parts, int piece, double most, double *partial, double *norms, cudaStream_t stream);
+size_t clip_workspace_bytes(const Context *ctx, const ClipPart *parts, int n, bool writes);
+int clip_updates(const Context *ctx, const ClipPart *parts, int n, bool writes, double most, double *partial, double *norms, cudaStream_t stream);
 
 } // namespace lb

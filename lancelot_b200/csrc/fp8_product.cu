@@ -19,7 +19,7 @@ namespace {
 constexpr int kM = 128, kK = 128; // rows of a tile, the summed axis of a block
 
 template <int BN> struct TileFp8 {
-    static constexpr int kOutWarps = 8, kThreads = 64 + kOutWarps * 32;
+    static constexpr int kOutWarps = 8, kThreads = 128 + kOutWarps * 32;
     static constexpr int kCols = BN / 2; // columns of a thread: the warps of a quarter of TMEM's lanes take a half each
     static constexpr int kStageBytes = (kM + BN) * kK;
     static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
@@ -51,6 +51,36 @@ __device__ __forceinline__ void tile_at(const Fp8Args &a, int t, int &tm, int &t
     tn = in / rows;
     tm = b * a.band + (in - tn * rows);
 }
+
+// Two 32-bit floats in a register pair
+__device__ __forceinline__ unsigned long long pair(float a, float b)
+{
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ unsigned long long pair(int a, int b)
+{
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+    return v;
+}
+__device__ __forceinline__ void unpair(unsigned long long v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b)
+{
+    unsigned long long v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ void fma2(unsigned long long &c, unsigned long long a, unsigned long long b)
+{
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+
+// Threads of the warps that take results out need more registers than an even share, those of the first warpgroup fewer: with 128 results each
+// 56 + 2 x 224 of the 3 x 168 that the block has (launch_tiles sees that it has them: the second call waits for what the first one gives up).
+constexpr int kChunk = 16;
+constexpr int kEven = 168, kFew = 56, kMany = 224;
 
 // PER_ROW: b has a scale for each of its rows, otherwise one for 128
 template <typename T, int BN, bool PER_ROW>
@@ -92,6 +122,8 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
     const unsigned tmem = *tmem_at;
     const int tiles = a.tiles_m * a.tiles_n;
 
+    if (warp < 4) {
+    if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFew));
     if (warp == 0) {
         if (lane == 0) {
             int it = 0;
@@ -148,10 +180,12 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
             for (int n = 0; n < 1 << 20; ++n)
                 if (mbar_try(drained, 0)) break;
         }
+    }
     } else {
+        if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMany));
         // a warp sees the 32 lanes of TMEM of its quarter; a thread has a row and half of the tile's columns
-        const int quarter = warp & 3, half = (warp - 2) / 4;
-        float *sb = scales + (warp - 2) * C::kCols;
+        const int quarter = warp & 3, half = (warp - 4) / 4;
+        float *sb = scales + (warp - 4) * C::kCols;
         int it = 0;
         bool ok = true;
         for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
@@ -159,10 +193,10 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
             tile_at(a, t, tm, tn);
             const int row = tm * kM + quarter * 32 + lane, col = tn * BN + half * C::kCols;
             const float *pa = a.a.at + (long)(min(row, a.m - 1) >> a.a.shift) * a.a.row;
-            const float *pb = a.b.at + (long)(min(PER_ROW ? col + lane : col, a.n - 1) >> a.b.shift) * a.b.row;
-            float acc[C::kCols];
+            const float *pb = a.b.at + (long)(min(col, a.n - 1) >> a.b.shift) * a.b.row;
+            unsigned long long acc[C::kCols / 2];
 #pragma unroll
-            for (int e = 0; e < C::kCols; ++e) acc[e] = 0.f;
+            for (int e = 0; e < C::kCols / 2; ++e) acc[e] = 0;
             float sa = __ldg(pa), one = 0.f, many[C::kCols / 32];
             auto fetch_b = [&](int k) { // the scales of block k of b
                 if (PER_ROW) {
@@ -176,7 +210,8 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
             fetch_b(0);
             for (int k = 0; k < a.k_blocks; ++k, ++it) {
                 const int buf = it % C::kBufs;
-                const float s = sa, s_one = one;
+                const float s = PER_ROW ? sa : sa * one;
+                const unsigned long long ss = pair(s, s);
                 if (PER_ROW) {
                     __syncwarp();
 #pragma unroll
@@ -187,29 +222,30 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
                     sa = __ldg(pa + (long)(k + 1) * a.a.block);
                     fetch_b(k + 1);
                 }
-                ok = mbar_wait(done + 8 * buf, (it / C::kBufs) & 1, failed);
+                ok = mbar_wait_inline(done + 8 * buf, (it / C::kBufs) & 1, failed);
                 if (!__all_sync(0xffffffffu, ok)) {
                     ok = false;
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned from = tmem + buf * BN + half * C::kCols + ((unsigned)quarter << 21);
+                int v[2][kChunk];
+                tmem_begin(from, v[0]);
 #pragma unroll
-                for (int c = 0; c < C::kCols; c += 32) {
-                    int v[32];
-                    tmem_load32(from + c, v);
-                    if (PER_ROW) {
+                for (int c = 0; c < C::kCols; c += kChunk) {
+                    int(&w)[kChunk] = v[c / kChunk & 1];
+                    tmem_ready(w);
+                    if (c + kChunk < C::kCols) tmem_begin(from + c + kChunk, v[(c / kChunk & 1) ^ 1]);
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 s4 = *reinterpret_cast<const float4 *>(sb + c + e);
-                            acc[c + e] = fmaf(__int_as_float(v[e]) * s, s4.x, acc[c + e]);
-                            acc[c + e + 1] = fmaf(__int_as_float(v[e + 1]) * s, s4.y, acc[c + e + 1]);
-                            acc[c + e + 2] = fmaf(__int_as_float(v[e + 2]) * s, s4.z, acc[c + e + 2]);
-                            acc[c + e + 3] = fmaf(__int_as_float(v[e + 3]) * s, s4.w, acc[c + e + 3]);
+                    for (int e = 0; e < kChunk; e += 4) {
+                        if (PER_ROW) {
+                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(sb + c + e);
+                            fma2(acc[(c + e) / 2], mul2(pair(w[e], w[e + 1]), ss), s4.x);
+                            fma2(acc[(c + e) / 2 + 1], mul2(pair(w[e + 2], w[e + 3]), ss), s4.y);
+                        } else {
+                            fma2(acc[(c + e) / 2], pair(w[e], w[e + 1]), ss);
+                            fma2(acc[(c + e) / 2 + 1], pair(w[e + 2], w[e + 3]), ss);
                         }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) acc[c + e] = fmaf(__int_as_float(v[e]) * s, s_one, acc[c + e]);
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -223,7 +259,7 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
                 for (int c = 0; c < C::kCols; c += 32) {
                     float f[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) f[e] = acc[c + e];
+                    for (int e = 0; e < 32; e += 2) unpair(acc[(c + e) / 2], f[e], f[e + 1]);
                     if (col + c < a.n) put32(out + c, f, a.n - col - c, a.align);
                 }
             }
@@ -242,6 +278,14 @@ template <typename T, int BN, bool PER_ROW> int launch_tiles(const Context *ctx,
     static std::atomic<bool> set[64]; // host threads that come here first at once all set the same attribute
     if (ctx->device >= 64 || !set[ctx->device]) {
         LB_CUDA(cudaFuncSetAttribute(fp8_product_kernel<T, BN, PER_ROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        if (BN == 256) {
+            cudaFuncAttributes has;
+            LB_CUDA(cudaFuncGetAttributes(&has, fp8_product_kernel<T, BN, PER_ROW>));
+            if (has.numRegs < kEven) {
+                set_error("the product's kernel was built with too few registers");
+                return LB_ERR_LOGIC;
+            }
+        }
         if (ctx->device < 64) set[ctx->device] = true;
     }
     const int tiles = a.tiles_m * a.tiles_n;

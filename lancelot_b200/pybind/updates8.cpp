@@ -352,10 +352,11 @@ Tensor clip_updates(int64_t context, int device, const py::object &updates, std:
     }
     const Tensor norms = c.empty({n}, at::kDouble);
     const int count = (int)sizes.size();
-    const size_t need = n ? lb_clip_updates_workspace_bytes(c.context, n, count, clients.data(), sizes.data()) : 0;
+    const int *writes = out || in_place ? out_dtypes.data() : nullptr;
+    const size_t need = n ? lb_clip_updates_workspace_bytes(c.context, n, count, clients.data(), dtypes.data(), sizes.data(), writes) : 0;
     const Tensor ws = c.workspace(need);
     check(lb_clip_updates(c.context, n, count, clients.data(), tensors.data(), dtypes.data(), sizes.data(), max_norm ? *max_norm : HUGE_VAL,
-                          out || in_place ? outs.data() : nullptr, out_dtypes.data(), address<double>(norms), address<void>(ws), need, c.stream()));
+                          out || in_place ? outs.data() : nullptr, writes, address<double>(norms), address<void>(ws), need, c.stream()));
     return norms;
 }
 
