@@ -919,10 +919,11 @@ int lb_dequantize_fp8(lb_context *h, const uint8_t *codes, int code_type, int64_
     if ((rc = code_type_ok(code_type))) return rc;
     REQUIRE(n_rows >= 0 && n_cols >= 0 && n_rows <= (int64_t)1 << 31 && n_cols <= (1 << 30), "n_rows or n_cols is out of range");
     if (n_rows == 0 || n_cols == 0) return LB_OK;
+    REQUIRE(blocks_of(n_rows) * blocks_of(n_cols) < (int64_t)1 << 31, "too many blocks for one call");
     if ((rc = rows_ok(codes, n_rows, n_cols, code_stride, 1))) return rc;
     if ((rc = rows_ok(scales, blocks == 1 ? n_rows : blocks_of(n_rows), blocks == 2 ? n_cols : blocks_of(n_cols), scale_stride, 4))) return rc;
     if ((rc = rows_ok(out, n_rows, n_cols, out_stride, value_size(dtype)))) return rc;
-    return dequantize_fp8(C(h), codes, code_type, code_stride, scales, scale_stride, blocks, n_rows, (int)n_cols, out, dtype, out_stride, S(stream));
+    return dequantize_fp8(codes, code_type, code_stride, scales, scale_stride, blocks, n_rows, (int)n_cols, out, dtype, out_stride, S(stream));
 }
 
 static Fp8Operand operand_of(const lb_fp8_operand *o)

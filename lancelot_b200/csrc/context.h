@@ -235,7 +235,7 @@ struct Fp8Operand {
 };
 int quantize_fp8(const void *values, int dtype, long rows, int cols, long stride, int blocks, int code_type, unsigned char *codes, long code_stride,
                  float *scales, long scale_stride, unsigned char *down, long down_stride, float *down_scales, long down_scale_stride, cudaStream_t stream);
-int dequantize_fp8(const Context *ctx, const unsigned char *codes, int code_type, long code_stride, const float *scales, long scale_stride, int blocks,
+int dequantize_fp8(const unsigned char *codes, int code_type, long code_stride, const float *scales, long scale_stride, int blocks,
                    long rows, int cols, void *out, int dtype, long out_stride, cudaStream_t stream);
 size_t fp8_matmul_workspace_bytes(int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b);
 int fp8_matmul(Context *ctx, int m, int n, int k, Fp8Operand a, Fp8Operand b, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream);

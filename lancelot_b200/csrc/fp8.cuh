@@ -32,60 +32,93 @@ template <bool E5M2> __device__ __forceinline__ float2 from_codes2(unsigned v)
     return __half22float2(*reinterpret_cast<const __half2 *>(&h));
 }
 
-// The code nearest to t / s, decided exactly, with one product.  q = t * (1 / s) in 32 bits is within two steps (2^-22 relative) of the quotient, so its
-// code is right unless q lies that near to a border between two codes.  There the border h, which has five bits at most, is
-// compared itself: the sign of h s - |t| is exact in one fused multiply-add for s >= 2^-100.  Below the least normal number the codes are evenly
-// spaced; adding that number brings their borders to the same bits of the sum.
-template <bool E5M2> __device__ __forceinline__ bool near_border(float q)
+// Two 32-bit floats in a register pair
+__device__ __forceinline__ unsigned long long pair(float a, float b)
+{
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ unsigned long long pair(int a, int b)
+{
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
+    return v;
+}
+__device__ __forceinline__ void unpair(unsigned long long v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b)
+{
+    unsigned long long v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ void fma2(unsigned long long &c, unsigned long long a, unsigned long long b)
+{
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ unsigned long long fma2_of(unsigned long long a, unsigned long long b, unsigned long long c)
+{
+    unsigned long long v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ float fma_sat(float a, float b, float c) // cut to [0, 1]
+{
+    float v;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+
+// The code nearest to m / s, m >= 0, decided exactly.  q = m * (1 / s) in 32 bits is within two steps of the quotient.  The codes on either side of q
+// have the border h between them, of five bits at most, and the sign of d = h s - m, exact in one fused multiply-add for s >= 2^-80, says on which
+// side of it the quotient lies, 0 that it lies on it.  So what is rounded to a code is not q but h (1 - 2^-10), h or h (1 + 2^-10): a tie goes to the
+// even code.  (Where q itself lies next to a code, on the wrong side of it, the border next to q still sends it to that code.)  Below the
+// least normal number the codes are evenly spaced; that number added to q brings their borders to the same bits.  Choices are made by
+// multiply-adds cut to [0, 1], which cost half of what comparisons do, and nothing depends on how often values lie next to a border: 16-bit
+// values often lie on one.
+constexpr float kTinyScale = 0x1p-80f;
+
+template <bool E5M2> __device__ __forceinline__ unsigned long long beside_border(unsigned long long m, unsigned long long s, unsigned long long f)
 {
     using F = Fp8<E5M2>;
-    const float m = fabsf(q);
-    const unsigned u = __float_as_uint(m < F::kNormal ? m + F::kNormal : m);
-    return ((u & F::kLow) - (F::kHalf - 4)) <= 8u;
+    const unsigned long long q = mul2(m, f);
+    float q0, q1, w0, w1, d0, d1;
+    unpair(q, q0, q1);
+    const unsigned long long y = pair(fma_sat(q0, -0x1p60f, F::kNormal * 0x1p60f), fma_sat(q1, -0x1p60f, F::kNormal * 0x1p60f)); // 1: below the normal numbers
+    unpair(fma2_of(y, pair(F::kNormal, F::kNormal), q), w0, w1);
+    const unsigned long long h = fma2_of(y, pair(-F::kNormal, -F::kNormal), pair(__uint_as_float((__float_as_uint(w0) & ~F::kLow) | F::kHalf),
+                                                                                 __uint_as_float((__float_as_uint(w1) & ~F::kLow) | F::kHalf)));
+    unpair(fma2_of(h, s, mul2(m, pair(-1.f, -1.f))), d0, d1);
+    const unsigned long long z = pair(fma_sat(d0, 0x1p125f, 0.5f), fma_sat(d1, 0x1p125f, 0.5f)); // d is a multiple of 2^-120
+    return mul2(h, fma2_of(z, pair(-0x1p-9f, -0x1p-9f), pair(1.f + 0x1p-10f, 1.f + 0x1p-10f)));
 }
-template <bool E5M2> __device__ __forceinline__ float settled(float q, float t, float s) // q, moved off the border to its right side, or onto it
+// smaller scales: a quotient of 64 bits, rounded to 24 in a way that keeps what lies beyond them in the last bit, so that rounding once more is
+// right.  0 where there is no scale, or one that is not finite
+__device__ __noinline__ float quotient_of_tiny(float m, float s)
 {
-    using F = Fp8<E5M2>;
-    if (!near_border<E5M2>(q)) return q;
-    const float m = fabsf(q);
-    const bool low = m < F::kNormal;
-    float h = __uint_as_float((__float_as_uint(low ? m + F::kNormal : m) & ~F::kLow) | F::kHalf);
-    if (low) h -= F::kNormal;
-    const float d = fmaf(h, s, -fabsf(t));
-    if (d != 0.f) h *= d > 0.f ? 1.f - 0x1p-12f : 1.f + 0x1p-12f;
-    return copysignf(h, t);
-}
-// scales below that (1 / s may pass the range, and h s the smallest numbers): a quotient of 64 bits, rounded to 24 in a way that keeps
-// what lies beyond them in the last bit, so that rounding once more is right
-__device__ __noinline__ float quotient_of_tiny(float t, float s)
-{
-    const double q = (double)t / (double)s;
+    if (!(s > 0.f)) return 0.f;
+    const double q = (double)m / (double)s;
     const float f = __double2float_rz(q);
     return (double)f == q ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
-
-constexpr float kTinyScale = 0x1p-100f;
-
-// the factor that takes a value to its quotient; 0 where the codes are 0 (a block of zeros, one that is not finite), and for the scales
-// that quotient_of_tiny serves
 __device__ __forceinline__ float inverse_of(float s) { return s >= kTinyScale ? __frcp_rn(s) : 0.f; }
+// whether a block's codes cannot be had with that
+__device__ __forceinline__ bool odd_scale(float s) { return !(s >= kTinyScale) && s != 0.f; }
 
-// four codes of one scale, or of a scale each
-template <bool E5M2> __device__ __forceinline__ unsigned codes4(const float *t, float s0, float s1, float s2, float s3, float i0, float i1, float i2, float i3)
+// The codes of four magnitudes (bits), of one scale or of a scale each (s), with the factors to their quotients (f).  odd: whether one of the scales is
+template <bool E5M2> __device__ __forceinline__ unsigned codes4(const uint4 &m, const float4 &s, const float4 &f, bool odd)
 {
-    float a = t[0] * i0, b = t[1] * i1, c = t[2] * i2, d = t[3] * i3;
-    if (i0 == 0.f || i1 == 0.f || i2 == 0.f || i3 == 0.f) { // seldom: none of this is on the way of ordinary blocks
-        a = i0 != 0.f ? settled<E5M2>(a, t[0], s0) : s0 > 0.f ? quotient_of_tiny(t[0], s0) : 0.f;
-        b = i1 != 0.f ? settled<E5M2>(b, t[1], s1) : s1 > 0.f ? quotient_of_tiny(t[1], s1) : 0.f;
-        c = i2 != 0.f ? settled<E5M2>(c, t[2], s2) : s2 > 0.f ? quotient_of_tiny(t[2], s2) : 0.f;
-        d = i3 != 0.f ? settled<E5M2>(d, t[3], s3) : s3 > 0.f ? quotient_of_tiny(t[3], s3) : 0.f;
-    } else if (near_border<E5M2>(a) | near_border<E5M2>(b) | near_border<E5M2>(c) | near_border<E5M2>(d)) {
-        a = settled<E5M2>(a, t[0], s0);
-        b = settled<E5M2>(b, t[1], s1);
-        c = settled<E5M2>(c, t[2], s2);
-        d = settled<E5M2>(d, t[3], s3);
+    const float a = __uint_as_float(m.x), b = __uint_as_float(m.y), c = __uint_as_float(m.z), d = __uint_as_float(m.w);
+    float q0, q1, q2, q3;
+    unpair(beside_border<E5M2>(pair(a, b), pair(s.x, s.y), pair(f.x, f.y)), q0, q1);
+    unpair(beside_border<E5M2>(pair(c, d), pair(s.z, s.w), pair(f.z, f.w)), q2, q3);
+    if (odd) {
+        if (!(s.x >= kTinyScale)) q0 = quotient_of_tiny(a, s.x);
+        if (!(s.y >= kTinyScale)) q1 = quotient_of_tiny(b, s.y);
+        if (!(s.z >= kTinyScale)) q2 = quotient_of_tiny(c, s.z);
+        if (!(s.w >= kTinyScale)) q3 = quotient_of_tiny(d, s.w);
     }
-    return to_codes2<E5M2>(a, b) | to_codes2<E5M2>(c, d) << 16;
+    return to_codes2<E5M2>(q0, q1) | to_codes2<E5M2>(q2, q3) << 16;
 }
 
 } // namespace

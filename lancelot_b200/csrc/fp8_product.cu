@@ -52,31 +52,6 @@ __device__ __forceinline__ void tile_at(const Fp8Args &a, int t, int &tm, int &t
     tm = b * a.band + (in - tn * rows);
 }
 
-// Two 32-bit floats in a register pair
-__device__ __forceinline__ unsigned long long pair(float a, float b)
-{
-    unsigned long long v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-    return v;
-}
-__device__ __forceinline__ unsigned long long pair(int a, int b)
-{
-    unsigned long long v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b));
-    return v;
-}
-__device__ __forceinline__ void unpair(unsigned long long v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b)
-{
-    unsigned long long v;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-__device__ __forceinline__ void fma2(unsigned long long &c, unsigned long long a, unsigned long long b)
-{
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
-}
-
 // Threads of the warps that take results out need more registers than an even share, those of the first warpgroup fewer: with 128 results each
 // 56 + 2 x 224 of the 3 x 168 that the block has (launch_tiles sees that it has them: the second call waits for what the first one gives up).
 constexpr int kChunk = 16;

@@ -5,6 +5,8 @@
 //
 // The reference has no 8-bit form of anything; products of such matrices (fp8_product.cu) sum over the axis along which a block
 // has 128 values, so the operand of a product and that of its gradient are the same matrix in two kinds of blocks.
+#include <type_traits>
+
 #include "fp8.cuh"
 #include "product.cuh"
 
@@ -22,45 +24,67 @@ __device__ __forceinline__ float number(float v) { return v; }
 __device__ __forceinline__ float number(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float number(__half v) { return __half2float(v); }
 
-// 16 values on a 16-byte boundary
-__device__ __forceinline__ void load16v(const float *p, float *v)
-{
-#pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-        const float4 x = __ldg(reinterpret_cast<const float4 *>(p + e));
-        v[e] = x.x, v[e + 1] = x.y, v[e + 2] = x.z, v[e + 3] = x.w;
+// Four values of a row as they lie.  Magnitudes are ordered like their bit patterns, with infinities and NaN above all numbers, in each of the types:
+// an integer maximum carries those along
+template <typename T> struct Four { // 16-bit types
+    using Raw = uint2;
+    static __device__ __forceinline__ Raw load(const T *p) { return __ldg(reinterpret_cast<const uint2 *>(p)); }
+    static __device__ __forceinline__ Raw make(const float (&v)[4]) { return make_uint2(pack2((T *)nullptr, v[0], v[1]), pack2((T *)nullptr, v[2], v[3])); }
+    static __device__ __forceinline__ unsigned wide(unsigned v) // the 32-bit float's bits of one of the type's in the upper half
+    {
+        if (sizeof(T) == 2 && std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)(v >> 16))));
+        return v;
     }
-}
-__device__ __forceinline__ void load16v(const __nv_bfloat16 *p, float *v)
-{
-#pragma unroll
-    for (int e = 0; e < 16; e += 8) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p + e));
-        const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[e + 2 * i] = __uint_as_float(w[i] << 16), v[e + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void load16v(const __half *p, float *v)
-{
-#pragma unroll
-    for (int e = 0; e < 16; e += 8) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p + e));
-        const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            v[e + 2 * i] = f.x, v[e + 2 * i + 1] = f.y;
+    static __device__ __forceinline__ uint4 magnitudes(const Raw &x)
+    {
+        const unsigned a = x.x & 0x7fff7fffu, b = x.y & 0x7fff7fffu;
+        if (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a)), g = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+            return make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(g.x), __float_as_uint(g.y));
         }
+        return make_uint4(a << 16, a & 0x7fff0000u, b << 16, b & 0x7fff0000u);
     }
+    static __device__ __forceinline__ unsigned signs(const Raw &x) { return __byte_perm(x.x, x.y, 0x7531) & 0x80808080u; }
+    // the largest magnitudes of several: column by column
+    using Most = uint2;
+    static __device__ __forceinline__ Most none() { return make_uint2(0, 0); }
+    static __device__ __forceinline__ Most more(const Most &m, const Raw &x) { return make_uint2(__vmaxu2(m.x, x.x & 0x7fff7fffu), __vmaxu2(m.y, x.y & 0x7fff7fffu)); }
+    static __device__ __forceinline__ uint4 columns(const Most &m) { return make_uint4(wide(m.x << 16), wide(m.x & 0xffff0000u), wide(m.y << 16), wide(m.y & 0xffff0000u)); }
+    static __device__ __forceinline__ unsigned all(const Most &m)
+    {
+        const unsigned v = __vmaxu2(m.x, m.y);
+        return wide(max(v << 16, v & 0xffff0000u));
+    }
+};
+template <> struct Four<float> {
+    using Raw = uint4;
+    static __device__ __forceinline__ Raw load(const float *p) { return __ldg(reinterpret_cast<const uint4 *>(p)); }
+    static __device__ __forceinline__ Raw make(const float (&v)[4]) { return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])); }
+    static __device__ __forceinline__ uint4 magnitudes(const Raw &x) { return make_uint4(x.x & 0x7fffffffu, x.y & 0x7fffffffu, x.z & 0x7fffffffu, x.w & 0x7fffffffu); }
+    static __device__ __forceinline__ unsigned signs(const Raw &x) { return __byte_perm(__byte_perm(x.x, x.y, 0x0073), __byte_perm(x.z, x.w, 0x0073), 0x5410) & 0x80808080u; }
+    using Most = uint4;
+    static __device__ __forceinline__ Most none() { return make_uint4(0, 0, 0, 0); }
+    static __device__ __forceinline__ Most more(const Most &m, const Raw &x)
+    {
+        const uint4 a = magnitudes(x);
+        return make_uint4(max(m.x, a.x), max(m.y, a.y), max(m.z, a.z), max(m.w, a.w));
+    }
+    static __device__ __forceinline__ uint4 columns(const Most &m) { return m; }
+    static __device__ __forceinline__ unsigned all(const Most &m) { return max(max(m.x, m.y), max(m.z, m.w)); }
+};
+template <typename T, bool VEC> __device__ __forceinline__ typename Four<T>::Raw load4(const T *p, int n) // the first n of them, zeros for the others
+{
+    if (VEC && n >= 4) return Four<T>::load(p);
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = e < n ? number(p[e]) : 0.f;
+    return Four<T>::make(v);
 }
-
-// magnitudes are ordered like their bit patterns, with infinities and NaN above all numbers: an integer maximum carries them along
-__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 template <bool E5M2> __device__ __forceinline__ float scale_of(unsigned most)
 {
     return most >= kInf ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(most), Fp8<E5M2>::kMost);
 }
+__device__ __forceinline__ float4 all(float v) { return make_float4(v, v, v, v); }
 
 struct QuantizeFp8Args {
     const void *values;
@@ -73,114 +97,90 @@ struct QuantizeFp8Args {
     long scale_stride, down_scale_stride;
 };
 
-__device__ __forceinline__ void put16(unsigned char *p, const unsigned (&q)[4], int n, bool vec)
+__device__ __forceinline__ void put4(unsigned char *p, unsigned q, int n, bool vec)
 {
-    if (vec && n >= 16) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(q[0], q[1], q[2], q[3]);
+    if (vec && n >= 4) {
+        *reinterpret_cast<unsigned *>(p) = q;
     } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (e < n) p[e] = (unsigned char)(q[e / 4] >> 8 * (e & 3));
+        for (int e = 0; e < 4; ++e)
+            if (e < n) p[e] = (unsigned char)(q >> 8 * e);
     }
 }
+__device__ __forceinline__ bool four_aligned(const unsigned char *p, long stride) { return stride % 4 == 0 && (uintptr_t)p % 4 == 0; }
 
-// A block takes a tile of 128 x 128: eight threads a row, 16 columns each, four rows a thread.  Maxima along a row stay in the eight threads,
-// those along a column go through shared memory.
-template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bounds__(256) quantize_fp8_kernel(const QuantizeFp8Args a)
+// A block takes a tile of 128 x 128, a warp eight of its rows, a lane four columns: the values of a row's block are one warp's, and
+// a thread's maxima along columns cover its eight rows and then go through shared memory.
+constexpr int kWarps = 16, kRowsOf = kB / kWarps;
+template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bounds__(kWarps * 32, 2) quantize_fp8_kernel(const QuantizeFp8Args a)
 {
-    __shared__ unsigned part[8][kB];
-    __shared__ float2 column[kB]; // scale and its inverse
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    __shared__ unsigned part[kWarps][kB];
+    __shared__ float column[kB];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long tr = blockIdx.x / a.tiles_c;
     const int tc = blockIdx.x - (unsigned)tr * a.tiles_c;
-    const int c0 = tc * kB + (t & 7) * 16, n = min(16, a.cols - c0);
-    const long r0 = tr * kB + (t >> 3);
-    float v[4][16];
+    const int c0 = tc * kB + lane * 4, n = a.cols - c0;
+    const long r0 = tr * kB + warp;
+    const int rows = (int)min((long)kRowsOf, max(0l, (a.rows - r0 + kWarps - 1) / kWarps)); // of this warp: r0, r0 + 16, ...
+    const T *p = reinterpret_cast<const T *>(a.values) + r0 * a.stride + c0;
+    typename Four<T>::Raw raw[kRowsOf];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long r = r0 + 32 * i;
-        const T *p = reinterpret_cast<const T *>(a.values) + r * a.stride + c0;
-        if (VEC && r < a.rows && n == 16) {
-            load16v(p, v[i]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[i][e] = r < a.rows && e < n ? number(p[e]) : 0.f;
-        }
-    }
-    const bool code_vec = a.code_stride % 16 == 0 && (uintptr_t)a.codes % 16 == 0, down_vec = a.down_stride % 16 == 0 && (uintptr_t)a.down % 16 == 0;
+    for (int i = 0; i < kRowsOf; ++i) raw[i] = load4<T, VEC>(p + i * kWarps * a.stride, i < rows ? n : 0);
+    using V = Four<T>;
+    auto put_row = [&](unsigned char *to, int i, const float4 &s, const float4 &f, bool odd, bool vec) {
+        put4(to, codes4<E5M2>(V::magnitudes(raw[i]), s, f, odd) | V::signs(raw[i]), n, vec);
+    };
     if (MODE == kRows || MODE == kBoth) {
+        const bool vec = four_aligned(a.codes, a.code_stride);
+        // lane i finds the scale of row i, for all lanes
+        unsigned mine = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const long r = r0 + 32 * i;
-            unsigned m = 0;
+        for (int i = 0; i < kRowsOf; ++i) {
+            const unsigned most = __reduce_max_sync(0xffffffffu, V::all(V::more(V::none(), raw[i])));
+            if (lane == i) mine = most;
+        }
+        const float scale = scale_of<E5M2>(mine), inverse = inverse_of(scale);
+        if (lane < rows) a.scales[(r0 + lane * kWarps) * a.scale_stride + tc] = scale;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) m = max(m, magnitude(v[i][e]));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-            const float s = scale_of<E5M2>(m), inv = inverse_of(s);
-            if (r >= a.rows || n <= 0) continue;
-            if ((t & 7) == 0) a.scales[r * a.scale_stride + tc] = s;
-            unsigned q[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = codes4<E5M2>(v[i] + 4 * e, s, s, s, s, inv, inv, inv, inv);
-            put16(a.codes + r * a.code_stride + c0, q, n, code_vec);
+        for (int i = 0; i < kRowsOf; ++i) {
+            const float s = __shfl_sync(0xffffffffu, scale, i), f = __shfl_sync(0xffffffffu, inverse, i);
+            if (i < rows) put_row(a.codes + (r0 + i * kWarps) * a.code_stride + c0, i, all(s), all(f), odd_scale(s), vec);
         }
     }
-    if constexpr (MODE == kSquare) {
-        unsigned m = 0;
+    if constexpr (MODE == kSquare || MODE == kColumns || MODE == kBoth) {
+        typename V::Most most = V::none();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kRowsOf; ++i) most = V::more(most, raw[i]);
+        if constexpr (MODE == kSquare) {
+            const bool vec = four_aligned(a.codes, a.code_stride);
+            unsigned m = __reduce_max_sync(0xffffffffu, V::all(most));
+            if (lane == 0) part[0][warp] = m;
+            __syncthreads();
+            m = __reduce_max_sync(0xffffffffu, part[0][lane & (kWarps - 1)]);
+            const float s = scale_of<E5M2>(m), f = inverse_of(s);
+            if (threadIdx.x == 0) a.scales[tr * a.scale_stride + tc] = s;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) m = max(m, magnitude(v[i][e]));
-        m = __reduce_max_sync(0xffffffffu, m);
-        if (lane == 0) part[0][warp] = m;
-        __syncthreads();
-        m = 0;
+            for (int i = 0; i < kRowsOf; ++i)
+                if (i < rows) put_row(a.codes + (r0 + i * kWarps) * a.code_stride + c0, i, all(s), all(f), odd_scale(s), vec);
+        } else {
+            const bool vec = four_aligned(a.down, a.down_stride);
+            *reinterpret_cast<uint4 *>(&part[warp][lane * 4]) = V::columns(most);
+            __syncthreads();
+            if (threadIdx.x < kB) {
+                unsigned m = 0;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) m = max(m, part[0][w]);
-        const float s = scale_of<E5M2>(m), inv = inverse_of(s);
-        if (t == 0) a.scales[tr * a.scale_stride + tc] = s;
+                for (int w = 0; w < kWarps; ++w) m = max(m, part[w][threadIdx.x]);
+                const float s = scale_of<E5M2>(m);
+                column[threadIdx.x] = s;
+                if (tc * kB + (int)threadIdx.x < a.cols) a.down_scales[tr * a.down_scale_stride + tc * kB + threadIdx.x] = s;
+            }
+            __syncthreads();
+            const float4 s = *reinterpret_cast<const float4 *>(column + lane * 4);
+            const float4 f = make_float4(inverse_of(s.x), inverse_of(s.y), inverse_of(s.z), inverse_of(s.w));
+            const bool odd = odd_scale(s.x) || odd_scale(s.y) || odd_scale(s.z) || odd_scale(s.w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const long r = r0 + 32 * i;
-            if (r >= a.rows || n <= 0) continue;
-            unsigned q[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = codes4<E5M2>(v[i] + 4 * e, s, s, s, s, inv, inv, inv, inv);
-            put16(a.codes + r * a.code_stride + c0, q, n, code_vec);
-        }
-    }
-    if constexpr (MODE == kColumns || MODE == kBoth) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            unsigned m = max(max(magnitude(v[0][e]), magnitude(v[1][e])), max(magnitude(v[2][e]), magnitude(v[3][e])));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            if (lane < 8) part[warp][lane * 16 + e] = m;
-        }
-        __syncthreads();
-        if (t < kB) {
-            unsigned m = 0;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) m = max(m, part[w][t]);
-            const float s = scale_of<E5M2>(m);
-            column[t] = make_float2(s, inverse_of(s));
-            if (tc * kB + t < a.cols) a.down_scales[tr * a.down_scale_stride + tc * kB + t] = s;
-        }
-        __syncthreads();
-        unsigned q[4][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 *s = column + (t & 7) * 16 + 4 * e;
-            const float2 s0 = s[0], s1 = s[1], s2 = s[2], s3 = s[3];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q[i][e] = codes4<E5M2>(v[i] + 4 * e, s0.x, s1.x, s2.x, s3.x, s0.y, s1.y, s2.y, s3.y);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const long r = r0 + 32 * i;
-            if (r < a.rows && n > 0) put16(a.down + r * a.down_stride + c0, q[i], n, down_vec);
+            for (int i = 0; i < kRowsOf; ++i)
+                if (i < rows) put_row(a.down + (r0 + i * kWarps) * a.down_stride + c0, i, s, f, odd, vec);
         }
     }
 }
@@ -188,7 +188,8 @@ template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bo
 struct DequantizeFp8Args {
     const unsigned char *codes;
     long code_stride, rows;
-    int cols, groups; // groups of 16 columns in a row
+    int cols;
+    unsigned tiles_c;
     const float *scales;
     long scale_stride;
     int row_shift, col_shift; // 7: a block spans 128 rows, 128 columns; 0: one
@@ -196,47 +197,55 @@ struct DequantizeFp8Args {
     long out_stride;
 };
 
-// a thread takes 16 codes of a row
-template <typename T, bool E5M2, bool VEC> __global__ void __launch_bounds__(256) dequantize_fp8_kernel(const DequantizeFp8Args a)
+// the same tiles: the scales of a lane's four columns serve its eight rows
+template <typename T, bool E5M2, bool VEC> __global__ void __launch_bounds__(kWarps * 32) dequantize_fp8_kernel(const DequantizeFp8Args a)
 {
-    const long total = a.rows * a.groups, step = (long)gridDim.x * 256;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-        const long r = i / a.groups;
-        const int c = (int)(i - r * a.groups) * 16, n = min(16, a.cols - c);
-        const unsigned char *p = a.codes + r * a.code_stride + c;
-        const float *s = a.scales + (r >> a.row_shift) * a.scale_stride;
-        T *to = reinterpret_cast<T *>(a.out) + r * a.out_stride + c;
-        unsigned w[4] = {0, 0, 0, 0};
-        if (VEC && n == 16) {
-            const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
-            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long tr = blockIdx.x / a.tiles_c;
+    const int tc = blockIdx.x - (unsigned)tr * a.tiles_c;
+    const int c0 = tc * kB + lane * 4, n = a.cols - c0;
+    const long r0 = tr * kB + warp;
+    const int rows = (int)min((long)kRowsOf, max(0l, (a.rows - r0 + kWarps - 1) / kWarps));
+    if (n <= 0) return;
+    const unsigned char *p = a.codes + r0 * a.code_stride + c0;
+    unsigned q[kRowsOf];
+    float4 s[kRowsOf];
+#pragma unroll
+    for (int i = 0; i < kRowsOf; ++i) {
+        if (i >= rows) break;
+        const unsigned char *at = p + i * kWarps * a.code_stride;
+        if (VEC && n >= 4) {
+            q[i] = __ldg(reinterpret_cast<const unsigned *>(at));
+        } else {
+            q[i] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < n) q[i] |= (unsigned)__ldg(at + e) << 8 * e;
+        }
+    }
+    if (a.col_shift) {
+#pragma unroll
+        for (int i = 0; i < kRowsOf; ++i)
+            if (i < rows) s[i] = all(__ldg(a.scales + ((r0 + i * kWarps) >> a.row_shift) * a.scale_stride + tc));
+    } else {
+        const float *of = a.scales + tr * a.scale_stride + c0;
+        s[0] = make_float4(__ldg(of), n > 1 ? __ldg(of + 1) : 0.f, n > 2 ? __ldg(of + 2) : 0.f, n > 3 ? __ldg(of + 3) : 0.f);
+#pragma unroll
+        for (int i = 1; i < kRowsOf; ++i) s[i] = s[0];
+    }
+    T *to = reinterpret_cast<T *>(a.out) + r0 * a.out_stride + c0;
+#pragma unroll
+    for (int i = 0; i < kRowsOf; ++i) {
+        if (i >= rows) break;
+        const float2 x = from_codes2<E5M2>(q[i]), y = from_codes2<E5M2>(q[i] >> 16);
+        const float v[4] = {x.x * s[i].x, x.y * s[i].y, y.x * s[i].z, y.y * s[i].w};
+        T *at = to + i * kWarps * a.out_stride;
+        if (VEC && n >= 4) {
+            *reinterpret_cast<typename Four<T>::Raw *>(at) = Four<T>::make(v);
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (e < n) w[e / 4] |= (unsigned)p[e] << 8 * (e & 3);
-        }
-        float v[16];
-        const float one = a.col_shift ? __ldg(s + (c >> 7)) : 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            const float2 f = from_codes2<E5M2>(w[e / 4] >> 8 * (e & 3));
-            v[e] = f.x * (a.col_shift ? one : e < n ? __ldg(s + c + e) : 0.f);
-            v[e + 1] = f.y * (a.col_shift ? one : e + 1 < n ? __ldg(s + c + e + 1) : 0.f);
-        }
-        if (VEC && n == 16) {
-            if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4 *>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; e += 8)
-                    *reinterpret_cast<uint4 *>(to + e) = make_uint4(pack2((T *)nullptr, v[e], v[e + 1]), pack2((T *)nullptr, v[e + 2], v[e + 3]),
-                                                                    pack2((T *)nullptr, v[e + 4], v[e + 5]), pack2((T *)nullptr, v[e + 6], v[e + 7]));
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (e < n) put(to + e, v[e]);
+            for (int e = 0; e < 4; ++e)
+                if (e < n) put(at + e, v[e]);
         }
     }
 }
@@ -244,9 +253,10 @@ template <typename T, bool E5M2, bool VEC> __global__ void __launch_bounds__(256
 template <typename T, bool E5M2, int MODE> int launch_quantize(const QuantizeFp8Args &a, cudaStream_t stream)
 {
     const long tiles = ((a.rows + kB - 1) / kB) * a.tiles_c;
-    const bool vec = (uintptr_t)a.values % 16 == 0 && (a.rows == 1 || a.stride * (long)sizeof(T) % 16 == 0);
-    if (vec) quantize_fp8_kernel<T, E5M2, MODE, true><<<(unsigned)tiles, 256, 0, stream>>>(a);
-    else quantize_fp8_kernel<T, E5M2, MODE, false><<<(unsigned)tiles, 256, 0, stream>>>(a);
+    const long unit = 4 * (long)sizeof(T);
+    const bool vec = (uintptr_t)a.values % unit == 0 && (a.rows == 1 || a.stride * (long)sizeof(T) % unit == 0);
+    if (vec) quantize_fp8_kernel<T, E5M2, MODE, true><<<(unsigned)tiles, kWarps * 32, 0, stream>>>(a);
+    else quantize_fp8_kernel<T, E5M2, MODE, false><<<(unsigned)tiles, kWarps * 32, 0, stream>>>(a);
     LB_CUDA(cudaGetLastError());
     return LB_OK;
 }
@@ -259,13 +269,12 @@ template <typename T, bool E5M2> int quantize_typed(const QuantizeFp8Args &a, in
     default: return launch_quantize<T, E5M2, kSquare>(a, stream);
     }
 }
-template <typename T, bool E5M2> int launch_dequantize(const Context *ctx, const DequantizeFp8Args &a, cudaStream_t stream)
+template <typename T, bool E5M2> int launch_dequantize(const DequantizeFp8Args &a, cudaStream_t stream)
 {
-    const long blocks = (a.rows * a.groups + 255) / 256, most = (long)ctx->sm_count * 32;
-    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-    const bool vec = (uintptr_t)a.codes % 16 == 0 && (uintptr_t)a.out % 16 == 0 && (a.rows == 1 || (a.code_stride % 16 == 0 && a.out_stride * (long)sizeof(T) % 16 == 0));
-    if (vec) dequantize_fp8_kernel<T, E5M2, true><<<grid, 256, 0, stream>>>(a);
-    else dequantize_fp8_kernel<T, E5M2, false><<<grid, 256, 0, stream>>>(a);
+    const long tiles = ((a.rows + kB - 1) / kB) * a.tiles_c, unit = 4 * (long)sizeof(T);
+    const bool vec = (uintptr_t)a.codes % 4 == 0 && (uintptr_t)a.out % unit == 0 && (a.rows == 1 || (a.code_stride % 4 == 0 && a.out_stride * (long)sizeof(T) % unit == 0));
+    if (vec) dequantize_fp8_kernel<T, E5M2, true><<<(unsigned)tiles, kWarps * 32, 0, stream>>>(a);
+    else dequantize_fp8_kernel<T, E5M2, false><<<(unsigned)tiles, kWarps * 32, 0, stream>>>(a);
     LB_CUDA(cudaGetLastError());
     return LB_OK;
 }
@@ -298,7 +307,7 @@ int quantize_fp8(const void *values, int dtype, long rows, int cols, long stride
     }
 }
 
-int dequantize_fp8(const Context *ctx, const unsigned char *codes, int code_type, long code_stride, const float *scales, long scale_stride, int blocks,
+int dequantize_fp8(const unsigned char *codes, int code_type, long code_stride, const float *scales, long scale_stride, int blocks,
                    long rows, int cols, void *out, int dtype, long out_stride, cudaStream_t stream)
 {
     DequantizeFp8Args a;
@@ -306,7 +315,7 @@ int dequantize_fp8(const Context *ctx, const unsigned char *codes, int code_type
     a.code_stride = code_stride;
     a.rows = rows;
     a.cols = cols;
-    a.groups = (cols + 15) / 16;
+    a.tiles_c = (unsigned)((cols + kB - 1) / kB);
     a.scales = scales;
     a.scale_stride = scale_stride;
     a.row_shift = blocks == kRows ? 0 : 7;
@@ -316,9 +325,9 @@ int dequantize_fp8(const Context *ctx, const unsigned char *codes, int code_type
     count_launch("fp8_dequantize", stream, (double)rows * cols * (1 + (dtype == 1 ? 4 : 2)));
     const bool e5m2 = code_type == 6;
     switch (dtype) {
-    case 1: return e5m2 ? launch_dequantize<float, true>(ctx, a, stream) : launch_dequantize<float, false>(ctx, a, stream);
-    case 3: return e5m2 ? launch_dequantize<__nv_bfloat16, true>(ctx, a, stream) : launch_dequantize<__nv_bfloat16, false>(ctx, a, stream);
-    default: return e5m2 ? launch_dequantize<__half, true>(ctx, a, stream) : launch_dequantize<__half, false>(ctx, a, stream);
+    case 1: return e5m2 ? launch_dequantize<float, true>(a, stream) : launch_dequantize<float, false>(a, stream);
+    case 3: return e5m2 ? launch_dequantize<__nv_bfloat16, true>(a, stream) : launch_dequantize<__nv_bfloat16, false>(a, stream);
+    default: return e5m2 ? launch_dequantize<__half, true>(a, stream) : launch_dequantize<__half, false>(a, stream);
     }
 }
 
