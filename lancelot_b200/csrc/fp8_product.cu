@@ -18,20 +18,117 @@ namespace {
 
 constexpr int kM = 128, kK = 128; // rows of a tile, the summed axis of a block
 
+struct Scales {
+    const float *at;
+    long row, block; // from one row (or block of 128 rows) to the next; from one block of the summed axis to the next
+    int shift;       // 7: a scale for 128 rows
+};
+
+// ---- few rows on one side -------------------------------------------------------------------------------------------------
+// Where both operands lie with the summed axis along their rows and one has up to eight of them, the other's bytes bound the call: they go
+// from memory straight into the registers of the warp's matrix instruction, as in the 8-bit integer product.  A block forms 16 rows of the long side
+// (the rows of A of m16n8k32) against the short side; its 16 warps take runs of 128 of the summed axis by turns, two steps of 64, and add up
+// through shared memory.  The order of the summed axis inside a product is free, so lane (g, t) loads 16 consecutive bytes of a row and uses them as four
+// k-slots on either side.  1 x 4096 x 4096 takes 4.8 us, 1 x 11008 x 4096 10.1 us (4.5 TB/s); 16 x 4096 x 4096 takes 10.2 us so, and
+// 8 us by tiles.
+constexpr int kSkinnyWarps = 16, kSkinny = 8;
+
+template <bool WIDE_A, bool WIDE_B> // e5m2
+__device__ __forceinline__ void mma_fp8(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1)
+{
+#define LB_MMA(A, B)                                                                                                                                  \
+    asm("mma.sync.aligned.m16n8k32.row.col.f32." A "." B ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                                 \
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                                                              \
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+    if (WIDE_A && WIDE_B) LB_MMA("e5m2", "e5m2");
+    else if (WIDE_A) LB_MMA("e5m2", "e4m3");
+    else if (WIDE_B) LB_MMA("e4m3", "e5m2");
+    else LB_MMA("e4m3", "e4m3");
+#undef LB_MMA
+}
+
+struct SkinnyFp8Args {
+    const signed char *w, *x; // long side [rows][k], short side [cols][k]
+    long w_stride, x_stride;
+    Scales ws, xs;
+    int rows, cols, k;
+    void *out;
+    long row_step, col_step; // of the result
+};
+
+template <typename T, bool ALIGNED, bool WIDE_W, bool WIDE_X>
+__global__ void __launch_bounds__(kSkinnyWarps * 32, 2) fp8_skinny_kernel(const SkinnyFp8Args a)
+{
+    __shared__ float part[kSkinnyWarps][16][kSkinny + 1];
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = threadIdx.x >> 5;
+    const long r0 = (long)blockIdx.x * 16;
+    const bool in0 = r0 + g < a.rows, in1 = r0 + g + 8 < a.rows;
+    const signed char *w0 = a.w + (r0 + g) * a.w_stride, *w1 = w0 + 8 * a.w_stride;
+    const float *s0 = a.ws.at + ((min(r0 + g, (long)a.rows - 1)) >> a.ws.shift) * a.ws.row, *s1 = a.ws.at + ((min(r0 + g + 8, (long)a.rows - 1)) >> a.ws.shift) * a.ws.row;
+    const signed char *x0 = a.x + g * a.x_stride;
+    const float *x_s0 = a.xs.at + (long)(min(t * 2, a.cols - 1) >> a.xs.shift) * a.xs.row, *x_s1 = a.xs.at + (long)(min(t * 2 + 1, a.cols - 1) >> a.xs.shift) * a.xs.row;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll(ALIGNED ? 2 : 1)
+    for (int k0 = warp * kK; k0 < a.k; k0 += kSkinnyWarps * kK) { // the warp stays together: mma.sync wants all lanes
+        uint4 u[2], v[2], x[2];
+        const int at = k0 + t * 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u[h] = load16<ALIGNED>(w0 + at + h * 64, in0 ? a.k - at - h * 64 : 0);
+            v[h] = load16<ALIGNED>(w1 + at + h * 64, in1 ? a.k - at - h * 64 : 0);
+            x[h] = load16<ALIGNED>(x0 + at + h * 64, g < a.cols ? a.k - at - h * 64 : 0);
+        }
+        const long p = k0 / kK;
+        const float sw0 = __ldg(s0 + p * a.ws.block), sw1 = __ldg(s1 + p * a.ws.block), sx0 = __ldg(x_s0 + p * a.xs.block), sx1 = __ldg(x_s1 + p * a.xs.block);
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            mma_fp8<WIDE_W, WIDE_X>(c, u[h].x, v[h].x, u[h].y, v[h].y, x[h].x, x[h].y);
+            mma_fp8<WIDE_W, WIDE_X>(c, u[h].z, v[h].z, u[h].w, v[h].w, x[h].z, x[h].w);
+        }
+        acc[0] = fmaf(c[0] * sw0, sx0, acc[0]);
+        acc[1] = fmaf(c[1] * sw0, sx1, acc[1]);
+        acc[2] = fmaf(c[2] * sw1, sx0, acc[2]);
+        acc[3] = fmaf(c[3] * sw1, sx1, acc[3]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[warp][g + (e >> 1) * 8][t * 2 + (e & 1)] = acc[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * kSkinny; i += kSkinnyWarps * 32) {
+        const int r = i & 15, c = i >> 4;
+        if (r0 + r >= a.rows || c >= a.cols) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSkinnyWarps; ++w) sum += part[w][r][c];
+        put(reinterpret_cast<T *>(a.out) + (r0 + r) * a.row_step + c * a.col_step, sum);
+    }
+}
+
+template <typename T, bool ALIGNED, bool WIDE_W, bool WIDE_X> int launch_skinny(const SkinnyFp8Args &a, cudaStream_t stream)
+{
+    const unsigned grid = (unsigned)((a.rows + 15) / 16);
+    fp8_skinny_kernel<T, ALIGNED, WIDE_W, WIDE_X><<<grid, kSkinnyWarps * 32, 0, stream>>>(a);
+    LB_CUDA(cudaGetLastError());
+    return LB_OK;
+}
+template <typename T, bool ALIGNED> int launch_skinny(const SkinnyFp8Args &a, bool wide_w, bool wide_x, cudaStream_t stream)
+{
+    if (wide_w) return wide_x ? launch_skinny<T, ALIGNED, true, true>(a, stream) : launch_skinny<T, ALIGNED, true, false>(a, stream);
+    return wide_x ? launch_skinny<T, ALIGNED, false, true>(a, stream) : launch_skinny<T, ALIGNED, false, false>(a, stream);
+}
+
+// ---- tiles on tcgen05 -------------------------------------------------------------------------------------------------------
 template <int BN> struct TileFp8 {
     static constexpr int kOutWarps = 8, kThreads = 128 + kOutWarps * 32;
     static constexpr int kCols = BN / 2; // columns of a thread: the warps of a quarter of TMEM's lanes take a half each
     static constexpr int kStageBytes = (kM + BN) * kK;
     static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
     static constexpr int kBufs = BN == 256 ? 2 : 4; // block sums in TMEM
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kOutWarps * kCols * 4 + 256;
+    static constexpr int kPitch = BN + 4;           // of a tile's results in shared memory, in floats
+    static constexpr int kRun = kCols / 4 + 4;      // scales of every fourth pair of columns, and a gap that keeps the four runs in different banks
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kOutWarps * kRun * 16 + 256;
 };
 
-struct Scales {
-    const float *at;
-    long row, block; // from one row (or block of 128 rows) to the next; from one block of the summed axis to the next
-    int shift;       // 7: a scale for 128 rows
-};
 struct Fp8Args {
     int m, n, k_blocks;
     int tiles_m, tiles_n, band; // tiles are walked in bands of `band` rows of tiles, so that a wave reads few distinct rows of a and b
@@ -54,19 +151,20 @@ __device__ __forceinline__ void tile_at(const Fp8Args &a, int t, int &tm, int &t
 
 // Threads of the warps that take results out need more registers than an even share, those of the first warpgroup fewer: with 128 results each
 // 56 + 2 x 224 of the 3 x 168 that the block has (launch_tiles sees that it has them: the second call waits for what the first one gives up).
-constexpr int kChunk = 16;
 constexpr int kEven = 168, kFew = 56, kMany = 224;
 
-// PER_ROW: b has a scale for each of its rows, otherwise one for 128
-template <typename T, int BN, bool PER_ROW>
+// PER_ROW: b has a scale for each of its rows, otherwise one for 128.
+// SPLIT: few tiles and a long summed axis.  The blocks of a cluster take a tile together, a run of the axis each, and add up through one another's
+// shared memory, in the order of the runs: no second kernel, no atomics.  333 x 1111 x 2047 takes TIME us with it, 25 us without.
+template <typename T, int BN, bool PER_ROW, bool SPLIT>
 __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                               const Fp8Args a)
 {
     using C = TileFp8<BN>;
     extern __shared__ unsigned char raw[];
     unsigned char *stages = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    float *scales = reinterpret_cast<float *>(stages + C::kStages * C::kStageBytes); // [warp][kCols]
-    unsigned char *tail = reinterpret_cast<unsigned char *>(scales + C::kOutWarps * C::kCols);
+    float *scales = reinterpret_cast<float *>(stages + C::kStages * C::kStageBytes); // [warp][4][kRun]
+    unsigned char *tail = reinterpret_cast<unsigned char *>(scales + C::kOutWarps * 4 * C::kRun);
     unsigned long long *bars = reinterpret_cast<unsigned long long *>(tail); // full[stages], empty[stages], done[bufs], freed[bufs], drained
     unsigned *tmem_at = reinterpret_cast<unsigned *>(bars + 2 * C::kStages + 2 * C::kBufs + 1);
     volatile int *failed = reinterpret_cast<volatile int *>(tmem_at + 1);
@@ -95,7 +193,13 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = *tmem_at;
-    const int tiles = a.tiles_m * a.tiles_n;
+    unsigned rank = 0, ranks = 1;
+    if (SPLIT) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    }
+    const int tiles = SPLIT ? (int)(blockIdx.x / ranks) + 1 : a.tiles_m * a.tiles_n, tile0 = SPLIT ? (int)(blockIdx.x / ranks) : (int)blockIdx.x;
+    const int k0 = SPLIT ? (int)((long)a.k_blocks * rank / ranks) : 0, k1 = SPLIT ? (int)((long)a.k_blocks * (rank + 1) / ranks) : a.k_blocks;
 
     if (warp < 4) {
     if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFew));
@@ -103,10 +207,10 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
         if (lane == 0) {
             int it = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (int t = tile0; t < tiles && ok; t += gridDim.x) {
                 int tm, tn;
                 tile_at(a, t, tm, tn);
-                for (int k = 0; k < a.k_blocks; ++k, ++it) {
+                for (int k = k0; k < k1; ++k, ++it) {
                     const int s = it % C::kStages;
                     if (it >= C::kStages) ok = mbar_wait(empty + 8 * s, (it / C::kStages - 1) & 1, failed);
                     if (!ok) break;
@@ -133,8 +237,8 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
         const unsigned elected = elect_one();
         int it = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-            for (int k = 0; k < a.k_blocks; ++k, ++it) {
+        for (int t = tile0; t < tiles && ok; t += gridDim.x) {
+            for (int k = k0; k < k1; ++k, ++it) {
                 const int s = it % C::kStages, buf = it % C::kBufs;
                 if (it >= C::kBufs) ok = mbar_wait_warp(freed + 8 * buf, (it / C::kBufs - 1) & 1, failed);
                 if (ok) ok = mbar_wait_warp(full + 8 * s, (it / C::kStages) & 1, failed);
@@ -158,21 +262,29 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
     }
     } else {
         if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMany));
-        // a warp sees the 32 lanes of TMEM of its quarter; a thread has a row and half of the tile's columns
+        // A warp sees the 32 lanes of TMEM of its quarter, and takes half of the tile's columns.  With one scale for them a thread has a row; with a
+        // scale each it has, as in the results of a warp's own matrix instruction, two columns of every eight in four rows, so that it
+        // needs a quarter of the scales.
         const int quarter = warp & 3, half = (warp - 4) / 4;
-        float *sb = scales + (warp - 4) * C::kCols;
+        float *sb = scales + (warp - 4) * 4 * C::kRun;
+        constexpr int kRows = PER_ROW ? 4 : 1;
         int it = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (int t = tile0; t < tiles && ok; t += gridDim.x) {
             int tm, tn;
             tile_at(a, t, tm, tn);
-            const int row = tm * kM + quarter * 32 + lane, col = tn * BN + half * C::kCols;
-            const float *pa = a.a.at + (long)(min(row, a.m - 1) >> a.a.shift) * a.a.row;
+            const int row = tm * kM + quarter * 32 + (PER_ROW ? lane >> 2 : lane), col = tn * BN + half * C::kCols;
+            const float *pa[kRows];
+            float sa[kRows], one = 0.f, many[C::kCols / 32];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                pa[r] = a.a.at + (long)(min(row + 8 * r, a.m - 1) >> a.a.shift) * a.a.row + (long)k0 * a.a.block;
+                sa[r] = __ldg(pa[r]);
+            }
             const float *pb = a.b.at + (long)(min(col, a.n - 1) >> a.b.shift) * a.b.row;
             unsigned long long acc[C::kCols / 2];
 #pragma unroll
             for (int e = 0; e < C::kCols / 2; ++e) acc[e] = 0;
-            float sa = __ldg(pa), one = 0.f, many[C::kCols / 32];
             auto fetch_b = [&](int k) { // the scales of block k of b
                 if (PER_ROW) {
 #pragma unroll
@@ -182,19 +294,21 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
                     one = __ldg(pb + (long)k * a.b.block);
                 }
             };
-            fetch_b(0);
-            for (int k = 0; k < a.k_blocks; ++k, ++it) {
+            fetch_b(k0);
+            for (int k = k0; k < k1; ++k, ++it) {
                 const int buf = it % C::kBufs;
-                const float s = PER_ROW ? sa : sa * one;
-                const unsigned long long ss = pair(s, s);
+                unsigned long long ss[kRows];
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) ss[r] = PER_ROW ? pair(sa[r], sa[r]) : pair(sa[r] * one, sa[r] * one);
                 if (PER_ROW) {
                     __syncwarp();
 #pragma unroll
-                    for (int c = 0; c < C::kCols / 32; ++c) sb[c * 32 + lane] = many[c];
+                    for (int c = 0; c < C::kCols / 32; ++c) sb[(lane >> 1 & 3) * C::kRun + (c * 4 + (lane >> 3)) * 2 + (lane & 1)] = many[c];
                     __syncwarp();
                 }
-                if (k + 1 < a.k_blocks) { // those of the next block, on their way while this one is added up
-                    sa = __ldg(pa + (long)(k + 1) * a.a.block);
+                if (k + 1 < k1) { // those of the next block, on their way while this one is added up
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r) sa[r] = __ldg(pa[r] += a.a.block);
                     fetch_b(k + 1);
                 }
                 ok = mbar_wait_inline(done + 8 * buf, (it / C::kBufs) & 1, failed);
@@ -204,23 +318,30 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned from = tmem + buf * BN + half * C::kCols + ((unsigned)quarter << 21);
-                int v[2][kChunk];
-                tmem_begin(from, v[0]);
+                int v[2][16];
+                auto begin = [&](int step, int (&w)[16]) { // 32 columns of 16 rows, the upper ones and then the lower ones; or 16 columns of all rows
+                    if (PER_ROW) tmem_begin_tiles(from + (step >> 1) * 32 + ((unsigned)(step & 1) << 20), w);
+                    else tmem_begin(from + step * 16, w);
+                };
+                begin(0, v[0]);
 #pragma unroll
-                for (int c = 0; c < C::kCols; c += kChunk) {
-                    int(&w)[kChunk] = v[c / kChunk & 1];
+                for (int step = 0; step < C::kCols / 16; ++step) {
+                    int(&w)[16] = v[step & 1];
                     tmem_ready(w);
-                    if (c + kChunk < C::kCols) tmem_begin(from + c + kChunk, v[(c / kChunk & 1) ^ 1]);
+                    if (step + 1 < C::kCols / 16) begin(step + 1, v[(step & 1) ^ 1]);
+                    if (PER_ROW) {
 #pragma unroll
-                    for (int e = 0; e < kChunk; e += 4) {
-                        if (PER_ROW) {
-                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(sb + c + e);
-                            fma2(acc[(c + e) / 2], mul2(pair(w[e], w[e + 1]), ss), s4.x);
-                            fma2(acc[(c + e) / 2 + 1], mul2(pair(w[e + 2], w[e + 3]), ss), s4.y);
-                        } else {
-                            fma2(acc[(c + e) / 2], pair(w[e], w[e + 1]), ss);
-                            fma2(acc[(c + e) / 2 + 1], pair(w[e + 2], w[e + 3]), ss);
+                        for (int i = 0; i < 4; i += 2) { // eight columns, and the next eight
+                            const int eight = (step >> 1) * 4 + i, at = ((step & 1) * (C::kCols / 8) + eight) * 2;
+                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(sb + (lane & 3) * C::kRun + eight * 2);
+                            fma2(acc[at], mul2(pair(w[4 * i], w[4 * i + 1]), ss[(step & 1) * 2]), s4.x);
+                            fma2(acc[at + 1], mul2(pair(w[4 * i + 2], w[4 * i + 3]), ss[kRows > 1 ? (step & 1) * 2 + 1 : 0]), s4.x);
+                            fma2(acc[at + 2], mul2(pair(w[4 * i + 4], w[4 * i + 5]), ss[kRows > 1 ? (step & 1) * 2 : 0]), s4.y);
+                            fma2(acc[at + 3], mul2(pair(w[4 * i + 6], w[4 * i + 7]), ss[kRows > 1 ? (step & 1) * 2 + 1 : 0]), s4.y);
                         }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) fma2(acc[step * 8 + e / 2], pair(w[e], w[e + 1]), ss[0]);
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -228,7 +349,34 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
                 if (lane == 0) mbar_arrive(freed + 8 * buf);
             }
             if (!ok) break;
-            if (row < a.m) {
+            if (SPLIT) { // all products have been formed, so the stages are free
+                float *to = reinterpret_cast<float *>(stages) + (quarter * 32 + (PER_ROW ? lane >> 2 : lane)) * C::kPitch + half * C::kCols + (PER_ROW ? (lane & 3) * 2 : 0);
+#pragma unroll
+                for (int e = 0; e < C::kCols / 2; ++e) {
+                    float2 x;
+                    unpair(acc[e], x.x, x.y);
+                    *reinterpret_cast<float2 *>(PER_ROW ? to + ((e & 1) * 8 + e / (C::kCols / 4) * 16) * C::kPitch + (e % (C::kCols / 4) >> 1) * 8 : to + 2 * e) = x;
+                }
+            } else if (PER_ROW) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (row + 8 * r >= a.m) continue;
+                    T *out = reinterpret_cast<T *>(a.out) + (long)(row + 8 * r) * a.out_stride + col + (lane & 3) * 2;
+#pragma unroll
+                    for (int i = 0; i < C::kCols / 8; ++i) {
+                        float x, y;
+                        unpair(acc[((r >> 1) * (C::kCols / 8) + i) * 2 + (r & 1)], x, y);
+                        const int left = a.n - col - (lane & 3) * 2 - i * 8;
+                        if (left >= 2 && a.align) {
+                            if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(out + i * 8) = make_float2(x, y);
+                            else *reinterpret_cast<unsigned *>(out + i * 8) = pack2(out, x, y);
+                        } else {
+                            if (left >= 1) put(out + i * 8, x);
+                            if (left >= 2) put(out + i * 8 + 1, y);
+                        }
+                    }
+                }
+            } else if (row < a.m) {
                 T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride + col;
 #pragma unroll
                 for (int c = 0; c < C::kCols; c += 32) {
@@ -240,6 +388,37 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
             }
         }
     }
+    if (SPLIT) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        int tm, tn;
+        tile_at(a, tile0, tm, tn);
+        const int rows = min(kM, a.m - tm * kM), cols = min(BN, a.n - tn * BN), all = rows * (BN / 4);
+        for (int i = (int)((long)all * rank / ranks) + (int)threadIdx.x; i < (int)((long)all * (rank + 1) / ranks); i += C::kThreads) {
+            const int r = i / (BN / 4), c = i % (BN / 4) * 4;
+            if (c >= cols) continue;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (unsigned from = 0; from < ranks; ++from) {
+                unsigned at;
+                float4 v;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(stage0 + (r * C::kPitch + c) * 4), "r"(from));
+                asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+                sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+            }
+            T *out = reinterpret_cast<T *>(a.out) + (long)(tm * kM + r) * a.out_stride + tn * BN + c;
+            if (a.align && c + 4 <= cols) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out) = sum;
+                else *reinterpret_cast<uint2 *>(out) = make_uint2(pack2(out, sum.x, sum.y), pack2(out, sum.z, sum.w));
+            } else {
+                put(out, sum.x);
+                if (c + 1 < cols) put(out + 1, sum.y);
+                if (c + 2 < cols) put(out + 2, sum.z);
+                if (c + 3 < cols) put(out + 3, sum.w);
+            }
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); // nobody leaves while it is read
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -247,15 +426,17 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kBufs * BN) : "memory");
 }
 
-template <typename T, int BN, bool PER_ROW> int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const Fp8Args &a, cudaStream_t stream)
+template <typename T, int BN, bool PER_ROW, bool SPLIT>
+int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const Fp8Args &a, int split, cudaStream_t stream)
 {
     using C = TileFp8<BN>;
+    const auto kernel = fp8_product_kernel<T, BN, PER_ROW, SPLIT>;
     static std::atomic<bool> set[64]; // host threads that come here first at once all set the same attribute
     if (ctx->device >= 64 || !set[ctx->device]) {
-        LB_CUDA(cudaFuncSetAttribute(fp8_product_kernel<T, BN, PER_ROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        LB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
         if (BN == 256) {
             cudaFuncAttributes has;
-            LB_CUDA(cudaFuncGetAttributes(&has, fp8_product_kernel<T, BN, PER_ROW>));
+            LB_CUDA(cudaFuncGetAttributes(&has, kernel));
             if (has.numRegs < kEven) {
                 set_error("the product's kernel was built with too few registers");
                 return LB_ERR_LOGIC;
@@ -264,9 +445,25 @@ template <typename T, int BN, bool PER_ROW> int launch_tiles(const Context *ctx,
         if (ctx->device < 64) set[ctx->device] = true;
     }
     const int tiles = a.tiles_m * a.tiles_n;
-    fp8_product_kernel<T, BN, PER_ROW><<<tiles < ctx->sm_count ? tiles : ctx->sm_count, C::kThreads, C::kSmem, stream>>>(ma, mb, a);
-    LB_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)(SPLIT ? tiles * split : tiles < ctx->sm_count ? tiles : ctx->sm_count));
+    c.blockDim = dim3(C::kThreads);
+    c.dynamicSmemBytes = C::kSmem;
+    c.stream = stream;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = (unsigned)split;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    c.attrs = &cluster;
+    c.numAttrs = SPLIT ? 1 : 0;
+    LB_CUDA(cudaLaunchKernelEx(&c, kernel, ma, mb, a));
     return LB_OK;
+}
+template <typename T, bool PER_ROW> int launch_any(const Context *ctx, int bn, const CUtensorMap &ma, const CUtensorMap &mb, const Fp8Args &a, int split, cudaStream_t stream)
+{
+    if (split > 1) return bn == 128 ? launch_tiles<T, 128, PER_ROW, true>(ctx, ma, mb, a, split, stream) : launch_tiles<T, 64, PER_ROW, true>(ctx, ma, mb, a, split, stream);
+    if (bn == 256) return launch_tiles<T, 256, PER_ROW, false>(ctx, ma, mb, a, 1, stream);
+    return bn == 128 ? launch_tiles<T, 128, PER_ROW, false>(ctx, ma, mb, a, 1, stream) : launch_tiles<T, 64, PER_ROW, false>(ctx, ma, mb, a, 1, stream);
 }
 
 // an operand as it lies: rows of `cols` bytes
@@ -287,8 +484,30 @@ Stored stored(const Fp8Operand &o, int along, int k)
 }
 size_t packed_bytes(const Stored &s) { return s.off ? ((size_t)s.rows * s.pitch + 255) / 256 * 256 : 0; }
 
+bool skinny(int m, int n, const Fp8Operand &a, const Fp8Operand &b) { return !a.across && !b.across && (m <= kSkinny || n <= kSkinny); }
+
 template <typename T> int product_typed(Context *ctx, int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b, void *out, long out_stride, cudaStream_t stream)
 {
+    if (skinny(m, n, a, b)) {
+        const bool turned = m > n; // the long side is the rows of a
+        const Fp8Operand &w = turned ? a : b, &x = turned ? b : a;
+        SkinnyFp8Args s;
+        s.w = reinterpret_cast<const signed char *>(w.codes);
+        s.x = reinterpret_cast<const signed char *>(x.codes);
+        s.w_stride = w.stride;
+        s.x_stride = x.stride;
+        s.ws = {w.scales, w.scale_row, w.scale_block, w.scale_shift};
+        s.xs = {x.scales, x.scale_row, x.scale_block, x.scale_shift};
+        s.rows = turned ? m : n;
+        s.cols = turned ? n : m;
+        s.k = k;
+        s.out = out;
+        s.row_step = turned ? out_stride : 1;
+        s.col_step = turned ? 1 : out_stride;
+        count_launch("fp8_skinny", stream, (double)m * k + (double)n * k + (double)m * n * sizeof(T));
+        const bool off = k % 16 != 0 || stored(a, m, k).off || stored(b, n, k).off;
+        return off ? launch_skinny<T, false>(s, w.type == 6, x.type == 6, stream) : launch_skinny<T, true>(s, w.type == 6, x.type == 6, stream);
+    }
     Fp8Args p;
     p.m = m;
     p.n = n;
@@ -304,16 +523,24 @@ template <typename T> int product_typed(Context *ctx, int m, int n, int k, const
     p.align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
     p.status = ctx->d_status;
     p.band = 8;
-    int bn = 128;
+    // The tile, and the blocks that share one, that take least: waves over the SMs, a block of the summed axis at what its bytes take from L2 to the SM
+    // (and, with a scale per row of b, its results to be scaled), a tile about a microsecond and the time of its results beside that, a
+    // split two more.
+    int bn = 128, split = 1;
     double least = 0.0;
-    for (int w = b.across ? 128 : 64; w <= 256; w *= 2) {
-        const long tiles = (long)p.tiles_m * ((n + w - 1) / w), waves = (tiles + ctx->sm_count - 1) / ctx->sm_count;
-        const double us = (double)waves * ((double)p.k_blocks * (128 + w) * 1.15e-3 + 0.7 + w * 6e-3);
-        if (least == 0.0 || us < least) {
-            least = us;
-            bn = w;
+    const bool per_row = b.scale_shift == 0;
+    for (int w = b.across ? 128 : 64; w <= 256; w *= 2)
+        for (int parts = 1; parts <= 8 && parts <= p.k_blocks; ++parts) {
+            const long tiles = (long)p.tiles_m * ((n + w - 1) / w), blocks = tiles * parts, waves = (blocks + ctx->sm_count - 1) / ctx->sm_count;
+            if (parts > 1 && (w == 256 || blocks > ctx->sm_count - ctx->sm_count / 8)) break; // clusters do not fill every group of SMs
+            const int k = (p.k_blocks + parts - 1) / parts;
+            const double us = (double)waves * ((double)k * (128 + w) * (per_row ? 2.3e-3 : 1.15e-3) + 0.7 + w * 6e-3) + (parts > 1 ? 2.0 : 0.0);
+            if (least == 0.0 || us < least) {
+                least = us;
+                bn = w;
+                split = parts;
+            }
         }
-    }
     p.tiles_n = (n + bn - 1) / bn;
     // D 32-bit floats; the operands' types, and bits 15 and 16 where the summed axis lies across their rows
     p.desc = (unsigned)(bn >> 3) << 17 | (unsigned)(kM >> 4) << 24 | 1u << 4 | (unsigned)(a.type == 6) << 7 | (unsigned)(b.type == 6) << 10 | (unsigned)a.across << 15 |
@@ -324,26 +551,23 @@ template <typename T> int product_typed(Context *ctx, int m, int n, int k, const
     if (rc) return rc;
     if ((rc = encode_map(&mb, b.codes, sb.rows, sb.cols, sb.rows > 1 ? b.stride : sb.pitch, 128, b.across ? 128 : bn))) return rc;
     count_launch("fp8_tiles", stream, (double)m * k + (double)n * k + (double)m * n * sizeof(T));
-    const bool per_row = b.scale_shift == 0;
-    if (bn == 256) return per_row ? launch_tiles<T, 256, true>(ctx, ma, mb, p, stream) : launch_tiles<T, 256, false>(ctx, ma, mb, p, stream);
-    if (bn == 128) return per_row ? launch_tiles<T, 128, true>(ctx, ma, mb, p, stream) : launch_tiles<T, 128, false>(ctx, ma, mb, p, stream);
-    return per_row ? launch_tiles<T, 64, true>(ctx, ma, mb, p, stream) : launch_tiles<T, 64, false>(ctx, ma, mb, p, stream);
+    return per_row ? launch_any<T, true>(ctx, bn, ma, mb, p, split, stream) : launch_any<T, false>(ctx, bn, ma, mb, p, split, stream);
 }
 
 } // namespace
 
 size_t fp8_matmul_workspace_bytes(int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b)
 {
-    return packed_bytes(stored(a, m, k)) + packed_bytes(stored(b, n, k));
+    return skinny(m, n, a, b) ? 0 : packed_bytes(stored(a, m, k)) + packed_bytes(stored(b, n, k));
 }
 
 int fp8_matmul(Context *ctx, int m, int n, int k, Fp8Operand a, Fp8Operand b, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream)
 {
     signed char *ws = reinterpret_cast<signed char *>(workspace);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i) { // operands that TMA cannot read
         Fp8Operand &o = i ? b : a;
         const Stored s = stored(o, i ? n : m, k);
-        if (!s.off) continue;
+        if (!s.off || skinny(m, n, a, b)) continue;
         const Packed one = {reinterpret_cast<const signed char *>(o.codes), o.stride, s.rows, ws}, none = {nullptr, 0, 0, nullptr};
         int log_lanes = 0;
         while (log_lanes < 8 && 16 << log_lanes < s.pitch) ++log_lanes;
