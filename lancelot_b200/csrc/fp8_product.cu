@@ -125,8 +125,11 @@ template <int BN> struct TileFp8 {
     static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
     static constexpr int kBufs = BN == 256 ? 2 : 4; // block sums in TMEM
     static constexpr int kPitch = BN + 4;           // of a tile's results in shared memory, in floats
+    static constexpr int kScaleStages = 8;          // blocks of the summed axis whose scales are on their way
     static constexpr int kRun = kCols / 4 + 4;      // scales of every fourth pair of columns, and a gap that keeps the four runs in different banks
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kOutWarps * kRun * 16 + 256;
+    static constexpr int kScaleFloats = kM + 8 * kRun; // of a stage: of the rows; of the columns of each half
+    static constexpr int kBars = 2 * kStages + 2 * kBufs + 2 * kScaleStages + 1;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleStages * kScaleFloats * 4 + 8 * kBars + 16;
 };
 
 struct Fp8Args {
@@ -153,6 +156,8 @@ __device__ __forceinline__ void tile_at(const Fp8Args &a, int t, int &tm, int &t
 // 56 + 2 x 224 of the 3 x 168 that the block has (launch_tiles sees that it has them: the second call waits for what the first one gives up).
 constexpr int kEven = 168, kFew = 56, kMany = 224;
 
+__device__ __forceinline__ void copy4(unsigned to, const float *from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory"); }
+
 // PER_ROW: b has a scale for each of its rows, otherwise one for 128.
 // SPLIT: few tiles and a long summed axis.  The blocks of a cluster take a tile together, a run of the axis each, and add up through one another's
 // shared memory, in the order of the runs: no second kernel, no atomics.  333 x 1111 x 2047 takes TIME us with it, 25 us without.
@@ -163,13 +168,14 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
     using C = TileFp8<BN>;
     extern __shared__ unsigned char raw[];
     unsigned char *stages = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    float *scales = reinterpret_cast<float *>(stages + C::kStages * C::kStageBytes); // [warp][4][kRun]
-    unsigned char *tail = reinterpret_cast<unsigned char *>(scales + C::kOutWarps * 4 * C::kRun);
-    unsigned long long *bars = reinterpret_cast<unsigned long long *>(tail); // full[stages], empty[stages], done[bufs], freed[bufs], drained
-    unsigned *tmem_at = reinterpret_cast<unsigned *>(bars + 2 * C::kStages + 2 * C::kBufs + 1);
+    float *scales = reinterpret_cast<float *>(stages + C::kStages * C::kStageBytes); // [scale stage][kScaleFloats]
+    unsigned long long *bars = reinterpret_cast<unsigned long long *>(scales + C::kScaleStages * C::kScaleFloats);
+    unsigned *tmem_at = reinterpret_cast<unsigned *>(bars + C::kBars);
     volatile int *failed = reinterpret_cast<volatile int *>(tmem_at + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned full = smem_u32(bars), empty = full + 8 * C::kStages, done = empty + 8 * C::kStages, freed = done + 8 * C::kBufs, drained = freed + 8 * C::kBufs;
+    // stages of the operands, block sums in TMEM, stages of the scales: filled, and free again
+    const unsigned full = smem_u32(bars), empty = full + 8 * C::kStages, done = empty + 8 * C::kStages, freed = done + 8 * C::kBufs, known = freed + 8 * C::kBufs,
+                   used = known + 8 * C::kScaleStages, drained = used + 8 * C::kScaleStages;
     const unsigned stage0 = smem_u32(stages);
 
     if (threadIdx.x == 0) {
@@ -180,6 +186,10 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
         for (int i = 0; i < C::kBufs; ++i) {
             mbar_init(done + 8 * i, 1);
             mbar_init(freed + 8 * i, C::kOutWarps);
+        }
+        for (int i = 0; i < C::kScaleStages; ++i) {
+            mbar_init(known + 8 * i, 64);
+            mbar_init(used + 8 * i, C::kOutWarps);
         }
         mbar_init(drained, 1);
         *failed = 0;
@@ -259,6 +269,46 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
             for (int n = 0; n < 1 << 20; ++n)
                 if (mbar_try(drained, 0)) break;
         }
+    } else if (PER_ROW) { // the scales, blocks ahead of their use: of the rows, and of the columns
+        int it = 0;
+        bool ok = true;
+        for (int t = tile0; t < tiles && ok; t += gridDim.x) {
+            int tm, tn;
+            tile_at(a, t, tm, tn);
+            constexpr int kMine = BN / 32;
+            const float *from[kMine > 4 ? kMine : 4];
+            unsigned to[kMine > 4 ? kMine : 4];
+            const long step = warp == 2 ? a.a.block : a.b.block;
+            if (warp == 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    from[i] = a.a.at + (long)(min(tm * kM + i * 32 + lane, a.m - 1) >> a.a.shift) * a.a.row + k0 * step;
+                    to[i] = i * 32 + lane;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    const int c = i * 32 + lane, in = c % C::kCols; // of each half of the columns four runs of every fourth pair
+                    from[i] = a.b.at + (long)(min(tn * BN + c, a.n - 1) >> a.b.shift) * a.b.row + k0 * step;
+                    to[i] = kM + c / C::kCols * 4 * C::kRun + (in >> 1 & 3) * C::kRun + (in >> 3) * 2 + (in & 1);
+                }
+            }
+            for (int k = k0; k < k1; ++k, ++it) {
+                const int s = it % C::kScaleStages;
+                if (it >= C::kScaleStages) ok = mbar_wait_warp(used + 8 * s, (it / C::kScaleStages - 1) & 1, failed);
+                if (!ok) break;
+                const unsigned at = smem_u32(scales + s * C::kScaleFloats);
+                if (warp == 2) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) copy4(at + 4 * to[i], from[i]), from[i] += step;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kMine; ++i) copy4(at + 4 * to[i], from[i]), from[i] += step;
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(known + 8 * s) : "memory");
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
     } else {
         if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMany));
@@ -266,7 +316,6 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
         // scale each it has, as in the results of a warp's own matrix instruction, two columns of every eight in four rows, so that it
         // needs a quarter of the scales.
         const int quarter = warp & 3, half = (warp - 4) / 4;
-        float *sb = scales + (warp - 4) * 4 * C::kRun;
         constexpr int kRows = PER_ROW ? 4 : 1;
         int it = 0;
         bool ok = true;
@@ -274,80 +323,64 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
             int tm, tn;
             tile_at(a, t, tm, tn);
             const int row = tm * kM + quarter * 32 + (PER_ROW ? lane >> 2 : lane), col = tn * BN + half * C::kCols;
-            const float *pa[kRows];
-            float sa[kRows], one = 0.f, many[C::kCols / 32];
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                pa[r] = a.a.at + (long)(min(row + 8 * r, a.m - 1) >> a.a.shift) * a.a.row + (long)k0 * a.a.block;
-                sa[r] = __ldg(pa[r]);
-            }
-            const float *pb = a.b.at + (long)(min(col, a.n - 1) >> a.b.shift) * a.b.row;
             unsigned long long acc[C::kCols / 2];
 #pragma unroll
             for (int e = 0; e < C::kCols / 2; ++e) acc[e] = 0;
-            auto fetch_b = [&](int k) { // the scales of block k of b
-                if (PER_ROW) {
-#pragma unroll
-                    for (int c = 0; c < C::kCols / 32; ++c)
-                        many[c] = __ldg(a.b.at + (long)min(col + c * 32 + lane, a.n - 1) * a.b.row + (long)k * a.b.block);
-                } else {
-                    one = __ldg(pb + (long)k * a.b.block);
-                }
-            };
-            fetch_b(k0);
+            // One scale for the columns: every thread fetches the two that it needs, a block ahead.  A scale each: two warps bring them into shared memory
+            const float *pa = a.a.at + (long)(min(row, a.m - 1) >> a.a.shift) * a.a.row + k0 * a.a.block, *pb = a.b.at + (long)(min(col, a.n - 1) >> a.b.shift) * a.b.row + k0 * a.b.block;
+            float next_row = 0.f, next_col = 0.f;
+            if (!PER_ROW && k0 < k1) next_row = __ldg(pa), next_col = __ldg(pb);
             for (int k = k0; k < k1; ++k, ++it) {
-                const int buf = it % C::kBufs;
+                const int buf = it % C::kBufs, stage = it % C::kScaleStages;
+                const float *row_scales = scales + stage * C::kScaleFloats + quarter * 32 + (lane >> 2);
+                const float *col_scales = scales + stage * C::kScaleFloats + kM + half * 4 * C::kRun + (lane & 3) * C::kRun;
                 unsigned long long ss[kRows];
-#pragma unroll
-                for (int r = 0; r < kRows; ++r) ss[r] = PER_ROW ? pair(sa[r], sa[r]) : pair(sa[r] * one, sa[r] * one);
                 if (PER_ROW) {
-                    __syncwarp();
+                    ok &= mbar_wait_inline(known + 8 * stage, (it / C::kScaleStages) & 1, failed);
 #pragma unroll
-                    for (int c = 0; c < C::kCols / 32; ++c) sb[(lane >> 1 & 3) * C::kRun + (c * 4 + (lane >> 3)) * 2 + (lane & 1)] = many[c];
-                    __syncwarp();
+                    for (int r = 0; r < kRows; ++r) ss[r] = pair(row_scales[8 * r], row_scales[8 * r]);
+                } else {
+                    ss[0] = pair(next_row * next_col, next_row * next_col);
+                    if (k + 1 < k1) next_row = __ldg(pa += a.a.block), next_col = __ldg(pb += a.b.block);
                 }
-                if (k + 1 < k1) { // those of the next block, on their way while this one is added up
-#pragma unroll
-                    for (int r = 0; r < kRows; ++r) sa[r] = __ldg(pa[r] += a.a.block);
-                    fetch_b(k + 1);
-                }
-                ok = mbar_wait_inline(done + 8 * buf, (it / C::kBufs) & 1, failed);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
+                ok &= mbar_wait_inline(done + 8 * buf, (it / C::kBufs) & 1, failed); // a warp whose wait ran out goes on, together, to the tile's end
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned from = tmem + buf * BN + half * C::kCols + ((unsigned)quarter << 21);
-                int v[2][16];
-                auto begin = [&](int step, int (&w)[16]) { // 32 columns of 16 rows, the upper ones and then the lower ones; or 16 columns of all rows
-                    if (PER_ROW) tmem_begin_tiles(from + (step >> 1) * 32 + ((unsigned)(step & 1) << 20), w);
-                    else tmem_begin(from + step * 16, w);
+                constexpr int kW = PER_ROW ? 16 : 32;
+                int v[2][kW];
+                auto begin = [&](int step, int (&w)[kW]) { // 32 columns of 16 rows, the upper ones and then the lower ones; or 16 columns of all rows
+                    if constexpr (PER_ROW) tmem_begin_tiles(from + (step >> 1) * 32 + ((unsigned)(step & 1) << 20), w);
+                    else tmem_begin(from + step * 32, w);
                 };
                 begin(0, v[0]);
 #pragma unroll
-                for (int step = 0; step < C::kCols / 16; ++step) {
-                    int(&w)[16] = v[step & 1];
+                for (int step = 0; step < C::kCols / kW; ++step) {
+                    int(&w)[kW] = v[step & 1];
                     tmem_ready(w);
-                    if (step + 1 < C::kCols / 16) begin(step + 1, v[(step & 1) ^ 1]);
-                    if (PER_ROW) {
+                    if (step + 1 < C::kCols / kW) begin(step + 1, v[(step & 1) ^ 1]);
+                    if constexpr (PER_ROW) {
 #pragma unroll
                         for (int i = 0; i < 4; i += 2) { // eight columns, and the next eight
-                            const int eight = (step >> 1) * 4 + i, at = ((step & 1) * (C::kCols / 8) + eight) * 2;
-                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(sb + (lane & 3) * C::kRun + eight * 2);
-                            fma2(acc[at], mul2(pair(w[4 * i], w[4 * i + 1]), ss[(step & 1) * 2]), s4.x);
-                            fma2(acc[at + 1], mul2(pair(w[4 * i + 2], w[4 * i + 3]), ss[kRows > 1 ? (step & 1) * 2 + 1 : 0]), s4.x);
-                            fma2(acc[at + 2], mul2(pair(w[4 * i + 4], w[4 * i + 5]), ss[kRows > 1 ? (step & 1) * 2 : 0]), s4.y);
-                            fma2(acc[at + 3], mul2(pair(w[4 * i + 6], w[4 * i + 7]), ss[kRows > 1 ? (step & 1) * 2 + 1 : 0]), s4.y);
+                            const int eight = (step >> 1) * 4 + i, at = ((step & 1) * (C::kCols / 8) + eight) * 2, r = (step & 1) * 2;
+                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(col_scales + eight * 2);
+                            fma2(acc[at], mul2(pair(w[4 * i], w[4 * i + 1]), ss[r]), s4.x);
+                            fma2(acc[at + 1], mul2(pair(w[4 * i + 2], w[4 * i + 3]), ss[r + 1]), s4.x);
+                            fma2(acc[at + 2], mul2(pair(w[4 * i + 4], w[4 * i + 5]), ss[r]), s4.y);
+                            fma2(acc[at + 3], mul2(pair(w[4 * i + 6], w[4 * i + 7]), ss[r + 1]), s4.y);
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) fma2(acc[step * 8 + e / 2], pair(w[e], w[e + 1]), ss[0]);
+                        for (int e = 0; e < kW; e += 2) fma2(acc[step * kW / 2 + e / 2], pair(w[e], w[e + 1]), ss[0]);
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(freed + 8 * buf);
+                if (lane == 0) {
+                    mbar_arrive(freed + 8 * buf);
+                    if (PER_ROW) mbar_arrive(used + 8 * stage);
+                }
             }
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             if (SPLIT) { // all products have been formed, so the stages are free
                 float *to = reinterpret_cast<float *>(stages) + (quarter * 32 + (PER_ROW ? lane >> 2 : lane)) * C::kPitch + half * C::kCols + (PER_ROW ? (lane & 3) * 2 : 0);

@@ -282,6 +282,88 @@ Tensor fp8_matmul(int64_t context, int device, const Tensor &a, const Tensor &a_
     return to;
 }
 
+// ---- a layer's training step: y = x w^T and the gradients of x and w, a call each ---------------------------------------------------
+// t [..., k] as a matrix whose rows are dense and apart: not so are transposed ones, and the gradient of a sum, one value for all
+Tensor matrix(const Tensor &t)
+{
+    const int64_t k = t.size(-1), rows = k ? t.numel() / k : t.sizes().size() < 2 ? 1 : c10::multiply_integers(t.sizes().slice(0, t.dim() - 1));
+    const Tensor m = t.dim() == 2 ? t : t.reshape({rows, k});
+    return m.stride(1) == 1 && (rows < 2 || m.stride(0) >= k) ? m : m.contiguous();
+}
+struct Coded {
+    Tensor codes, scales, down, down_scales;
+};
+Coded coded(const Call &c, const Tensor &m, int blocks, int type)
+{
+    Maybe codes, scales, down, down_scales;
+    const int64_t n = m.size(0), cols = m.size(1);
+    c.tensor(m, 2, "an operand");
+    const int dtype = value_type(m.scalar_type());
+    if (!dtype) refuse("an operand must be float32, bfloat16 or float16");
+    if (blocks != 2) blocks_into(c, codes, scales, n, cols, blocks == 4 ? blocks_of(n) : n, blocks_of(cols), type);
+    if (blocks == 2 || blocks == 3) blocks_into(c, down, down_scales, n, cols, blocks_of(n), cols, type);
+    auto stride = [](const Maybe &t) { return t ? row_stride(*t) : 0; };
+    check(lb_quantize_fp8(c.context, address<void>(m), dtype, n, cols, row_stride(m), blocks, type, address<uint8_t>(codes), stride(codes),
+                          address<float>(scales), stride(scales), address<uint8_t>(down), stride(down), address<float>(down_scales),
+                          stride(down_scales), c.stream()));
+    return {codes.value_or(Tensor()), scales.value_or(Tensor()), down.value_or(Tensor()), down_scales.value_or(Tensor())};
+}
+// codes and their scales as they lie, or both with their axes exchanged
+lb_fp8_operand stored_operand(const Tensor &codes, const Tensor &scales, bool across, int scale_rows, int type)
+{
+    lb_fp8_operand o = {};
+    o.codes = address<uint8_t>(codes);
+    o.stride = row_stride(codes);
+    o.across = across;
+    o.code_type = type;
+    o.scales = address<float>(scales);
+    o.scale_row = across ? 1 : row_stride(scales);
+    o.scale_block = across ? row_stride(scales) : 1;
+    o.scale_rows = scale_rows;
+    return o;
+}
+Tensor product(const Call &c, int64_t m, int64_t n, int64_t k, const lb_fp8_operand &x, const lb_fp8_operand &y, at::IntArrayRef shape, at::ScalarType type)
+{
+    const Tensor to = c.empty(shape, type);
+    const size_t need = lb_fp8_matmul_workspace_bytes(m, n, k, &x, &y);
+    const Tensor ws = c.workspace(need);
+    check(lb_fp8_matmul(c.context, m, n, k, &x, &y, address<void>(to), value_type(type), n, address<void>(ws), need, c.stream()));
+    return to;
+}
+
+// y, and what the gradients need: x in blocks along its rows' axis (for that of w), w's codes (for that of x)
+py::tuple fp8_linear_forward(int64_t context, int device, const Tensor &x, const Tensor &w, bool need_x, bool need_w)
+{
+    const Call c = call_of(context, device);
+    const Tensor xm = matrix(x), wm = matrix(w);
+    const Coded xc = coded(c, xm, need_w ? 3 : 1, 5), wc = coded(c, wm, 4, 5);
+    const int64_t m = xm.size(0), n = wm.size(0), k = xm.size(1);
+    at::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = n;
+    const Tensor y = product(c, m, n, k, stored_operand(xc.codes, xc.scales, false, 1, 5), stored_operand(wc.codes, wc.scales, false, 128, 5), shape, x.scalar_type());
+    auto kept = [](const Tensor &t, bool keep) { return keep ? py::cast(t) : py::none(); };
+    return py::make_tuple(y, kept(xc.down, need_w), kept(xc.down_scales, need_w), kept(wc.codes, need_x), kept(wc.scales, need_x));
+}
+py::tuple fp8_linear_backward(int64_t context, int device, const Tensor &g, const Maybe &xd, const Maybe &xds, const Maybe &w8, const Maybe &ws, int type,
+                              int x_dtype, int w_dtype)
+{
+    const Call c = call_of(context, device);
+    if (type != 5 && type != 6) refuse("dtype must be float8_e4m3fn or float8_e5m2");
+    const Tensor gm = matrix(g);
+    const Coded gc = coded(c, gm, w8 ? (xd ? 3 : 1) : 2, type);
+    const int64_t m = gm.size(0), n = gm.size(1);
+    py::object dx = py::none(), dw = py::none();
+    if (w8) {
+        at::DimVector shape(g.sizes().begin(), g.sizes().end());
+        shape.back() = w8->size(1);
+        dx = py::cast(product(c, m, w8->size(1), n, stored_operand(gc.codes, gc.scales, false, 1, type), stored_operand(*w8, *ws, true, 128, 5), shape, scalar_type(x_dtype)));
+    }
+    if (xd)
+        dw = py::cast(product(c, n, xd->size(1), m, stored_operand(gc.down, gc.down_scales, true, 1, type), stored_operand(*xd, *xds, true, 1, 5), {n, xd->size(1)},
+                              scalar_type(w_dtype)));
+    return py::make_tuple(dx, dw);
+}
+
 // ---- clipping -------------------------------------------------------------------------------------------------------------------
 Tensor clip_updates(int64_t context, int device, const py::object &updates, std::optional<double> max_norm, const Maybe &out)
 {
@@ -382,4 +464,6 @@ PYBIND11_MODULE(_updates8, m)
     m.def("dequantize_fp8", &dequantize_fp8);
     m.def("fp8_matmul", &fp8_matmul);
     m.def("clip_updates", &clip_updates);
+    m.def("fp8_linear_forward", &fp8_linear_forward);
+    m.def("fp8_linear_backward", &fp8_linear_backward);
 }

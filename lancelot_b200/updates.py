@@ -111,45 +111,18 @@ def low_rank_update(lb, factors, out=None):
     return out
 
 
-def _matrix(t):
-    """t [..., k] as a matrix whose rows are dense and apart: not so are transposed ones, and the gradient of a sum, one value for all"""
-    rows = t.reshape(t.shape[:-1].numel(), t.shape[-1])
-    return rows if rows.stride(1) == 1 and (rows.shape[0] < 2 or rows.stride(0) >= rows.shape[1]) else rows.contiguous()
-
-
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, lb, x, w, grad_dtype):
-        need_x, need_w = ctx.needs_input_grad[1:3]
-        rows = _matrix(x)
-        if need_w:
-            x8, xs, xd, xds = lb.quantize_fp8_both(rows)
-        else:
-            (x8, xs), xd, xds = lb.quantize_fp8(rows), None, None
-        w8, ws = lb.quantize_fp8(_matrix(w), (128, 128))
-        ctx.lb, ctx.grad_dtype, ctx.dtypes = lb, grad_dtype, (x.dtype, w.dtype)
-        ctx.save_for_backward(xd, xds, *((w8, ws) if need_x else (None, None)))
-        return lb.fp8_matmul(x8, xs, w8, ws, dtype=x.dtype).view(*x.shape[:-1], w.shape[0])
+        y, *kept = lb.fp8_linear_forward(x, w, *ctx.needs_input_grad[1:3])
+        ctx.lb, ctx.types = lb, (grad_dtype, x.dtype, w.dtype)
+        ctx.save_for_backward(*kept)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        lb = ctx.lb
-        xd, xds, w8, ws = ctx.saved_tensors
-        need_x, need_w = ctx.needs_input_grad[1:3]
-        rows = _matrix(g)
-        dx = dw = None
-        if need_x and need_w:
-            g8, gs, gd, gds = lb.quantize_fp8_both(rows, dtype=ctx.grad_dtype)
-        elif need_x:
-            g8, gs = lb.quantize_fp8(rows, dtype=ctx.grad_dtype)
-        else:
-            gd, gds = lb.quantize_fp8(rows, (128, 1), dtype=ctx.grad_dtype)
-        if need_x:
-            dx = lb.fp8_matmul(g8, gs, w8.t(), ws.t(), dtype=ctx.dtypes[0]).view(*g.shape[:-1], w8.shape[1])
-        if need_w:
-            dw = lb.fp8_matmul(gd.t(), gds.t(), xd.t(), xds.t(), dtype=ctx.dtypes[1])
-        return None, dx, dw, None
+        return None, *ctx.lb.fp8_linear_backward(g, *ctx.saved_tensors, *ctx.types), None
 
 
 def fp8_linear(lb, x, w, grad_dtype=torch.float8_e4m3fn):
