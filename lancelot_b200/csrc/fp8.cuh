@@ -105,14 +105,14 @@ __device__ __forceinline__ float inverse_of(float s) { return s >= kTinyScale ? 
 // whether a block's codes cannot be had with that
 __device__ __forceinline__ bool odd_scale(float s) { return !(s >= kTinyScale) && s != 0.f; }
 
-// The codes of four magnitudes (bits), of one scale or of a scale each (s), with the factors to their quotients (f).  odd: whether one of the scales is
-template <bool E5M2> __device__ __forceinline__ unsigned codes4(const uint4 &m, const float4 &s, const float4 &f, bool odd)
+// The codes of four magnitudes (bits), of one scale or of a scale each (s), with the factors to their quotients (f).  ODD: one of the scales may be
+template <bool E5M2, bool ODD> __device__ __forceinline__ unsigned codes4(const uint4 &m, const float4 &s, const float4 &f)
 {
     const float a = __uint_as_float(m.x), b = __uint_as_float(m.y), c = __uint_as_float(m.z), d = __uint_as_float(m.w);
     float q0, q1, q2, q3;
     unpair(beside_border<E5M2>(pair(a, b), pair(s.x, s.y), pair(f.x, f.y)), q0, q1);
     unpair(beside_border<E5M2>(pair(c, d), pair(s.z, s.w), pair(f.z, f.w)), q2, q3);
-    if (odd) {
+    if constexpr (ODD) {
         if (!(s.x >= kTinyScale)) q0 = quotient_of_tiny(a, s.x);
         if (!(s.y >= kTinyScale)) q1 = quotient_of_tiny(b, s.y);
         if (!(s.z >= kTinyScale)) q2 = quotient_of_tiny(c, s.z);

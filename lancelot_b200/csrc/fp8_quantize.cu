@@ -125,13 +125,43 @@ template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bo
     const T *p = reinterpret_cast<const T *>(a.values) + r0 * a.stride + c0;
     typename Four<T>::Raw raw[kRowsOf];
 #pragma unroll
-    for (int i = 0; i < kRowsOf; ++i) raw[i] = load4<T, VEC>(p + i * kWarps * a.stride, i < rows ? n : 0);
+    for (int i = 0; i < kRowsOf; ++i, p += kWarps * a.stride) raw[i] = load4<T, VEC>(p, i < rows ? n : 0);
     using V = Four<T>;
-    auto put_row = [&](unsigned char *to, int i, const float4 &s, const float4 &f, bool odd, bool vec) {
-        put4(to, codes4<E5M2>(V::magnitudes(raw[i]), s, f, odd) | V::signs(raw[i]), n, vec);
+    // a whole tile of ordinary scales goes without a question asked for each of its rows
+    const bool whole = rows == kRowsOf && tc * kB + kB <= a.cols;
+    auto put_rows = [&](unsigned char *to, long stride, auto scale_of_row, bool odd) {
+        to += r0 * stride + c0;
+        const long step = kWarps * stride;
+        if (whole && !odd && four_aligned(to - c0 - r0 * stride, stride)) {
+#pragma unroll
+            for (int i = 0; i < kRowsOf; ++i, to += step) {
+                float4 s, f;
+                scale_of_row(i, s, f);
+                *reinterpret_cast<unsigned *>(to) = codes4<E5M2, false>(V::magnitudes(raw[i]), s, f) | V::signs(raw[i]);
+            }
+        } else if (!odd) {
+            const bool vec = four_aligned(to - c0 - r0 * stride, stride);
+#pragma unroll
+            for (int i = 0; i < kRowsOf; ++i, to += step) {
+                if (i >= rows) break;
+                float4 s, f;
+                scale_of_row(i, s, f);
+                put4(to, codes4<E5M2, false>(V::magnitudes(raw[i]), s, f) | V::signs(raw[i]), n, vec);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < kRowsOf; ++i, to += step) {
+                float4 s, f;
+                scale_of_row(i, s, f);
+                typename V::Raw x = raw[0];
+#pragma unroll
+                for (int j = 1; j < kRowsOf; ++j)
+                    if (i == j) x = raw[j];
+                if (i < rows) put4(to, codes4<E5M2, true>(V::magnitudes(x), s, f) | V::signs(x), n, false);
+            }
+        }
     };
     if (MODE == kRows || MODE == kBoth) {
-        const bool vec = four_aligned(a.codes, a.code_stride);
         // lane i finds the scale of row i, for all lanes
         unsigned mine = 0;
 #pragma unroll
@@ -141,29 +171,22 @@ template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bo
         }
         const float scale = scale_of<E5M2>(mine), inverse = inverse_of(scale);
         if (lane < rows) a.scales[(r0 + lane * kWarps) * a.scale_stride + tc] = scale;
-#pragma unroll
-        for (int i = 0; i < kRowsOf; ++i) {
-            const float s = __shfl_sync(0xffffffffu, scale, i), f = __shfl_sync(0xffffffffu, inverse, i);
-            if (i < rows) put_row(a.codes + (r0 + i * kWarps) * a.code_stride + c0, i, all(s), all(f), odd_scale(s), vec);
-        }
+        put_rows(a.codes, a.code_stride, [&](int i, float4 &s, float4 &f) { s = all(__shfl_sync(0xffffffffu, scale, i)), f = all(__shfl_sync(0xffffffffu, inverse, i)); },
+                 __any_sync(0xffffffffu, odd_scale(scale)));
     }
     if constexpr (MODE == kSquare || MODE == kColumns || MODE == kBoth) {
         typename V::Most most = V::none();
 #pragma unroll
         for (int i = 0; i < kRowsOf; ++i) most = V::more(most, raw[i]);
         if constexpr (MODE == kSquare) {
-            const bool vec = four_aligned(a.codes, a.code_stride);
             unsigned m = __reduce_max_sync(0xffffffffu, V::all(most));
             if (lane == 0) part[0][warp] = m;
             __syncthreads();
             m = __reduce_max_sync(0xffffffffu, part[0][lane & (kWarps - 1)]);
-            const float s = scale_of<E5M2>(m), f = inverse_of(s);
-            if (threadIdx.x == 0) a.scales[tr * a.scale_stride + tc] = s;
-#pragma unroll
-            for (int i = 0; i < kRowsOf; ++i)
-                if (i < rows) put_row(a.codes + (r0 + i * kWarps) * a.code_stride + c0, i, all(s), all(f), odd_scale(s), vec);
+            const float scale = scale_of<E5M2>(m), inverse = inverse_of(scale);
+            if (threadIdx.x == 0) a.scales[tr * a.scale_stride + tc] = scale;
+            put_rows(a.codes, a.code_stride, [&](int, float4 &s, float4 &f) { s = all(scale), f = all(inverse); }, odd_scale(scale));
         } else {
-            const bool vec = four_aligned(a.down, a.down_stride);
             *reinterpret_cast<uint4 *>(&part[warp][lane * 4]) = V::columns(most);
             __syncthreads();
             if (threadIdx.x < kB) {
@@ -175,12 +198,10 @@ template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bo
                 if (tc * kB + (int)threadIdx.x < a.cols) a.down_scales[tr * a.down_scale_stride + tc * kB + threadIdx.x] = s;
             }
             __syncthreads();
-            const float4 s = *reinterpret_cast<const float4 *>(column + lane * 4);
-            const float4 f = make_float4(inverse_of(s.x), inverse_of(s.y), inverse_of(s.z), inverse_of(s.w));
-            const bool odd = odd_scale(s.x) || odd_scale(s.y) || odd_scale(s.z) || odd_scale(s.w);
-#pragma unroll
-            for (int i = 0; i < kRowsOf; ++i)
-                if (i < rows) put_row(a.down + (r0 + i * kWarps) * a.down_stride + c0, i, s, f, odd, vec);
+            const float4 c = *reinterpret_cast<const float4 *>(column + lane * 4);
+            const float4 inverse = make_float4(inverse_of(c.x), inverse_of(c.y), inverse_of(c.z), inverse_of(c.w));
+            put_rows(a.down, a.down_stride, [&](int, float4 &s, float4 &f) { s = c, f = inverse; },
+                     __any_sync(0xffffffffu, odd_scale(c.x) || odd_scale(c.y) || odd_scale(c.z) || odd_scale(c.w)));
         }
     }
 }
