@@ -227,46 +227,89 @@ template <typename T, bool E5M2, bool VEC> __global__ void __launch_bounds__(kWa
     const int c0 = tc * kB + lane * 4, n = a.cols - c0;
     const long r0 = tr * kB + warp;
     const int rows = (int)min((long)kRowsOf, max(0l, (a.rows - r0 + kWarps - 1) / kWarps));
-    if (n <= 0) return;
-    const unsigned char *p = a.codes + r0 * a.code_stride + c0;
-    unsigned q[kRowsOf];
-    float4 s[kRowsOf];
+    if (!VEC) { // rows off their alignment: a lane takes every 32nd column, so that a warp's loads and stores are runs all the same
+        const int first = tc * kB + lane;
+        float s[4];
+        if (!a.col_shift) {
 #pragma unroll
-    for (int i = 0; i < kRowsOf; ++i) {
-        if (i >= rows) break;
-        const unsigned char *at = p + i * kWarps * a.code_stride;
-        if (VEC && n >= 4) {
-            q[i] = __ldg(reinterpret_cast<const unsigned *>(at));
-        } else {
-            q[i] = 0;
+            for (int e = 0; e < 4; ++e) s[e] = first + 32 * e < a.cols ? __ldg(a.scales + tr * a.scale_stride + first + 32 * e) : 0.f;
+        }
+        const unsigned char *p = a.codes + r0 * a.code_stride + first;
+        T *to = reinterpret_cast<T *>(a.out) + r0 * a.out_stride + first;
+#pragma unroll 4
+        for (int i = 0; i < rows; ++i) {
+            const unsigned char *at = p + i * kWarps * a.code_stride;
+            unsigned q[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = first + 32 * e < a.cols ? __ldg(at + 32 * e) : 0;
+            const float2 x = from_codes2<E5M2>(q[0] | q[1] << 8), y = from_codes2<E5M2>(q[2] | q[3] << 8);
+            const float v[4] = {x.x, x.y, y.x, y.y};
+            const float one = a.col_shift ? __ldg(a.scales + ((r0 + i * kWarps) >> a.row_shift) * a.scale_stride + tc) : 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (e < n) q[i] |= (unsigned)__ldg(at + e) << 8 * e;
+                if (first + 32 * e < a.cols) put(to + i * kWarps * a.out_stride + 32 * e, v[e] * (a.col_shift ? one : s[e]));
         }
+        return;
     }
-    if (a.col_shift) {
-#pragma unroll
-        for (int i = 0; i < kRowsOf; ++i)
-            if (i < rows) s[i] = all(__ldg(a.scales + ((r0 + i * kWarps) >> a.row_shift) * a.scale_stride + tc));
-    } else {
+    if (n <= 0) return;
+    const unsigned char *p = a.codes + r0 * a.code_stride + c0;
+    T *to = reinterpret_cast<T *>(a.out) + r0 * a.out_stride + c0;
+    const long step = kWarps * a.code_stride, out_step = kWarps * a.out_stride;
+    float4 s[kRowsOf];
+    if (!a.col_shift) {
         const float *of = a.scales + tr * a.scale_stride + c0;
         s[0] = make_float4(__ldg(of), n > 1 ? __ldg(of + 1) : 0.f, n > 2 ? __ldg(of + 2) : 0.f, n > 3 ? __ldg(of + 3) : 0.f);
 #pragma unroll
         for (int i = 1; i < kRowsOf; ++i) s[i] = s[0];
-    }
-    T *to = reinterpret_cast<T *>(a.out) + r0 * a.out_stride + c0;
+    } else if (a.row_shift) {
+        s[0] = all(__ldg(a.scales + tr * a.scale_stride + tc));
 #pragma unroll
-    for (int i = 0; i < kRowsOf; ++i) {
+        for (int i = 1; i < kRowsOf; ++i) s[i] = s[0];
+    } else {
+        const float *of = a.scales + r0 * a.scale_stride + tc;
+#pragma unroll
+        for (int i = 0; i < kRowsOf; ++i, of += kWarps * a.scale_stride) s[i] = all(i < rows ? __ldg(of) : 0.f);
+    }
+    auto value = [&](unsigned q, const float4 &f, float (&v)[4]) {
+        const float2 x = from_codes2<E5M2>(q), y = from_codes2<E5M2>(q >> 16);
+        v[0] = x.x * f.x, v[1] = x.y * f.y, v[2] = y.x * f.z, v[3] = y.y * f.w;
+    };
+    if (rows == kRowsOf && tc * kB + kB <= a.cols) { // a whole tile
+        unsigned q[kRowsOf];
+#pragma unroll
+        for (int i = 0; i < kRowsOf; ++i, p += step) q[i] = __ldg(reinterpret_cast<const unsigned *>(p));
+#pragma unroll
+        for (int i = 0; i < kRowsOf; ++i, to += out_step) {
+            float v[4];
+            value(q[i], s[i], v);
+            *reinterpret_cast<typename Four<T>::Raw *>(to) = Four<T>::make(v);
+        }
+        return;
+    }
+    unsigned q[kRowsOf];
+#pragma unroll
+    for (int i = 0; i < kRowsOf; ++i, p += step) {
+        q[i] = 0;
         if (i >= rows) break;
-        const float2 x = from_codes2<E5M2>(q[i]), y = from_codes2<E5M2>(q[i] >> 16);
-        const float v[4] = {x.x * s[i].x, x.y * s[i].y, y.x * s[i].z, y.y * s[i].w};
-        T *at = to + i * kWarps * a.out_stride;
-        if (VEC && n >= 4) {
-            *reinterpret_cast<typename Four<T>::Raw *>(at) = Four<T>::make(v);
+        if (n >= 4) {
+            q[i] = __ldg(reinterpret_cast<const unsigned *>(p));
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (e < n) put(at + e, v[e]);
+                if (e < n) q[i] |= (unsigned)__ldg(p + e) << 8 * e;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsOf; ++i, to += out_step) {
+        if (i >= rows) break;
+        float v[4];
+        value(q[i], s[i], v);
+        if (n >= 4) {
+            *reinterpret_cast<typename Four<T>::Raw *>(to) = Four<T>::make(v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < n) put(to + e, v[e]);
         }
     }
 }
