@@ -332,9 +332,8 @@ LB_API int lb_fp8_matmul(lb_context *ctx, int64_t m, int64_t n, int64_t k, const
  * outs (HOST array, NULL: norms only): out = v * f, in 32 bits, then rounded to its type, with f = 1 where norms[c] <= max_norm,
  * max_norm / norms[c] rounded to 32 bits where it is larger, NaN where it is not finite.  tensors, outs: HOST arrays of n_tensors device
  * pointers to sizes[i] contiguous values of type dtypes[i], out_dtypes[i]; clients[i], not decreasing: whose tensor it is.
- * outs[i] is tensors[i] itself or apart from all tensors and all other results.  (out_dtypes of the first call: NULL where outs is.) */
-LB_API size_t lb_clip_updates_workspace_bytes(const lb_context *ctx, int n_clients, int n_tensors, const int *clients, const int *dtypes,
-                    const int64_t *sizes, const int *out_dtypes);
+ * outs[i] is tensors[i] itself or apart from all tensors and all other results. */
+LB_API size_t lb_clip_updates_workspace_bytes(int n_clients, int n_tensors, const int64_t *sizes);
 LB_API int lb_clip_updates(lb_context *ctx, int n_clients, int n_tensors, const int *clients, const void *const *tensors, const int *dtypes,
                     const int64_t *sizes, double max_norm, void *const *outs, const int *out_dtypes, double *norms, void *workspace,
                     size_t workspace_bytes, void *stream);

@@ -1041,14 +1041,17 @@ static int clip_apart(const std::vector<ClipPart> &parts)
     return LB_OK;
 }
 
-size_t lb_clip_updates_workspace_bytes(const lb_context *h, int n_clients, int n_tensors, const int *clients, const int *dtypes, const int64_t *sizes,
-                                       const int *out_dtypes)
-try {
-    if (!h || !h->c || n_clients < 1 || clip_ok(n_clients, n_tensors, clients, dtypes, sizes, out_dtypes)) return 0;
-    const std::vector<ClipPart> parts = clip_parts(n_clients, n_tensors, clients, dtypes, sizes, out_dtypes);
-    return clip_workspace_bytes(h->c, parts.data(), (int)parts.size(), out_dtypes != nullptr);
-} catch (const std::bad_alloc &) {
-    return 0;
+static size_t clip_bytes(int n_clients, int n_tensors, const int64_t *sizes)
+{
+    size_t sums = (size_t)n_clients; // clients without values
+    for (int i = 0; i < n_tensors; ++i) sums += sizes[i] ? clip_sums(sizes[i]) : 0;
+    return sums * 8;
+}
+
+size_t lb_clip_updates_workspace_bytes(int n_clients, int n_tensors, const int64_t *sizes)
+{
+    if (n_clients < 1 || n_tensors < 0 || (n_tensors && !sizes)) return 0;
+    return clip_bytes(n_clients, n_tensors, sizes);
 }
 
 int lb_clip_updates(lb_context *h, int n_clients, int n_tensors, const int *clients, const void *const *tensors, const int *dtypes,
@@ -1064,7 +1067,6 @@ try {
     REQUIRE(norms && (n_tensors == 0 || (tensors && (!outs || out_dtypes))), "operand is null");
     REQUIRE((uintptr_t)norms % 8 == 0, "an operand is not aligned to its type");
     std::vector<ClipPart> parts = clip_parts(n_clients, n_tensors, clients, dtypes, sizes, out_dtypes);
-    const size_t need = clip_workspace_bytes(C(h), parts.data(), (int)parts.size(), outs != nullptr);
     for (ClipPart &p : parts) {
         const int i = p.index;
         if (i < 0) continue;
@@ -1076,7 +1078,7 @@ try {
         p.out = outs[i];
     }
     if ((rc = clip_apart(parts))) return rc;
-    if ((rc = workspace_ok(workspace, workspace_bytes, need))) return rc;
+    if ((rc = workspace_ok(workspace, workspace_bytes, clip_bytes(n_clients, n_tensors, sizes)))) return rc;
     return clip_updates(C(h), parts.data(), (int)parts.size(), outs != nullptr, max_norm, reinterpret_cast<double *>(workspace), norms, S(stream));
 } catch (const std::bad_alloc &) {
     set_error("out of host memory");

@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostTensors = 640;    // of one launch: they travel as its argument
+constexpr int kLeastPiece = 1024; // elements: clip_workspace_bytes counts on it
 constexpr double kRoundBytes = 48e6; // of values: what stays in L2 until they are read again, beside the results
 
 struct Part {
@@ -346,8 +347,8 @@ struct Launch {
 
 double part_bytes(const ClipPart &p) { return (double)p.n * (p.in_type == 1 ? 4 : 2); }
 
-// The launches of a call, and (with `parts`) their tables; returns the number of sums
-long plan(const Context *ctx, const ClipPart *in, int n, bool writes, std::vector<Launch> &launches, std::vector<Part> *parts)
+// The launches of a call, and their tables
+void plan(const Context *ctx, const ClipPart *in, int n, bool writes, std::vector<Launch> &launches, std::vector<Part> &parts)
 {
     long slots = 0;
     auto pieces_of = [](long size, int piece) { return size ? (int)((size + piece - 1) / piece) : 1; };
@@ -356,11 +357,11 @@ long plan(const Context *ctx, const ClipPart *in, int n, bool writes, std::vecto
         for (int j = i; j < end; ++j) all += (double)in[j].n;
         // some eight pieces an SM, of 64 KB of 32-bit values at most: every block of the second kernel reads the sums of all pieces of its client
         const double even = all / (8.0 * ctx->sm_count);
-        const int piece = even <= 1024 ? 1024 : even >= 16384 && all < 16384.0 * (1 << 20) ? 16384 : ((int)(even / 1024) + 1) * 1024;
+        const int piece = even <= kLeastPiece ? kLeastPiece : even >= 16384 && all < 16384.0 * (1 << 20) ? 16384 : ((int)(even / 1024) + 1) * 1024;
         Launch l = {i, end - i, piece, 0, false};
         for (int j = i; j < end; ++j) {
             const int pieces = pieces_of(in[j].n, piece);
-            if (parts) (*parts)[j] = {in[j].in, in[j].out, in[j].n, l.pieces, (int)slots, 0, (int)slots + pieces, in[j].client, j == 0 || in[j].client != in[j - 1].client};
+            parts[j] = {in[j].in, in[j].out, in[j].n, l.pieces, (int)slots, 0, (int)slots + pieces, in[j].client, j == 0 || in[j].client != in[j - 1].client};
             l.pieces += pieces;
             slots += pieces;
         }
@@ -397,14 +398,12 @@ long plan(const Context *ctx, const ClipPart *in, int n, bool writes, std::vecto
             }
         i = whole;
     }
-    if (parts)
-        for (int i = 0; i < n;) { // a client's sums lie together, those of several launches too
-            int end = i;
-            while (end < n && in[end].client == in[i].client) ++end;
-            for (int j = i; j < end; ++j) (*parts)[j].slots = (*parts)[i].slot, (*parts)[j].slots_end = (*parts)[end - 1].slots_end;
-            i = end;
-        }
-    return slots;
+    for (int i = 0; i < n;) { // a client's sums lie together, those of several launches too
+        int end = i;
+        while (end < n && in[end].client == in[i].client) ++end;
+        for (int j = i; j < end; ++j) parts[j].slots = parts[i].slot, parts[j].slots_end = parts[end - 1].slots_end;
+        i = end;
+    }
 }
 
 // The first kernel of a call waits for what came before it; the others are set up, and those of sums begin, while their predecessor ends
@@ -448,17 +447,12 @@ template <int MOST> const void *kernel_of(int in_type, int out_type)
 
 } // namespace
 
-size_t clip_workspace_bytes(const Context *ctx, const ClipPart *parts, int n, bool writes)
-{
-    std::vector<Launch> launches;
-    return (size_t)plan(ctx, parts, n, writes, launches, nullptr) * 8;
-}
-
 int clip_updates(const Context *ctx, const ClipPart *in, int n, bool writes, double most, double *partial, double *norms, cudaStream_t stream)
 {
     std::vector<Launch> launches;
+    launches.reserve(8);
     std::vector<Part> parts(n);
-    plan(ctx, in, n, writes, launches, &parts);
+    plan(ctx, in, n, writes, launches, parts);
     int rc = LB_OK;
     for (const Launch &l : launches) {
         double bytes = 0.0;
@@ -466,8 +460,8 @@ int clip_updates(const Context *ctx, const ClipPart *in, int n, bool writes, dou
         count_launch(l.writes ? "clip_scale" : "clip_norm", stream, bytes);
         const int in_type = in[l.first].in_type, out_type = l.writes ? in[l.first].out_type : 0;
         const bool first = &l == launches.data();
-        if (l.count <= 16) rc = launch<16>(parts, l, kernel_of<16>(in_type, out_type), most, partial, norms, first, stream);
-        else if (l.count <= 96) rc = launch<96>(parts, l, kernel_of<96>(in_type, out_type), most, partial, norms, first, stream);
+        if (l.count <= 32) rc = launch<32>(parts, l, kernel_of<32>(in_type, out_type), most, partial, norms, first, stream);
+        else if (l.count <= 128) rc = launch<128>(parts, l, kernel_of<128>(in_type, out_type), most, partial, norms, first, stream);
         else rc = launch<kMostTensors>(parts, l, kernel_of<kMostTensors>(in_type, out_type), most, partial, norms, first, stream);
         if (rc) return rc;
     }

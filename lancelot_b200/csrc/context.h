@@ -248,7 +248,7 @@ struct ClipPart {
     int client, in_type, out_type;
     int index; // of the call's tensors; -1: none of them
 };
-size_t clip_workspace_bytes(const Context *ctx, const ClipPart *parts, int n, bool writes);
+inline size_t clip_sums(long n) { return n ? (size_t)((n + 1023) / 1024) : 1; } // of a tensor, at most: a sum for 1024 elements
 int clip_updates(const Context *ctx, const ClipPart *parts, int n, bool writes, double most, double *partial, double *norms, cudaStream_t stream);
 
 } // namespace lb

@@ -392,15 +392,18 @@ Tensor clip_updates(int64_t context, int device, const py::object &updates, std:
         if (!py::isinstance<py::sequence>(updates)) refuse("updates must be a matrix, or for each client a list of tensors");
         for (const py::handle client : py::reinterpret_borrow<py::sequence>(updates)) {
             if (THPVariable_Check(client.ptr()) || !py::isinstance<py::sequence>(client)) refuse("updates must be a matrix, or for each client a list of tensors");
-            for (const py::handle item : py::reinterpret_borrow<py::sequence>(client)) {
+            const py::object items = py::reinterpret_steal<py::object>(PySequence_Fast(client.ptr(), "updates"));
+            if (!items) throw py::error_already_set();
+            for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(items.ptr()); ++i) {
+                const py::handle item = PySequence_Fast_GET_ITEM(items.ptr(), i);
                 if (!THPVariable_Check(item.ptr())) refuse("updates must be a matrix, or for each client a list of tensors");
-                const Tensor t = THPVariable_Unpack(item.ptr());
+                const Tensor &t = THPVariable_Unpack(item.ptr());
                 if (!t.is_cuda() || t.get_device() != c.device || t.layout() != at::kStrided) refuse("an update's tensors must be on cuda:" + std::to_string(device));
                 if (!value_type(t.scalar_type())) refuse("an update's tensors must be float32, bfloat16 or float16");
                 // the order of the values is the result's where they are copied
                 if (out ? !t.is_contiguous() : !t.is_non_overlapping_and_dense()) refuse(out ? "an update's tensors must be contiguous" : "an update's tensors must be dense");
                 add(t, t.numel(), 0);
-                held.push_back(t);
+                if (in_place) held.push_back(t);
             }
             ++n;
         }
@@ -435,7 +438,7 @@ Tensor clip_updates(int64_t context, int device, const py::object &updates, std:
     const Tensor norms = c.empty({n}, at::kDouble);
     const int count = (int)sizes.size();
     const int *writes = out || in_place ? out_dtypes.data() : nullptr;
-    const size_t need = n ? lb_clip_updates_workspace_bytes(c.context, n, count, clients.data(), dtypes.data(), sizes.data(), writes) : 0;
+    const size_t need = n ? lb_clip_updates_workspace_bytes(n, count, sizes.data()) : 0;
     const Tensor ws = c.workspace(need);
     check(lb_clip_updates(c.context, n, count, clients.data(), tensors.data(), dtypes.data(), sizes.data(), max_norm ? *max_norm : HUGE_VAL,
                           out || in_place ? outs.data() : nullptr, writes, address<double>(norms), address<void>(ws), need, c.stream()));
