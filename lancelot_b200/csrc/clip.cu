@@ -11,7 +11,10 @@
 //
 // Two kernels, for some clients at a time (a round): the values are read for their sums, and read again, out of L2, the last ones first, and
 // written.  The sums of a round start while the results of the one before are still being written (programmatic launches).
-// Bound by HBM: TIMES
+// Bound by HBM: norms of 20 x 11 M in 130 us (6.9 TB/s).  As flat rows 20 x 11 M take 426 us: DRAM reads every value once, but the reading and the writing of a
+// round (45 MB) come one after the other, with the start and the end of a kernel each (one round of everything, whose values are read twice, takes 490 us; the
+// writing alone 330 us).  11 M values in bf16 as a row of 32 bits: 19 us.  A single persistent kernel whose blocks meet between a round's two parts took
+// 480 us: a meeting costs some 6 us of idle memory.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -237,7 +237,7 @@ def check_product(out, a, b, k):
 FORMS = {"forward": ((1, 128), (128, 128), False, False), "input": ((1, 128), (128, 128), False, True), "weight": ((1, 128), (1, 128), True, True),
          "factors": ((1, 128), (1, 128), False, False), "turned": ((128, 128), (1, 128), True, False), "squares": ((128, 128), (128, 128), False, False)}
 PRODUCTS = [(1, 64, 64), (1, 1, 1), (7, 33, 129), (32, 200, 1000), (33, 65, 31), (64, 64, 128), (100, 300, 200), (128, 128, 128), (129, 257, 385), (333, 1111, 511),
-            (200, 640, 2048), (1000, 1500, 640), (2, 4096, 300), (700, 3, 260)]
+            (200, 640, 2048), (1000, 1500, 640), (2, 4096, 300), (700, 3, 260), (1100, 5003, 390), (3001, 1300, 130)]
 
 
 @pytest.mark.parametrize("form", sorted(FORMS))
@@ -407,6 +407,81 @@ def test_a_layers_step(ctx, dtype, shape, n, grad):
     y = updates.fp8_linear(ctx, x, w.detach())
     y.float().sum().backward()
     check_product(x.grad.reshape(m, k), held(ones, (1, 128), "e4m3"), w8.t(), n)
+
+
+def test_a_layers_step_on_an_empty_batch_and_on_transposed_operands(ctx):
+    import torch
+
+    from lancelot_b200 import updates
+
+    g = gen(12)
+    w = torch.randn(200, 64, generator=g, device="cuda").t().requires_grad_()  # [64][200], its rows not dense
+    x = torch.zeros(0, 200, device="cuda", requires_grad=True)
+    y = updates.fp8_linear(ctx, x, w)
+    assert y.shape == (0, 64)
+    dx, dw = torch.autograd.grad(y, (x, w), y.detach())
+    assert dx.shape == (0, 200) and dw.shape == (64, 200) and not dw.any()
+    x = torch.randn(200, 30, generator=g, device="cuda").t()
+    assert torch.equal(updates.fp8_linear(ctx, x, w), updates.fp8_linear(ctx, x.contiguous(), w.detach().contiguous()))
+    one = torch.randn(200, generator=g, device="cuda")
+    # one value for several rows; the sums of 12 rows and those of one are formed in other orders, so both are held to the formula
+    codes, scales = quantized(one[None], (1, 128), "e4m3")
+    x8 = codes * spread(scales, 1, 200, (1, 128)).double()
+    codes, scales = quantized(w.detach().contiguous(), (128, 128), "e4m3")
+    w8 = codes * spread(scales, 64, 200, (128, 128)).double()
+    check_product(updates.fp8_linear(ctx, one.expand(4, 3, 200), w).detach().reshape(12, 64), x8.expand(12, 200), w8, 200)
+    check_product(updates.fp8_linear(ctx, one, w).detach()[None], x8, w8, 200)
+    # what is kept for the backward pass are codes: the layer's operands may change in between
+    x = torch.randn(20, 200, generator=g, device="cuda").requires_grad_()
+    y = updates.fp8_linear(ctx, x, w)
+    want = torch.autograd.grad(y, (x, w), torch.ones_like(y), retain_graph=True)
+    with torch.no_grad():
+        w.zero_()
+        x.zero_()
+    for p, q in zip(torch.autograd.grad(y, (x, w), torch.ones_like(y)), want):
+        assert torch.equal(p, q)
+
+
+def test_a_captured_step(ctx):
+    """forward and gradients replayed with other inputs, in two graphs at once that share the operands"""
+    import torch
+
+    from lancelot_b200 import updates
+
+    g = gen(13)
+    x = torch.randn(70, 200, generator=g, device="cuda").requires_grad_()
+    w = torch.randn(90, 200, generator=g, device="cuda").requires_grad_()
+    dy = torch.randn(70, 90, generator=g, device="cuda")
+
+    def step():
+        y = updates.fp8_linear(ctx, x, w)
+        return (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    got = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            got.append(step())
+    with torch.no_grad():
+        x.normal_(generator=g)
+        w.normal_(generator=g)
+        dy.normal_(generator=g)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for graph, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            graph.replay()
+    torch.cuda.synchronize()
+    for want, *replayed in zip(step(), *got):
+        for r in replayed:
+            assert torch.equal(r, want)
+    ctx.check_status()
 
 
 def test_gradients_against_differences(ctx):
