@@ -6,15 +6,15 @@
 // (lancelot-main-GPU/utils/byzantine_fl.py:162-171,527-536); the reference has none.
 //
 // Squares of 32-bit floats are exact in 64 bits, and so are summed there: no sum passes the range, and small entries are not lost behind
-// large ones.  The tensors are cut into pieces, dealt out to the blocks; a block's sum for a client goes to its own slot, and every block that needs a
-// client's norm adds its slots up in the same order, so that results do not depend on which block was first.
+// large ones.  The tensors are cut into pieces, a block each; a piece's sum goes to its own place, and every block that needs a client's norm adds
+// its pieces' sums up in the same order, so that results do not depend on which block was first.
 //
-// Two kernels, for some clients at a time (a round): the values are read for their sums, and read again, out of L2, the last ones first, and
-// written.  The sums of a round start while the results of the one before are still being written (programmatic launches).
-// Bound by HBM: norms of 20 x 11 M in 130 us (6.9 TB/s).  As flat rows 20 x 11 M take 426 us: DRAM reads every value once, but the reading and the writing of a
-// round (45 MB) come one after the other, with the start and the end of a kernel each (one round of everything, whose values are read twice, takes 490 us; the
-// writing alone 330 us).  11 M values in bf16 as a row of 32 bits: 19 us.  A single persistent kernel whose blocks meet between a round's two parts took
-// 480 us: a meeting costs some 6 us of idle memory.
+// The values of some clients (a round) are read for their sums by one kernel, and read again, the last ones first, and written by the next one, whose other
+// blocks sum up the round after that.  Every kernel starts while its predecessor ends (programmatic launches).  Bound by memory: the norms of
+// 20 x 11 M take 130 us (6.9 TB/s).  As flat rows 20 x 11 M take 403 us (floor 277): a third of the second reading misses L2 (61 MB of DRAM read for a
+// client's 45), and a round's kernel has a start and an end of some microseconds.  Without rounds, every value read twice from DRAM, it takes 451 us,
+// with rounds of one client 422, with sums and results in kernels of their own 425; a persistent kernel whose blocks meet between a round's two parts takes
+// 480 us, 6 of them for each meeting.  11 M values in bf16 as a row of 32 bits: 18.5 us; four clients of eight tensors: 4.3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -30,8 +30,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostTensors = 640;    // of one launch: they travel as its argument
-constexpr int kLeastPiece = 1024; // elements: clip_workspace_bytes counts on it
-constexpr double kRoundBytes = 48e6; // of values: what stays in L2 until they are read again, beside the results
+constexpr int kLeastPiece = 1024;    // elements: clip_sums counts on it
+constexpr double kRoundBytes = 96e6; // of values, unless a single client has more: most of them stay in L2 until they are read again
 
 struct Part {
     const void *in;
@@ -44,7 +44,9 @@ struct Part {
 };
 template <int MOST> struct ClipArgs {
     Part tensor[MOST];
-    int n_tensors, piece; // piece: elements of a piece
+    int n_scale, n_tensors;       // the first n_scale tensors are written, the others are summed up
+    int scale_piece, sum_piece;   // elements of their pieces
+    int scale_pieces, sum_pieces; // how many
     double most;
     double *partial, *norms;
 };
@@ -98,10 +100,10 @@ __device__ __forceinline__ double block_sum(double v, double *shared)
     return v;
 }
 
-// the tensor that holds a piece
-template <int MOST> __device__ __forceinline__ const Part &tensor_of(const ClipArgs<MOST> &a, int piece)
+// the tensor that holds a piece, of tensors lo to hi - 1
+template <int MOST> __device__ __forceinline__ const Part &tensor_of(const ClipArgs<MOST> &a, int lo, int hi, int piece)
 {
-    int lo = 0, hi = a.n_tensors - 1;
+    --hi;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (a.tensor[mid].first <= piece) lo = mid;
@@ -285,16 +287,19 @@ __device__ __forceinline__ void predecessor_done() { asm volatile("griddepcontro
 // the next kernel's blocks may come as soon as there is room
 __device__ __forceinline__ void successor_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+template <typename T, int MOST> __device__ __forceinline__ void sum_up(const ClipArgs<MOST> &a, int i, double *shared)
+{
+    const Part &t = tensor_of(a, a.n_scale, a.n_tensors, i);
+    const long e = (long)(i - t.first) * a.sum_piece;
+    const double sum = block_sum(squares(reinterpret_cast<const T *>(t.in) + e, (int)min((long)a.sum_piece, t.n - e)), shared);
+    if (threadIdx.x == 0) a.partial[t.slot + (i - t.first)] = sum;
+    predecessor_done(); // nothing of it is used: whoever waits for this kernel has then waited for that one too
+}
 template <typename T, int MOST> __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ ClipArgs<MOST> a)
 {
     __shared__ double shared[kThreads / 32];
     successor_may_start();
-    const int i = (int)blockIdx.x;
-    const Part &t = tensor_of(a, i);
-    const long e = (long)(i - t.first) * a.piece;
-    const double sum = block_sum(squares(reinterpret_cast<const T *>(t.in) + e, (int)min((long)a.piece, t.n - e)), shared);
-    if (threadIdx.x == 0) a.partial[t.slot + (i - t.first)] = sum;
-    predecessor_done(); // nothing of it is used: whoever waits for this kernel has then waited for that one too
+    sum_up<T>(a, (int)blockIdx.x, shared);
 }
 
 __device__ __forceinline__ double norm_of(const double *partial, int from, int to, double *shared)
@@ -304,15 +309,23 @@ __device__ __forceinline__ double norm_of(const double *partial, int from, int t
     return sqrt(block_sum(sum, shared));
 }
 
+// Blocks that write the results of some clients, and blocks that sum up the next clients' values, by turns: memory is read and written at once
 template <typename T, typename O, int MOST> __global__ void __launch_bounds__(kThreads) clip_kernel(const __grid_constant__ ClipArgs<MOST> a)
 {
     __shared__ double shared[kThreads / 32];
     successor_may_start();
-    const int i = (int)(gridDim.x - 1 - blockIdx.x); // what was read last is read first
-    const Part &t = tensor_of(a, i);
-    const long e = (long)(i - t.first) * a.piece;
+    const int pairs = min(a.scale_pieces, a.sum_pieces), block = (int)blockIdx.x;
+    const bool sums = block < 2 * pairs ? block & 1 : a.sum_pieces > pairs;
+    int i = block < 2 * pairs ? block >> 1 : block - pairs;
+    if (sums) {
+        sum_up<T>(a, i, shared);
+        return;
+    }
+    i = a.scale_pieces - 1 - i; // what was read last is read first
+    const Part &t = tensor_of(a, 0, a.n_scale, i);
+    const long e = (long)(i - t.first) * a.scale_piece;
     // values on their way while the norm is found: no kernel before this one that may still run writes them
-    Scaling<T, O> s(reinterpret_cast<const T *>(t.in) + e, t.out ? reinterpret_cast<O *>(t.out) + e : nullptr, (int)min((long)a.piece, t.n - e));
+    Scaling<T, O> s(reinterpret_cast<const T *>(t.in) + e, t.out ? reinterpret_cast<O *>(t.out) + e : nullptr, (int)min((long)a.scale_piece, t.n - e));
     s.load(threadIdx.x * s.N);
     predecessor_done();
     const double norm = norm_of(a.partial, t.slots, t.slots_end, shared);
@@ -425,16 +438,23 @@ int start(const void *kernel, int grid, void *args, bool first, cudaStream_t str
     LB_CUDA(cudaLaunchKernelExC(&c, kernel, list));
     return LB_OK;
 }
-template <int MOST> int launch(const std::vector<Part> &parts, const Launch &l, const void *kernel, double most, double *partial, double *norms, bool first, cudaStream_t stream)
+template <int MOST>
+int launch(const std::vector<Part> &parts, const Launch &l, const Launch *next, const void *kernel, double most, double *partial, double *norms, bool first, cudaStream_t stream)
 {
     ClipArgs<MOST> a;
-    std::copy(parts.begin() + l.first, parts.begin() + l.first + l.count, a.tensor);
-    a.n_tensors = l.count;
-    a.piece = l.piece;
+    const int count = l.count + (next ? next->count : 0);
+    std::copy(parts.begin() + l.first, parts.begin() + l.first + count, a.tensor);
+    const Launch *sums = l.writes ? next : &l;
+    a.n_scale = l.writes ? l.count : 0;
+    a.n_tensors = count;
+    a.scale_piece = l.piece;
+    a.scale_pieces = l.writes ? l.pieces : 0;
+    a.sum_piece = sums ? sums->piece : 0;
+    a.sum_pieces = sums ? sums->pieces : 0;
     a.most = most;
     a.partial = partial;
     a.norms = norms;
-    return start(kernel, l.pieces, &a, first, stream);
+    return start(kernel, a.scale_pieces + a.sum_pieces, &a, first, stream);
 }
 template <typename T, int MOST> const void *kernel_of(int out_type)
 {
@@ -457,15 +477,23 @@ int clip_updates(const Context *ctx, const ClipPart *in, int n, bool writes, dou
     std::vector<Part> parts(n);
     plan(ctx, in, n, writes, launches, parts);
     int rc = LB_OK;
-    for (const Launch &l : launches) {
+    for (size_t j = 0; j < launches.size(); ++j) {
+        const Launch &l = launches[j];
+        const bool first = j == 0;
+        // the results of some clients go with the sums of the next ones
+        const Launch *next = l.writes && j + 1 < launches.size() && !launches[j + 1].writes && l.count + launches[j + 1].count <= kMostTensors &&
+                                     l.first + l.count == launches[j + 1].first && in[l.first].in_type == in[launches[j + 1].first].in_type
+                                 ? &launches[++j]
+                                 : nullptr;
         double bytes = 0.0;
-        for (int i = l.first; i < l.first + l.count; ++i) bytes += !l.writes ? part_bytes(in[i]) : in[i].out ? (double)in[i].n * (in[i].out_type == 1 ? 4 : 2) : 0.0;
+        const int count = l.count + (next ? next->count : 0);
+        for (int i = l.first; i < l.first + count; ++i)
+            bytes += !l.writes || i >= l.first + l.count ? part_bytes(in[i]) : in[i].out ? (double)in[i].n * (in[i].out_type == 1 ? 4 : 2) : 0.0;
         count_launch(l.writes ? "clip_scale" : "clip_norm", stream, bytes);
         const int in_type = in[l.first].in_type, out_type = l.writes ? in[l.first].out_type : 0;
-        const bool first = &l == launches.data();
-        if (l.count <= 32) rc = launch<32>(parts, l, kernel_of<32>(in_type, out_type), most, partial, norms, first, stream);
-        else if (l.count <= 128) rc = launch<128>(parts, l, kernel_of<128>(in_type, out_type), most, partial, norms, first, stream);
-        else rc = launch<kMostTensors>(parts, l, kernel_of<kMostTensors>(in_type, out_type), most, partial, norms, first, stream);
+        if (count <= 32) rc = launch<32>(parts, l, next, kernel_of<32>(in_type, out_type), most, partial, norms, first, stream);
+        else if (count <= 128) rc = launch<128>(parts, l, next, kernel_of<128>(in_type, out_type), most, partial, norms, first, stream);
+        else rc = launch<kMostTensors>(parts, l, next, kernel_of<kMostTensors>(in_type, out_type), most, partial, norms, first, stream);
         if (rc) return rc;
     }
     if (writes) return LB_OK;

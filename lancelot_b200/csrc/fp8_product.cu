@@ -160,12 +160,13 @@ __device__ __forceinline__ void copy4(unsigned to, const float *from) { asm vola
 
 // One CTA per SM walks over tiles of 128 x BN.  Warp 0 brings 128 bytes of the summed axis of either operand by TMA into a ring of stages, warp 1 issues the
 // products (four of k = 32 a block) into one of two or four places in TMEM, and warps 4 to 11 scale a block's sums and add them to results that they keep
-// in registers: a scale is for 128 of the summed axis, so the sums have to leave TMEM that often.  Bound by shared memory, which takes in and gives out 96 KB for a
-// block of a tile 256 wide (768 of the 1070 cycles that a block takes; the products themselves take 512), and by the chain from the products' end to the sums' and back:
-// 8192 x 8192 x 8192 in 495 us (2.2 P operations a second), without the accumulating warps 423 us, without the products 323 us.  Two CTAs on a tile of 256 x 256
-// move 64 KB a block, but wait longer for one another than that saves (732 us).  With a scale per row of b there is a product more for every sum:
-// 4096 x 11008 x 4096 in 305 us.  Votes and waits in the accumulating warps cost what they take: a vote a block 3 %, scales through
-// shared memory instead of a load ahead 25 % (with a scale per row, where loads are many, they gain 8 %).
+// in registers: a scale is for 128 of the summed axis, so the sums have to leave TMEM that often.  A block of a tile 256 wide takes some 1050 cycles, of which the
+// products are 512 (the tensor cores are active in 51 % of the cycles): what bounds it is the chain from the products' end over the sums' way to the registers to the
+// next products, with two places for the sums, beside the 96 KB that shared memory takes in and gives out.  8192 x 8192 x 8192 takes 485 to 495 us (2.2 to 2.3 P
+// operations a second; among others of its kind 594 us, under the power cap), without the accumulating warps' work 423 us, without the products 323 us.  Two CTAs on
+// a tile of 256 x 256, which move 64 KB a block, wait longer for one another than that saves (732 us).  With a scale per row of b there is a product
+// more for every sum: 4096 x 11008 x 4096 in 305 us.  Everything in the accumulating warps' chain costs what it takes: a vote a block 3 %,
+// scales through shared memory instead of a load ahead 25 % (with a scale per row, where loads are many, they gain 8 %).
 //
 // PER_ROW: b has a scale for each of its rows, otherwise one for 128.
 // SPLIT: few tiles and a long summed axis.  The blocks of a cluster take a tile together, a run of the axis each, and add up through one another's
