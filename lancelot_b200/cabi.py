@@ -468,15 +468,9 @@ class Context:
         fp8_matmul(gd.t(), gds.t(), xd.t(), xds.t()) from the codes in blocks (128, 1)"""
         return _updates8().fp8_matmul(self._handle(), self.device, a, a_scale, b, b_scale, VALUE_TYPES.get(dtype, 0), out)
 
-    def fp8_linear_forward(self, x, w, need_x=True, need_w=True):
-        """x [..., k], w [n][k] -> (y = x w^T, and what fp8_linear_backward takes): x in blocks (1, 128), w in blocks (128, 128), multiplied.  need_x, need_w:
-        whether the gradients of x and w will be asked for"""
-        return _updates8().fp8_linear_forward(self._handle(), self.device, x, w, need_x, need_w)
-
-    def fp8_linear_backward(self, g, x_down, x_down_scales, w8, w_scales, grad_dtype=torch.float8_e4m3fn, x_dtype=torch.bfloat16, w_dtype=torch.bfloat16):
-        """g [..., n], the gradient of y, and what fp8_linear_forward kept (None where a gradient is not needed) -> the gradients of x and w"""
-        return _updates8().fp8_linear_backward(self._handle(), self.device, g, x_down, x_down_scales, w8, w_scales, FP8_TYPES.get(grad_dtype, 0),
-                                               VALUE_TYPES.get(x_dtype, 0), VALUE_TYPES.get(w_dtype, 0))
+    def fp8_linear(self, x, w, grad_dtype=torch.float8_e4m3fn):
+        """y = x w^T with gradients, x [..., k], w [n][k]: see ``updates.fp8_linear``"""
+        return _updates8().fp8_linear(self, self.device, x, w, FP8_TYPES.get(grad_dtype, 0))
 
     def clip_updates(self, updates, max_norm=None, out=None):
         """The norm of each client's update over all its tensors -> [n_clients] float64, on the device.  updates: for each client a list of tensors

@@ -6,6 +6,8 @@
 #include <ATen/ops/empty_strided.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -331,37 +333,91 @@ Tensor product(const Call &c, int64_t m, int64_t n, int64_t k, const lb_fp8_oper
     return to;
 }
 
-// y, and what the gradients need: x in blocks along its rows' axis (for that of w), w's codes (for that of x)
-py::tuple fp8_linear_forward(int64_t context, int device, const Tensor &x, const Tensor &w, bool need_x, bool need_w)
-{
-    const Call c = call_of(context, device);
-    const Tensor xm = matrix(x), wm = matrix(w);
-    const Coded xc = coded(c, xm, need_w ? 3 : 1, 5), wc = coded(c, wm, 4, 5);
-    const int64_t m = xm.size(0), n = wm.size(0), k = xm.size(1);
-    at::DimVector shape(x.sizes().begin(), x.sizes().end());
-    shape.back() = n;
-    const Tensor y = product(c, m, n, k, stored_operand(xc.codes, xc.scales, false, 1, 5), stored_operand(wc.codes, wc.scales, false, 128, 5), shape, x.scalar_type());
-    auto kept = [](const Tensor &t, bool keep) { return keep ? py::cast(t) : py::none(); };
-    return py::make_tuple(y, kept(xc.down, need_w), kept(xc.down_scales, need_w), kept(wc.codes, need_x), kept(wc.scales, need_x));
-}
-py::tuple fp8_linear_backward(int64_t context, int device, const Tensor &g, const Maybe &xd, const Maybe &xds, const Maybe &w8, const Maybe &ws, int type,
-                              int x_dtype, int w_dtype)
-{
-    const Call c = call_of(context, device);
-    if (type != 5 && type != 6) refuse("dtype must be float8_e4m3fn or float8_e5m2");
-    const Tensor gm = matrix(g);
-    const Coded gc = coded(c, gm, w8 ? (xd ? 3 : 1) : 2, type);
-    const int64_t m = gm.size(0), n = gm.size(1);
-    py::object dx = py::none(), dw = py::none();
-    if (w8) {
-        at::DimVector shape(g.sizes().begin(), g.sizes().end());
-        shape.back() = w8->size(1);
-        dx = py::cast(product(c, m, w8->size(1), n, stored_operand(gc.codes, gc.scales, false, 1, type), stored_operand(*w8, *ws, true, 128, 5), shape, scalar_type(x_dtype)));
+// The context's owner, a Python object: asked for the handle again in the backward pass, so that a context closed in between is refused
+struct Owner : torch::CustomClassHolder {
+    PyObject *object;
+    explicit Owner(const py::handle &o) : object(o.inc_ref().ptr()) {}
+    ~Owner() override
+    {
+        if (!Py_IsInitialized()) return;
+        py::gil_scoped_acquire gil;
+        Py_DECREF(object);
     }
-    if (xd)
-        dw = py::cast(product(c, n, xd->size(1), m, stored_operand(gc.down, gc.down_scales, true, 1, type), stored_operand(*xd, *xds, true, 1, 5), {n, xd->size(1)},
-                              scalar_type(w_dtype)));
-    return py::make_tuple(dx, dw);
+    int64_t handle() const
+    {
+        py::gil_scoped_acquire gil;
+        return py::handle(object).attr("_handle")().cast<int64_t>();
+    }
+};
+
+struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const Call &c, const c10::intrusive_ptr<Owner> &owner, int type,
+                          bool need_x, bool need_w)
+    {
+        const Tensor xm = matrix(x), wm = matrix(w);
+        const Coded xc = coded(c, xm, need_w ? 3 : 1, 5), wc = coded(c, wm, 4, 5);
+        const int64_t m = xm.size(0), n = wm.size(0), k = xm.size(1);
+        at::DimVector shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = n;
+        // x in blocks along its rows' axis is for the gradient of w, w's codes are for that of x
+        ctx->save_for_backward({need_w ? xc.down : Tensor(), need_w ? xc.down_scales : Tensor(), need_x ? wc.codes : Tensor(), need_x ? wc.scales : Tensor()});
+        ctx->saved_data["owner"] = c10::IValue::make_capsule(owner);
+        ctx->saved_data["device"] = (int64_t)c.device;
+        ctx->saved_data["type"] = (int64_t)type;
+        ctx->saved_data["x"] = x.scalar_type();
+        ctx->saved_data["w"] = w.scalar_type();
+        return product(c, m, n, k, stored_operand(xc.codes, xc.scales, false, 1, 5), stored_operand(wc.codes, wc.scales, false, 128, 5), shape, x.scalar_type());
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, const torch::autograd::variable_list &grads)
+    {
+        torch::autograd::variable_list out(7);
+        const Tensor &g = grads[0];
+        const auto kept = ctx->get_saved_variables();
+        const Tensor &xd = kept[0], &xds = kept[1], &w8 = kept[2], &ws = kept[3];
+        if (!g.defined() || (!xd.defined() && !w8.defined())) return out;
+        const bool again = at::GradMode::is_enabled();
+        try {
+            at::NoGradGuard none;
+            const Call c = call_of(c10::static_intrusive_pointer_cast<Owner>(ctx->saved_data["owner"].toCapsule())->handle(), (int)ctx->saved_data["device"].toInt());
+            const int type = (int)ctx->saved_data["type"].toInt();
+            const Tensor gm = matrix(g);
+            const Coded gc = coded(c, gm, w8.defined() ? (xd.defined() ? 3 : 1) : 2, type);
+            const int64_t m = gm.size(0), n = gm.size(1);
+            if (w8.defined()) {
+                at::DimVector shape(g.sizes().begin(), g.sizes().end());
+                shape.back() = w8.size(1);
+                out[0] = product(c, m, w8.size(1), n, stored_operand(gc.codes, gc.scales, false, 1, type), stored_operand(w8, ws, true, 128, 5), shape,
+                                 ctx->saved_data["x"].toScalarType());
+            }
+            if (xd.defined())
+                out[1] = product(c, n, xd.size(1), m, stored_operand(gc.down, gc.down_scales, true, 1, type), stored_operand(xd, xds, true, 1, 5), {n, xd.size(1)},
+                                 ctx->saved_data["w"].toScalarType());
+        } catch (const Refused &e) { // this may be a thread of the autograd engine, which carries torch's exceptions to the caller
+            TORCH_CHECK_VALUE(e.code != LB_ERR_INVALID_ARG, e.message);
+            TORCH_CHECK(false, e.message);
+        }
+        if (again) { // gradients of the gradients are not there: whoever asks for them is told
+            torch::autograd::variable_list found;
+            for (Tensor &t : out)
+                if (t.defined()) found.push_back(t.detach().set_requires_grad(true));
+            const auto error = std::make_shared<torch::autograd::DelayedError>("the gradients of fp8_linear are not differentiable", (int64_t)found.size());
+            found = (*error)(std::move(found));
+            size_t i = 0;
+            for (Tensor &t : out)
+                if (t.defined()) t = found[i++];
+        }
+        return out;
+    }
+};
+
+Tensor fp8_linear(const py::object &lb, int device, const Tensor &x, const Tensor &w, int type)
+{
+    const Call c = call_of(lb.attr("_handle")().cast<int64_t>(), device);
+    if (x.dim() < 1 || w.dim() != 2 || x.size(-1) != w.size(1)) refuse("x must be [..., k] and w [n][k]");
+    if (type != 5 && type != 6) refuse("grad_dtype must be float8_e4m3fn or float8_e5m2");
+    const bool grad = at::GradMode::is_enabled();
+    return Fp8Linear::apply(x, w, c, c10::make_intrusive<Owner>(lb), type, grad && x.requires_grad(), grad && w.requires_grad());
 }
 
 // ---- clipping -------------------------------------------------------------------------------------------------------------------
@@ -467,6 +523,5 @@ PYBIND11_MODULE(_updates8, m)
     m.def("dequantize_fp8", &dequantize_fp8);
     m.def("fp8_matmul", &fp8_matmul);
     m.def("clip_updates", &clip_updates);
-    m.def("fp8_linear_forward", &fp8_linear_forward);
-    m.def("fp8_linear_backward", &fp8_linear_backward);
+    m.def("fp8_linear", &fp8_linear);
 }

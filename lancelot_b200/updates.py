@@ -111,29 +111,16 @@ def low_rank_update(lb, factors, out=None):
     return out
 
 
-class _Fp8Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, lb, x, w, grad_dtype):
-        y, *kept = lb.fp8_linear_forward(x, w, *ctx.needs_input_grad[1:3])
-        ctx.lb, ctx.types = lb, (grad_dtype, x.dtype, w.dtype)
-        ctx.save_for_backward(*kept)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        return None, *ctx.lb.fp8_linear_backward(g, *ctx.saved_tensors, *ctx.types), None
-
-
 def fp8_linear(lb, x, w, grad_dtype=torch.float8_e4m3fn):
     """y = x w^T with gradients, x [..., k], w [n][k] (float32, bfloat16, float16, on the device of lb): the three products of a training step in
     8-bit floating point.  x is quantised in blocks of 128 values along what a product sums over, w in blocks of 128 x 128; the gradient of y as x,
-    to grad_dtype.  y and the gradients have the types of x and of their tensors.  What is kept for the backward pass are the codes"""
+    to grad_dtype.  y and the gradients have the types of x and of their tensors.  What is kept for the backward pass are the codes.  The gradients
+    themselves are not differentiable.  In a graph capture take them with ``torch.autograd.grad``"""
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError("x must be [..., k] and w [n][k]")
     if grad_dtype not in FP8_TYPES:
         raise ValueError("grad_dtype must be float8_e4m3fn or float8_e5m2")
-    return _Fp8Linear.apply(lb, x, w, grad_dtype)
+    return lb.fp8_linear(x, w, grad_dtype)
 
 
 def flat_updates(lb, updates, max_norm=None, out=None, dtype=torch.float32):

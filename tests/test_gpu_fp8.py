@@ -442,6 +442,50 @@ def test_a_layers_step_on_an_empty_batch_and_on_transposed_operands(ctx):
         assert torch.equal(p, q)
 
 
+def test_gradients_of_gradients_and_a_context_closed_in_between():
+    import torch
+
+    from lancelot_b200 import cabi, updates
+
+    c = cabi.Context(12, cabi.coeff_modulus_create(1 << 12, [40, 40]), 1)
+    g = gen(14)
+    x = torch.randn(20, 150, generator=g, device="cuda").requires_grad_()
+    w = torch.randn(30, 150, generator=g, device="cuda").requires_grad_()
+    dx, dw = torch.autograd.grad(updates.fp8_linear(c, x, w).square().sum(), (x, w), create_graph=True)
+    want = torch.autograd.grad(updates.fp8_linear(c, x, w).square().sum(), (x, w))
+    assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        (dx.sum() + dw.sum()).backward()
+    y = updates.fp8_linear(c, x, w)
+    with torch.no_grad():
+        assert not updates.fp8_linear(c, x, w).requires_grad
+    c.close()
+    with pytest.raises(ValueError):
+        y.sum().backward()
+    with pytest.raises(ValueError):
+        updates.fp8_linear(c, x, w)
+
+
+def test_a_backward_pass_on_another_stream(ctx):
+    import torch
+
+    from lancelot_b200 import updates
+
+    g = gen(15)
+    x = torch.randn(200, 300, generator=g, device="cuda").requires_grad_()
+    w = torch.randn(100, 300, generator=g, device="cuda").requires_grad_()
+    dy = torch.randn(200, 100, generator=g, device="cuda")
+    want = torch.autograd.grad(updates.fp8_linear(ctx, x, w), (x, w), dy)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            y = updates.fp8_linear(ctx, x, w)
+            got = torch.autograd.grad(y, (x, w), dy)
+        side.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_a_captured_step(ctx):
     """forward and gradients replayed with other inputs, in two graphs at once that share the operands"""
     import torch
