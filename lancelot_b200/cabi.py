@@ -446,7 +446,7 @@ class Context:
         row, scales [n][ceil(cols / 128)]; (128, 1), 128 rows of a column, scales [ceil(n / 128)][cols]; (128, 128).  scale = the block's largest
         magnitude / the largest value of dtype; a code is the value nearest to value / scale, ties to even.  A block that holds an infinity or
         NaN reads as NaN.  codes, scales: where the results go (made here if not given, the codes' rows on 16-byte boundaries)"""
-        blocks = FP8_BLOCKS.get(tuple(block) if isinstance(block, (tuple, list)) else block, 0)
+        blocks = FP8_BLOCKS.get(block if isinstance(block, (tuple, int)) else tuple(block), 0)
         if blocks == 2:
             return _updates8().quantize_fp8(self._handle(), self.device, values, blocks, FP8_TYPES.get(dtype, 0), None, None, codes, scales)
         return _updates8().quantize_fp8(self._handle(), self.device, values, blocks, FP8_TYPES.get(dtype, 0), codes, scales, None, None)

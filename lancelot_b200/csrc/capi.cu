@@ -1051,6 +1051,8 @@ static size_t clip_bytes(int n_clients, int n_tensors, const int64_t *sizes)
 size_t lb_clip_updates_workspace_bytes(int n_clients, int n_tensors, const int64_t *sizes)
 {
     if (n_clients < 1 || n_tensors < 0 || (n_tensors && !sizes)) return 0;
+    for (int i = 0; i < n_tensors; ++i)
+        if (sizes[i] < 0) return 0;
     return clip_bytes(n_clients, n_tensors, sizes);
 }
 

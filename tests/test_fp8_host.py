@@ -62,6 +62,18 @@ def test_a_product_asks_for_a_workspace_only_where_rows_are_off_their_alignment(
     assert need(300, 500, 200, operand(1 << 20, 333, across=1), operand(1 << 20, 200)) == -(-200 * 304 // 256) * 256 + -(-500 * 208 // 256) * 256
 
 
+def test_clipping_asks_for_a_sum_for_every_piece():
+    import ctypes as C
+
+    from lancelot_b200 import lib
+
+    f = lib.lb_clip_updates_workspace_bytes
+    f.restype = C.c_size_t
+    sizes = (C.c_int64 * 4)(1, 1024, 1025, 0)
+    assert f(2, 4, sizes) == 8 * (2 + 1 + 1 + 2) and f(3, 0, None) == 24
+    assert f(0, 4, sizes) == 0 and f(2, 4, None) == 0 and f(1, 1, (C.c_int64 * 1)(-5)) == 0
+
+
 def test_a_layer_checks_its_shapes():
     from lancelot_b200 import updates
 
