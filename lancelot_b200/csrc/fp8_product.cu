@@ -118,7 +118,7 @@ template <typename T, bool ALIGNED> int launch_skinny(const SkinnyFp8Args &a, bo
 }
 
 // ---- tiles on tcgen05 -------------------------------------------------------------------------------------------------------
-template <int BN> struct TileFp8 {
+template <int BN, bool OFF> struct TileFp8 {
     static constexpr int kOutWarps = 8, kThreads = 128 + kOutWarps * 32;
     static constexpr int kCols = BN / 2; // columns of a thread: the warps of a quarter of TMEM's lanes take a half each
     static constexpr int kStageBytes = (kM + BN) * kK;
@@ -129,7 +129,8 @@ template <int BN> struct TileFp8 {
     static constexpr int kRun = kCols / 4 + 4;      // scales of every fourth pair of columns, and a gap that keeps the four runs in different banks
     static constexpr int kScaleFloats = kM + 8 * kRun; // of a stage: of the rows; of the columns of each half
     static constexpr int kBars = 2 * kStages + 2 * kBufs + 2 * kScaleStages + 1;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kScaleStages * kScaleFloats * 4 + 8 * kBars + 16;
+    static constexpr int kTurn = OFF ? 16 * 33 : 0; // of a warp: 16 rows of 32 results, to be written row by row
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + (kScaleStages * kScaleFloats + kOutWarps * kTurn) * 4 + 8 * kBars + 16;
 };
 
 struct Fp8Args {
@@ -162,8 +163,8 @@ __device__ __forceinline__ void copy4(unsigned to, const float *from) { asm vola
 // products (four of k = 32 a block) into one of two or four places in TMEM, and warps 4 to 11 scale a block's sums and add them to results that they keep
 // in registers: a scale is for 128 of the summed axis, so the sums have to leave TMEM that often.  A block of a tile 256 wide takes some 1050 cycles, of which the
 // products are 512 (the tensor cores are active in 51 % of the cycles): what bounds it is the chain from the products' end over the sums' way to the registers to the
-// next products, with two places for the sums, beside the 96 KB that shared memory takes in and gives out.  8192 x 8192 x 8192 takes 485 to 495 us (2.2 to 2.3 P
-// operations a second; among others of its kind 594 us, under the power cap), without the accumulating warps' work 423 us, without the products 323 us.  Two CTAs on
+// next products, with two places for the sums, beside the 96 KB that shared memory takes in and gives out.  8192 x 8192 x 8192 takes 485 to 505 us (2.2 P
+// operations a second; among others of its kind 570 us, under the power cap), without the accumulating warps' work 423 us, without the products 323 us.  Two CTAs on
 // a tile of 256 x 256, which move 64 KB a block, wait longer for one another than that saves (732 us).  With a scale per row of b there is a product
 // more for every sum: 4096 x 11008 x 4096 in 305 us.  Everything in the accumulating warps' chain costs what it takes: a vote a block 3 %,
 // scales through shared memory instead of a load ahead 25 % (with a scale per row, where loads are many, they gain 8 %).
@@ -171,15 +172,18 @@ __device__ __forceinline__ void copy4(unsigned to, const float *from) { asm vola
 // PER_ROW: b has a scale for each of its rows, otherwise one for 128.
 // SPLIT: few tiles and a long summed axis.  The blocks of a cluster take a tile together, a run of the axis each, and add up through one another's
 // shared memory, in the order of the runs: no second kernel, no atomics.  333 x 1111 x 2047 takes 8.2 us with it, 25.7 us without.
-template <typename T, int BN, bool PER_ROW, bool SPLIT>
-__global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+// OFF: the result's rows start on no 16-byte boundary: results are turned through shared memory, so that a warp writes 32 of a row at a time.
+// 8000 x 7999 x 1024 in bf16 takes 146 us so, 680 us where every thread writes its own row, and with 8000 columns 82 us.
+template <typename T, int BN, bool PER_ROW, bool SPLIT, bool OFF>
+__global__ void __launch_bounds__(TileFp8<BN, OFF>::kThreads, 1) fp8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                                               const Fp8Args a)
 {
-    using C = TileFp8<BN>;
+    using C = TileFp8<BN, OFF>;
     extern __shared__ unsigned char raw[];
     unsigned char *stages = reinterpret_cast<unsigned char *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     float *scales = reinterpret_cast<float *>(stages + C::kStages * C::kStageBytes); // [scale stage][kScaleFloats]
-    unsigned long long *bars = reinterpret_cast<unsigned long long *>(scales + C::kScaleStages * C::kScaleFloats);
+    float *turns = scales + C::kScaleStages * C::kScaleFloats; // [warp][kTurn]
+    unsigned long long *bars = reinterpret_cast<unsigned long long *>(turns + C::kOutWarps * C::kTurn);
     unsigned *tmem_at = reinterpret_cast<unsigned *>(bars + C::kBars);
     volatile int *failed = reinterpret_cast<volatile int *>(tmem_at + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -320,315 +324,352 @@ __global__ void __launch_bounds__(TileFp8<BN>::kThreads, 1) fp8_product_kernel(c
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
-        } else {
-            if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMany));
-            // A warp sees the 32 lanes of TMEM of its quarter, and takes half of the tile's columns.  With one scale for them a thread has a row; with a
-            // scale each it has, as in the results of a warp's own matrix instruction, two columns of every eight in four rows, so that it
-            // needs a quarter of the scales.
-            const int quarter = warp & 3, half = (warp - 4) / 4;
-            constexpr int kRows = PER_ROW ? 4 : 1;
-            int it = 0;
-            bool ok = true;
-            for (int t = tile0; t < tiles && ok; t += gridDim.x) {
-                int tm, tn;
-                tile_at(a, t, tm, tn);
-                const int row = tm * kM + quarter * 32 + (PER_ROW ? lane >> 2 : lane), col = tn * BN + half * C::kCols;
-                unsigned long long acc[C::kCols / 2];
-#pragma unroll
-                for (int e = 0; e < C::kCols / 2; ++e) acc[e] = 0;
-                // One scale for the columns: every thread fetches the two that it needs, a block ahead.  A scale each: two warps bring them into shared memory
-                const float *pa = a.a.at + (long)(min(row, a.m - 1) >> a.a.shift) * a.a.row + k0 * a.a.block, *pb = a.b.at + (long)(min(col, a.n - 1) >> a.b.shift) * a.b.row + k0 * a.b.block;
-                float next_row = 0.f, next_col = 0.f;
-                if (!PER_ROW && k0 < k1) next_row = __ldg(pa), next_col = __ldg(pb);
-                for (int k = k0; k < k1; ++k, ++it) {
-                    const int buf = it % C::kBufs, stage = it % C::kScaleStages;
-                    const float *row_scales = scales + stage * C::kScaleFloats + quarter * 32 + (lane >> 2);
-                    const float *col_scales = scales + stage * C::kScaleFloats + kM + half * 4 * C::kRun + (lane & 3) * C::kRun;
-                    unsigned long long ss[kRows];
-                    if (PER_ROW) {
-                        ok &= mbar_wait_inline(known + 8 * stage, (it / C::kScaleStages) & 1, failed);
-#pragma unroll
-                        for (int r = 0; r < kRows; ++r) ss[r] = pair(row_scales[8 * r], row_scales[8 * r]);
-                    } else {
-                        ss[0] = pair(next_row * next_col, next_row * next_col);
-                        if (k + 1 < k1) next_row = __ldg(pa += a.a.block), next_col = __ldg(pb += a.b.block);
-                    }
-                    ok &= mbar_wait_inline(done + 8 * buf, (it / C::kBufs) & 1, failed); // a warp whose wait ran out goes on, together, to the tile's end
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const unsigned from = tmem + buf * BN + half * C::kCols + ((unsigned)quarter << 21);
-                    constexpr int kW = PER_ROW ? 16 : 32;
-                    int v[2][kW];
-                    auto begin = [&](int step, int (&w)[kW]) { // 32 columns of 16 rows, the upper ones and then the lower ones; or 16 columns of all rows
-                        if constexpr (PER_ROW) tmem_begin_tiles(from + (step >> 1) * 32 + ((unsigned)(step & 1) << 20), w);
-                        else tmem_begin(from + step * 32, w);
-                    };
-                    begin(0, v[0]);
-#pragma unroll
-                    for (int step = 0; step < C::kCols / kW; ++step) {
-                        int(&w)[kW] = v[step & 1];
-                        tmem_ready(w);
-                        if (step + 1 < C::kCols / kW) begin(step + 1, v[(step & 1) ^ 1]);
-                        if constexpr (PER_ROW) {
-#pragma unroll
-                            for (int i = 0; i < 4; i += 2) { // eight columns, and the next eight
-                                const int eight = (step >> 1) * 4 + i, at = ((step & 1) * (C::kCols / 8) + eight) * 2, r = (step & 1) * 2;
-                                const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(col_scales + eight * 2);
-                                fma2(acc[at], mul2(pair(w[4 * i], w[4 * i + 1]), ss[r]), s4.x);
-                                fma2(acc[at + 1], mul2(pair(w[4 * i + 2], w[4 * i + 3]), ss[r + 1]), s4.x);
-                                fma2(acc[at + 2], mul2(pair(w[4 * i + 4], w[4 * i + 5]), ss[r]), s4.y);
-                                fma2(acc[at + 3], mul2(pair(w[4 * i + 6], w[4 * i + 7]), ss[r + 1]), s4.y);
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < kW; e += 2) fma2(acc[step * kW / 2 + e / 2], pair(w[e], w[e + 1]), ss[0]);
-                        }
-                    }
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(freed + 8 * buf);
-                        if (PER_ROW) mbar_arrive(used + 8 * stage);
-                    }
-                }
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (SPLIT) { // all products have been formed, so the stages are free
-                    float *to = reinterpret_cast<float *>(stages) + (quarter * 32 + (PER_ROW ? lane >> 2 : lane)) * C::kPitch + half * C::kCols + (PER_ROW ? (lane & 3) * 2 : 0);
-#pragma unroll
-                    for (int e = 0; e < C::kCols / 2; ++e) {
-                        float2 x;
-                        unpair(acc[e], x.x, x.y);
-                        *reinterpret_cast<float2 *>(PER_ROW ? to + ((e & 1) * 8 + e / (C::kCols / 4) * 16) * C::kPitch + (e % (C::kCols / 4) >> 1) * 8 : to + 2 * e) = x;
-                    }
-                } else if (PER_ROW) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (row + 8 * r >= a.m) continue;
-                        T *out = reinterpret_cast<T *>(a.out) + (long)(row + 8 * r) * a.out_stride + col + (lane & 3) * 2;
-#pragma unroll
-                        for (int i = 0; i < C::kCols / 8; ++i) {
-                            float x, y;
-                            unpair(acc[((r >> 1) * (C::kCols / 8) + i) * 2 + (r & 1)], x, y);
-                            const int left = a.n - col - (lane & 3) * 2 - i * 8;
-                            if (left >= 2 && a.align) {
-                                if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(out + i * 8) = make_float2(x, y);
-                                else *reinterpret_cast<unsigned *>(out + i * 8) = pack2(out, x, y);
-                            } else {
-                                if (left >= 1) put(out + i * 8, x);
-                                if (left >= 2) put(out + i * 8 + 1, y);
-                            }
-                        }
-                    }
-                } else if (row < a.m) {
-                    T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride + col;
-#pragma unroll
-                    for (int c = 0; c < C::kCols; c += 32) {
-                        float f[32];
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) unpair(acc[(c + e) / 2], f[e], f[e + 1]);
-                        if (col + c < a.n) put32(out + c, f, a.n - col - c, a.align);
-                    }
-                }
-            }
-        }
-        if (SPLIT) {
-            __syncwarp();
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMany));
+        // A warp sees the 32 lanes of TMEM of its quarter, and takes half of the tile's columns.  With one scale for them a thread has a row; with a
+        // scale each it has, as in the results of a warp's own matrix instruction, two columns of every eight in four rows, so that it
+        // needs a quarter of the scales.
+        const int quarter = warp & 3, half = (warp - 4) / 4;
+        constexpr int kRows = PER_ROW ? 4 : 1;
+        int it = 0;
+        bool ok = true;
+        for (int t = tile0; t < tiles && ok; t += gridDim.x) {
             int tm, tn;
-            tile_at(a, tile0, tm, tn);
-            const int rows = min(kM, a.m - tm * kM), cols = min(BN, a.n - tn * BN), all = rows * (BN / 4);
-            for (int i = (int)((long)all * rank / ranks) + (int)threadIdx.x; i < (int)((long)all * (rank + 1) / ranks); i += C::kThreads) {
-                const int r = i / (BN / 4), c = i % (BN / 4) * 4;
-                if (c >= cols) continue;
-                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (unsigned from = 0; from < ranks; ++from) {
-                    unsigned at;
-                    float4 v;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(stage0 + (r * C::kPitch + c) * 4), "r"(from));
-                    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-                    sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
-                }
-                T *out = reinterpret_cast<T *>(a.out) + (long)(tm * kM + r) * a.out_stride + tn * BN + c;
-                if (a.align && c + 4 <= cols) {
-                    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out) = sum;
-                    else *reinterpret_cast<uint2 *>(out) = make_uint2(pack2(out, sum.x, sum.y), pack2(out, sum.z, sum.w));
+            tile_at(a, t, tm, tn);
+            const int row = tm * kM + quarter * 32 + (PER_ROW ? lane >> 2 : lane), col = tn * BN + half * C::kCols;
+            unsigned long long acc[C::kCols / 2];
+#pragma unroll
+            for (int e = 0; e < C::kCols / 2; ++e) acc[e] = 0;
+            // One scale for the columns: every thread fetches the two that it needs, a block ahead.  A scale each: two warps bring them into shared memory
+            const float *pa = a.a.at + (long)(min(row, a.m - 1) >> a.a.shift) * a.a.row + k0 * a.a.block, *pb = a.b.at + (long)(min(col, a.n - 1) >> a.b.shift) * a.b.row + k0 * a.b.block;
+            float next_row = 0.f, next_col = 0.f;
+            if (!PER_ROW && k0 < k1) next_row = __ldg(pa), next_col = __ldg(pb);
+            for (int k = k0; k < k1; ++k, ++it) {
+                const int buf = it % C::kBufs, stage = it % C::kScaleStages;
+                const float *row_scales = scales + stage * C::kScaleFloats + quarter * 32 + (lane >> 2);
+                const float *col_scales = scales + stage * C::kScaleFloats + kM + half * 4 * C::kRun + (lane & 3) * C::kRun;
+                unsigned long long ss[kRows];
+                if (PER_ROW) {
+                    ok &= mbar_wait_inline(known + 8 * stage, (it / C::kScaleStages) & 1, failed);
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r) ss[r] = pair(row_scales[8 * r], row_scales[8 * r]);
                 } else {
-                    put(out, sum.x);
-                    if (c + 1 < cols) put(out + 1, sum.y);
-                    if (c + 2 < cols) put(out + 2, sum.z);
-                    if (c + 3 < cols) put(out + 3, sum.w);
+                    ss[0] = pair(next_row * next_col, next_row * next_col);
+                    if (k + 1 < k1) next_row = __ldg(pa += a.a.block), next_col = __ldg(pb += a.b.block);
+                }
+                ok &= mbar_wait_inline(done + 8 * buf, (it / C::kBufs) & 1, failed); // a warp whose wait ran out goes on, together, to the tile's end
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned from = tmem + buf * BN + half * C::kCols + ((unsigned)quarter << 21);
+                constexpr int kW = PER_ROW || OFF ? 16 : 32;
+                int v[2][kW];
+                auto begin = [&](int step, int (&w)[kW]) { // 32 columns of 16 rows, the upper ones and then the lower ones; or 16 columns of all rows
+                    if constexpr (PER_ROW) tmem_begin_tiles(from + (step >> 1) * 32 + ((unsigned)(step & 1) << 20), w);
+                    else tmem_begin(from + step * kW, w);
+                };
+                begin(0, v[0]);
+#pragma unroll
+                for (int step = 0; step < C::kCols / kW; ++step) {
+                    int(&w)[kW] = v[step & 1];
+                    tmem_ready(w);
+                    if (step + 1 < C::kCols / kW) begin(step + 1, v[(step & 1) ^ 1]);
+                    if constexpr (PER_ROW) {
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2) { // eight columns, and the next eight
+                            const int eight = (step >> 1) * 4 + i, at = ((step & 1) * (C::kCols / 8) + eight) * 2, r = (step & 1) * 2;
+                            const ulonglong2 s4 = *reinterpret_cast<const ulonglong2 *>(col_scales + eight * 2);
+                            fma2(acc[at], mul2(pair(w[4 * i], w[4 * i + 1]), ss[r]), s4.x);
+                            fma2(acc[at + 1], mul2(pair(w[4 * i + 2], w[4 * i + 3]), ss[r + 1]), s4.x);
+                            fma2(acc[at + 2], mul2(pair(w[4 * i + 4], w[4 * i + 5]), ss[r]), s4.y);
+                            fma2(acc[at + 3], mul2(pair(w[4 * i + 6], w[4 * i + 7]), ss[r + 1]), s4.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kW; e += 2) fma2(acc[step * kW / 2 + e / 2], pair(w[e], w[e + 1]), ss[0]);
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(freed + 8 * buf);
+                    if (PER_ROW) mbar_arrive(used + 8 * stage);
                 }
             }
-            __syncwarp();
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); // nobody leaves while it is read
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncthreads();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (threadIdx.x == 0 && *failed) atomicOr(a.status, 2);
-        if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kBufs * BN) : "memory");
-    }
-
-    template <typename T, int BN, bool PER_ROW, bool SPLIT>
-    int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const Fp8Args &a, int split, cudaStream_t stream)
-    {
-        using C = TileFp8<BN>;
-        const auto kernel = fp8_product_kernel<T, BN, PER_ROW, SPLIT>;
-        static std::atomic<bool> set[64]; // host threads that come here first at once all set the same attribute
-        if (ctx->device >= 64 || !set[ctx->device]) {
-            LB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-            if (BN == 256) {
-                cudaFuncAttributes has;
-                LB_CUDA(cudaFuncGetAttributes(&has, kernel));
-                if (has.numRegs < kEven) {
-                    set_error("the product's kernel was built with too few registers");
-                    return LB_ERR_LOGIC;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (SPLIT) { // all products have been formed, so the stages are free
+                float *to = reinterpret_cast<float *>(stages) + (quarter * 32 + (PER_ROW ? lane >> 2 : lane)) * C::kPitch + half * C::kCols + (PER_ROW ? (lane & 3) * 2 : 0);
+#pragma unroll
+                for (int e = 0; e < C::kCols / 2; ++e) {
+                    float2 x;
+                    unpair(acc[e], x.x, x.y);
+                    *reinterpret_cast<float2 *>(PER_ROW ? to + ((e & 1) * 8 + e / (C::kCols / 4) * 16) * C::kPitch + (e % (C::kCols / 4) >> 1) * 8 : to + 2 * e) = x;
+                }
+            } else if (OFF) { // turned through shared memory, so that a warp writes 32 results of a row at a time
+                float *turn = turns + (warp - 4) * C::kTurn;
+                const int first = tm * kM + quarter * 32;
+#pragma unroll
+                for (int c = 0; c < C::kCols; c += 32) {
+#pragma unroll
+                    for (int upper = 0; upper < 2; ++upper) {
+                        __syncwarp();
+                        if (PER_ROW) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int r = 0; r < 2; ++r) {
+                                    float x, y;
+                                    unpair(acc[(upper * (C::kCols / 8) + c / 8 + i) * 2 + r], x, y);
+                                    float *to = turn + ((lane >> 2) + 8 * r) * 33 + i * 8 + (lane & 3) * 2;
+                                    to[0] = x, to[1] = y;
+                                }
+                        } else if ((lane >> 4) == upper) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                float x, y;
+                                unpair(acc[(c + e) / 2], x, y);
+                                turn[(lane & 15) * 33 + e] = x, turn[(lane & 15) * 33 + e + 1] = y;
+                            }
+                        }
+                        __syncwarp();
+                        const int rows = min(16, a.m - first - upper * 16);
+                        T *to = reinterpret_cast<T *>(a.out) + (long)(first + upper * 16) * a.out_stride + col + c + lane;
+                        if (col + c + lane < a.n)
+                            for (int i = 0; i < rows; ++i, to += a.out_stride) put(to, turn[i * 33 + lane]);
+                    }
+                }
+            } else if (PER_ROW) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (row + 8 * r >= a.m) continue;
+                    T *out = reinterpret_cast<T *>(a.out) + (long)(row + 8 * r) * a.out_stride + col + (lane & 3) * 2;
+#pragma unroll
+                    for (int i = 0; i < C::kCols / 8; ++i) {
+                        float x, y;
+                        unpair(acc[((r >> 1) * (C::kCols / 8) + i) * 2 + (r & 1)], x, y);
+                        const int left = a.n - col - (lane & 3) * 2 - i * 8;
+                        if (left >= 2) {
+                            if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(out + i * 8) = make_float2(x, y);
+                            else *reinterpret_cast<unsigned *>(out + i * 8) = pack2(out, x, y);
+                        } else {
+                            if (left >= 1) put(out + i * 8, x);
+                            if (left >= 2) put(out + i * 8 + 1, y);
+                        }
+                    }
+                }
+            } else if (row < a.m) {
+                T *out = reinterpret_cast<T *>(a.out) + (long)row * a.out_stride + col;
+#pragma unroll
+                for (int c = 0; c < C::kCols; c += 32) {
+                    float f[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) unpair(acc[(c + e) / 2], f[e], f[e + 1]);
+                    if (col + c < a.n) put32(out + c, f, a.n - col - c, a.align);
                 }
             }
-            if (ctx->device < 64) set[ctx->device] = true;
         }
-        const int tiles = a.tiles_m * a.tiles_n;
-        cudaLaunchConfig_t c = {};
-        c.gridDim = dim3((unsigned)(SPLIT ? tiles * split : tiles < ctx->sm_count ? tiles : ctx->sm_count));
-        c.blockDim = dim3(C::kThreads);
-        c.dynamicSmemBytes = C::kSmem;
-        c.stream = stream;
-        cudaLaunchAttribute cluster;
-        cluster.id = cudaLaunchAttributeClusterDimension;
-        cluster.val.clusterDim.x = (unsigned)split;
-        cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-        c.attrs = &cluster;
-        c.numAttrs = SPLIT ? 1 : 0;
-        LB_CUDA(cudaLaunchKernelEx(&c, kernel, ma, mb, a));
-        return LB_OK;
     }
-    template <typename T, bool PER_ROW> int launch_any(const Context *ctx, int bn, const CUtensorMap &ma, const CUtensorMap &mb, const Fp8Args &a, int split, cudaStream_t stream)
-    {
-        if (split > 1) return bn == 128 ? launch_tiles<T, 128, PER_ROW, true>(ctx, ma, mb, a, split, stream) : launch_tiles<T, 64, PER_ROW, true>(ctx, ma, mb, a, split, stream);
-        if (bn == 256) return launch_tiles<T, 256, PER_ROW, false>(ctx, ma, mb, a, 1, stream);
-        return bn == 128 ? launch_tiles<T, 128, PER_ROW, false>(ctx, ma, mb, a, 1, stream) : launch_tiles<T, 64, PER_ROW, false>(ctx, ma, mb, a, 1, stream);
-    }
-
-    // an operand as it lies: rows of `cols` bytes
-    struct Stored {
-        long rows;
-        int cols;
-        bool off; // rows off a 16-byte boundary: TMA cannot read them
-        int pitch;
-    };
-    Stored stored(const Fp8Operand &o, int along, int k)
-    {
-        Stored s;
-        s.rows = o.across ? k : along;
-        s.cols = o.across ? along : k;
-        s.off = (uintptr_t)o.codes % 16 != 0 || (s.rows > 1 && o.stride % 16 != 0);
-        s.pitch = (s.cols + 15) / 16 * 16;
-        return s;
-    }
-    size_t packed_bytes(const Stored &s) { return s.off ? ((size_t)s.rows * s.pitch + 255) / 256 * 256 : 0; }
-
-    bool skinny(int m, int n, const Fp8Operand &a, const Fp8Operand &b) { return !a.across && !b.across && (m <= kSkinny || n <= kSkinny); }
-
-    template <typename T> int product_typed(Context *ctx, int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b, void *out, long out_stride, cudaStream_t stream)
-    {
-        if (skinny(m, n, a, b)) {
-            const bool turned = m > n; // the long side is the rows of a
-            const Fp8Operand &w = turned ? a : b, &x = turned ? b : a;
-            SkinnyFp8Args s;
-            s.w = reinterpret_cast<const signed char *>(w.codes);
-            s.x = reinterpret_cast<const signed char *>(x.codes);
-            s.w_stride = w.stride;
-            s.x_stride = x.stride;
-            s.ws = {w.scales, w.scale_row, w.scale_block, w.scale_shift};
-            s.xs = {x.scales, x.scale_row, x.scale_block, x.scale_shift};
-            s.rows = turned ? m : n;
-            s.cols = turned ? n : m;
-            s.k = k;
-            s.out = out;
-            s.row_step = turned ? out_stride : 1;
-            s.col_step = turned ? 1 : out_stride;
-            count_launch("fp8_skinny", stream, (double)m * k + (double)n * k + (double)m * n * sizeof(T));
-            const bool off = k % 16 != 0 || stored(a, m, k).off || stored(b, n, k).off;
-            return off ? launch_skinny<T, false>(s, w.type == 6, x.type == 6, stream) : launch_skinny<T, true>(s, w.type == 6, x.type == 6, stream);
-        }
-        Fp8Args p;
-        p.m = m;
-        p.n = n;
-        p.k_blocks = (k + kK - 1) / kK;
-        p.tiles_m = (m + kM - 1) / kM;
-        p.a_across = a.across;
-        p.b_across = b.across;
-        p.a = {a.scales, a.scale_row, a.scale_block, a.scale_shift};
-        p.b = {b.scales, b.scale_row, b.scale_block, b.scale_shift};
-        p.out = out;
-        p.out_stride = out_stride;
-        const uintptr_t at = (uintptr_t)out | (uintptr_t)(out_stride * (long)sizeof(T));
-        p.align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
-        p.status = ctx->d_status;
-        p.band = 8;
-        // The tile, and the CTAs that share one, that take least, in microseconds as measured: waves over the SMs, in each a block of the summed axis at
-        // what one takes (by shared memory and the accumulating warps; with a scale per row of b by the latter), and a tile's results; a split adds two.
-        // 2048 x 2048 x 2048 takes 12.7 us with tiles 256 wide and 16.3 with 128, 4096 x 4096 x 64 14.3 and 13.5; 100 x 100 x 4096 7.0 us split
-        // over eight and 18.8 by one.
-        int bn = 128, split = 1;
-        double least = 0.0;
-        const bool per_row = b.scale_shift == 0;
-        for (int w = b.across ? 128 : 64; w <= 256; w *= 2)
-            for (int parts = 1; parts <= 8 && parts <= p.k_blocks; ++parts) {
-                const long tiles = (long)p.tiles_m * ((n + w - 1) / w), blocks = tiles * parts, waves = (blocks + ctx->sm_count - 1) / ctx->sm_count;
-                if (parts > 1 && (w == 256 || blocks > ctx->sm_count - ctx->sm_count / 8)) break; // clusters do not fill every group of SMs
-                const int k = (p.k_blocks + parts - 1) / parts;
-                const double block = per_row ? 0.06 + w * 3.3e-3 : w == 64 ? 0.3 : 0.16 + w * 1.33e-3;
-                const double us = (double)waves * (k * block + w * 14e-3) + (parts > 1 ? 2.0 : 0.0);
-                if (least == 0.0 || us < least) {
-                    least = us;
-                    bn = w;
-                    split = parts;
-                }
+    if (SPLIT) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        int tm, tn;
+        tile_at(a, tile0, tm, tn);
+        const int rows = min(kM, a.m - tm * kM), cols = min(BN, a.n - tn * BN), all = rows * (BN / 4);
+        for (int i = (int)((long)all * rank / ranks) + (int)threadIdx.x; i < (int)((long)all * (rank + 1) / ranks); i += C::kThreads) {
+            const int r = i / (BN / 4), c = i % (BN / 4) * 4;
+            if (c >= cols) continue;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (unsigned from = 0; from < ranks; ++from) {
+                unsigned at;
+                float4 v;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(stage0 + (r * C::kPitch + c) * 4), "r"(from));
+                asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+                sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
             }
-        p.tiles_n = (n + bn - 1) / bn;
-        // D 32-bit floats; the operands' types, and bits 15 and 16 where the summed axis lies across their rows
-        p.desc = (unsigned)(bn >> 3) << 17 | (unsigned)(kM >> 4) << 24 | 1u << 4 | (unsigned)(a.type == 6) << 7 | (unsigned)(b.type == 6) << 10 | (unsigned)a.across << 15 |
-                 (unsigned)b.across << 16;
-        const Stored sa = stored(a, m, k), sb = stored(b, n, k);
-        CUtensorMap ma, mb;
-        int rc = encode_map(&ma, a.codes, sa.rows, sa.cols, sa.rows > 1 ? a.stride : sa.pitch, 128, 128);
-        if (rc) return rc;
-        if ((rc = encode_map(&mb, b.codes, sb.rows, sb.cols, sb.rows > 1 ? b.stride : sb.pitch, 128, b.across ? 128 : bn))) return rc;
-        count_launch("fp8_tiles", stream, (double)m * k + (double)n * k + (double)m * n * sizeof(T));
-        return per_row ? launch_any<T, true>(ctx, bn, ma, mb, p, split, stream) : launch_any<T, false>(ctx, bn, ma, mb, p, split, stream);
-    }
-
-    } // namespace
-
-    size_t fp8_matmul_workspace_bytes(int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b)
-    {
-        return skinny(m, n, a, b) ? 0 : packed_bytes(stored(a, m, k)) + packed_bytes(stored(b, n, k));
-    }
-
-    int fp8_matmul(Context *ctx, int m, int n, int k, Fp8Operand a, Fp8Operand b, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream)
-    {
-        signed char *ws = reinterpret_cast<signed char *>(workspace);
-        for (int i = 0; i < 2; ++i) { // operands that TMA cannot read
-            Fp8Operand &o = i ? b : a;
-            const Stored s = stored(o, i ? n : m, k);
-            if (!s.off || skinny(m, n, a, b)) continue;
-            const Packed one = {reinterpret_cast<const signed char *>(o.codes), o.stride, s.rows, ws}, none = {nullptr, 0, 0, nullptr};
-            int log_lanes = 0;
-            while (log_lanes < 8 && 16 << log_lanes < s.pitch) ++log_lanes;
-            const long blocks = (s.rows + (256 >> log_lanes) - 1) >> (8 - log_lanes), most = (long)ctx->sm_count * 32;
-            count_launch("fp8_pack", stream, 2.0 * s.rows * s.cols);
-            pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(one, none, s.cols, s.pitch, log_lanes);
-            LB_CUDA(cudaGetLastError());
-            o.codes = reinterpret_cast<unsigned char *>(ws);
-            o.stride = s.pitch;
-            ws += packed_bytes(s);
+            T *out = reinterpret_cast<T *>(a.out) + (long)(tm * kM + r) * a.out_stride + tn * BN + c;
+            if (a.align && c + 4 <= cols) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out) = sum;
+                else *reinterpret_cast<uint2 *>(out) = make_uint2(pack2(out, sum.x, sum.y), pack2(out, sum.z, sum.w));
+            } else {
+                put(out, sum.x);
+                if (c + 1 < cols) put(out + 1, sum.y);
+                if (c + 2 < cols) put(out + 2, sum.z);
+                if (c + 3 < cols) put(out + 3, sum.w);
+            }
         }
-        switch (dtype) {
-        case 1: return product_typed<float>(ctx, m, n, k, a, b, out, out_stride, stream);
-        case 3: return product_typed<__nv_bfloat16>(ctx, m, n, k, a, b, out, out_stride, stream);
-        default: return product_typed<__half>(ctx, m, n, k, a, b, out, out_stride, stream);
-        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); // nobody leaves while it is read
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (threadIdx.x == 0 && *failed) atomicOr(a.status, 2);
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kBufs * BN) : "memory");
+}
 
-    } // namespace lb
+template <typename T, int BN, bool PER_ROW, bool SPLIT, bool OFF>
+int launch_tiles(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const Fp8Args &a, int split, cudaStream_t stream)
+{
+    using C = TileFp8<BN, OFF>;
+    const auto kernel = fp8_product_kernel<T, BN, PER_ROW, SPLIT, OFF>;
+    static std::atomic<bool> set[64]; // host threads that come here first at once all set the same attribute
+    if (ctx->device >= 64 || !set[ctx->device]) {
+        LB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        if (BN == 256) {
+            cudaFuncAttributes has;
+            LB_CUDA(cudaFuncGetAttributes(&has, kernel));
+            if (has.numRegs < kEven) {
+                set_error("the product's kernel was built with too few registers");
+                return LB_ERR_LOGIC;
+            }
+        }
+        if (ctx->device < 64) set[ctx->device] = true;
+    }
+    const int tiles = a.tiles_m * a.tiles_n;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)(SPLIT ? tiles * split : tiles < ctx->sm_count ? tiles : ctx->sm_count));
+    c.blockDim = dim3(C::kThreads);
+    c.dynamicSmemBytes = C::kSmem;
+    c.stream = stream;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = (unsigned)split;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    c.attrs = &cluster;
+    c.numAttrs = SPLIT ? 1 : 0;
+    LB_CUDA(cudaLaunchKernelEx(&c, kernel, ma, mb, a));
+    return LB_OK;
+}
+template <typename T, int BN, bool PER_ROW> int launch_whole(const Context *ctx, const CUtensorMap &ma, const CUtensorMap &mb, const Fp8Args &a, cudaStream_t stream)
+{
+    return a.align ? launch_tiles<T, BN, PER_ROW, false, false>(ctx, ma, mb, a, 1, stream) : launch_tiles<T, BN, PER_ROW, false, true>(ctx, ma, mb, a, 1, stream);
+}
+template <typename T, bool PER_ROW> int launch_any(const Context *ctx, int bn, const CUtensorMap &ma, const CUtensorMap &mb, const Fp8Args &a, int split, cudaStream_t stream)
+{
+    if (split > 1) return bn == 128 ? launch_tiles<T, 128, PER_ROW, true, false>(ctx, ma, mb, a, split, stream) : launch_tiles<T, 64, PER_ROW, true, false>(ctx, ma, mb, a, split, stream);
+    if (bn == 256) return launch_whole<T, 256, PER_ROW>(ctx, ma, mb, a, stream);
+    return bn == 128 ? launch_whole<T, 128, PER_ROW>(ctx, ma, mb, a, stream) : launch_whole<T, 64, PER_ROW>(ctx, ma, mb, a, stream);
+}
+
+// an operand as it lies: rows of `cols` bytes
+struct Stored {
+    long rows;
+    int cols;
+    bool off; // rows off a 16-byte boundary: TMA cannot read them
+    int pitch;
+};
+Stored stored(const Fp8Operand &o, int along, int k)
+{
+    Stored s;
+    s.rows = o.across ? k : along;
+    s.cols = o.across ? along : k;
+    s.off = (uintptr_t)o.codes % 16 != 0 || (s.rows > 1 && o.stride % 16 != 0);
+    s.pitch = (s.cols + 15) / 16 * 16;
+    return s;
+}
+size_t packed_bytes(const Stored &s) { return s.off ? ((size_t)s.rows * s.pitch + 255) / 256 * 256 : 0; }
+
+bool skinny(int m, int n, const Fp8Operand &a, const Fp8Operand &b) { return !a.across && !b.across && (m <= kSkinny || n <= kSkinny); }
+
+template <typename T> int product_typed(Context *ctx, int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b, void *out, long out_stride, cudaStream_t stream)
+{
+    if (skinny(m, n, a, b)) {
+        const bool turned = m > n; // the long side is the rows of a
+        const Fp8Operand &w = turned ? a : b, &x = turned ? b : a;
+        SkinnyFp8Args s;
+        s.w = reinterpret_cast<const signed char *>(w.codes);
+        s.x = reinterpret_cast<const signed char *>(x.codes);
+        s.w_stride = w.stride;
+        s.x_stride = x.stride;
+        s.ws = {w.scales, w.scale_row, w.scale_block, w.scale_shift};
+        s.xs = {x.scales, x.scale_row, x.scale_block, x.scale_shift};
+        s.rows = turned ? m : n;
+        s.cols = turned ? n : m;
+        s.k = k;
+        s.out = out;
+        s.row_step = turned ? out_stride : 1;
+        s.col_step = turned ? 1 : out_stride;
+        count_launch("fp8_skinny", stream, (double)m * k + (double)n * k + (double)m * n * sizeof(T));
+        const bool off = k % 16 != 0 || stored(a, m, k).off || stored(b, n, k).off;
+        return off ? launch_skinny<T, false>(s, w.type == 6, x.type == 6, stream) : launch_skinny<T, true>(s, w.type == 6, x.type == 6, stream);
+    }
+    Fp8Args p;
+    p.m = m;
+    p.n = n;
+    p.k_blocks = (k + kK - 1) / kK;
+    p.tiles_m = (m + kM - 1) / kM;
+    p.a_across = a.across;
+    p.b_across = b.across;
+    p.a = {a.scales, a.scale_row, a.scale_block, a.scale_shift};
+    p.b = {b.scales, b.scale_row, b.scale_block, b.scale_shift};
+    p.out = out;
+    p.out_stride = out_stride;
+    const uintptr_t at = (uintptr_t)out | (uintptr_t)(out_stride * (long)sizeof(T));
+    p.align = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
+    p.status = ctx->d_status;
+    p.band = 8;
+    // The tile, and the CTAs that share one, that take least, in microseconds as measured: waves over the SMs, in each a block of the summed axis at
+    // what one takes (by shared memory and the accumulating warps; with a scale per row of b by the latter), and a tile's results; a split adds two.
+    // 2048 x 2048 x 2048 takes 12.7 us with tiles 256 wide and 16.3 with 128, 4096 x 4096 x 64 14.3 and 13.5; 100 x 100 x 4096 7.0 us split
+    // over eight and 18.8 by one.
+    int bn = 128, split = 1;
+    double least = 0.0;
+    const bool per_row = b.scale_shift == 0;
+    for (int w = b.across ? 128 : 64; w <= 256; w *= 2)
+        for (int parts = 1; parts <= 8 && parts <= p.k_blocks; ++parts) {
+            const long tiles = (long)p.tiles_m * ((n + w - 1) / w), blocks = tiles * parts, waves = (blocks + ctx->sm_count - 1) / ctx->sm_count;
+            if (parts > 1 && (w == 256 || blocks > ctx->sm_count - ctx->sm_count / 8)) break; // clusters do not fill every group of SMs
+            const int k = (p.k_blocks + parts - 1) / parts;
+            const double block = per_row ? 0.06 + w * 3.3e-3 : w == 64 ? 0.3 : 0.16 + w * 1.33e-3;
+            const double us = (double)waves * (k * block + w * 14e-3) + (parts > 1 ? 2.0 : 0.0);
+            if (least == 0.0 || us < least) {
+                least = us;
+                bn = w;
+                split = parts;
+            }
+        }
+    p.tiles_n = (n + bn - 1) / bn;
+    // D 32-bit floats; the operands' types, and bits 15 and 16 where the summed axis lies across their rows
+    p.desc = (unsigned)(bn >> 3) << 17 | (unsigned)(kM >> 4) << 24 | 1u << 4 | (unsigned)(a.type == 6) << 7 | (unsigned)(b.type == 6) << 10 | (unsigned)a.across << 15 |
+             (unsigned)b.across << 16;
+    const Stored sa = stored(a, m, k), sb = stored(b, n, k);
+    CUtensorMap ma, mb;
+    int rc = encode_map(&ma, a.codes, sa.rows, sa.cols, sa.rows > 1 ? a.stride : sa.pitch, 128, 128);
+    if (rc) return rc;
+    if ((rc = encode_map(&mb, b.codes, sb.rows, sb.cols, sb.rows > 1 ? b.stride : sb.pitch, 128, b.across ? 128 : bn))) return rc;
+    count_launch("fp8_tiles", stream, (double)m * k + (double)n * k + (double)m * n * sizeof(T));
+    return per_row ? launch_any<T, true>(ctx, bn, ma, mb, p, split, stream) : launch_any<T, false>(ctx, bn, ma, mb, p, split, stream);
+}
+
+} // namespace
+
+size_t fp8_matmul_workspace_bytes(int m, int n, int k, const Fp8Operand &a, const Fp8Operand &b)
+{
+    return skinny(m, n, a, b) ? 0 : packed_bytes(stored(a, m, k)) + packed_bytes(stored(b, n, k));
+}
+
+int fp8_matmul(Context *ctx, int m, int n, int k, Fp8Operand a, Fp8Operand b, void *out, int dtype, long out_stride, void *workspace, cudaStream_t stream)
+{
+    signed char *ws = reinterpret_cast<signed char *>(workspace);
+    for (int i = 0; i < 2; ++i) { // operands that TMA cannot read
+        Fp8Operand &o = i ? b : a;
+        const Stored s = stored(o, i ? n : m, k);
+        if (!s.off || skinny(m, n, a, b)) continue;
+        const Packed one = {reinterpret_cast<const signed char *>(o.codes), o.stride, s.rows, ws}, none = {nullptr, 0, 0, nullptr};
+        int log_lanes = 0;
+        while (log_lanes < 8 && 16 << log_lanes < s.pitch) ++log_lanes;
+        const long blocks = (s.rows + (256 >> log_lanes) - 1) >> (8 - log_lanes), most = (long)ctx->sm_count * 32;
+        count_launch("fp8_pack", stream, 2.0 * s.rows * s.cols);
+        pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(one, none, s.cols, s.pitch, log_lanes);
+        LB_CUDA(cudaGetLastError());
+        o.codes = reinterpret_cast<unsigned char *>(ws);
+        o.stride = s.pitch;
+        ws += packed_bytes(s);
+    }
+    switch (dtype) {
+    case 1: return product_typed<float>(ctx, m, n, k, a, b, out, out_stride, stream);
+    case 3: return product_typed<__nv_bfloat16>(ctx, m, n, k, a, b, out, out_stride, stream);
+    default: return product_typed<__half>(ctx, m, n, k, a, b, out, out_stride, stream);
+    }
+}
+
+} // namespace lb
