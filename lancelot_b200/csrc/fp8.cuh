@@ -70,7 +70,7 @@ __device__ __forceinline__ float fma_sat(float a, float b, float c) // cut to [0
 }
 
 // The code nearest to m / s, m >= 0, decided exactly.  q = m * (1 / s) in 32 bits is within two steps of the quotient.  The codes on either side of q
-// have the border h between them, of five bits at most, and the sign of d = h s - m, exact in one fused multiply-add for s >= 2^-80, says on which
+// have the border h between them, of five bits at most, and the sign of d = m - h s, exact in one fused multiply-add for s >= 2^-80, says on which
 // side of it the quotient lies, 0 that it lies on it.  So what is rounded to a code is not q but h (1 - 2^-10), h or h (1 + 2^-10): a tie goes to the
 // even code.  (Where q itself lies next to a code, on the wrong side of it, the border next to q still sends it to that code.)  Below the
 // least normal number the codes are evenly spaced; that number added to q brings their borders to the same bits.  Choices are made by
@@ -86,11 +86,12 @@ template <bool E5M2> __device__ __forceinline__ unsigned long long beside_border
     unpair(q, q0, q1);
     const unsigned long long y = pair(fma_sat(q0, -0x1p60f, F::kNormal * 0x1p60f), fma_sat(q1, -0x1p60f, F::kNormal * 0x1p60f)); // 1: below the normal numbers
     unpair(fma2_of(y, pair(F::kNormal, F::kNormal), q), w0, w1);
-    const unsigned long long h = fma2_of(y, pair(-F::kNormal, -F::kNormal), pair(__uint_as_float((__float_as_uint(w0) & ~F::kLow) | F::kHalf),
-                                                                                 __uint_as_float((__float_as_uint(w1) & ~F::kLow) | F::kHalf)));
-    unpair(fma2_of(h, s, mul2(m, pair(-1.f, -1.f))), d0, d1);
+    // -h, which spares turning m
+    const unsigned long long h = fma2_of(y, pair(F::kNormal, F::kNormal), pair(__uint_as_float((__float_as_uint(w0) & ~F::kLow) | (F::kHalf | 0x80000000u)),
+                                                                               __uint_as_float((__float_as_uint(w1) & ~F::kLow) | (F::kHalf | 0x80000000u))));
+    unpair(fma2_of(h, s, m), d0, d1);
     const unsigned long long z = pair(fma_sat(d0, 0x1p125f, 0.5f), fma_sat(d1, 0x1p125f, 0.5f)); // d is a multiple of 2^-120
-    return mul2(h, fma2_of(z, pair(-0x1p-9f, -0x1p-9f), pair(1.f + 0x1p-10f, 1.f + 0x1p-10f)));
+    return mul2(h, fma2_of(z, pair(-0x1p-9f, -0x1p-9f), pair(-1.f + 0x1p-10f, -1.f + 0x1p-10f)));
 }
 // smaller scales: a quotient of 64 bits, rounded to 24 in a way that keeps what lies beyond them in the last bit, so that rounding once more is
 // right.  0 where there is no scale, or one that is not finite
