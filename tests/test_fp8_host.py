@@ -22,6 +22,50 @@ def test_the_extension_refuses_tensors_that_are_not_on_the_device():
         m.clip_updates(0, 0, [], -1.0, None)
 
 
+class Made:
+    """a sequence that makes its items when they are asked for, and keeps none"""
+
+    def __init__(self, make, n, log=None, name=None):
+        self.make, self.n, self.log, self.name = make, n, log if log is not None else [], name
+
+    def __len__(self):
+        return self.n
+
+    def __getitem__(self, i):
+        if i >= self.n:
+            raise IndexError(i)
+        self.log.append(("read", self.name))
+        return self.make(i)
+
+    def __del__(self):
+        self.log.append(("gone", self.name))
+
+
+def test_clients_that_are_made_on_access_are_held_while_they_are_read():
+    from lancelot_b200._lib import InvalidArgument
+    from lancelot_b200.pybind import _updates8 as m
+
+    for out, most in ((None, None), (None, 1.0), (torch.zeros(2, 6), 1.0)):
+        log = []
+        updates = Made(lambda c: Made(lambda i: torch.zeros(3), 2, log, c), 2)
+        with pytest.raises(InvalidArgument, match="cuda:0"):
+            m.clip_updates(0, 0, updates, most, out)
+        for c in range(2):
+            mine = [what for what, name in log if name == c]
+            assert mine and "gone" not in mine[:-1] and mine.count("read") == 2
+    # an inner list that its owner fills anew for every client, and a sequence that fails
+    box = []
+
+    def refill(c):
+        box[:] = [torch.zeros(3)]
+        return box
+
+    with pytest.raises(InvalidArgument, match="cuda:0"):
+        m.clip_updates(0, 0, Made(refill, 3), 1.0, None)
+    with pytest.raises(ZeroDivisionError):
+        m.clip_updates(0, 0, Made(lambda c: 1 // 0, 3), 1.0, None)
+    with pytest.raises(ZeroDivisionError):
+        m.clip_updates(0, 0, [Made(lambda c: 1 // 0, 3)], 1.0, None)
 
 
 def operand(codes, stride, across=0, code_type=5, scales=4096, scale_row=1, scale_block=1, scale_rows=1):

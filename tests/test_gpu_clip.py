@@ -148,6 +148,41 @@ def test_clients_without_values_and_without_tensors(ctx):
     assert ctx.clip_updates(torch.zeros(3, 0, device="cuda"), 1.0).tolist() == [0, 0, 0]
 
 
+def test_updates_that_are_made_on_access(ctx):
+    """nobody but the call holds the tensors: their memory is not for its scratch and its results"""
+    import torch
+
+    class Made:
+        def __init__(self, make, n):
+            self.make, self.n = make, n
+
+        def __len__(self):
+            return self.n
+
+        def __getitem__(self, i):
+            if i >= self.n:
+                raise IndexError(i)
+            return self.make(i)
+
+    sizes = [3, 64, 40, 70001]  # some of the size of the norms and the scratch
+    base = [torch.randn(sum(sizes), generator=gen(20 + c), device="cuda") for c in range(8)]
+    at = [sum(sizes[:i]) for i in range(5)]
+    plain = [[b[x:y] for x, y in zip(at, at[1:])] for b in base]
+    box = []
+
+    def refill(c):  # the same list for every client
+        box[:] = [t.clone() for t in plain[c]]
+        return box
+
+    for updates in (Made(lambda c: Made(lambda i: plain[c][i] * 1, 4), 8), Made(refill, 8)):
+        norms = ctx.clip_updates(updates)
+        assert torch.equal(norms, ctx.clip_updates(plain))
+        out = torch.empty(8, sum(sizes), device="cuda")
+        assert torch.equal(ctx.clip_updates(updates, 200.0, out=out), norms)
+        for o, b, norm in zip(out, base, norms.tolist()):
+            assert torch.equal(o, clipped(b, factor(norm, 200.0)))
+
+
 def test_values_that_are_not_finite_large_and_small(ctx):
     import torch
 
