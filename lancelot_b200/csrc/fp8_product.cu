@@ -357,7 +357,8 @@ __global__ void __launch_bounds__(TileFp8<BN, OFF>::kThreads, 1) fp8_product_ker
                     ss[0] = pair(next_row * next_col, next_row * next_col);
                     if (k + 1 < k1) next_row = __ldg(pa += a.a.block), next_col = __ldg(pb += a.b.block);
                 }
-                ok &= mbar_wait_inline(done + 8 * buf, (it / C::kBufs) & 1, failed); // a warp whose wait ran out goes on, together, to the tile's end
+                ok &= mbar_wait_inline(done + 8 * buf, (it / C::kBufs) & 1, failed); // a warp whose wait ran out goes on to the tile's end
+                __syncwarp(); // every lane has waited for itself, in as many turns as it took: loads out of TMEM want the whole warp at once
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned from = tmem + buf * BN + half * C::kCols + ((unsigned)quarter << 21);
                 constexpr int kW = PER_ROW || OFF ? 16 : 32;

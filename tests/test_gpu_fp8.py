@@ -301,6 +301,27 @@ def test_scales_that_are_not_finite_or_zero_in_products(ctx):
     assert bool((out[1] == math.inf).all()) and bool(out[2].isnan().all()) and not out[0].any() and not out[3].any()
 
 
+@pytest.mark.parametrize("form", ["forward", "weight", "squares"])
+@pytest.mark.parametrize("m,n,k", [(300, 1100, 1300), (2500, 2300, 2100), (129, 65, 4000)])
+def test_products_among_others_are_the_same_every_time(ctx, form, m, n, k):
+    """two streams at once, so that the warps that take sums out wait in ever other turns; whole tiles, and rows that end within one"""
+    import torch
+
+    g = gen(m)
+    block_a, block_b, across_a, across_b = FORMS[form]
+    a, sa, va = operand(g, m, k, "e4m3", block_a, across_a)
+    b, sb, vb = operand(g, n, k, "e4m3", block_b, across_b)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(ctx.fp8_matmul(a, sa, b, sb, dtype=torch.float32))
+    torch.cuda.synchronize()
+    assert all(torch.equal(outs[0], o) for o in outs)
+    check_product(outs[0], va, vb, k)
+    ctx.check_status()
+
+
 def test_empty_products_and_scales_of_any_stride(ctx):
     import torch
 
