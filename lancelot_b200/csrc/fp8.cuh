@@ -62,6 +62,12 @@ __device__ __forceinline__ unsigned long long fma2_of(unsigned long long a, unsi
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
     return v;
 }
+__device__ __forceinline__ unsigned long long fma2_towards_zero(unsigned long long a, unsigned long long b, unsigned long long c)
+{
+    unsigned long long v;
+    asm("fma.rz.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
 __device__ __forceinline__ float fma_sat(float a, float b, float c) // cut to [0, 1]
 {
     float v;
@@ -73,7 +79,8 @@ __device__ __forceinline__ float fma_sat(float a, float b, float c) // cut to [0
 // have the border h between them, of five bits at most, and the sign of d = m - h s, exact in one fused multiply-add for s >= 2^-80, says on which
 // side of it the quotient lies, 0 that it lies on it.  So what is rounded to a code is not q but h (1 - 2^-10), h or h (1 + 2^-10): a tie goes to the
 // even code.  (Where q itself lies next to a code, on the wrong side of it, the border next to q still sends it to that code.)  Below the
-// least normal number the codes are evenly spaced; that number added to q brings their borders to the same bits.  Choices are made by
+// least normal number the codes are evenly spaced; that number added to q brings their borders to the same bits (rounded towards zero: the last q below it,
+// rounded to nearest, would make twice that number, where borders are spaced twice as far).  Choices are made by
 // multiply-adds cut to [0, 1], which cost half of what comparisons do, and nothing depends on how often values lie next to a border: 16-bit
 // values often lie on one.
 constexpr float kTinyScale = 0x1p-80f;
@@ -85,7 +92,7 @@ template <bool E5M2> __device__ __forceinline__ unsigned long long beside_border
     float q0, q1, w0, w1, d0, d1;
     unpair(q, q0, q1);
     const unsigned long long y = pair(fma_sat(q0, -0x1p60f, F::kNormal * 0x1p60f), fma_sat(q1, -0x1p60f, F::kNormal * 0x1p60f)); // 1: below the normal numbers
-    unpair(fma2_of(y, pair(F::kNormal, F::kNormal), q), w0, w1);
+    unpair(fma2_towards_zero(y, pair(F::kNormal, F::kNormal), q), w0, w1);
     // -h, which spares turning m
     const unsigned long long h = fma2_of(y, pair(F::kNormal, F::kNormal), pair(__uint_as_float((__float_as_uint(w0) & ~F::kLow) | (F::kHalf | 0x80000000u)),
                                                                                __uint_as_float((__float_as_uint(w1) & ~F::kLow) | (F::kHalf | 0x80000000u))));

@@ -124,6 +124,63 @@ def test_borders_between_codes_are_decided_exactly(ctx, code, block):
 
 @pytest.mark.parametrize("code", sorted(CODES))
 @pytest.mark.parametrize("block", sorted(BLOCKS))
+def test_values_at_and_beside_every_code_and_every_border(ctx, code, block):
+    """up to two steps of 32 bits beside, under many scales; the quotient that decides may itself be two steps off"""
+    import torch
+
+    _, bits, least, most = CODES[code]
+    levels = [math.ldexp(f, least - bits) for f in range(1 << bits)]
+    levels += [math.ldexp((1 << bits) + f, e + least - bits) for e in range(40) for f in range(1 << bits)]
+    levels = torch.tensor([x for x in levels if x <= most], dtype=torch.float64, device="cuda")
+    every = torch.cat([levels, (levels[1:] + levels[:-1]) / 2])
+    every = torch.cat([every, every[(every >= 2.0 ** (least - 1)) & (every <= 2.0 ** (least + 1))].repeat(8)])  # around the least normal number
+    h, w = BLOCKS[block]
+    rows, cols = {"rows": (4096, 1024), "columns": (1024, 4096), "square": (6400, 6400)}[block]
+    for seed in range(2):
+        g = gen(30 + seed)
+        top = torch.rand(-(-rows // h), -(-cols // w), generator=g, device="cuda") * 10 + 0.1
+        s = spread(top / torch.full_like(top, most), rows, cols, (h, w))
+        v = (every[torch.randint(0, len(every), (rows, cols), generator=g, device="cuda")] * s.double()).float()
+        step = torch.randint(-2, 3, (rows, cols), generator=g, device="cuda", dtype=torch.int32)
+        v = (v.view(torch.int32) + step).clamp(min=0).view(torch.float32)
+        v = torch.minimum(v, s * most)
+        v[::h, ::w] = top  # the largest of each block
+        codes, scales = ctx.quantize_fp8(v, (h, w), dtype=dt(CODES[code][0]))
+        want, want_scales = quantized(v, (h, w), code)
+        assert torch.equal(scales, want_scales)
+        wrong = (codes.double() != want).sum().item()
+        assert wrong == 0, (wrong, v.numel())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("code", sorted(CODES))
+def test_16_bit_values_at_the_least_normal_number(ctx, dtype, code):
+    """every significand of a block's largest value, against the values of its type next to the least normal number times the scale; among them 41/1024 beside 1148 in
+    16 bits, whose quotient is 2^-6"""
+    import torch
+
+    _, bits, least, most = CODES[code]
+    kind = dt(dtype)
+    n = 1024 if dtype == "float16" else 128
+    top = ((1 + torch.arange(n, device="cuda").double() / n) * 1024).to(kind)
+    s = (top.float() / torch.full((n,), most, device="cuda")).double()
+    v = torch.zeros(n, 128, dtype=kind, device="cuda")
+    near = (s * 2.0 ** least).to(kind)
+    for i, step in enumerate(range(-3, 4)):
+        v[:, i] = (near.view(torch.int16) + step).view(kind)
+        v[:, 8 + i] = -v[:, i]
+    v[:, 127] = top
+    codes, scales = ctx.quantize_fp8(v, dtype=dt(CODES[code][0]))
+    want, want_scales = quantized(v.float(), (1, 128), code)
+    assert torch.equal(scales, want_scales) and torch.equal(codes.double(), want)
+    if dtype == "float16" and code == "e4m3":
+        x = torch.zeros(1, 128, dtype=kind, device="cuda")
+        x[0, 0], x[0, 1] = 1148, 41 / 1024
+        assert ctx.quantize_fp8(x)[0][0, 1].item() == 2.0 ** -6
+
+
+@pytest.mark.parametrize("code", sorted(CODES))
+@pytest.mark.parametrize("block", sorted(BLOCKS))
 def test_blocks_of_zeros_tiny_huge_and_values_that_are_not_finite(ctx, code, block):
     import torch
 
