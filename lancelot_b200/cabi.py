@@ -462,7 +462,8 @@ class Context:
 
     def fp8_matmul(self, a, a_scale, b, b_scale, dtype=torch.bfloat16, out=None):
         """a [m][k], b [n][k] of 8-bit floats -> [m][n]: for each block of 128 of k, the sum of products times a's and b's scales, added up in 32
-        bits.  a_scale [m][ceil(k / 128)] or [ceil(m / 128)][ceil(k / 128)], b_scale likewise.  An operand is dense along either
+        bits.  a_scale [m][ceil(k / 128)] or [ceil(m / 128)][ceil(k / 128)], b_scale likewise; the product of two scales that meet, and that of a block's
+        sum and a's scale, have to be normal numbers of 32 bits or 0.  An operand is dense along either
         axis: transposed views (of codes and scales) give the gradients of a product without a copy.  With x8, xs = quantize_fp8(x), w8, ws =
         quantize_fp8(w, (128, 128)) and y = fp8_matmul(x8, xs, w8, ws), the gradient of x is fp8_matmul(g8, gs, w8.t(), ws.t()), that of w
         fp8_matmul(gd.t(), gds.t(), xd.t(), xds.t()) from the codes in blocks (128, 1)"""

@@ -114,7 +114,8 @@ def low_rank_update(lb, factors, out=None):
 def fp8_linear(lb, x, w, grad_dtype=torch.float8_e4m3fn):
     """y = x w^T with gradients, x [..., k], w [n][k] (float32, bfloat16, float16, on the device of lb): the three products of a training step in
     8-bit floating point.  x is quantised in blocks of 128 values along what a product sums over, w in blocks of 128 x 128; the gradient of y as x,
-    to grad_dtype.  y and the gradients have the types of x and of their tensors.  What is kept for the backward pass are the codes.  The gradients
+    to grad_dtype.  y and the gradients have the types of x and of their tensors.  Gradients of y below some 1e-30 lose bits (the products of scales leave the
+    normal numbers of 32 bits): a loss that small is scaled up first.  What is kept for the backward pass are the codes.  The gradients
     themselves are not differentiable.  In a graph capture take them with ``torch.autograd.grad``"""
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError("x must be [..., k] and w [n][k]")

@@ -334,6 +334,41 @@ def test_products_of_operands_off_their_alignment(ctx, form, m, n, k):
                 assert bool((held == 3.0).all())
 
 
+# Exponents of the scales of a and b, the largest code (of 8 bits), and how many scales are of ordinary size: the product of two scales, and that of a block's sum and
+# a's scale, are up to the ends of the normal numbers; the block's sum times b's scale need not be in range
+APART = [(-62, -62, 127, 0.3), (64, 63, 1, 0.3), (-20, 110, 127, 0.0), (-100, 126, 127, 0.0), (-140, 20, 127, 0.0), (-70, 70, 127, 0.3), (70, -70, 1, 0.3),
+         (110, -20, 1, 0.3)]
+
+
+@pytest.mark.parametrize("form", sorted(FORMS))
+@pytest.mark.parametrize("m,n,k", [(3, 200, 300), (200, 3, 300), (40, 200, 300), (129, 65, 2100), (1300, 2500, 400), (1301, 2501, 400)])
+def test_scales_far_apart(ctx, form, m, n, k):
+    """Scales of ordinary size beside others in the same tile.  The bound is that of check_product; a term may lose half a step of the subnormal numbers
+    twice beside it, once before it is multiplied by b's scale"""
+    import torch
+
+    block_a, block_b, across_a, across_b = FORMS[form]
+    for i, (ea, eb, top, ordinary) in enumerate(APART):
+        g = gen(m + n + i)
+        a, sa, _ = operand(g, m, k, "e4m3", block_a, across_a)
+        b, sb, _ = operand(g, n, k, "e4m3", block_b, across_b)
+        if top == 1:  # zeros and 2^-9
+            for t in (a, b):
+                t.view(torch.uint8).copy_(torch.randint(0, 2, t.shape, generator=g, device="cuda"))
+            a.view(torch.uint8)[::5] = 0
+            b.view(torch.uint8)[1::3] = 0
+        for s, e in ((sa, ea), (sb, eb)):
+            s.clamp_(0.5, 1.0).mul_(torch.where(torch.rand(s.shape, generator=g, device="cuda") < ordinary, 1.0, 2.0 ** (e // 2)))
+            s.mul_(torch.where(s > 1.5, 2.0 ** (e - e // 2), 1.0) if e > 0 else torch.where(s < 0.4, 2.0 ** (e - e // 2), 1.0))
+        va, vb = a.double() * spread(sa, m, k, block_a).double(), b.double() * spread(sb, n, k, block_b).double()
+        out = ctx.fp8_matmul(a, sa, b, sb, dtype=torch.float32)
+        want, size = va @ vb.t(), va.abs() @ vb.abs().t()
+        blocks = -(-k // 128)
+        bound = (128 + blocks + 4) * 2.0 ** -23 * size + 2.0 ** -24 * want.abs() + blocks * 2.0 ** -149 * (1 + sb.max().item())
+        off = (out.double() - want).abs() - bound
+        assert not out.isnan().any() and off.max().item() <= 0, (ea, eb, off.max().item())
+
+
 def test_scales_that_are_not_finite_or_zero_in_products(ctx):
     import torch
 
