@@ -298,7 +298,8 @@ LB_API int lb_int8_distances(lb_context *ctx, const int8_t *codes, int64_t code_
  * shorter.  dtype, strides and workspaces as in the calls above. */
 
 /* m = max|v| of a block, scale = m / M rounded to 32 bits, code = the type's value nearest to v / scale, ties to even, at most M in
- * magnitude.  A block of zeros has scale 0; one that holds an infinity or NaN has scale NaN and codes 0, so that it reads as NaN.
+ * magnitude.  A block of zeros, or of values so small that m / M rounds to 0, has scale 0; one that holds an infinity or NaN has scale NaN, so that it
+ * reads as NaN.  The codes of either are zeros, with the signs of the values.
  * blocks 1 and 4 fill codes and scales, 2 codes_down and scales_down, 3 all four, with the blocks of 1 and of 2.  Results must not overlap
  * values or one another. */
 LB_API int lb_quantize_fp8(lb_context *ctx, const void *values, int dtype, int64_t n_rows, int64_t n_cols, int64_t value_stride, int blocks,

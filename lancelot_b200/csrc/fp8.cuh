@@ -101,7 +101,7 @@ template <bool E5M2> __device__ __forceinline__ unsigned long long beside_border
     return mul2(h, fma2_of(z, pair(-0x1p-9f, -0x1p-9f), pair(-1.f + 0x1p-10f, -1.f + 0x1p-10f)));
 }
 // smaller scales: a quotient of 64 bits, rounded to 24 in a way that keeps what lies beyond them in the last bit, so that rounding once more is
-// right.  0 where there is no scale, or one that is not finite
+// right.  0 where the scale is not finite
 __device__ __noinline__ float quotient_of_tiny(float m, float s)
 {
     if (!(s > 0.f)) return 0.f;
@@ -111,7 +111,7 @@ __device__ __noinline__ float quotient_of_tiny(float m, float s)
 }
 __device__ __forceinline__ float inverse_of(float s) { return s >= kTinyScale ? __frcp_rn(s) : 0.f; }
 // whether a block's codes cannot be had with that
-__device__ __forceinline__ bool odd_scale(float s) { return !(s >= kTinyScale) && s != 0.f; }
+__device__ __forceinline__ bool odd_scale(float s) { return !(s >= kTinyScale); }
 
 // The codes of four magnitudes (bits), of one scale or of a scale each (s), with the factors to their quotients (f).  ODD: one of the scales may be
 template <bool E5M2, bool ODD> __device__ __forceinline__ unsigned codes4(const uint4 &m, const float4 &s, const float4 &f)

@@ -88,6 +88,8 @@ template <bool E5M2> __device__ __forceinline__ float scale_of(unsigned most)
 {
     return most >= kInf ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(most), Fp8<E5M2>::kMost);
 }
+// What codes are decided by: the scale, and for a block without one (of zeros, or of values so small that their scale rounds to 0) any that makes its codes 0
+__device__ __forceinline__ float divisor_of(float scale) { return scale == 0.f ? 1.f : scale; }
 __device__ __forceinline__ float4 all(float v) { return make_float4(v, v, v, v); }
 
 struct QuantizeFp8Args {
@@ -173,10 +175,10 @@ template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bo
             const unsigned most = __reduce_max_sync(0xffffffffu, V::all(V::more(V::none(), raw[i])));
             if (lane == i) mine = most;
         }
-        const float scale = scale_of<E5M2>(mine), inverse = inverse_of(scale);
+        const float scale = scale_of<E5M2>(mine), divisor = divisor_of(scale), inverse = inverse_of(divisor);
         if (lane < rows) a.scales[(r0 + lane * kWarps) * a.scale_stride + tc] = scale;
-        put_rows(a.codes, a.code_stride, [&](int i, float4 &s, float4 &f) { s = all(__shfl_sync(0xffffffffu, scale, i)), f = all(__shfl_sync(0xffffffffu, inverse, i)); },
-                 __any_sync(0xffffffffu, odd_scale(scale)));
+        put_rows(a.codes, a.code_stride, [&](int i, float4 &s, float4 &f) { s = all(__shfl_sync(0xffffffffu, divisor, i)), f = all(__shfl_sync(0xffffffffu, inverse, i)); },
+                 __any_sync(0xffffffffu, odd_scale(divisor)));
     }
     if constexpr (MODE == kSquare || MODE == kColumns || MODE == kBoth) {
         typename V::Most most = V::none();
@@ -187,9 +189,9 @@ template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bo
             if (lane == 0) part[0][warp] = m;
             __syncthreads();
             m = __reduce_max_sync(0xffffffffu, part[0][lane & (kWarps - 1)]);
-            const float scale = scale_of<E5M2>(m), inverse = inverse_of(scale);
+            const float scale = scale_of<E5M2>(m), divisor = divisor_of(scale), inverse = inverse_of(divisor);
             if (threadIdx.x == 0) a.scales[tr * a.scale_stride + tc] = scale;
-            put_rows(a.codes, a.code_stride, [&](int, float4 &s, float4 &f) { s = all(scale), f = all(inverse); }, odd_scale(scale));
+            put_rows(a.codes, a.code_stride, [&](int, float4 &s, float4 &f) { s = all(divisor), f = all(inverse); }, odd_scale(divisor));
         } else {
             *reinterpret_cast<uint4 *>(&part[warp][lane * 4]) = V::columns(most);
             __syncthreads();
@@ -198,7 +200,7 @@ template <typename T, bool E5M2, int MODE, bool VEC> __global__ void __launch_bo
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) m = max(m, part[w][threadIdx.x]);
                 const float s = scale_of<E5M2>(m);
-                column[threadIdx.x] = s;
+                column[threadIdx.x] = divisor_of(s);
                 if (tc * kB + (int)threadIdx.x < a.cols) a.down_scales[tr * a.down_scale_stride + tc * kB + threadIdx.x] = s;
             }
             __syncthreads();

@@ -208,6 +208,26 @@ def test_blocks_of_zeros_tiny_huge_and_values_that_are_not_finite(ctx, code, blo
     assert ctx.dequantize_fp8(*ctx.quantize_fp8(x)).isnan().sum() == 2
 
 
+@pytest.mark.parametrize("code", sorted(CODES))
+@pytest.mark.parametrize("block", sorted(BLOCKS))
+def test_scales_that_round_to_zero(ctx, code, block):
+    """blocks whose largest value is so small that no scale is left have codes 0, whatever the blocks beside them are"""
+    import torch
+
+    h, w = BLOCKS[block]
+    rows, cols = 256, 512
+    for e in range(-149, -125):
+        top = torch.full((-(-rows // h), -(-cols // w)), 2.0 ** e, dtype=torch.float64, device="cuda").float()
+        for beside in (None, 2.0 ** -120, 1.0, math.inf):
+            if beside is not None:
+                top.view(-1)[1::2] = beside
+            v = spread(top, rows, cols, (h, w)).contiguous()
+            v[1::2] *= -1
+            codes, scales = ctx.quantize_fp8(v, (h, w), dtype=dt(CODES[code][0]))
+            want, want_scales = quantized(v, (h, w), code)
+            assert same(scales, want_scales) and torch.equal(codes.double(), want), (e, beside)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
 @pytest.mark.parametrize("shift,pitch", [(0, 520), (1, 520), (0, 517), (3, 515), (8, 528)])
 def test_strided_values_and_given_results(ctx, dtype, shift, pitch):
