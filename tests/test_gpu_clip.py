@@ -219,6 +219,94 @@ def test_more_tensors_than_one_launch_holds(ctx):
         assert all(torch.equal(t, clipped(b, f)) for t, b in zip(updates[i], before[i]))
 
 
+ROUNDS = {"by count": (5, [3 + i * 37 % 91 for i in range(150)], "float32"), "by count, 16 bits": (7, [1 + i * 53 % 701 for i in range(201)], "bfloat16"),
+          "by bytes": (4, [9999999, 1, 77, 123457], "float32"), "by bytes, 16 bits": (5, [17000003, 5, 2999], "float16"),
+          "one client a round": (3, [26000001, 13], "float32"), "clients of more tensors than a launch holds": (3, [5 + i % 7 for i in range(700)], "float32")}
+
+
+@pytest.mark.parametrize("case", sorted(ROUNDS))
+@pytest.mark.parametrize("bad", [None, 2])
+def test_several_rounds_of_clients(ctx, case, bad):
+    """results of some clients are written while the next ones are summed up: in place, as rows of either width, norms alone"""
+    import torch
+
+    clients, sizes, dtype = ROUNDS[case]
+    g = gen(40)
+    base = [make(g, sizes, dtype, 0.01 * (1 + c)) for c in range(clients)]
+    if bad is not None:
+        base[bad][len(sizes) // 2][0] = math.inf
+    # every tensor lies somewhere else between two boundaries of 16 bytes, in memory that is otherwise left as it was
+    pads = [[(i + c) % 9 for i in range(len(sizes))] for c in range(clients)]
+
+    def laid_out():
+        held = [[torch.full((n + 16,), 3.0, dtype=dt(dtype), device="cuda") for n in sizes] for _ in range(clients)]
+        views = [[h[p:p + n] for h, p, n in zip(hs, ps, sizes)] for hs, ps in zip(held, pads)]
+        for vs, bs in zip(views, base):
+            for v, b in zip(vs, bs):
+                v.copy_(b)
+        return held, views
+
+    held, views = laid_out()
+    norms = ctx.clip_updates(views)
+    good = [c for c in range(clients) if c != bad]
+    check_norms(norms[good], [base[c] for c in good])
+    assert bad is None or norms[bad].item() == math.inf
+    most = norms[good].median().item()
+    factors = [math.nan if c == bad else factor(norms[c].item(), most) for c in range(clients)]
+    dim = sum(sizes)
+    for into in ("float32", dtype):
+        want = torch.stack([torch.cat([clipped(b, f, dt(into)) for b in bs]) for bs, f in zip(base, factors)])
+        for _ in range(3):
+            room = torch.full((clients, dim + 5), 9.0, dtype=dt(into), device="cuda")
+            assert torch.equal(ctx.clip_updates(views, most, out=room[:, 2:2 + dim]), norms)
+            assert same(room[:, 2:2 + dim], want)
+            assert bool((room[:, :2] == 9).all() and (room[:, 2 + dim:] == 9).all())
+        del want, room
+    for _ in range(2):
+        assert torch.equal(ctx.clip_updates(views, most), norms)
+        for vs, hs, bs, ps, f in zip(views, held, base, pads, factors):
+            for v, h, b, p in zip(vs, hs, bs, ps):
+                assert same(v, clipped(b, f))
+                assert bool((h[:p] == 3).all() and (h[p + v.numel():] == 3).all())
+        held, views = laid_out()
+
+
+def test_rounds_in_a_captured_graph(ctx):
+    import torch
+
+    clients, sizes, dtype = ROUNDS["by count"]
+    g = gen(41)
+    updates = [make(g, sizes, dtype, 1 + c) for c in range(clients)]
+    out = torch.empty(clients, sum(sizes), device="cuda")
+    ctx.clip_updates(updates, 100.0, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norms = ctx.clip_updates(updates, 100.0, out=out)
+    for seed in (1, 2):
+        for ts in updates:
+            for t in ts:
+                t.normal_(generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone(), norms.clone()
+        want = torch.empty_like(out)
+        assert torch.equal(ctx.clip_updates(updates, 100.0, out=want), got[1]) and torch.equal(got[0], want)
+
+
+def test_norms_of_more_clients_than_one_launch_holds(ctx):
+    import torch
+
+    m = torch.randn(4321, 37, generator=gen(42), device="cuda")
+    norms = ctx.clip_updates(m)
+    want = m.double().square().sum(1).sqrt()
+    assert bool(((norms - want).abs() <= want * 2.0 ** -53 * 41).all())
+    out = torch.empty_like(m)
+    assert torch.equal(ctx.clip_updates(m, 6.0, out=out), norms)
+    f = torch.where(norms > 6.0, 6.0 / norms, torch.ones_like(norms)).float()
+    assert torch.equal(out, m * f[:, None])
+
+
 def test_the_same_result_every_time_and_on_two_streams(ctx):
     import torch
 
