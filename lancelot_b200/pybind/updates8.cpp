@@ -106,6 +106,15 @@ Tensor result(const Call &c, const Maybe &out, int64_t rows, int64_t cols, int d
     if (out->size(0) != rows || out->size(1) != cols) refuse("out must be [" + std::to_string(rows) + "][" + std::to_string(cols) + "]");
     return *out;
 }
+// a caller's tensor that a call has written: autograd sees from its version that it is no longer what was saved
+void written(const Tensor &t)
+{
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(const Maybe &t)
+{
+    if (t) written(*t);
+}
 Call call_of(int64_t context, int device) { return Call{reinterpret_cast<lb_context *>(context), device}; }
 
 void quantize_rows(int64_t context, int device, const Tensor &values, const Tensor &codes, const Tensor &scales, int64_t group, const Maybe &slots,
@@ -135,6 +144,9 @@ void quantize_rows(int64_t context, int device, const Tensor &values, const Tens
     check(lb_quantize_rows(c.context, address<void>(values), type, n, cols, row_stride(values), address<int32_t>(lengths), address<float>(residual),
                            address<float>(residual_out), stride, table, k.slots, k.page, group, k.codes, k.code_stride, k.scales, k.scale_stride,
                            address<void>(ws), need, c.stream()));
+    written(codes);
+    written(scales);
+    written(residual_out);
 }
 
 Tensor dequantize_rows(int64_t context, int device, const Tensor &codes, const Tensor &scales, int64_t n_cols, int64_t group, const Maybe &slots,
@@ -150,6 +162,7 @@ Tensor dequantize_rows(int64_t context, int device, const Tensor &codes, const T
     const Tensor to = result(c, out, n, n_cols, dtype);
     check(lb_dequantize_rows(c.context, k.codes, k.code_stride, k.scales, k.scale_stride, k.slots, k.page, group, table, n, n_cols, address<void>(to),
                              value_type(to.scalar_type()), row_stride(to), c.stream()));
+    written(out);
     return to;
 }
 
@@ -170,6 +183,7 @@ Tensor int8_matmul(int64_t context, int device, const Tensor &a, const Tensor &b
     const Tensor ws = c.workspace(need);
     check(lb_int8_matmul(c.context, m, n, k, pa, sa, address<float>(a_scale), pb, sb, address<float>(b_scale), address<void>(to),
                          value_type(to.scalar_type()), row_stride(to), address<void>(ws), need, c.stream()));
+    written(out);
     return to;
 }
 
@@ -219,12 +233,14 @@ py::tuple quantize_fp8(int64_t context, int device, const Tensor &values, int bl
     if (blocks < 1 || blocks > 4) refuse("block must be (1, 128), (128, 1) or (128, 128)");
     if (type != 5 && type != 6) refuse("dtype must be float8_e4m3fn or float8_e5m2");
     const int64_t n = values.size(0), cols = values.size(1);
+    const Maybe given[] = {codes, scales, codes_down, scales_down};
     if (blocks != 2) blocks_into(c, codes, scales, n, cols, blocks == 4 ? blocks_of(n) : n, blocks_of(cols), type);
     if (blocks == 2 || blocks == 3) blocks_into(c, codes_down, scales_down, n, cols, blocks_of(n), cols, type);
     auto stride = [](const Maybe &t) { return t ? row_stride(*t) : 0; };
     check(lb_quantize_fp8(c.context, address<void>(values), dtype, n, cols, row_stride(values), blocks, type, address<uint8_t>(codes), stride(codes),
                           address<float>(scales), stride(scales), address<uint8_t>(codes_down), stride(codes_down), address<float>(scales_down),
                           stride(scales_down), c.stream()));
+    for (const Maybe &t : given) written(t);
     if (blocks == 3) return py::make_tuple(*codes, *scales, *codes_down, *scales_down);
     return blocks == 2 ? py::make_tuple(*codes_down, *scales_down) : py::make_tuple(*codes, *scales);
 }
@@ -242,6 +258,7 @@ Tensor dequantize_fp8(int64_t context, int device, const Tensor &codes, const Te
     const Tensor to = result(c, out, n, cols, dtype);
     check(lb_dequantize_fp8(c.context, address<uint8_t>(codes), type, row_stride(codes), address<float>(scales), row_stride(scales), blocks, n, cols,
                             address<void>(to), value_type(to.scalar_type()), row_stride(to), c.stream()));
+    written(out);
     return to;
 }
 
@@ -281,6 +298,7 @@ Tensor fp8_matmul(int64_t context, int device, const Tensor &a, const Tensor &a_
     const size_t need = lb_fp8_matmul_workspace_bytes(m, n, k, &x, &y);
     const Tensor ws = c.workspace(need);
     check(lb_fp8_matmul(c.context, m, n, k, &x, &y, address<void>(to), value_type(to.scalar_type()), row_stride(to), address<void>(ws), need, c.stream()));
+    written(out);
     return to;
 }
 
@@ -496,8 +514,6 @@ Tensor clip_updates(int64_t context, int device, const py::object &updates, std:
     } else if (in_place) {
         for (const void *p : tensors) outs.push_back(const_cast<void *>(p));
         out_dtypes = dtypes;
-        for (const Tensor &t : held)
-            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
     }
     const Tensor norms = c.empty({n}, at::kDouble);
     const int count = (int)sizes.size();
@@ -506,6 +522,9 @@ Tensor clip_updates(int64_t context, int device, const py::object &updates, std:
     const Tensor ws = c.workspace(need);
     check(lb_clip_updates(c.context, n, count, clients.data(), tensors.data(), dtypes.data(), sizes.data(), max_norm ? *max_norm : HUGE_VAL,
                           out || in_place ? outs.data() : nullptr, writes, address<double>(norms), address<void>(ws), need, c.stream()));
+    written(out);
+    if (in_place)
+        for (const Tensor &t : held) written(t);
     return norms;
 }
 

@@ -690,6 +690,57 @@ def test_gradients_against_differences(ctx):
             assert said != 0 and found == said
 
 
+def test_what_is_written_counts_as_changed(ctx):
+    """autograd notices that a tensor which it saved was overwritten; a call that is refused changes nothing"""
+    import torch
+
+    from lancelot_b200 import updates
+    from lancelot_b200._lib import InvalidArgument
+
+    g = gen(16)
+    x = torch.randn(64, 256, generator=g, device="cuda")
+    x8, xs, xd, xds = ctx.quantize_fp8_both(x)
+    y = torch.zeros(64, 64, device="cuda")
+    wide, rows = torch.zeros(64, 256, device="cuda"), torch.zeros(2, 256, device="cuda")
+    i8, i8s = torch.zeros(64, 256, dtype=torch.int8, device="cuda"), torch.zeros(64, 1, device="cuda")
+    res = torch.zeros(64, 256, device="cuda")
+    a, b = torch.ones(256, device="cuda"), torch.ones(256, device="cuda")
+    for call, written in ((lambda: ctx.quantize_fp8(x, codes=x8, scales=xs), (x8, xs)),
+                          (lambda: ctx.quantize_fp8(x, (128, 1), codes=xd, scales=xds), (xd, xds)),
+                          (lambda: ctx.dequantize_fp8(x8, xs, out=wide), (wide,)),
+                          (lambda: ctx.fp8_matmul(x8, xs, x8, xs, out=y), (y,)),
+                          (lambda: ctx.clip_updates([[a], [b]], 1.0, out=rows), (rows,)),
+                          (lambda: ctx.clip_updates([[a], [b]], 1.0), (a, b)),
+                          (lambda: ctx.clip_updates(rows, 1.0), (rows,)),
+                          (lambda: ctx.quantize_rows(x, i8, i8s, residual=res, residual_out=res), (i8, i8s, res)),
+                          (lambda: ctx.dequantize_rows(i8, i8s, 256, out=wide), (wide,)),
+                          (lambda: ctx.int8_matmul(i8, i8, i8s.view(-1), i8s.view(-1), out=y), (y,))):
+        before = [t._version for t in written]
+        others = [(t, t._version) for t in (x, x8, xs, xd, xds, y, wide, rows, i8, i8s, res, a, b) if not any(t is u for u in written)]
+        call()
+        assert all(t._version > v for t, v in zip(written, before))
+        assert all(t._version == v for t, v in others)
+    for call, kept in ((lambda: ctx.clip_updates([[a], [a]], 1.0), a), (lambda: ctx.clip_updates([[a, b[:3]], [b]], 1.0), a),
+                       (lambda: ctx.clip_updates([[rows[0]], [a]], 1.0, out=rows.view(2, 256).flip(0)[:, :255]), rows)):
+        before = kept._version
+        with pytest.raises(InvalidArgument):
+            call()
+        assert kept._version == before
+    # nothing is read for the norms alone, and a saved result that a later call overwrites is found out
+    before = a._version
+    ctx.clip_updates([[a], [b]])
+    assert a._version == before
+    p = torch.ones(64, 64, device="cuda", requires_grad=True)
+    z = (p * y).sum()
+    ctx.fp8_matmul(x8, xs, x8, xs, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    with torch.inference_mode():
+        t = torch.zeros(64, 64, device="cuda")
+        ctx.fp8_matmul(x8, xs, x8, xs, out=t)
+        ctx.clip_updates([[t]], 1.0)
+
+
 def test_updates_of_low_rank_from_8_bit_floats(ctx):
     import torch
 
