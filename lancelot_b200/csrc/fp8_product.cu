@@ -454,9 +454,8 @@ __global__ void __launch_bounds__(TileFp8<BN, OFF>::kThreads, 1) fp8_product_ker
                         if (left >= 2) {
                             if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(out + i * 8) = make_float2(x, y);
                             else *reinterpret_cast<unsigned *>(out + i * 8) = pack2(out, x, y);
-                        } else {
-                            if (left >= 1) put(out + i * 8, x);
-                            if (left >= 2) put(out + i * 8 + 1, y);
+                        } else if (left == 1) {
+                            put(out + i * 8, x);
                         }
                     }
                 }
