@@ -323,7 +323,8 @@ typedef struct lb_fp8_operand {
 
 /* out[i][j] = sum over blocks p of (sum over k in p of a[i][k] b[j][k]) * a's scale * b's scale: sums and products in 32-bit floats, one rounding to
  * dtype.  Two products have to be normal numbers (from 2^-126 on, finite) or 0: that of the two scales, and that of a block's sum and a's scale.
- * Which one is formed goes by the shapes; below that range bits are lost, above it results are infinite or NaN.
+ * Which one is formed goes by the shapes.  Below that range a term is off by up to the block's sum times 2^-150, or b's scale times 2^-150; above it
+ * results are infinite or NaN.
  * Any alignment of the codes' rows: those off a 16-byte boundary may be copied into the workspace first, and are read in whole
  * aligned pieces of 16 bytes (up to 15 bytes on either side are read along and dropped).  out must not overlap an operand. */
 LB_API size_t lb_fp8_matmul_workspace_bytes(int64_t m, int64_t n, int64_t k, const lb_fp8_operand *a, const lb_fp8_operand *b);

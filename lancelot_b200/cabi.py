@@ -477,7 +477,8 @@ class Context:
         """The norm of each client's update over all its tensors -> [n_clients] float64, on the device.  updates: for each client a list of tensors
         (float32, bfloat16, float16, also mixed), or a matrix with a row for each client.  With max_norm, updates of a larger norm are
         scaled down to it, in place; one whose norm is not finite becomes NaN throughout.  out [n_clients][values] (float32, bfloat16,
-        float16): the (scaled) values of each client, tensor by tensor, go there instead, and the tensors stay as they are"""
+        float16): the (scaled) values of each client, tensor by tensor, go there instead, and the tensors stay as they are; NaN throughout where the
+        norm is not finite, without max_norm too"""
         return _updates8().clip_updates(self._handle(), self.device, updates, max_norm, out)
 
     def check_status(self):

@@ -165,11 +165,12 @@ __device__ __forceinline__ void copy4(unsigned to, const float *from) { asm vola
 // One CTA per SM walks over tiles of 128 x BN.  Warp 0 brings 128 bytes of the summed axis of either operand by TMA into a ring of stages, warp 1 issues the
 // products (four of k = 32 a block) into one of two or four places in TMEM, and warps 4 to 11 scale a block's sums and add them to results that they keep
 // in registers: a scale is for 128 of the summed axis, so the sums have to leave TMEM that often.  A block of a tile 256 wide takes some 1050 cycles, of which the
-// products are 512 (the tensor cores are active in 51 % of the cycles): what bounds it is the chain from the products' end over the sums' way to the registers to the
-// next products, with two places for the sums, beside the 96 KB that shared memory takes in and gives out.  8192 x 8192 x 8192 takes 485 to 505 us (2.2 P
-// operations a second; among others of its kind 570 us, under the power cap), without the accumulating warps' work 423 us, without the products 323 us.  Two CTAs on
+// products are 512 (the tensor cores are active in 51 % of the cycles): what bounds it is the 96 KB that shared memory takes in and gives out a block, and the chain from
+// the products' end over the sums' way to the registers to the next products, with two places for the sums.  8192 x 8192 x 8192 takes 480 to 500 us (2.2 P
+// operations a second; among others of its kind 570 to 597 us, under the power cap), without the accumulating warps' work 423 us, without the products 323 us,
+// without either 281 us.  Two CTAs on
 // a tile of 256 x 256, which move 64 KB a block, wait longer for one another than that saves (732 us).  With a scale per row of b there is a product
-// more for every sum: 4096 x 11008 x 4096 in 305 us.  Everything in the accumulating warps' chain costs what it takes: a vote a block 3 %,
+// more for every sum, and TMEM is read 16 registers at a time: 4096 x 11008 x 4096 in 307 us, without that product 276, without the accumulating warps' work 169.  Everything in the accumulating warps' chain costs what it takes: a vote a block 3 %,
 // scales through shared memory instead of a load ahead 25 % (with a scale per row, where loads are many, they gain 8 %).
 //
 // PER_ROW: b has a scale for each of its rows, otherwise one for 128.
@@ -614,7 +615,7 @@ template <typename T> int product_typed(Context *ctx, int m, int n, int k, const
     // The tile, and the CTAs that share one, that take least, in microseconds as measured: waves over the SMs, in each a block of the summed axis at
     // what one takes (by shared memory and the accumulating warps; with a scale per row of b by the latter), and a tile's results; a split adds two.
     // 2048 x 2048 x 2048 takes 12.7 us with tiles 256 wide and 16.3 with 128, 4096 x 4096 x 64 14.3 and 13.5; 100 x 100 x 4096 7.0 us split
-    // over eight and 18.8 by one.
+    // over eight and 18.8 by one.  Results off a 16-byte boundary, which take longer to write, get the same tiles: the times are those of aligned ones.
     int bn = 128, split = 1;
     double least = 0.0;
     const bool per_row = b.scale_shift == 0;

@@ -7,8 +7,8 @@
 // has 128 values, so the operand of a product and that of its gradient are the same matrix in two kinds of blocks.
 //
 // Both kernels work on tiles of 128 x 128 and are bound by their instructions (some 20 a value and kind of blocks, issued in 70 % of the cycles) rather than by memory:
-// 8192 x 4096 in bf16 in rows 32 us (3.2 TB/s), in squares 29, in both kinds 52; in 32 bits 35, 34 and 55 (3.7 to 4.9 TB/s); 4096 x 11008 in 32 bits in squares
-// 45 us (5.0 TB/s).  Read back to bf16 23 to 25 us (4.3 TB/s).  Rows off their alignment: 8192 x 4095 in bf16 54 and 40 us.
+// 8192 x 4096 in bf16 in rows 31 us (3.2 TB/s), in columns 32, in squares 28.5, in both kinds 50; in 32 bits 34, 35, 33.5 and 54 (3.7 to 4.9 TB/s); 4096 x 11008
+// in 32 bits in squares 43.5 us (5.2 TB/s).  Read back to bf16 20 to 24 us (4.3 TB/s).  Rows off their alignment: 8192 x 4095 in bf16 52 and 40 us.
 #include <type_traits>
 
 #include "fp8.cuh"
