@@ -463,31 +463,46 @@ Tensor clip_updates(int64_t context, int device, const py::object &updates, std:
         for (; n < t.size(0); ++n) add(t, t.size(1), n * t.stride(0));
         held.push_back(t);
     } else {
-        // A sequence may make its items when they are asked for: all tensors are held, from here to the launch, before the first address is taken
         if (!py::isinstance<py::sequence>(updates)) refuse("updates must be a matrix, or for each client a list of tensors");
-        std::vector<size_t> ends; // of each client's tensors
-        for (const py::object client : py::reinterpret_borrow<py::sequence>(updates)) {
+        auto add_tensor = [&](const Tensor &t) {
+            if (!t.is_cuda() || t.get_device() != c.device || t.layout() != at::kStrided) refuse("an update's tensors must be on cuda:" + std::to_string(device));
+            if (!value_type(t.scalar_type())) refuse("an update's tensors must be float32, bfloat16 or float16");
+            // the order of the values is the result's where they are copied
+            if (out ? !t.is_contiguous() : !t.is_non_overlapping_and_dense()) refuse(out ? "an update's tensors must be contiguous" : "an update's tensors must be dense");
+            add(t, t.numel(), 0);
+        };
+        auto each = [&](const py::handle &client, auto &&use) {
             if (THPVariable_Check(client.ptr()) || !py::isinstance<py::sequence>(client)) refuse("updates must be a matrix, or for each client a list of tensors");
             const py::object items = py::reinterpret_steal<py::object>(PySequence_Fast(client.ptr(), "updates"));
             if (!items) throw py::error_already_set();
             for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(items.ptr()); ++i) {
                 const py::handle item = PySequence_Fast_GET_ITEM(items.ptr(), i);
                 if (!THPVariable_Check(item.ptr())) refuse("updates must be a matrix, or for each client a list of tensors");
-                held.push_back(THPVariable_Unpack(item.ptr()));
+                use(THPVariable_Unpack(item.ptr()));
             }
-            ends.push_back(held.size());
-        }
-        size_t i = 0;
-        for (const size_t end : ends) {
-            for (; i < end; ++i) {
-                const Tensor &t = held[i];
-                if (!t.is_cuda() || t.get_device() != c.device || t.layout() != at::kStrided) refuse("an update's tensors must be on cuda:" + std::to_string(device));
-                if (!value_type(t.scalar_type())) refuse("an update's tensors must be float32, bfloat16 or float16");
-                // the order of the values is the result's where they are copied
-                if (out ? !t.is_contiguous() : !t.is_non_overlapping_and_dense()) refuse(out ? "an update's tensors must be contiguous" : "an update's tensors must be dense");
-                add(t, t.numel(), 0);
+        };
+        // Lists and tuples keep their tensors, and nothing runs in this thread's place, or in another's, that could take them away before the launch.  Any other
+        // sequence may make its items when they are asked for, and change lists meanwhile: then all tensors are held, before the first address is taken
+        auto keeps = [](PyObject *of) { return PyList_CheckExact(of) || PyTuple_CheckExact(of); };
+        bool lasting = keeps(updates.ptr());
+        for (Py_ssize_t k = 0; lasting && k < PySequence_Fast_GET_SIZE(updates.ptr()); ++k) lasting = keeps(PySequence_Fast_GET_ITEM(updates.ptr(), k));
+        if (lasting) {
+            for (; n < PySequence_Fast_GET_SIZE(updates.ptr()); ++n)
+                each(PySequence_Fast_GET_ITEM(updates.ptr(), n), [&](const Tensor &t) {
+                    add_tensor(t);
+                    if (in_place) held.push_back(t);
+                });
+        } else {
+            std::vector<size_t> ends; // of each client's tensors
+            for (const py::object client : py::reinterpret_borrow<py::sequence>(updates)) {
+                each(client, [&](const Tensor &t) { held.push_back(t); });
+                ends.push_back(held.size());
             }
-            ++n;
+            size_t i = 0;
+            for (const size_t end : ends) {
+                for (; i < end; ++i) add_tensor(held[i]);
+                ++n;
+            }
         }
     }
     if (max_norm && !(*max_norm >= 0.0)) refuse("max_norm is a number that is not negative");
